@@ -153,6 +153,68 @@ int tfa_b200_fwd_decode_noalloc(const void* Q, const void* K, const void* V, voi
                                 int seqLenQ, int seqLenKV, int numHeadsQ, int numHeadsKV, int headDim, int isCausal,
                                 int numSplits, void* stream);
 
+/*
+ * Attention whose scores are capped, biased by distance, or masked by prefix or document.  No counterpart in the reference.
+ * Tensors, layouts and limits of tfa_b200_fwd.  Query row i of every batch entry has position qStart + i, key j position j (qStart:
+ * a chunk or a single token behind keys that are there already).
+ *   s = q . k / sqrt(headDim);  softcap > 0: s <- softcap * tanh(s / softcap);  alibiSlopes [numHeadsQ]: s <- s - slope_h * |position - j|
+ *   A row sees key j if (not isCausal, or j <= position, or j < prefixLens[b]) and (no documents, or docIdsQ[b][i] == docIdsKV[b][j] >= 0).
+ * prefixLens int32 [batchSize] (with isCausal only); docIdsQ int32 [batchSize, seqLenQ], docIdsKV int32 [batchSize, seqLenKV]: both or
+ * neither; negative ids belong to no document (padding): such a key is seen by no row and such a row sees no key.  Ids may come in any
+ * order; keys outside the range of blocks that a 128-row tile of queries can see are not read, so runs of equal ids in ascending order
+ * are fast.  A row that sees no key is zero.  softcap 0 and null pointers switch a part off.
+ */
+int tfa_b200_fwd_scored(const void* Q, const void* K, const void* V, void* O, int dtype, int batchSize, int seqLenQ, int seqLenKV,
+                        int numHeadsQ, int numHeadsKV, int headDim, int isCausal, int qStart, float softcap, const float* alibiSlopes,
+                        const int* prefixLens, const int* docIdsQ, const int* docIdsKV, void* stream);
+
+/*
+ * The paged 8-bit K/V cache.  K and V each are codes [numBlocks, numHeadsKV, blockTokens, headDim] (int8, or e4m3 as uint8) and one fp32
+ * scale per (block, head) [numBlocks, numHeadsKV]: value = code * scale.  blockTokens is 16, 32, 64 or 128.  Token t of request b lies in
+ * cell t % blockTokens of block blockTable[b][t / blockTokens] (int32 [batchSize, maxBlocks]); its slot is block * blockTokens + cell.
+ */
+#define TFA_B200_CACHE_INT8 1
+#define TFA_B200_CACHE_E4M3 2
+
+/*
+ * Block tables and slot maps from request lengths, on the device.  seqLens: tokens that each request holds; newLens: tokens that it
+ * gets now (negative counts as none); finished (may be null): requests that give all their blocks back and start anew from length zero.
+ * freeBlocks [freeCapacity] is a stack of free block ids with its top at *numFree - 1: first the blocks of finished requests go on top, in
+ * the order of the requests and of their tables, then every request in order takes the blocks it needs from the top.  A request whose
+ * blocks would not all be there, counting every request ahead of it, or that would need more than maxBlocks, gets none: its length stays
+ * and its rows have slot -1.  blockTable and freeBlocks are updated in place; written are
+ *   cuSeqLens [batchSize + 1]: prefix sums of newLens;  slots int64 [totalNew]: the slot of every packed row, -1 behind the last request;
+ *   seqLensAfter [batchSize];  *numFreeAfter.
+ * totalNew is the row count of the packed tensors, at least the sum of newLens (rows past it get no slot).
+ */
+int tfa_b200_kv_cache_plan(int* blockTable, const int* seqLens, const int* newLens, const unsigned char* finished, int* freeBlocks,
+                           const int* numFree, long long* slots, int* cuSeqLens, int* seqLensAfter, int* numFreeAfter, int batchSize,
+                           int maxBlocks, int freeCapacity, int blockTokens, long long totalNew, void* stream);
+
+/*
+ * Rows of K and V [totalNew, numHeadsKV, headDim] (dtype code) -> their slots of the cache.  A block's scale grows to what its new
+ * rows need: scale <- max(scale, max |x| / 127 or / 448), codes = round(x / scale) with a new scale taken before it is rounded to the fp32
+ * that is stored, and codes that were there before are rounded anew when it
+ * grows; rows that begin at a block's first cell begin it, whatever its scale was.  Infinities become the largest code and NaN zero, and
+ * neither counts for the scale.  Slots below 0 or past the cache are skipped.  The rows of one block have to follow one another, and no slot
+ * may come twice (as tfa_b200_kv_cache_plan gives them): what such a call leaves in that block is undefined.
+ */
+int tfa_b200_kv_cache_store(const void* K, const void* V, void* kCache, void* vCache, float* kScales, float* vScales, const long long* slots,
+                            int dtype, int cacheType, long long totalNew, int numBlocks, int numHeadsKV, int headDim, int blockTokens,
+                            void* stream);
+
+/*
+ * Attention of packed queries over the cache.  Q, O [totalQ, numHeadsQ, headDim] fp16 / bf16; cuSeqLensQ int32 [batchSize + 1]; seqLens
+ * int32 [batchSize]: tokens of each request, those of its queries included - they are its last positions.  isCausal: a query sees the
+ * keys up to its own position, else all of the request's.  softcap and alibiSlopes as in tfa_b200_fwd_scored.  maxSeqLenQ / maxSeqLenKV
+ * only size the launch.  Every row of O is written: rows of no request, of a request without tokens and rows in front of its first position
+ * are zero.  Keys in blocks whose id is outside [0, numBlocks) are not seen.
+ */
+int tfa_b200_fwd_cache(const void* Q, void* O, const void* kCache, const void* vCache, const float* kScales, const float* vScales,
+                       const int* blockTable, const int* seqLens, const int* cuSeqLensQ, int dtype, int cacheType, int batchSize,
+                       int maxSeqLenQ, int maxSeqLenKV, long long totalQ, int numBlocks, int maxBlocks, int blockTokens, int numHeadsQ,
+                       int numHeadsKV, int headDim, int isCausal, float softcap, const float* alibiSlopes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,202 @@
+"""flash_attn_scored_forward on the GPU against 64 bits: caps, distance bias, prefix and document masks, first positions."""
+import math
+
+import pytest
+import torch
+
+import tinyfa_b200 as tfa
+from plain64 import U, attend, check, visible
+
+pytestmark = pytest.mark.gpu
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def _inputs(dtype, B, Sq, Skv, Hq, Hkv, D, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return tuple(torch.randn(B, s, h, D, device="cuda", generator=g).to(DT[dtype]) for s, h in ((Sq, Hq), (Skv, Hkv), (Skv, Hkv)))
+
+
+def _slopes(H):
+    return torch.tensor([2.0 ** (-8.0 * (h + 1) / H) for h in range(H)], device="cuda")
+
+
+def _compare(got, Q, K, V, causal, cap=0.0, slopes=None, prefix=None, dq=None, dk=None, q_start=0):
+    for b in range(Q.shape[0]):
+        see, dist = visible(Q.shape[1], K.shape[1], causal, q_start, None if prefix is None else int(prefix[b]), None if dq is None else dq[b],
+                            None if dk is None else dk[b])
+        o, off, a = attend(Q[b].double(), K[b].double(), V[b].double(), see, cap, slopes, dist,
+                            2.0 ** -21 if Q.dtype == torch.float32 else 8.6e-5)
+        check(got[b], o, off, a, U[Q.dtype], K.shape[1] * 2.0 ** -25 * V[b].abs().max().item() if Q.dtype == torch.float16 else 0.0)
+
+
+SHAPES = [  # dtype, B, Sq, Skv, Hq, Hkv, D
+    ("fp16", 1, 1, 1, 1, 1, 32), ("bf16", 2, 7, 9, 3, 1, 64), ("fp16", 2, 130, 257, 4, 2, 96), ("bf16", 1, 300, 300, 8, 2, 128),
+    ("fp16", 1, 200, 461, 2, 2, 192), ("bf16", 1, 131, 300, 4, 1, 256), ("bf16", 2, 517, 333, 6, 3, 32), ("fp16", 3, 257, 129, 4, 4, 64),
+    ("fp32", 1, 1, 3, 2, 1, 32), ("fp32", 2, 65, 130, 4, 2, 64), ("fp32", 1, 130, 67, 2, 2, 96), ("fp32", 1, 100, 129, 2, 1, 128),
+    ("fp32", 1, 66, 66, 1, 1, 192), ("fp32", 1, 70, 140, 2, 1, 256),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(map(str, s)))
+@pytest.mark.parametrize("what", ["mask", "cap", "bias", "both"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_cap_and_bias(shape, what, causal):
+    dtype, B, Sq, Skv, Hq, Hkv, D = shape
+    Q, K, V = _inputs(dtype, B, Sq, Skv, Hq, Hkv, D)
+    cap = 2.5 if what in ("cap", "both") else 0.0
+    slopes = _slopes(Hq) if what in ("bias", "both") else None
+    got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=causal, softcap=cap, alibi_slopes=slopes)
+    _compare(got, Q, K, V, causal, cap, slopes)
+    tfa.device_status()
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(map(str, s)))
+def test_prefix(shape):
+    dtype, B, Sq, Skv, Hq, Hkv, D = shape
+    Q, K, V = _inputs(dtype, B, Sq, Skv, Hq, Hkv, D, 1)
+    prefix = torch.tensor([[0, Skv // 3 + 1, Skv + 500][b % 3] for b in range(B)], dtype=torch.int32, device="cuda")
+    slopes = _slopes(Hq)
+    got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, prefix_lens=prefix, alibi_slopes=slopes)
+    _compare(got, Q, K, V, True, slopes=slopes, prefix=prefix)
+
+
+def _documents(B, S, mean, seed, pad=True, shuffle=False):
+    g = torch.Generator().manual_seed(seed)
+    rows = []
+    for b in range(B):
+        row, d = [], 3 * b
+        while len(row) < S:
+            row += [d] * (1 + int(torch.empty(1).exponential_(1.0 / mean, generator=g)))
+            d += 1
+        row = row[:S]
+        if pad:
+            row[S - S // 5:] = [-1] * (S // 5)
+        if shuffle:
+            row = [row[i] for i in torch.randperm(S, generator=g).tolist()]
+        rows.append(row)
+    return torch.tensor(rows, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype,B,S,Hq,Hkv,D", [("fp16", 2, 700, 4, 2, 64), ("bf16", 1, 1100, 8, 2, 128), ("bf16", 3, 130, 2, 2, 32), ("fp16", 1, 600, 2, 1, 256),
+                                                ("fp32", 2, 300, 4, 2, 64), ("fp32", 1, 200, 1, 1, 256), ("bf16", 1, 20, 4, 1, 96), ("fp16", 1, 500, 2, 2, 192)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("kind", ["ascending", "shuffled", "all_padding", "one"])
+def test_documents(dtype, B, S, Hq, Hkv, D, causal, kind):
+    Q, K, V = _inputs(dtype, B, S, S, Hq, Hkv, D, 2)
+    if kind == "all_padding":
+        docs = torch.full((B, S), -1, dtype=torch.int32, device="cuda")
+    elif kind == "one":
+        docs = torch.full((B, S), 7, dtype=torch.int32, device="cuda")
+    else:
+        docs = _documents(B, S, 90, 5, shuffle=kind == "shuffled")
+    got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=causal, softcap=4.0, doc_ids_q=docs, doc_ids_kv=docs)
+    _compare(got, Q, K, V, causal, 4.0, dq=docs, dk=docs)
+    assert (got[docs < 0] == 0).all()
+
+
+def test_documents_of_other_keys_with_prefix_and_start():
+    Q, K, V = _inputs("bf16", 2, 150, 900, 4, 2, 128, 3)
+    dk = _documents(2, 900, 200, 8, pad=False)
+    dq = dk[:, 400:550].contiguous()
+    prefix = torch.tensor([450, 0], dtype=torch.int32, device="cuda")
+    got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, prefix_lens=prefix, doc_ids_q=dq, doc_ids_kv=dk, q_start=400)
+    _compare(got, Q, K, V, True, prefix=prefix, dq=dq, dk=dk, q_start=400)
+
+
+@pytest.mark.parametrize("dtype,B,n,L,Hq,Hkv,D", [("bf16", 3, 1, 1000, 8, 2, 128), ("fp16", 2, 4, 5000, 4, 1, 64), ("bf16", 1, 1, 9001, 32, 8, 96), ("fp16", 5, 3, 300, 5, 1, 32),
+                                                  ("bf16", 1, 2, 3000, 4, 2, 192), ("fp16", 1, 1, 2049, 2, 1, 256), ("fp32", 2, 3, 700, 4, 2, 128),
+                                                  ("bf16", 2, 40, 6000, 8, 2, 128), ("fp16", 3, 5, 6455, 4, 1, 96), ("bf16", 1, 60, 9000, 2, 1, 32), ("fp16", 1, 50, 5000, 4, 1, 192), ("fp16", 1, 17, 12000, 4, 4, 64), ("bf16", 1, 100, 4000, 2, 1, 256)])
+@pytest.mark.parametrize("extra", [0, 77])
+def test_tokens_and_chunks_behind_keys(dtype, B, n, L, Hq, Hkv, D, extra):
+    """Single tokens, draft tokens and chunks at the end of the keys (or with keys behind them that they do not see)."""
+    Q, K, V = _inputs(dtype, B, n, L + n + extra, Hq, Hkv, D, 4)
+    slopes = _slopes(Hq)
+    got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, softcap=20.0, alibi_slopes=slopes, q_start=L)
+    _compare(got, Q, K, V, True, 20.0, slopes, q_start=L)
+    if n > 1:  # without the mask
+        _compare(tfa.flash_attn_scored_forward(Q, K, V, softcap=20.0), Q, K, V, False, 20.0)
+    tfa.device_status()
+
+
+def test_matches_the_plain_call_without_options():
+    for dtype, D in (("bf16", 128), ("fp16", 64)):
+        Q, K, V = _inputs(dtype, 2, 500, 500, 4, 2, D, 6)
+        for causal in (False, True):
+            want = tfa.flash_attn_forward(Q, K, V, causal)
+            assert torch.equal(tfa.flash_attn_scored_forward(Q, K, V, causal), want)
+
+
+def test_scores_far_past_the_cap():
+    """Scores of hundreds against a cap of 1 and 30: all weights are within e^2c of each other, nothing overflows."""
+    for dtype in ("fp16", "bf16", "fp32"):
+        Q, K, V = _inputs(dtype, 1, 200, 300, 2, 1, 64, 7)
+        for cap in (1.0, 30.0):
+            got = tfa.flash_attn_scored_forward(Q * 30, K * 30, V, softcap=cap)
+            assert torch.isfinite(got).all()
+            if cap == 1.0:
+                # a score of hundreds is +-1 after the cap, but the few near zero follow their error: 900 D 2^-24 sum |q k|
+                _compare(got, Q * 30, K * 30, V, False, cap)
+
+
+def test_large_q_start_keeps_distances():
+    Q, K, V = _inputs("bf16", 1, 1, 4000, 4, 1, 64, 8)
+    slopes = _slopes(4) * 0.01
+    got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, alibi_slopes=slopes, q_start=5000)
+    _compare(got, Q, K, V, True, slopes=slopes, q_start=5000)
+
+
+def test_replayed_graph_and_side_stream():
+    Q, K, V = _inputs("bf16", 2, 300, 300, 8, 2, 128, 9)
+    docs = _documents(2, 300, 70, 1)
+    args = dict(is_causal=True, softcap=30.0, doc_ids_q=docs, doc_ids_kv=docs)
+    want = tfa.flash_attn_scored_forward(Q, K, V, **args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = tfa.flash_attn_scored_forward(Q, K, V, **args)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = tfa.flash_attn_scored_forward(Q, K, V, **args)
+    for seed in (10, 11):
+        q2, k2, v2 = _inputs("bf16", 2, 300, 300, 8, 2, 128, seed)
+        Q.copy_(q2), K.copy_(k2), V.copy_(v2)
+        graph.replay()
+        assert torch.equal(captured, tfa.flash_attn_scored_forward(Q, K, V, **args))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_nan_keys_and_values_in_places_nobody_sees(dtype):
+    """Padding of a batch may hold anything; keys that a row masks may be NaN."""
+    Q, K, V = _inputs(dtype, 2, 260, 260, 4, 2, 64, 12)
+    docs = _documents(2, 260, 60, 3)
+    want = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, doc_ids_q=docs, doc_ids_kv=docs)
+    pad = docs < 0
+    Q[pad], K[pad] = math.nan, math.inf
+    got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, doc_ids_q=docs, doc_ids_kv=docs)
+    assert torch.equal(got, want)
+    K[:, 200:] = math.nan  # the causal mask hides them from the rows before
+    got = tfa.flash_attn_scored_forward(Q[:, :200].contiguous(), K, V, is_causal=True, doc_ids_q=docs[:, :200].contiguous(), doc_ids_kv=docs)
+    assert torch.equal(got, want[:, :200])
+
+
+def test_refusals():
+    Q, K, V = _inputs("fp16", 1, 8, 8, 2, 1, 64)
+    ids = torch.zeros(1, 8, dtype=torch.int32, device="cuda")
+    f = tfa.flash_attn_scored_forward
+    for kw, text in ((dict(softcap=-1.0), "softcap"), (dict(softcap=math.inf), "softcap"), (dict(softcap=math.nan), "softcap"), (dict(q_start=-1), "q_start"),
+                     (dict(q_start=1.5), "q_start"), (dict(prefix_lens=ids[:, 0]), "causal"), (dict(doc_ids_q=ids), "together"),
+                     (dict(doc_ids_q=ids.long(), doc_ids_kv=ids), "int32"), (dict(doc_ids_q=ids[:, :4], doc_ids_kv=ids), "contiguous|shape"),
+                     (dict(alibi_slopes=torch.ones(1, device="cuda")), "shape"), (dict(alibi_slopes=torch.ones(2)), "CUDA"),
+                     (dict(alibi_slopes=torch.ones(2, device="cuda", dtype=torch.float64)), "float32")):
+        with pytest.raises(RuntimeError, match=text):
+            f(Q, K, V, **kw)
+    with pytest.raises(RuntimeError, match="forward only"):
+        f(Q.requires_grad_(), K, V)
+    with torch.no_grad():
+        f(Q, K, V)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        f(Q.detach().transpose(1, 2), K, V)
+    empty = f(Q.detach(), K[:, :0], V[:, :0])
+    assert (empty == 0).all()

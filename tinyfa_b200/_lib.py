@@ -30,6 +30,10 @@ EXPORTED_SYMBOLS = (
     "tfa_b200_set_option",
     "tfa_b200_version",
     "tfa_b200_fwd_decode_noalloc",
+    "tfa_b200_fwd_scored",
+    "tfa_b200_kv_cache_plan",
+    "tfa_b200_kv_cache_store",
+    "tfa_b200_fwd_cache",
 )
 
 _lib = None
@@ -63,6 +67,15 @@ def load():
     lib.tfa_b200_set_option.restype = ci
     lib.tfa_b200_fwd_decode_noalloc.argtypes = [vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, ci, vp]
     lib.tfa_b200_fwd_decode_noalloc.restype = ci
+    cf = ctypes.c_float
+    lib.tfa_b200_fwd_scored.argtypes = [vp, vp, vp, vp] + [ci] * 9 + [cf, vp, vp, vp, vp, vp]
+    lib.tfa_b200_fwd_scored.restype = ci
+    lib.tfa_b200_kv_cache_plan.argtypes = [vp] * 10 + [ci] * 4 + [ll, vp]
+    lib.tfa_b200_kv_cache_plan.restype = ci
+    lib.tfa_b200_kv_cache_store.argtypes = [vp] * 7 + [ci, ci, ll, ci, ci, ci, ci, vp]
+    lib.tfa_b200_kv_cache_store.restype = ci
+    lib.tfa_b200_fwd_cache.argtypes = [vp] * 9 + [ci] * 5 + [ll] + [ci] * 7 + [cf, vp, vp]
+    lib.tfa_b200_fwd_cache.restype = ci
     lib.tfa_b200_version.argtypes = []
     lib.tfa_b200_version.restype = ctypes.c_char_p
     _lib = lib

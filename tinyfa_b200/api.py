@@ -167,6 +167,72 @@ def flash_attn_varlen_forward(Q, K, V, cu_seqlens_q, cu_seqlens_kv, max_seqlen_q
         return _run_varlen(lib, device, Q, K, V, cu_seqlens_q, cu_seqlens_kv, max_seqlen_q, max_seqlen_kv, code, is_causal)
 
 
+def _check_no_grad(*tensors):
+    """These operators have no backward pass: better an error than gradients that are silently missing."""
+    if torch.is_grad_enabled():
+        _check(not any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors),
+               "forward only: call under torch.no_grad(), or on tensors that do not require gradients")
+
+
+def _check_aux(x, name, dtype, shape, device):
+    """An optional tensor beside Q: its address, None where there is none."""
+    if x is None:
+        return None
+    _check_input(x, name)
+    _check(x.dtype == dtype, f"{name} must be {str(dtype).replace('torch.', '')}")
+    _check(tuple(x.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+    _check(x.get_device() == device, f"{name} must be on the device of Q")
+    return x.data_ptr()
+
+
+def _check_softcap(softcap):
+    softcap = float(softcap)
+    _check(0.0 <= softcap < float("inf"), "softcap must be 0 (none) or a positive finite number")
+    return softcap
+
+
+def _run_scored(lib, device, Q, K, V, code, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv):
+    batch, seq_q, heads_q, head_dim = Q.shape
+    seq_kv, heads_kv = K.shape[1], K.shape[2]
+    O = torch.empty_like(Q) if (seq_kv > 0 and Q.numel() > 0) else torch.zeros_like(Q)
+    rc = lib.tfa_b200_fwd_scored(Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), code, batch, seq_q, seq_kv, heads_q, heads_kv,
+                                 head_dim, 1 if is_causal else 0, q_start, softcap, slopes, prefix, docs_q, docs_kv, _raw_stream(device))
+    if rc != 0:
+        _lib.check(rc, "flash_attn_scored_forward")
+    return O
+
+
+def flash_attn_scored_forward(Q, K, V, is_causal=False, softcap=0.0, alibi_slopes=None, prefix_lens=None, doc_ids_q=None, doc_ids_kv=None,
+                              q_start=0):
+    """Fixed-length attention forward with scores that are capped, biased by distance, or masked by prefix or document.
+
+    Q [B,Sq,Hq,D]; K,V [B,Skv,Hkv,D]; returns O like Q.  Query row i has position p = q_start + i, key j position j.
+      s = q.k / sqrt(D);  softcap > 0: s = softcap * tanh(s / softcap);  alibi_slopes (float32 [Hq]): s -= slope * |p - j|
+    Row i sees key j if (not is_causal, or j <= p, or j < prefix_lens[b]) and (no documents, or doc_ids_q[b,i] == doc_ids_kv[b,j] >= 0).
+    prefix_lens int32 [B] needs is_causal; doc_ids_q int32 [B,Sq] and doc_ids_kv int32 [B,Skv] are given together, negative ids are padding.
+    A row that sees no key is zero.  Forward only.
+    """
+    if not _usable(Q, K, V):
+        _check_fixed(Q, K, V)
+    q_shape, kv_shape = Q.shape, K.shape
+    _check_fixed(Q, K, V)
+    _check(kv_shape[0] == q_shape[0], "Batch sizes must match")
+    _check_no_grad(Q, K, V, alibi_slopes)
+    _check(isinstance(q_start, int) and q_start >= 0, "q_start must be an integer >= 0")
+    _check(prefix_lens is None or is_causal, "prefix_lens widens the causal mask: it needs is_causal")
+    _check((doc_ids_q is None) == (doc_ids_kv is None), "doc_ids_q and doc_ids_kv must be given together")
+    code, device, softcap = _DTYPE_CODE[Q.dtype], Q.get_device(), _check_softcap(softcap)
+    slopes = _check_aux(alibi_slopes, "alibi_slopes", torch.float32, (q_shape[2],), device)
+    prefix = _check_aux(prefix_lens, "prefix_lens", torch.int32, (q_shape[0],), device)
+    docs_q = _check_aux(doc_ids_q, "doc_ids_q", torch.int32, (q_shape[0], q_shape[1]), device)
+    docs_kv = _check_aux(doc_ids_kv, "doc_ids_kv", torch.int32, (q_shape[0], kv_shape[1]), device)
+    lib = _lib.load()
+    if _current_device() == device:
+        return _run_scored(lib, device, Q, K, V, code, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv)
+    with torch.cuda.device(device):
+        return _run_scored(lib, device, Q, K, V, code, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv)
+
+
 def is_head_dim_compiled(head_dim):
     """Mirror of tfa::isHeadDimCompiled (reference csrc/flash_attn/config.cuh:102-131)."""
     return bool(_lib.load().tfa_b200_head_dim_supported(int(head_dim)))

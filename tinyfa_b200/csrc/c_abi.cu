@@ -11,6 +11,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 #include <thread>
@@ -203,6 +204,29 @@ int* device_work_counter(int device, cudaStream_t stream, int* rc, CUtensorMap**
   return base + 1 + 2 * it->second;
 }
 
+// Arrival counters of the cache attention kernel, by which the parts of a unit that several runs share find out who comes last:
+// zero between launches (the last one puts its counter back), and never shared by launches that can run at the same time - a slot
+// of kJoinCounters for every counter pair above, with the same rule.
+constexpr int kJoinCounters = 1024;
+static int* g_joinBlock[64] = {nullptr};
+int* device_join_counters(int device, cudaStream_t stream, int* rc) {
+  int* pair = device_work_counter(device, stream, rc, nullptr);
+  if (pair == nullptr) return nullptr;
+  std::lock_guard<std::mutex> lock(g_devMutex);
+  if (g_joinBlock[device] == nullptr) {
+    const size_t bytes = sizeof(int) * kJoinCounters * (kStreamPairs + kCapturePairs);
+    int* p = nullptr;
+    if (cudaMalloc(&p, bytes) != cudaSuccess || cudaMemset(p, 0, bytes) != cudaSuccess) {
+      set_error_string("could not allocate the arrival counters: %s", cudaGetErrorString(cudaGetLastError()));
+      *rc = kCudaError;
+      return nullptr;
+    }
+    g_joinBlock[device] = p;
+  }
+  const long long slot = (pair - (g_statusWord[device] + 1)) / 2;
+  return g_joinBlock[device] + slot * kJoinCounters;
+}
+
 // Completes the tensor maps of a packed variable-length launch on the device: the three maps arrive as kernel
 // arguments with a placeholder row count, the real counts are cuQ[batch] and cuKV[batch] (the reference reads its
 // lengths on the device as well, reference csrc/flash_attn/params.cuh:89-94).  One warp; the maps go to `out` in
@@ -332,7 +356,7 @@ static int not_compiled(const FwdProblem& p) {
   return dtype_compiled(p.dtype) ? kBadHeadDim : kBadDtype;
 }
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static int pick_pack_shift(const FwdProblem& p) {
   const int group = p.headsQ / p.headsKV;
@@ -349,6 +373,9 @@ static int pick_pack_shift(const FwdProblem& p) {
   return (p.seqLenQ < 128 || p.causal) ? shift : 0;
 }
 
+int pack_shift_of(const FwdProblem& p) { return pick_pack_shift(p); }
+int split_kv_option() { return g_optSplitKv.load(); }
+
 static int num_sms() {
   static int cached[64] = {0};
   int device = 0;
@@ -359,6 +386,17 @@ static int num_sms() {
     cached[device] = n;
   }
   return cached[device];
+}
+
+int scratch_alloc(void** ptr, size_t bytes, int device, cudaStream_t stream) {
+  cudaMemPool_t pool = scratch_pool(device);
+  const cudaError_t e = (pool != nullptr) ? cudaMallocFromPoolAsync(ptr, bytes, pool, stream) : cudaMallocAsync(ptr, bytes, stream);
+  if (e != cudaSuccess) {
+    set_error_string("cudaMallocAsync(%zu bytes) for partial results: %s", bytes, cudaGetErrorString(e));
+    (void)cudaGetLastError();
+    return kCudaError;
+  }
+  return kOk;
 }
 
 // Short query blocks: stream K/V once for all Q heads of a KV head and split the key range over CTAs.  The partial
@@ -480,14 +518,15 @@ static int run_tc(const FwdProblem& p, int ps, const TcSplit& split) {
 // at 256 (1.4 in the pair form, which key ranges do not have).  What it decides, us per call whole -> in ranges: 2 x 8 rows x
 // 12289 keys, 32 over 8 heads of 128 152 -> 36, 1 x 8 x 32768 386 -> 45, 1 x 512 x 2048 16 heads 38 -> 30, causal 1 x 2048 4 heads
 // 38 -> 29; left whole: 1 x 1024 x 1024 8 heads 25.2 (27.1 in four), causal 1 x 2048 4 heads of 256 34 (39 in two).
-static TcSplit tc_split_plan(const FwdProblem& p, int packShift) {
+static TcSplit tc_split_plan(const FwdProblem& p, int packShift, int qStart = 0) {
   TcSplit s;
   const int opt = g_optSplitTc.load();
   if (opt == 0 || p.cuQ != nullptr || !dtype_compiled(p.dtype) || !head_dim_compiled(p.headDim)) return s;
   const int rowsPerItem = 128 >> packShift;
   const long long items = (long long)((p.seqLenQ + rowsPerItem - 1) / rowsPerItem) * (p.headsQ >> packShift) * p.batch;
   const long long slots = (long long)num_sms() * (p.headDim <= 128 ? 2 : 1);
-  const int seen = p.causal ? (p.seqLenQ < p.seqLenKV ? p.seqLenQ : p.seqLenKV) : p.seqLenKV;
+  const int reach = p.seqLenQ + qStart;  // causal: keys that the last row sees
+  const int seen = p.causal ? (reach < p.seqLenKV ? reach : p.seqLenKV) : p.seqLenKV;
   const int blocks = (seen + 127) / 128;
   long long parts = opt;
   if (opt < 0) {
@@ -497,7 +536,7 @@ static TcSplit tc_split_plan(const FwdProblem& p, int packShift) {
     const double usPart = (double)p.totalQ * p.headsQ * p.headDim * 8.0 / 3.3e6;  // write and read one part, 3.3 TB/s
     // mean key blocks of an item
     const double sq = p.seqLenQ, skv = p.seqLenKV;
-    const double mean = !p.causal ? blocks : 0.5 + (sq <= skv ? sq * 0.5 : skv - skv * skv * 0.5 / sq) / 128.0;
+    const double mean = !p.causal ? blocks : qStart > 0 ? fmin(skv, qStart + sq * 0.5) / 128.0 : 0.5 + (sq <= skv ? sq * 0.5 : skv - skv * skv * 0.5 / sq) / 128.0;
     const double share = items * mean / slots;  // key blocks per CTA slot when spread evenly
     double best = 0.0;
     for (int n = 1; n <= 32 && n <= blocks; n++) {
@@ -521,6 +560,8 @@ static TcSplit tc_split_plan(const FwdProblem& p, int packShift) {
   s.parts = (blocks + s.partBlocks - 1) / s.partBlocks;
   return s;
 }
+
+TcSplit tc_split_of(const FwdProblem& p, int packShift, int qStart) { return tc_split_plan(p, packShift, qStart); }
 
 // The tensor-core path.  Key ranges need scratch for their partial results: like the fp32 workspace they are not used
 // under stream capture (these calls capture as one kernel without an allocation), and without scratch the call runs whole.

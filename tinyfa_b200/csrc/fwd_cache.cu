@@ -1,0 +1,864 @@
+// Attention over the paged 8-bit K/V cache, few query rows per request (decode steps, draft tokens): sm_100a.
+//
+//   S = (q . k) / sqrt(D), k = code * scale[block, head];  capped: S <- c tanh(S / c);  biased: S <- S - slope_h |pos - j|
+//   O = sum_j exp(S_j) v_j / sum_j exp(S_j) over the keys j <= pos of a query at position pos (all keys without the causal mask)
+//
+// Bound by HBM: every code is read once per KV head, the products are a few per cent of the time.  So the kernel is a stream:
+//   * the query rows that share a KV head form tiles of 16 rows; the 64-key blocks of all (request, tile) units in a row are cut
+//     into equal runs, one CTA per run and KV head, whatever the lengths are - which only the device knows;
+//   * each of a CTA's four warps takes every fourth 16-key slice, with a ring of its own that cp.async fills several slices ahead,
+//     across the ends of requests, and a running maximum and sum of its own.  Nothing but the end of a unit synchronises the CTA;
+//   * codes become fp16 exactly (int8 and e4m3 both fit its 11 bits), so mma.sync sees the codes themselves: the scale of a block of
+//     keys multiplies the scores, the scale of a block of values the weights.  bf16 queries become fp16 with a power of two per row
+//     taken out, which loses only what lies 2^-31 below the row's largest element;
+//   * the contraction index of Q.K^T and the column index of P.V are permuted so that a lane's operands are 16 (D = 128) contiguous
+//     bytes of a cache row; P.V needs two byte permutes per four codes to bring two keys together;
+//   * weights are stored relative to the largest block scale of V seen so far and 2^10 up, so that the fp16 weights of a block
+//     whose scale is 2^-23 of the largest still have all their bits;
+//   * a unit that several runs share is put together by the CTA that finishes last, which it learns from a counter.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <mutex>
+
+#include "../../include/tinyfa_b200.h"
+#include "build_config.cuh"
+#include "ptx_sm100.cuh"
+#include "tfa_common.cuh"
+
+namespace tfa_b200 {
+
+int device_num_sms(int device);  // c_abi.cu
+int* device_join_counters(int device, cudaStream_t stream, int* rc);  // c_abi.cu
+
+namespace cache {
+
+constexpr int kThreads = 128;
+constexpr int kBlockKeys = 64;  // unit of the partition: a slice of 16 keys for each warp
+constexpr int kRows = 16;       // query rows of a tile (MMA M)
+constexpr float kUp = 1024.f;   // weights are stored this much larger
+
+struct Params {
+  const void* Q;
+  void* O;
+  const uint8_t* kCodes;
+  const uint8_t* vCodes;
+  const float* kScales;
+  const float* vScales;
+  const int* table;  // [batch][width]
+  const int* lens;   // [batch] tokens of each request, its new ones included
+  const int* cuQ;    // [batch + 1]
+  const float* slopes;  // [headsQ] or null
+  int batch, width, numBlocks, blockShift;
+  int headsQ, headsKV, group;
+  int causal;
+  int runs;
+  int totalQ;
+  float scaleLog2;  // log2(e) / sqrt(D)
+  float cap;        // 0: none
+  float* partO;     // [runs][headsKV][2][16][D] normalised
+  float* partLse;   // [runs][headsKV][2][16]
+  int* join;        // [runs][headsKV], zero
+};
+
+// Bytes of a row of K and V in shared memory: a multiple of 16 that keeps the lanes of a load on different banks (K: eight rows of
+// 64 bytes; V: rows 2 apart) for D = 32, 64, 128, 192 (V at 192 and 256, K at 96: two lanes to a bank).
+template <int D>
+constexpr int k_pitch() {
+  return D % 128 == 0 ? D + 64 : D;
+}
+template <int D>
+constexpr int v_pitch() {
+  return D + 16;
+}
+template <int D>
+constexpr int stages() {
+  return D <= 64 ? 6 : 4;
+}
+constexpr int kHeader = 16;  // scale of K, scale of V, whether the block exists
+template <int D>
+constexpr int stage_bytes() {
+  return 16 * (k_pitch<D>() + v_pitch<D>()) + kHeader;
+}
+template <int D>
+constexpr int ring_bytes() {
+  return 4 * stages<D>() * stage_bytes<D>();
+}
+template <int D>
+constexpr int merge_bytes() {
+  return (kRows * (D + 8) + 8 * kRows) * (int)sizeof(float);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int bytes = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
+  const int bytes = valid ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// Four codes of a word -> two pairs of halves, exactly.  int8: 0x6400 | (code ^ 0x80) is 1024 + 128 + code.
+template <bool kInt8>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (kInt8) {
+    w ^= 0x80808080u;
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+
+// kWords consecutive words of a lane from shared memory, in the widest loads that its alignment (kAlign bytes) allows.
+template <int kWords, int kAlign>
+__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[kWords]) {
+  if constexpr (kAlign >= 16 && kWords % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) {
+      asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(addr + i * 4));
+    }
+  } else if constexpr (kAlign >= 8 && kWords % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[i]), "=r"(w[i + 1]) : "r"(addr + i * 4));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWords; i++) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(addr + i * 4));
+  }
+}
+
+// Where a lane's bytes of a K row lie, and which elements of Q meet them: lane q of a quad has 16 bytes of every 64, and 8 of the
+// last 32 where D is an odd multiple of 32.  Word w of the row's D / 16 words per lane is k-step w of the contraction.
+template <int D>
+__device__ __forceinline__ constexpr int k_byte(int w, int q) {
+  return w / 4 * 64 + (w / 4 < D / 64 ? q * 16 + w % 4 * 4 : q * 8 + w % 4 * 4);
+}
+
+// A run's position in the row of units: blocks [blk, blocks) of query tile `tile` of request b.
+struct Segment {
+  int b, tile;
+  int blk, end;       // key blocks of the segment
+  int blocks;         // key blocks of the unit
+  int q0, nq, len;    // request: first row of Q, rows, tokens
+  int keyEnd;         // keys that some row of the tile sees
+};
+
+template <int D>
+__device__ __forceinline__ int tiles_of(int nq, int group) {
+  return (int)(((long long)nq * group + kRows - 1) / kRows);
+}
+
+// Run that holds block u of `total` blocks, i.e. the c with total * c / runs <= u < total * (c + 1) / runs.
+__device__ __forceinline__ int run_of_block(long long u, long long total, int runs) { return (int)(((u + 1) * runs - 1) / total); }
+
+template <int D, bool kInt8, bool kBf16>
+__global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) {
+  constexpr int kS = stages<D>(), kStage = stage_bytes<D>(), KP = k_pitch<D>(), VP = v_pitch<D>();
+  constexpr int kNT = D / 8;   // 8-wide column tiles of O
+  constexpr int kLdO = D + 8;  // row pitch of the merge buffer
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long sScan[kThreads / 32];
+  __shared__ long long sPlace[3];  // unit that holds the run's first block: request, unit's first block, 1 if found
+  __shared__ int sLast;
+  float* sO = reinterpret_cast<float*>(smem + ring_bytes<D>());  // [16][kLdO]
+  float* sM = sO + kRows * kLdO;                                 // [4][16]
+  float* sL = sM + 4 * kRows;                                    // [4][16]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, tig = lane & 3;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kS * kStage;
+
+  ptx::grid_wait_previous();
+  ptx::grid_allow_next();
+  // neighbouring CTAs are the KV heads of one run: they read neighbouring tiles of the same blocks at the same time
+  const int run = (int)blockIdx.x / p.headsKV;
+  const int hkv = (int)blockIdx.x - run * p.headsKV;
+  const int capacity = p.width << p.blockShift;
+
+  auto request = [&](int b, int& q0, int& nq, int& len) {
+    q0 = min(max(p.cuQ[b], 0), p.totalQ);
+    nq = min(max(p.cuQ[b + 1] - q0, 0), p.totalQ - q0);
+    len = min(max(p.lens[b], 0), capacity);
+  };
+  auto unit_blocks = [&](int len) { return (len + kBlockKeys - 1) / kBlockKeys; };
+  auto blocks_of_request = [&](int b) -> long long {
+    int q0, nq, len;
+    request(b, q0, nq, len);
+    return (long long)tiles_of<D>(nq, p.group) * unit_blocks(len);
+  };
+  // ---- the blocks of all requests, and where this run begins among them
+  long long mine = 0, total = 0;
+  for (int b = threadIdx.x; b < p.batch; b += kThreads) mine += blocks_of_request(b);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+  if (lane == 0) sScan[warp] = mine;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; w++) total += sScan[w];
+  __syncthreads();
+
+  // ---- rows that no unit has: those of no request, and those of requests without a token; a share for every CTA
+  {
+    uint16_t* O = static_cast<uint16_t*>(p.O);
+    auto zero_rows = [&](int r0, int r1) {  // this head's part of them
+      constexpr int kVec = D / 8;
+      const int per = p.group * kVec;
+      for (long long i = threadIdx.x; i < (long long)(r1 - r0) * per; i += kThreads) {
+        const long long row = r0 + i / per;
+        *reinterpret_cast<uint4*>(O + (row * p.headsQ + hkv * p.group) * D + (i % per) * 8) = make_uint4(0, 0, 0, 0);
+      }
+    };
+    if (run == 0) {
+      zero_rows(0, min(max(p.cuQ[0], 0), p.totalQ));
+      zero_rows(min(max(p.cuQ[p.batch], 0), p.totalQ), p.totalQ);
+    }
+    for (int b = run; b < p.batch; b += p.runs) {
+      int q0, nq, len;
+      request(b, q0, nq, len);
+      if (len == 0) zero_rows(q0, q0 + nq);
+    }
+  }
+  // The host sized the grid for the largest lengths: with fewer blocks, fewer runs of at least two blocks.  (Every run has to have a
+  // block: the parts of a unit are counted by the runs between its first block's and its last one's.)
+  const int runs = (int)min((long long)p.runs, (total + 1) / 2);
+  if (run >= runs) return;
+  const long long u0 = total * run / runs, u1 = total * (run + 1) / runs;
+  long long carry = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    const long long n = b < p.batch ? blocks_of_request(b) : 0;
+    long long v = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += o;
+    }
+    if (lane == 31) sScan[warp] = v;
+    __syncthreads();
+    long long sum = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; w++) {
+      if (w < warp) v += sScan[w];
+      sum += sScan[w];
+    }
+    v += carry - n;  // blocks ahead of request b
+    if (u0 >= v && u0 < v + n) {
+      sPlace[0] = b;
+      sPlace[1] = v;
+    }
+    carry += sum;
+    __syncthreads();
+    if (carry > u0) break;
+  }
+
+  auto finish = [&](Segment& s) {  // the fields that follow from the request and the tile
+    const int lastRow = min((s.tile + 1) * kRows, s.nq * p.group) - 1;
+    s.keyEnd = p.causal ? min(s.len, s.len - s.nq + lastRow / p.group + 1) : s.len;
+  };
+  long long left;  // blocks of the run behind the segment
+  auto first_segment = [&](Segment& s, long long& rest) {
+    s.b = (int)sPlace[0];
+    request(s.b, s.q0, s.nq, s.len);
+    s.blocks = unit_blocks(s.len);
+    const long long at = u0 - sPlace[1];
+    s.tile = (int)(at / s.blocks);
+    s.blk = (int)(at - (long long)s.tile * s.blocks);
+    s.end = (int)min((long long)s.blocks, s.blk + (u1 - u0));
+    rest = (u1 - u0) - (s.end - s.blk);
+    finish(s);
+  };
+  auto next_segment = [&](Segment& s, long long& rest) {  // rest > 0
+    s.tile++;
+    if (s.tile >= tiles_of<D>(s.nq, p.group)) {
+      s.tile = 0;
+      do {  // ends: `rest` blocks are still to come
+        s.b++;
+        request(s.b, s.q0, s.nq, s.len);
+      } while (s.nq == 0 || s.len == 0);
+      s.blocks = unit_blocks(s.len);
+    }
+    s.blk = 0;
+    s.end = (int)min((long long)s.blocks, rest);
+    rest -= s.end;
+    finish(s);
+  };
+
+  // ---- the loads: a cursor of its own, kS - 1 slices ahead
+  Segment ls;
+  long long lsRest;
+  first_segment(ls, lsRest);
+  bool loading = true;
+  int ldKey = ls.blk * kBlockKeys + warp * 16, ldStage = 0;
+  const long long headBytes = (long long)D << p.blockShift;
+  auto seg_key_end = [&](const Segment& s) { return min(s.end * kBlockKeys, s.keyEnd); };
+  auto settle = [&]() {  // on to the next slice that exists
+    while (loading && ldKey >= seg_key_end(ls)) {
+      if (lsRest == 0) {
+        loading = false;
+      } else {
+        next_segment(ls, lsRest);
+        ldKey = warp * 16;
+      }
+    }
+  };
+  settle();
+  int ldPage = loading ? p.table[(long long)ls.b * p.width + (ldKey >> p.blockShift)] : 0;
+  auto issue = [&]() {
+    if (loading) {
+      const uint32_t st = ring + ldStage * kStage;
+      const bool ok = ldPage >= 0 && ldPage < p.numBlocks;
+      const long long tile = ok ? (long long)ldPage * p.headsKV + hkv : 0;
+      const int rows = ok ? min(16, ls.len - ldKey) : 0;  // keys of the slice
+      const uint8_t* k = p.kCodes + tile * headBytes + (ldKey & ((1 << p.blockShift) - 1)) * D;
+      const uint8_t* v = p.vCodes + tile * headBytes + (ldKey & ((1 << p.blockShift) - 1)) * D;
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) {
+        const int c = lane + i * 32, r = c / (D / 16), col = c % (D / 16) * 16;
+        cp_async16(st + r * KP + col, k + (r < rows ? c * 16 : 0), r < rows);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) {
+        const int c = lane + i * 32, r = c / (D / 16), col = c % (D / 16) * 16;
+        cp_async16(st + 16 * KP + r * VP + col, v + (r < rows ? c * 16 : 0), r < rows);
+      }
+      const uint32_t head = st + 16 * (KP + VP);
+      if (lane == 0) {
+        cp_async4(head, p.kScales + tile, ok);
+        cp_async4(head + 4, p.vScales + tile, ok);
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(head + 8), "r"(ok ? 1 : 0) : "memory");
+      }
+      ldStage = ldStage + 1 == kS ? 0 : ldStage + 1;
+      ldKey += kBlockKeys;
+      settle();
+      if (loading) ldPage = p.table[(long long)ls.b * p.width + (ldKey >> p.blockShift)];
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kS - 1; i++) issue();
+
+  // ---- the units of the run
+  const int rowA = g, rowB = g + 8;
+  Segment s;
+  first_segment(s, left);
+  bool firstSegment = true;
+  int stage = 0;
+  for (;;) {
+    const int nRows = min(s.nq * p.group - s.tile * kRows, kRows);
+    const int flatA = s.tile * kRows + rowA, flatB = s.tile * kRows + rowB;
+    const bool validA = rowA < nRows, validB = rowB < nRows;
+    const int tokA = validA ? flatA / p.group : 0, tokB = validB ? flatB / p.group : 0;
+    const int headA = hkv * p.group + (validA ? flatA % p.group : 0), headB = hkv * p.group + (validB ? flatB % p.group : 0);
+    const int posA = s.len - s.nq + tokA, posB = s.len - s.nq + tokB;
+    const float slopeA = p.slopes != nullptr ? p.slopes[headA] * 1.44269504f : 0.f;
+    const float slopeB = p.slopes != nullptr ? p.slopes[headB] * 1.44269504f : 0.f;
+    // Q fragments, permuted like the lanes' bytes of K; factors of the scores
+    uint32_t qf[D / 16][4];
+    float facA = p.scaleLog2, facB = p.scaleLog2;
+    {
+      const uint16_t* gQ = static_cast<const uint16_t*>(p.Q);
+      const uint16_t* qa = gQ + ((long long)(s.q0 + tokA) * p.headsQ + headA) * D;
+      const uint16_t* qb = gQ + ((long long)(s.q0 + tokB) * p.headsQ + headB) * D;
+#pragma unroll
+      for (int w = 0; w < D / 16; w++) {
+        const uint2 a = *reinterpret_cast<const uint2*>(qa + k_byte<D>(w, tig)), b = *reinterpret_cast<const uint2*>(qb + k_byte<D>(w, tig));
+        qf[w][0] = validA ? a.x : 0u;
+        qf[w][1] = validB ? b.x : 0u;
+        qf[w][2] = validA ? a.y : 0u;
+        qf[w][3] = validB ? b.y : 0u;
+      }
+      if constexpr (kBf16) {
+        // largest exponent of the row -> the power of two that brings its largest element into [2^13, 2^14)
+        uint32_t ma = 0, mb = 0;
+#pragma unroll
+        for (int w = 0; w < D / 16; w++) {
+          ma = max(max(ma, qf[w][0] & 0x7F80u), max(qf[w][0] >> 16 & 0x7F80u, max(qf[w][2] & 0x7F80u, qf[w][2] >> 16 & 0x7F80u)));
+          mb = max(max(mb, qf[w][1] & 0x7F80u), max(qf[w][1] >> 16 & 0x7F80u, max(qf[w][3] & 0x7F80u, qf[w][3] >> 16 & 0x7F80u)));
+        }
+        ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
+        ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 2));
+        mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+        mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
+        // exponent field e of the row's maximum: the factor is 2^(13 - (e - 127)); kept inside what a float's exponent holds
+        const int ea = min(max((int)(ma >> 7), 14), 253), eb = min(max((int)(mb >> 7), 14), 253);
+        const float upA = __int_as_float((267 - ea) << 23), upB = __int_as_float((267 - eb) << 23);  // 2^(140 - e), e - 127 = exponent
+        const float dnA = __int_as_float((ea - 13) << 23), dnB = __int_as_float((eb - 13) << 23);
+        facA *= dnA;
+        facB *= dnB;
+        auto conv = [](uint32_t x, float f) {
+          return half2_of(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xFFFF0000u) * f);
+        };
+#pragma unroll
+        for (int w = 0; w < D / 16; w++) {
+          qf[w][0] = conv(qf[w][0], upA);
+          qf[w][1] = conv(qf[w][1], upB);
+          qf[w][2] = conv(qf[w][2], upA);
+          qf[w][3] = conv(qf[w][3], upB);
+        }
+      }
+    }
+    const float capLog2 = p.cap * 1.44269504f;
+    if (p.cap > 0.f) {  // scores as arguments 2 log2(e) S / c of the exponential that gives the tanh
+      const float f = 2.f / p.cap;
+      facA *= f;
+      facB *= f;
+    }
+
+    float o[kNT][4];
+#pragma unroll
+    for (int i = 0; i < kNT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
+    float vRef = 0.f, vRefInv = 0.f;  // largest scale of V so far; O holds sums of 2^10 p v / vRef
+
+    const int keyStop = seg_key_end(s);
+    for (int key0 = s.blk * kBlockKeys + warp * 16; key0 < keyStop; key0 += kBlockKeys) {
+      cp_async_wait<kS - 2>();
+      __syncwarp();
+      const uint32_t st = ring + stage * kStage;
+      float ks, vs;
+      uint32_t there;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks) : "r"(st + 16 * (KP + VP)));
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs) : "r"(st + 16 * (KP + VP) + 4));
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(there) : "r"(st + 16 * (KP + VP) + 8));
+      // ---- S = Q K^T for 16 rows x 16 keys
+      float sc[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; n++) {
+        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+        const uint32_t row = st + (n * 8 + g) * KP;
+#pragma unroll
+        for (int c = 0; c < D / 64; c++) {
+          uint32_t w[4];
+          lds_words<4, 16>(row + c * 64 + tig * 16, w);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            uint32_t b0, b1;
+            widen<kInt8>(w[i], b0, b1);
+            mma_f16(sc[n], qf[c * 4 + i], b0, b1);
+          }
+        }
+        if constexpr (D % 64 != 0) {
+          uint32_t w[2];
+          lds_words<2, 8>(row + D / 64 * 64 + tig * 8, w);
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            uint32_t b0, b1;
+            widen<kInt8>(w[i], b0, b1);
+            mma_f16(sc[n], qf[D / 64 * 4 + i], b0, b1);
+          }
+        }
+      }
+      // ---- scores in units of log2, capped, biased, masked
+      const float fA = facA * ks, fB = facB * ks;
+#pragma unroll
+      for (int n = 0; n < 2; n++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) sc[n][e] *= e < 2 ? fA : fB;
+      }
+      if (p.cap > 0.f) {  // c tanh(x) = c - 2 c / (e^2x + 1)
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) sc[n][e] = fmaf(-2.f * capLog2, rcp(ex2(sc[n][e]) + 1.f), capLog2);
+        }
+      }
+      if (p.slopes != nullptr) {
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int key = key0 + n * 8 + 2 * tig + (e & 1);
+            sc[n][e] = fmaf(e < 2 ? -slopeA : -slopeB, fabsf((float)((e < 2 ? posA : posB) - key)), sc[n][e]);
+          }
+        }
+      }
+      if (!there || key0 + 16 > s.len || (p.causal && key0 + 15 > s.len - s.nq + s.tile * kRows / p.group)) {
+        const int limA = !there ? 0 : p.causal ? min(s.len, posA + 1) : s.len, limB = !there ? 0 : p.causal ? min(s.len, posB + 1) : s.len;
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (key0 + n * 8 + 2 * tig + (e & 1) >= (e < 2 ? limA : limB)) sc[n][e] = -INFINITY;
+          }
+        }
+      }
+      // ---- running maximum and sum for rows g (A) and g + 8 (B)
+      float mxA = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
+      float mxB = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+      mxA = fmaxf(mxA, __shfl_xor_sync(0xffffffffu, mxA, 1));
+      mxA = fmaxf(mxA, __shfl_xor_sync(0xffffffffu, mxA, 2));
+      mxB = fmaxf(mxB, __shfl_xor_sync(0xffffffffu, mxB, 1));
+      mxB = fmaxf(mxB, __shfl_xor_sync(0xffffffffu, mxB, 2));
+      const float mnA = fmaxf(mA, mxA), mnB = fmaxf(mB, mxB);
+      if (__any_sync(0xffffffffu, mnA > mA || mnB > mB || vs > vRef)) {
+        const float vNew = fmaxf(vRef, vs);
+        const float fv = vNew > vRef ? vRef / vNew : 1.f;
+        const float scA = mA == -INFINITY ? 0.f : ex2(mA - mnA), scB = mB == -INFINITY ? 0.f : ex2(mB - mnB);
+        lA *= scA;
+        lB *= scB;
+        const float oA = scA * fv, oB = scB * fv;
+#pragma unroll
+        for (int i = 0; i < kNT; i++) {
+          o[i][0] *= oA;
+          o[i][1] *= oA;
+          o[i][2] *= oB;
+          o[i][3] *= oB;
+        }
+        mA = mnA;
+        mB = mnB;
+        vRef = vNew;
+        vRefInv = vNew > 0.f ? kUp / vNew : 0.f;
+      }
+      const float muA = mA == -INFINITY ? 0.f : mA, muB = mB == -INFINITY ? 0.f : mB;
+      const float wv = vs * vRefInv;
+      float pA[4], pB[4];
+#pragma unroll
+      for (int n = 0; n < 2; n++) {
+        pA[n * 2 + 0] = ex2(sc[n][0] - muA);
+        pA[n * 2 + 1] = ex2(sc[n][1] - muA);
+        pB[n * 2 + 0] = ex2(sc[n][2] - muB);
+        pB[n * 2 + 1] = ex2(sc[n][3] - muB);
+      }
+      lA += (pA[0] + pA[1]) + (pA[2] + pA[3]);  // per-thread partial, reduced over the quad at the end
+      lB += (pB[0] + pB[1]) + (pB[2] + pB[3]);
+      uint32_t pf[4];  // weights to 11 bits: half a step is 2^-12 of a weight
+      pf[0] = half2_of(pA[0] * wv, pA[1] * wv);
+      pf[1] = half2_of(pB[0] * wv, pB[1] * wv);
+      pf[2] = half2_of(pA[2] * wv, pA[3] * wv);
+      pf[3] = half2_of(pB[2] * wv, pB[3] * wv);
+      // ---- O += P V: column n of tile j is head-dim element n * D / 8 + j, so that a lane's D / 8 codes of a key are contiguous
+      constexpr int kAlign = (D / 8) % 16 == 0 ? 16 : (D / 8) % 8 == 0 ? 8 : 4;
+      constexpr int kPiece = kAlign / 4;
+      const uint32_t vr = st + 16 * KP + g * (D / 8);
+#pragma unroll
+      for (int c = 0; c < D / 32; c += kPiece) {
+        uint32_t w[4][kPiece];
+#pragma unroll
+        for (int i = 0; i < 4; i++) lds_words<kPiece, kAlign>(vr + (2 * tig + (i & 1) + (i >> 1) * 8) * VP + c * 4, w[i]);
+#pragma unroll
+        for (int i = 0; i < kPiece; i++) {
+          uint32_t b0[4], b1[4];
+          widen<kInt8>(__byte_perm(w[0][i], w[1][i], 0x5140), b0[0], b0[1]);
+          widen<kInt8>(__byte_perm(w[0][i], w[1][i], 0x7362), b0[2], b0[3]);
+          widen<kInt8>(__byte_perm(w[2][i], w[3][i], 0x5140), b1[0], b1[1]);
+          widen<kInt8>(__byte_perm(w[2][i], w[3][i], 0x7362), b1[2], b1[3]);
+#pragma unroll
+          for (int j = 0; j < 4; j++) mma_f16(o[(c + i) * 4 + j], pf, b0[j], b1[j]);
+        }
+      }
+      __syncwarp();  // every lane has read the stage before the next issue overwrites it
+      stage = stage + 1 == kS ? 0 : stage + 1;
+      issue();
+    }
+
+    // ---- the four warps' shares of the unit, one after the other
+    lA += __shfl_xor_sync(0xffffffffu, lA, 1);
+    lA += __shfl_xor_sync(0xffffffffu, lA, 2);
+    lB += __shfl_xor_sync(0xffffffffu, lB, 1);
+    lB += __shfl_xor_sync(0xffffffffu, lB, 2);
+    if (tig == 0) {
+      sM[warp * kRows + rowA] = mA;
+      sM[warp * kRows + rowB] = mB;
+      sL[warp * kRows + rowA] = lA;
+      sL[warp * kRows + rowB] = lB;
+    }
+    __syncthreads();
+    {
+      float MA = -INFINITY, MB = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        MA = fmaxf(MA, sM[w * kRows + rowA]);
+        MB = fmaxf(MB, sM[w * kRows + rowB]);
+      }
+      const float down = vRef * (1.f / kUp);
+      const float fA = (mA == -INFINITY ? 0.f : ex2(mA - MA)) * down, fB = (mB == -INFINITY ? 0.f : ex2(mB - MB)) * down;
+#pragma unroll 1
+      for (int w = 0; w < 4; w++) {
+        if (w == warp) {
+#pragma unroll
+          for (int j = 0; j < kNT; j++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              float* at = sO + (e < 2 ? rowA : rowB) * kLdO + (2 * tig + (e & 1)) * (D / 8) + j;
+              *at = fmaf(o[j][e], e < 2 ? fA : fB, w == 0 ? 0.f : *at);
+            }
+          }
+        }
+        __syncthreads();
+      }
+    }
+    const bool whole = s.blk == 0 && s.end == s.blocks;
+    const long long slot = ((long long)run * p.headsKV + hkv) * 2 + (firstSegment ? 0 : 1);
+    auto store = [&](int r, int c4, float4 acc) {
+      const int flat = s.tile * kRows + r;
+      uint16_t* dst = static_cast<uint16_t*>(p.O) + ((long long)(s.q0 + flat / p.group) * p.headsQ + hkv * p.group + flat % p.group) * D + c4 * 4;
+      uint2 out;
+      if constexpr (kBf16) {
+        __nv_bfloat162 x = __floats2bfloat162_rn(acc.x, acc.y), y = __floats2bfloat162_rn(acc.z, acc.w);
+        out.x = *reinterpret_cast<uint32_t*>(&x);
+        out.y = *reinterpret_cast<uint32_t*>(&y);
+      } else {
+        out.x = half2_of(acc.x, acc.y);
+        out.y = half2_of(acc.z, acc.w);
+      }
+      *reinterpret_cast<uint2*>(dst) = out;
+    };
+    for (int idx = threadIdx.x; idx < nRows * (D / 4); idx += kThreads) {
+      const int r = idx / (D / 4), c4 = idx % (D / 4);
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) m = fmaxf(m, sM[w * kRows + r]);
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        const float mw = sM[w * kRows + r];
+        l += sL[w * kRows + r] * (mw == -INFINITY ? 0.f : ex2(mw - m));
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
+      float4 acc = *reinterpret_cast<const float4*>(sO + r * kLdO + c4 * 4);
+      acc.x *= inv;
+      acc.y *= inv;
+      acc.z *= inv;
+      acc.w *= inv;
+      if (whole) {
+        store(r, c4, acc);
+      } else {
+        __stcg(reinterpret_cast<float4*>(p.partO + (slot * kRows + r) * D + c4 * 4), acc);
+        if (c4 == 0) __stcg(p.partLse + slot * kRows + r, l == 0.f ? -INFINITY : m + log2f(l));
+      }
+    }
+    if (!whole) {
+      // ---- the unit is shared by runs c0 .. c1: whoever comes last puts the parts together
+      const long long a = (u1 - left) - s.end;  // the unit's first block (u1 - left: the block behind the segment)
+      const int c0 = run_of_block(a, total, runs), c1 = run_of_block(a + s.blocks - 1, total, runs);
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int* counter = p.join + (long long)c0 * p.headsKV + hkv;
+        const bool last = atomicAdd(counter, 1) == c1 - c0;
+        if (last) *counter = 0;  // for the next call
+        sLast = last;
+        __threadfence();
+      }
+      __syncthreads();
+      if (sLast) {
+        // the unit is the first segment of every run but possibly c0, which it begins in unless it begins the run
+        const int at0 = total * c0 / runs == a ? 0 : 1;
+        auto part = [&](int c) { return ((long long)c * p.headsKV + hkv) * 2 + (c == c0 ? at0 : 0); };
+        for (int idx = threadIdx.x; idx < nRows * (D / 4); idx += kThreads) {
+          const int r = idx / (D / 4), c4 = idx % (D / 4);
+          float M = -INFINITY;
+          bool nan = false;
+#pragma unroll 8
+          for (int c = c0; c <= c1; c++) {
+            const float lse = __ldcg(p.partLse + part(c) * kRows + r);
+            nan = nan || lse != lse;
+            M = fmaxf(M, lse);
+          }
+          if (M == -INFINITY) M = 0.f;
+          if (nan) M = NAN;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float sum = 0.f;
+#pragma unroll 4
+          for (int c = c0; c <= c1; c++) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partO + (part(c) * kRows + r) * D + c4 * 4));
+            const float w = ex2(__ldcg(p.partLse + part(c) * kRows + r) - M);
+            acc.x = fmaf(w, v.x, acc.x);
+            acc.y = fmaf(w, v.y, acc.y);
+            acc.z = fmaf(w, v.z, acc.z);
+            acc.w = fmaf(w, v.w, acc.w);
+            sum += w;
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          store(r, c4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        }
+      }
+    }
+    if (left == 0) break;
+    next_segment(s, left);
+    firstSegment = false;
+    __syncthreads();  // the merge buffer is written again
+  }
+  cp_async_wait<0>();
+}
+
+// CTAs of an SM: what shared memory and registers (255 a thread at most) hold.
+constexpr int ctas_per_sm(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
+
+template <int D, bool kInt8, bool kBf16>
+int launch(Params& p, int maxRuns, int device, cudaStream_t stream) {
+  constexpr int kSmem = ring_bytes<D>() + merge_bytes<D>();
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  auto kernel = cache_decode_kernel<D, kInt8, kBf16>;
+  static std::once_flag once[64];
+  static cudaError_t attrErr[64];
+  std::call_once(once[device], [&] {
+    attrErr[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (attrErr[device] == cudaSuccess) {
+      attrErr[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    }
+  });
+  if (attrErr[device] != cudaSuccess) {
+    set_error_string("cudaFuncSetAttribute(%d bytes): %s", kSmem, cudaGetErrorString(attrErr[device]));
+    return kCudaError;
+  }
+  const cudaError_t e = launch_kernel(kernel, dim3((unsigned)(maxRuns * p.headsKV)), kThreads, kSmem, stream, may_overlap(stream), p);
+  if (e != cudaSuccess) {
+    set_error_string("cache attention kernel launch failed: %s", cudaGetErrorString(e));
+    return kCudaError;
+  }
+  return kOk;
+}
+
+template <int D>
+int launch_typed(Params& p, bool int8, bool bf16, int runs, int device, cudaStream_t stream) {
+  (void)p; (void)int8; (void)runs; (void)device; (void)stream;
+  if (bf16) {
+    if constexpr (TFA_HAVE_BF16) return int8 ? launch<D, true, true>(p, runs, device, stream) : launch<D, false, true>(p, runs, device, stream);
+  } else {
+    if constexpr (TFA_HAVE_FP16) return int8 ? launch<D, true, false>(p, runs, device, stream) : launch<D, false, false>(p, runs, device, stream);
+  }
+  return kBadDtype;
+}
+
+int dispatch(Params& p, int headDim, bool int8, bool bf16, int runs, int device, cudaStream_t stream) {
+  switch (headDim) {
+#if TFA_HAVE_HD32
+    case 32: return launch_typed<32>(p, int8, bf16, runs, device, stream);
+#endif
+#if TFA_HAVE_HD64
+    case 64: return launch_typed<64>(p, int8, bf16, runs, device, stream);
+#endif
+#if TFA_HAVE_HD96
+    case 96: return launch_typed<96>(p, int8, bf16, runs, device, stream);
+#endif
+#if TFA_HAVE_HD128
+    case 128: return launch_typed<128>(p, int8, bf16, runs, device, stream);
+#endif
+#if TFA_HAVE_HD192
+    case 192: return launch_typed<192>(p, int8, bf16, runs, device, stream);
+#endif
+#if TFA_HAVE_HD256
+    case 256: return launch_typed<256>(p, int8, bf16, runs, device, stream);
+#endif
+    default: return kBadHeadDim;
+  }
+}
+
+}  // namespace cache
+}  // namespace tfa_b200
+
+using namespace tfa_b200;
+
+extern "C" int tfa_b200_fwd_cache(const void* Q, void* O, const void* kCache, const void* vCache, const float* kScales, const float* vScales,
+                                  const int* blockTable, const int* seqLens, const int* cuSeqLensQ, int dtype, int cacheType, int batchSize,
+                                  int maxSeqLenQ, int maxSeqLenKV, long long totalQ, int numBlocks, int maxBlocks, int blockTokens, int numHeadsQ,
+                                  int numHeadsKV, int headDim, int isCausal, float softcap, const float* alibiSlopes, void* stream) {
+  using namespace cache;
+  int rc = validate_common(Q, kCache, vCache, O, dtype, batchSize, maxSeqLenQ, maxSeqLenKV, numHeadsQ, numHeadsKV, headDim);
+  if (rc != kOk) return rc;
+  if (dtype == kFp32) {
+    set_error_string("attention over an 8-bit cache takes fp16 and bf16 queries");
+    return kBadDtype;
+  }
+  if (cacheType != TFA_B200_CACHE_INT8 && cacheType != TFA_B200_CACHE_E4M3) {
+    set_error_string("unsupported cache type %d (1 = int8, 2 = e4m3)", cacheType);
+    return kBadDtype;
+  }
+  int shift = 4;
+  while (shift < 8 && (1 << shift) != blockTokens) shift++;
+  if (shift == 8) {
+    set_error_string("blocks hold 16, 32, 64 or 128 tokens (got %d)", blockTokens);
+    return kBadArgument;
+  }
+  if (totalQ < 0 || numBlocks < 0 || maxBlocks < 0 || !(softcap >= 0.f) || isinf(softcap)) {
+    set_error_string("negative size or softcap (totalQ=%lld numBlocks=%d maxBlocks=%d softcap=%g)", totalQ, numBlocks, maxBlocks, softcap);
+    return kBadArgument;
+  }
+  if (totalQ == 0) return kOk;
+  if (totalQ > 0x7FFFFFFFll || totalQ * numHeadsQ > 0x7FFFFFFFll || ((long long)maxBlocks << shift) > 0x7FFFFFFFll - kBlockKeys) {
+    set_error_string("totalQ * numHeadsQ and maxBlocks * blockTokens must stay below 2^31");
+    return kTooLarge;
+  }
+  if (cuSeqLensQ == nullptr || Q == nullptr || O == nullptr || (batchSize > 0 && (seqLens == nullptr || (maxBlocks > 0 && blockTable == nullptr))) ||
+      (numBlocks > 0 && (kCache == nullptr || vCache == nullptr || kScales == nullptr || vScales == nullptr))) {
+    set_error_string("null pointer");
+    return kBadArgument;
+  }
+  if ((rc = check_device()) != kOk) return rc;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kCudaError;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  Params p;
+  p.Q = Q;
+  p.O = O;
+  p.kCodes = static_cast<const uint8_t*>(kCache);
+  p.vCodes = static_cast<const uint8_t*>(vCache);
+  p.kScales = kScales;
+  p.vScales = vScales;
+  p.table = blockTable;
+  p.lens = seqLens;
+  p.cuQ = cuSeqLensQ;
+  p.slopes = alibiSlopes;
+  p.batch = batchSize;
+  p.width = maxBlocks;
+  p.numBlocks = numBlocks;
+  p.blockShift = shift;
+  p.headsQ = numHeadsQ;
+  p.headsKV = numHeadsKV;
+  p.group = numHeadsQ / numHeadsKV;
+  p.causal = isCausal ? 1 : 0;
+  p.totalQ = (int)totalQ;
+  p.scaleLog2 = (float)(1.4426950408889634 / sqrt((double)headDim));
+  p.cap = softcap;
+  // as many runs as the GPU holds CTAs, and no more than there can be pairs of key blocks
+  const long long slots = (long long)device_num_sms(device) * ctas_per_sm(headDim);
+  const long long tiles = ((long long)(maxSeqLenQ > 0 ? maxSeqLenQ : 1) * p.group + kRows - 1) / kRows;
+  const long long most = (tiles * ((maxSeqLenKV + kBlockKeys - 1) / kBlockKeys) * batchSize + 1) / 2;
+  long long runs = slots / numHeadsKV;
+  if (runs > most) runs = most;
+  if (runs < 1) runs = 1;
+  p.runs = (int)runs;
+  p.partO = p.partLse = nullptr;
+  p.join = nullptr;
+  void* scratch = nullptr;
+  if (runs > 1) {
+    p.join = device_join_counters(device, s, &rc);
+    if (p.join == nullptr) return rc;
+    const size_t rows = (size_t)runs * numHeadsKV * 2 * kRows;
+    rc = scratch_alloc(&scratch, rows * (headDim + 1) * sizeof(float), device, s);
+    if (rc != kOk) return rc;
+    p.partO = static_cast<float*>(scratch);
+    p.partLse = p.partO + rows * headDim;
+  }
+  rc = cache::dispatch(p, headDim, cacheType == TFA_B200_CACHE_INT8, dtype == kBf16, p.runs, device, s);
+  if (scratch != nullptr) cudaFreeAsync(scratch, s);
+  return rc;
+}

@@ -30,6 +30,7 @@
 #include "../../include/tinyfa_b200.h"
 #include "build_config.cuh"
 #include "ptx_sm100.cuh"
+#include "score.cuh"
 #include "tfa_common.cuh"
 
 namespace tfa_b200 {
@@ -68,6 +69,18 @@ struct Params {
   long long totalQ;  // rows of Q (for the partial buffers' stride)
   float scaleLog2;
 };
+// ... of a call whose scores are capped, biased or masked by prefix or document (score.cuh); fixed length
+struct ScoreParams : Params, ScoreFields {
+  int keyEnd;  // keys that some row may see
+};
+template <bool kScore>
+struct ParamsOf {
+  using type = Params;
+};
+template <>
+struct ParamsOf<true> {
+  using type = ScoreParams;
+};
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   const int bytes = valid ? 16 : 0;
@@ -103,6 +116,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float fmax_nan(float a, float b) {  // NaN is kept
@@ -168,8 +186,9 @@ __host__ __device__ __forceinline__ int run_of_block(long long u, long long tota
 // anew for every block: the code that carries a run on into the next entry cost calls of whole pairs up to 3 % (16 x 16384 keys, 32 heads over 32
 // of 128 667 -> 641 us).  The number of CTAs per SM is stated because without it the compiler keeps to 168 registers at head dim 128, where two
 // CTAs have 255 each: runs 665 -> 617 us there.  Head dim 32 is better off with 8 CTAs than with 7 of 65 registers.
-template <int D, bool kBf16, bool kEven>
-__global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_splitkv_kernel(const Params p) {
+// kScore: scores are capped, biased and masked (score.cuh) on the way, and multiples of log2(e) from there on.
+template <int D, bool kBf16, bool kEven, bool kScore = false>
+__global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_splitkv_kernel(const typename ParamsOf<kScore>::type p) {
   constexpr int kTileBytes = kBlockKeys * D * 2;
   constexpr int kNT = D / 8;  // 8-wide output column tiles
   constexpr int kLdO = merge_ld<D>();
@@ -205,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
     qRow0 = (long long)b * sq;
     kvRow0 = (long long)b * skv;
     keyEnd = p.causal ? min(skv, sq) : skv;  // top-left causal: key j needs j <= i <= sq-1
+    if constexpr (kScore) keyEnd = p.keyEnd;
   } else {
     part = blockIdx.x;
     hkv = blockIdx.y;
@@ -223,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
     if (sq <= 0) return;
     if (skv <= 0) return;  // nothing to write
     keyEnd = p.causal ? min(skv, sq) : skv;
+    if constexpr (kScore) keyEnd = p.keyEnd;
     // keysPerSplit comes from the caller's maximum key length, which only sizes the launch: the last split runs to
     // the real end of the sequence, so an understated maximum loses no keys (the reference derives its key loop from
     // the actual length as well, reference csrc/flash_attn/params.cuh:156-163).
@@ -242,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
   const int rowA = g, rowB = g + 8;
   const int qposA = rowA / p.group, qposB = rowB / p.group;
   const bool validA = rowA < nRows, validB = rowB < nRows;
-  const float c = p.scaleLog2;
+  const float c = kScore ? 1.f : p.scaleLog2;
 
   float o[kNT][4];
   float mA, mB, lA, lB;
@@ -335,6 +356,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
       acc.y *= inv;
       acc.z *= inv;
       acc.w *= inv;
+      if (kScore && l == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // a row that sees no key is zero even where 0 times a value is not
       const long long orow = (qRow0 + r / p.group) * p.headsQ + hkv * p.group + r % p.group;
       if (whole) {
         uint2 out;
@@ -400,8 +422,45 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
         mma16816<kBf16>(sc[0], qf[ks], kf[0], kf[1]);
         mma16816<kBf16>(sc[1], qf[ks], kf[2], kf[3]);
       }
+      if constexpr (kScore) {
+        // c tanh(x) = c - 2 c / (e^2x + 1): off by about 2^-23 c whatever x is, which is what the exponential behind it sees
+        const float capLog2 = p.cap * 1.44269504f, factor = p.cap > 0.f ? 2.f * p.scaleLog2 / p.cap : p.scaleLog2;
+        const int posA = p.qStart + qposA, posB = p.qStart + qposB;
+        int limA = keyEnd, limB = keyEnd;
+        if (p.causal) {
+          const int prefix = p.prefix != nullptr ? p.prefix[b] : 0;
+          limA = min(limA, max(posA + 1, prefix));
+          limB = min(limB, max(posB + 1, prefix));
+        }
+        float slopeA = 0.f, slopeB = 0.f;
+        if (p.slopes != nullptr) {
+          slopeA = validA ? p.slopes[hkv * p.group + rowA % p.group] * 1.44269504f : 0.f;
+          slopeB = validB ? p.slopes[hkv * p.group + rowB % p.group] * 1.44269504f : 0.f;
+        }
+        int docA = -1, docB = -1;
+        if (p.docKV != nullptr) {
+          docA = validA ? p.docQ[qRow0 + qposA] : -1;
+          docB = validB ? p.docQ[qRow0 + qposB] : -1;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int key = kb + n * 8 + 2 * tig + (e & 1);
+            float x = sc[n][e] * factor;
+            if (p.cap > 0.f) x = fmaf(-2.f * capLog2, rcp(ex2(x) + 1.f), capLog2);
+            if (p.slopes != nullptr) x = fmaf(e < 2 ? -slopeA : -slopeB, fabsf((float)((e < 2 ? posA : posB) - key)), x);
+            bool see = key < (e < 2 ? limA : limB);
+            if (p.docKV != nullptr) {
+              const int doc = e < 2 ? docA : docB;
+              see = see && doc >= 0 && p.docKV[(long long)b * skv + key] == doc;
+            }
+            sc[n][e] = see ? x : -INFINITY;
+          }
+        }
+      }
       // ---- mask (tail of the key range, top-left causal)
-      const bool needMask = (kb + 16 > keyEnd) || p.causal;
+      const bool needMask = !kScore && ((kb + 16 > keyEnd) || p.causal);
       if (needMask) {
 #pragma unroll
         for (int n = 0; n < 2; n++) {
@@ -563,7 +622,7 @@ combine_kernel(const float* partO, const float* partLse, void* O, long long rows
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kCombineThreads)
 combine_parts_kernel(const float* partO, const float* partLse, void* O, long long rows, int partBlocks,
-                     int seqLenQ, int seqLenKV, int headsQ, int causal, int rowsPerTile) {
+                     int seqLenQ, int seqLenKV, int headsQ, int causal, int rowsPerTile, int qStart) {
   constexpr int kVec = D / 4, kGroups = kCombineThreads / kVec;
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
@@ -573,7 +632,7 @@ combine_parts_kernel(const float* partO, const float* partLse, void* O, long lon
   int blocks = (seqLenKV + 127) / 128;
   if (causal) {  // key blocks of this row's query tile, as in make_work
     const int tile = (int)(row / headsQ % seqLenQ) / rowsPerTile;
-    blocks = min(blocks, (min((tile + 1) * rowsPerTile, seqLenQ) + 127) / 128);
+    blocks = min(blocks, (qStart + min((tile + 1) * rowsPerTile, seqLenQ) + 127) / 128);
   }
   const int parts = (blocks + partBlocks - 1) / partBlocks;
   if (parts == 1) return;  // the attention kernel has written the output
@@ -615,7 +674,7 @@ int launch_combine(const FwdProblem& p, int packShift, const TcSplit& split) {
   } else {
     e = launch_kernel(combine_parts_kernel<D, kBf16>, dim3((unsigned)((rows + kGroups - 1) / kGroups)), kCombineThreads, 0, p.stream,
                       p.overlap, split.partO, split.partLse, p.O, rows, split.partBlocks, p.seqLenQ, p.seqLenKV, p.headsQ, p.causal,
-                      128 >> packShift);
+                      128 >> packShift, p.score != nullptr ? p.score->qStart : 0);
   }
   if (e != cudaSuccess) {
     set_error_string("combine kernel launch failed: %s", cudaGetErrorString(e));
@@ -636,26 +695,35 @@ constexpr int quarter_ctas_per_sm(int D) { return D == 32 ? 16 : D == 64 ? 12 : 
 // CTAs of an SM without the even partition: the stated 8, registers up to head dim 96, shared memory above.
 constexpr int whole_ctas_per_sm(int D) { return D == 32 ? 8 : D == 64 ? 4 : D == 96 ? 3 : D == 128 ? 2 : 1; }
 
-template <int D, bool kBf16>
+// Keys that some row of the call may see.
+int splitkv_seen(const FwdProblem& p) {
+  if (!p.causal) return p.seqLenKV;
+  long long reach = p.seqLenQ;
+  if (p.score != nullptr) reach += p.score->qStart;
+  if (p.score != nullptr && p.score->prefix != nullptr) reach = p.seqLenKV;  // which only the device knows
+  return (int)(reach < p.seqLenKV ? reach : p.seqLenKV);
+}
+
+template <int D, bool kBf16, bool kScore = false>
 int launch(const FwdProblem& pr, const SplitPlan& plan, float* partO, float* partLse) {
   constexpr int kSmem = ring_bytes(D) + merge_bytes(D, 1);
   static_assert(kSmem <= kMaxSmem && merge_bytes(D, 4) <= ring_bytes(D) && merge_ld<D>() == D + 8, "shared memory");
-  auto kernel = plan.runs > 0 ? fwd_splitkv_kernel<D, kBf16, true> : fwd_splitkv_kernel<D, kBf16, false>;
+  auto kernel = plan.runs > 0 ? fwd_splitkv_kernel<D, kBf16, true, kScore> : fwd_splitkv_kernel<D, kBf16, false, kScore>;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kCudaError;
   static std::once_flag once[64];
   static cudaError_t attrErr[64];
   std::call_once(once[device], [&] {
-    attrErr[device] = cudaFuncSetAttribute(fwd_splitkv_kernel<D, kBf16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    attrErr[device] = cudaFuncSetAttribute(fwd_splitkv_kernel<D, kBf16, true, kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
     if (attrErr[device] == cudaSuccess) {
-      attrErr[device] = cudaFuncSetAttribute(fwd_splitkv_kernel<D, kBf16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+      attrErr[device] = cudaFuncSetAttribute(fwd_splitkv_kernel<D, kBf16, false, kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
     }
     // all of it as shared memory: the spread below counts on it
     if (attrErr[device] == cudaSuccess) {
-      attrErr[device] = cudaFuncSetAttribute(fwd_splitkv_kernel<D, kBf16, true>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+      attrErr[device] = cudaFuncSetAttribute(fwd_splitkv_kernel<D, kBf16, true, kScore>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     }
     if (attrErr[device] == cudaSuccess) {
-      attrErr[device] = cudaFuncSetAttribute(fwd_splitkv_kernel<D, kBf16, false>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+      attrErr[device] = cudaFuncSetAttribute(fwd_splitkv_kernel<D, kBf16, false, kScore>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     }
   });
   if (attrErr[device] != cudaSuccess) {
@@ -663,7 +731,7 @@ int launch(const FwdProblem& pr, const SplitPlan& plan, float* partO, float* par
     return kCudaError;
   }
   const int numSMs = device_num_sms(device);
-  Params p;
+  typename ParamsOf<kScore>::type p;
   p.Q = pr.Q;
   p.K = pr.K;
   p.V = pr.V;
@@ -686,6 +754,11 @@ int launch(const FwdProblem& pr, const SplitPlan& plan, float* partO, float* par
   p.keysPerSplit = ((blocks + plan.splits - 1) / plan.splits) * kBlockKeys;
   p.totalQ = pr.totalQ;
   p.scaleLog2 = (float)(1.4426950408889634 / sqrt((double)D));
+  if constexpr (kScore) {
+    static_cast<ScoreFields&>(p) = *pr.score;
+    p.keyEnd = splitkv_seen(pr);
+    p.keysPerSplit = (((p.keyEnd + kBlockKeys - 1) / kBlockKeys + plan.splits - 1) / plan.splits) * kBlockKeys;
+  }
   const dim3 grid = plan.runs > 0 ? dim3((unsigned)(plan.runs * pr.headsKV)) : dim3((unsigned)plan.splits, (unsigned)pr.headsKV, (unsigned)pr.batch);
   // head dim 96 fits three CTAs per SM without the merge buffer, two with it: packed, 223 x up to 5432 keys, 2 heads 138 -> 118 us
   size_t smem = plan.runs > 0 ? kSmem : ring_bytes(D);
@@ -745,7 +818,7 @@ SplitPlan splitkv_plan(const FwdProblem& p, int numSMs, int forced) {
     plan.splits = forced < maxSplits ? forced : maxSplits;
     return plan;
   }
-  const int seen = p.causal ? (p.seqLenQ < p.seqLenKV ? p.seqLenQ : p.seqLenKV) : p.seqLenKV;
+  const int seen = decode::splitkv_seen(p);
   const long long blocks = (seen + decode::kBlockKeys - 1) / decode::kBlockKeys;
   const long long slots = (long long)numSMs * decode::quarter_ctas_per_sm(p.headDim) / 4;
   if (p.cuQ == nullptr && blocks >= 4 && pairs < 8 * slots && p.headsKV <= slots) {
@@ -828,13 +901,19 @@ int launch_fwd_splitkv(const FwdProblem& p, const SplitPlan& plan, float* scratc
   float* partO = scratch;
   float* partLse = scratch ? scratch + (size_t)plan.splits * rows * p.headDim : nullptr;
   const bool bf = (p.dtype == kBf16);
-#define TFA_DECODE_CASE(D)                                                                   \
-  case D:                                                                                    \
-    if (bf) {                                                                                \
-      if constexpr (TFA_HAVE_BF16) return decode::launch<D, true>(p, plan, partO, partLse);  \
-    } else {                                                                                 \
-      if constexpr (TFA_HAVE_FP16) return decode::launch<D, false>(p, plan, partO, partLse); \
-    }                                                                                        \
+#define TFA_DECODE_CASE(D)                                                                           \
+  case D:                                                                                            \
+    if (bf) {                                                                                        \
+      if constexpr (TFA_HAVE_BF16) {                                                                 \
+        return p.score != nullptr ? decode::launch<D, true, true>(p, plan, partO, partLse)           \
+                                  : decode::launch<D, true>(p, plan, partO, partLse);                \
+      }                                                                                              \
+    } else {                                                                                         \
+      if constexpr (TFA_HAVE_FP16) {                                                                 \
+        return p.score != nullptr ? decode::launch<D, false, true>(p, plan, partO, partLse)          \
+                                  : decode::launch<D, false>(p, plan, partO, partLse);               \
+      }                                                                                              \
+    }                                                                                                \
     return kBadDtype;
   (void)bf; (void)partO; (void)partLse;
   switch (p.headDim) {

@@ -18,6 +18,7 @@
 
 #include "build_config.cuh"
 #include "ptx_sm100.cuh"
+#include "score.cuh"
 #include "tfa_common.cuh"
 
 namespace tfa_b200 {
@@ -43,7 +44,21 @@ struct Fp32Params {
   int gateEpoch;
 };
 
+// ... of a call whose scores are capped, biased or masked by prefix or document; key blocks and query tiles of its tables are this file's
+struct Fp32ScoreParams : Fp32Params, ScoreFields {
+  float scale;  // 1 / sqrt(D)
+};
+
 namespace fp32 {
+
+template <bool kScore>
+struct ParamsOf {
+  using type = Fp32Params;
+};
+template <>
+struct ParamsOf<true> {
+  using type = Fp32ScoreParams;
+};
 
 // kGated instantiations run behind the tensor-core kernel and return at once unless it left the call to them.  Calls that
 // come here straight away have instantiations of their own: the check at the top cost a 23 us call 4 %.
@@ -103,8 +118,8 @@ __device__ __forceinline__ void load_tile(float* sm, const float* base, long lon
   }
 }
 
-template <int D, int BR, bool kGated>
-__global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const Fp32Params p) {
+template <int D, int BR, bool kGated, bool kScore = false>
+__global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const typename ParamsOf<kScore>::type p) {
   constexpr int kThreads = BR * 8 / kRowsPerThread;
   constexpr int LD = D + 4;
   constexpr int LDP = kBC + 4;
@@ -141,6 +156,19 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
   const int qEnd = min(q0 + BR, sq);
   int nblk = (skv + kBC - 1) / kBC;
   if (p.causal) nblk = min(nblk, (qEnd + kBC - 1) / kBC);
+  int blk0 = 0;
+  [[maybe_unused]] int prefix = 0;
+  if constexpr (kScore) {
+    nblk = (skv + kBC - 1) / kBC;
+    if (p.prefix != nullptr) prefix = p.prefix[b];
+    if (p.tileRange != nullptr) {
+      const int2 range = p.tileRange[(long long)b * p.tiles + tileIdx];
+      blk0 = range.x;
+      nblk = range.y;
+    } else if (p.causal) {
+      nblk = min(nblk, (max(p.qStart + qEnd, prefix) + kBC - 1) / kBC);
+    }
+  }
 
   const long long qStride = (long long)p.headsQ * D;
   const long long kvStride = (long long)p.headsKV * D;
@@ -151,7 +179,7 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
   const int ty = threadIdx.x >> 3, tx = threadIdx.x & 7;
 
   load_tile<D, BR, LD, kThreads>(sQ, gQ, qRow0 + q0, qRow0 + sq, qStride);
-  load_tile<D, kBC, LD, kThreads>(sK, gK, kvRow0, kvRow0 + skv, kvStride);
+  load_tile<D, kBC, LD, kThreads>(sK, gK, kvRow0 + blk0 * kBC, kvRow0 + skv, kvStride);
   cp_async_commit();
 
   float o[RPT][NCH][4];
@@ -165,9 +193,9 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
       o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.f;
     }
   }
-  const float c = p.scaleLog2;
+  const float c = kScore ? 1.f : p.scaleLog2;
 
-  for (int j = 0; j < nblk; j++) {
+  for (int j = blk0; j < nblk; j++) {
     const int kbase = j * kBC;
     load_tile<D, kBC, LD, kThreads>(sV, gV, kvRow0 + kbase, kvRow0 + skv, kvStride);
     cp_async_commit();
@@ -230,8 +258,31 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
       }
     }
 
+    if constexpr (kScore) {  // capped, biased, masked; multiples of log2(e) from here on
+      int doc[8];
+      if (p.docKV != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) doc[i] = kbase + tx + 8 * i < skv ? p.docKV[kvRow0 + kbase + tx + 8 * i] : -1;
+      }
+      const float slope = p.slopes != nullptr ? p.slopes[h] : 0.f;
+#pragma unroll
+      for (int r = 0; r < RPT; r++) {
+        const int row = q0 + ty * RPT + r, pos = p.qStart + row;
+        const int lim = p.causal ? min(skv, max(pos + 1, prefix)) : skv;
+        const int rowDoc = (p.docKV != nullptr && row < sq) ? p.docQ[qRow0 + row] : -1;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int key = kbase + tx + 8 * i;
+          float x = s[r][i] * p.scale;
+          if (p.cap > 0.f) x = p.cap * tanhf(x / p.cap);
+          if (p.slopes != nullptr) x = fmaf(-slope, fabsf((float)(pos - key)), x);
+          const bool see = key < lim && (p.docKV == nullptr || (rowDoc >= 0 && doc[i] == rowDoc));
+          s[r][i] = see ? x * 1.44269504f : -INFINITY;
+        }
+      }
+    }
     // ---- mask + online softmax
-    const bool needMask = (kbase + kBC > skv) || (p.causal && (kbase + kBC - 1 > q0));
+    const bool needMask = !kScore && ((kbase + kBC > skv) || (p.causal && (kbase + kBC - 1 > q0)));
 #pragma unroll
     for (int r = 0; r < RPT; r++) {
       const int qpos = q0 + ty * RPT + r;
@@ -337,6 +388,7 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
         v.y = o[r][i][1] * inv;
         v.z = o[r][i][2] * inv;
         v.w = o[r][i][3] * inv;
+        if (kScore && sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);  // sees no key: zero even where 0 times a value is not
         *reinterpret_cast<float4*>(dst + (tx + 8 * i) * 4) = v;
       }
     }
@@ -888,18 +940,21 @@ int launch_t8(const FwdProblem& pr) {
   return kOk;
 }
 
-template <int D, int BR>
+template <int D, int BR, bool kScore = false>
 int launch(const FwdProblem& pr) {
   constexpr int LD = D + 4;
   constexpr int kSmem = (BR * LD + 2 * kBC * LD + BR * (kBC + 4)) * (int)sizeof(float);
-  auto kernel = pr.gate != nullptr ? fwd_fp32_kernel<D, BR, true> : fwd_fp32_kernel<D, BR, false>;
+  auto kernel = fwd_fp32_kernel<D, BR, false, kScore>;
+  if constexpr (!kScore) {
+    if (pr.gate != nullptr) kernel = fwd_fp32_kernel<D, BR, true>;
+  }
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kCudaError;
   static std::once_flag once[64];
   static cudaError_t attrErr[64];
   std::call_once(once[device], [&] {
-    attrErr[device] = cudaFuncSetAttribute(fwd_fp32_kernel<D, BR, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (attrErr[device] == cudaSuccess) {
+    attrErr[device] = cudaFuncSetAttribute(fwd_fp32_kernel<D, BR, false, kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (!kScore && attrErr[device] == cudaSuccess) {
       attrErr[device] = cudaFuncSetAttribute(fwd_fp32_kernel<D, BR, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     }
   });
@@ -907,7 +962,7 @@ int launch(const FwdProblem& pr) {
     set_error_string("cudaFuncSetAttribute(%d bytes): %s", kSmem, cudaGetErrorString(attrErr[device]));
     return kCudaError;
   }
-  Fp32Params p;
+  typename ParamsOf<kScore>::type p;
   p.Q = static_cast<const float*>(pr.Q);
   p.K = static_cast<const float*>(pr.K);
   p.V = static_cast<const float*>(pr.V);
@@ -923,6 +978,10 @@ int launch(const FwdProblem& pr) {
   p.gate = pr.gate;
   p.gateEpoch = pr.gateEpoch;
   p.scaleLog2 = (float)(1.4426950408889634 / sqrt((double)D));
+  if constexpr (kScore) {
+    static_cast<ScoreFields&>(p) = *pr.score;
+    p.scale = (float)(1.0 / sqrt((double)D));
+  }
   dim3 grid((unsigned)((pr.seqLenQ + BR - 1) / BR), (unsigned)pr.headsQ, (unsigned)pr.batch);
   const cudaError_t e = launch_kernel(kernel, grid, BR * 8 / kRowsPerThread, kSmem, pr.stream, pr.overlap, p);
   if (e != cudaSuccess) {
@@ -934,7 +993,38 @@ int launch(const FwdProblem& pr) {
 
 }  // namespace fp32
 
+// Capped, biased or masked scores: 64 query rows and 64 keys at every head dim (kScoreTileRows and kScoreBlockKeys of fwd_score.cu).
+static int launch_fwd_fp32_scored(const FwdProblem& pr) {
+#if TFA_HAVE_FP32
+  switch (pr.headDim) {
+#if TFA_HAVE_HD32
+    case 32: return fp32::launch<32, 64, true>(pr);
+#endif
+#if TFA_HAVE_HD64
+    case 64: return fp32::launch<64, 64, true>(pr);
+#endif
+#if TFA_HAVE_HD96
+    case 96: return fp32::launch<96, 64, true>(pr);
+#endif
+#if TFA_HAVE_HD128
+    case 128: return fp32::launch<128, 64, true>(pr);
+#endif
+#if TFA_HAVE_HD192
+    case 192: return fp32::launch<192, 64, true>(pr);
+#endif
+#if TFA_HAVE_HD256
+    case 256: return fp32::launch<256, 64, true>(pr);
+#endif
+    default: break;
+  }
+#else
+  (void)pr;
+#endif
+  return kBadHeadDim;
+}
+
 int launch_fwd_fp32(const FwdProblem& pr) {
+  if (pr.score != nullptr) return launch_fwd_fp32_scored(pr);
 #if TFA_HAVE_FP32
   switch (pr.headDim) {
 #if TFA_HAVE_HD32

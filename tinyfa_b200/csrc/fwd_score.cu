@@ -1,0 +1,255 @@
+// Attention with capped, biased or masked scores (score.cuh): argument checks, choice of the kernel, and the two small kernels that tell
+// the attention kernels which key blocks a query tile can see when keys and queries belong to documents.
+#include <cuda_runtime.h>
+#include <limits.h>
+#include <math.h>
+
+#include "../../include/tinyfa_b200.h"
+#include "build_config.cuh"
+#include "ptx_sm100.cuh"
+#include "score.cuh"
+#include "tfa_common.cuh"
+
+namespace tfa_b200 {
+
+int device_num_sms(int device);  // c_abi.cu
+int pack_shift_of(const FwdProblem& p);
+int split_kv_option();
+TcSplit tc_split_of(const FwdProblem& p, int packShift, int qStart);
+bool splitkv_applicable(const FwdProblem& p);  // fwd_decode.cu
+SplitPlan splitkv_plan(const FwdProblem& p, int numSMs, int forced);
+size_t splitkv_scratch_floats(const FwdProblem& p, const SplitPlan& plan);
+int launch_fwd_splitkv(const FwdProblem& p, const SplitPlan& plan, float* scratch);
+int launch_combine_parts(const FwdProblem& p, int packShift, const TcSplit& split);
+
+#define TFA_DECLARE_SCORE(HDP)                                                             \
+  int launch_fwd_tc_score_hdp##HDP##_bf0(const FwdProblem&, int, const TcSplit&);          \
+  int launch_fwd_tc_score_hdp##HDP##_bf1(const FwdProblem&, int, const TcSplit&);          \
+  static inline int score_call_hdp##HDP(const FwdProblem& p, int ps, const TcSplit& split) { \
+    (void)p; (void)ps; (void)split;                                                        \
+    if (p.dtype == kBf16) {                                                                \
+      if constexpr (TFA_HAVE_BF16) return launch_fwd_tc_score_hdp##HDP##_bf1(p, ps, split); \
+    } else {                                                                               \
+      if constexpr (TFA_HAVE_FP16) return launch_fwd_tc_score_hdp##HDP##_bf0(p, ps, split); \
+    }                                                                                      \
+    return kBadDtype;                                                                      \
+  }
+#if TFA_HAVE_HDP64
+TFA_DECLARE_SCORE(64)
+#endif
+#if TFA_HAVE_HDP128
+TFA_DECLARE_SCORE(128)
+#endif
+#if TFA_HAVE_HDP192
+TFA_DECLARE_SCORE(192)
+#endif
+#if TFA_HAVE_HDP256
+TFA_DECLARE_SCORE(256)
+#endif
+#undef TFA_DECLARE_SCORE
+
+namespace score {
+
+constexpr int kWarps = 8;
+constexpr int kScoreTileRows = 64, kScoreBlockKeys = 64;  // of the fp32 kernel; the tensor-core kernel has 128 >> packShift and 128
+
+// Smallest and largest document of every key block, a warp each.
+__global__ void __launch_bounds__(kWarps * 32) key_blocks_kernel(const int* docKV, int2* out, int seqLenKV, int blockKeys, int blocks, long long all) {
+  ptx::grid_wait_previous();
+  ptx::grid_allow_next();
+  const long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (i >= all) return;
+  const long long b = i / blocks;
+  const int k0 = (int)(i - b * blocks) * blockKeys, k1 = min(k0 + blockKeys, seqLenKV);
+  int lo = INT_MAX, hi = INT_MIN;
+  for (int k = k0 + (threadIdx.x & 31); k < k1; k += 32) {
+    const int d = docKV[b * seqLenKV + k];
+    lo = min(lo, d);
+    hi = max(hi, d);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if ((threadIdx.x & 31) == 0) out[i] = make_int2(lo, hi);
+}
+
+// Key blocks [x, y) that some row of a query tile may see, a warp for each tile: from the first to the last block whose range of
+// documents meets the tile's (documents in ascending order: exactly those with a visible key), as far as the causal mask reaches.
+// Never empty: a tile that sees nothing gets one block, in which everything is masked, so that its rows are written.
+__global__ void __launch_bounds__(kWarps * 32) tile_range_kernel(const int* docQ, const int2* keyBlocks, const int* prefix, int2* out, int seqLenQ,
+                                                                 int seqLenKV, int tileRows, int tiles, int blockKeys, int blocks, int causal, int qStart,
+                                                                 long long all) {
+  ptx::grid_wait_previous();
+  ptx::grid_allow_next();
+  const long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (i >= all) return;
+  const int lane = threadIdx.x & 31;
+  const long long b = i / tiles;
+  const int r0 = (int)(i - b * tiles) * tileRows, r1 = min(r0 + tileRows, seqLenQ);
+  int lo = INT_MAX, hi = INT_MIN;
+  for (int r = r0 + lane; r < r1; r += 32) {
+    const int d = docQ[b * seqLenQ + r];
+    if (d >= 0) {
+      lo = min(lo, d);
+      hi = max(hi, d);
+    }
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  int end = blocks;
+  if (causal) {
+    long long see = (long long)qStart + r1;
+    if (prefix != nullptr) see = max(see, (long long)prefix[b]);
+    end = (int)min((long long)blocks, (see - 1) / blockKeys + 1);
+  }
+  int first = INT_MAX, last = -1;
+  for (int k = lane; k < end; k += 32) {
+    const int2 ids = keyBlocks[b * blocks + k];
+    if (ids.y >= lo && ids.x <= hi) {
+      first = min(first, k);
+      last = k;
+    }
+  }
+  first = __reduce_min_sync(0xffffffffu, first);
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 0) out[i] = last < 0 ? make_int2(0, 1) : make_int2(first, last + 1);
+}
+
+int run_tc(const FwdProblem& p, int ps, const TcSplit& split) {
+  switch (p.headDim) {
+#if TFA_HAVE_HDP64
+    case 32:
+    case 64: return score_call_hdp64(p, ps, split);
+#endif
+#if TFA_HAVE_HDP128
+    case 96:
+    case 128: return score_call_hdp128(p, ps, split);
+#endif
+#if TFA_HAVE_HDP192
+    case 192: return score_call_hdp192(p, ps, split);
+#endif
+#if TFA_HAVE_HDP256
+    case 256: return score_call_hdp256(p, ps, split);
+#endif
+    default: return kBadHeadDim;
+  }
+}
+
+// The partial results of a call that is cut over its keys, and the tables of documents, live in one stream-ordered allocation that is
+// released behind the last kernel.
+int dispatch(FwdProblem p, ScoreFields& f, int device) {
+  p.score = &f;
+  p.overlap = may_overlap(p.stream);
+  const bool docs = f.docKV != nullptr;
+  const bool fp32 = p.dtype == kFp32;
+  const int sms = device_num_sms(device);
+  const int forced = split_kv_option();
+  // few query rows: the split-KV kernel, which reads every key - with documents most keys may be none of the row's
+  const bool rows = !fp32 && !docs && forced != 0 && splitkv_applicable(p);
+  SplitPlan plan = {1, 0, 0};
+  size_t floats = 0;
+  int ps = 0;
+  TcSplit split;
+  if (rows) {
+    plan = splitkv_plan(p, sms, forced);
+    floats = splitkv_scratch_floats(p, plan);
+  } else if (!fp32) {
+    ps = pack_shift_of(p);
+    if (!docs && f.prefix == nullptr) split = tc_split_of(p, ps, f.qStart);
+    if (split.parts > 1) floats = (size_t)split.parts * p.totalQ * p.headsQ * (p.headDim + 1);
+  }
+  const int tileRows = fp32 ? kScoreTileRows : 128 >> ps, blockKeys = fp32 ? kScoreBlockKeys : 128;
+  const int blocks = (p.seqLenKV + blockKeys - 1) / blockKeys;
+  f.tiles = (p.seqLenQ + tileRows - 1) / tileRows;
+  const size_t tableBytes = docs ? sizeof(int2) * (size_t)p.batch * (blocks + f.tiles) : 0;
+  void* scratch = nullptr;
+  int rc = kOk;
+  if (floats > 0 || tableBytes > 0) {
+    rc = scratch_alloc(&scratch, tableBytes > 0 ? tableBytes : floats * sizeof(float), device, p.stream);
+    if (rc != kOk) return rc;
+  }
+  if (docs) {
+    int2* keyBlocks = static_cast<int2*>(scratch);
+    int2* tileRange = keyBlocks + (size_t)p.batch * blocks;
+    const long long allBlocks = (long long)p.batch * blocks, allTiles = (long long)p.batch * f.tiles;
+    cudaError_t e = launch_kernel(key_blocks_kernel, dim3((unsigned)((allBlocks + kWarps - 1) / kWarps)), kWarps * 32, 0, p.stream, p.overlap, f.docKV,
+                                  keyBlocks, p.seqLenKV, blockKeys, blocks, allBlocks);
+    if (e == cudaSuccess) {
+      e = launch_kernel(tile_range_kernel, dim3((unsigned)((allTiles + kWarps - 1) / kWarps)), kWarps * 32, 0, p.stream, p.overlap, f.docQ, keyBlocks,
+                        f.prefix, tileRange, p.seqLenQ, p.seqLenKV, tileRows, f.tiles, blockKeys, blocks, p.causal, f.qStart, allTiles);
+    }
+    if (e != cudaSuccess) {
+      set_error_string("document table kernel launch failed: %s", cudaGetErrorString(e));
+      rc = kCudaError;
+    }
+    f.keyBlocks = keyBlocks;
+    f.tileRange = tileRange;
+  }
+  if (rc == kOk) {
+    if (fp32) {
+      rc = launch_fwd_fp32(p);
+    } else if (rows) {
+      rc = launch_fwd_splitkv(p, plan, static_cast<float*>(scratch));
+    } else {
+      if (split.parts > 1) {
+        split.partO = static_cast<float*>(scratch);
+        split.partLse = split.partO + (size_t)split.parts * p.totalQ * p.headsQ * p.headDim;
+      }
+      rc = run_tc(p, ps, split);
+      if (rc == kOk && split.parts > 1) rc = launch_combine_parts(p, ps, split);
+    }
+  }
+  if (scratch != nullptr) cudaFreeAsync(scratch, p.stream);
+  return rc;
+}
+
+}  // namespace score
+}  // namespace tfa_b200
+
+using namespace tfa_b200;
+
+extern "C" int tfa_b200_fwd_scored(const void* Q, const void* K, const void* V, void* O, int dtype, int batchSize, int seqLenQ, int seqLenKV,
+                                   int numHeadsQ, int numHeadsKV, int headDim, int isCausal, int qStart, float softcap, const float* alibiSlopes,
+                                   const int* prefixLens, const int* docIdsQ, const int* docIdsKV, void* stream) {
+  int rc = validate_common(Q, K, V, O, dtype, batchSize, seqLenQ, seqLenKV, numHeadsQ, numHeadsKV, headDim);
+  if (rc != kOk) return rc;
+  if (qStart < 0 || !(softcap >= 0.f) || isinf(softcap)) {
+    set_error_string("qStart and softcap must not be negative (qStart=%d softcap=%g)", qStart, softcap);
+    return kBadArgument;
+  }
+  if (prefixLens != nullptr && !isCausal) {
+    set_error_string("prefix lengths widen the causal mask: they need isCausal");
+    return kBadArgument;
+  }
+  if ((docIdsQ == nullptr) != (docIdsKV == nullptr)) {
+    set_error_string("document ids are given for queries and keys or for neither");
+    return kBadArgument;
+  }
+  if (batchSize == 0 || seqLenQ == 0 || seqLenKV == 0) return kOk;  // nothing to write
+  if ((long long)batchSize * seqLenQ > 0x7FFFFFFFll || (long long)batchSize * seqLenKV > 0x7FFFFFFFll || (long long)qStart + seqLenQ > 0x7FFFFF00ll) {
+    set_error_string("batchSize * seqLen and qStart + seqLenQ must stay below 2^31 rows");
+    return kTooLarge;
+  }
+  if ((rc = check_device()) != kOk) return rc;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kCudaError;
+  FwdProblem p;
+  p.Q = Q;
+  p.K = K;
+  p.V = V;
+  p.O = O;
+  p.cuQ = nullptr;
+  p.cuKV = nullptr;
+  p.dtype = dtype;
+  p.batch = batchSize;
+  p.seqLenQ = seqLenQ;
+  p.seqLenKV = seqLenKV;
+  p.totalQ = (long long)batchSize * seqLenQ;
+  p.totalKV = (long long)batchSize * seqLenKV;
+  p.headsQ = numHeadsQ;
+  p.headsKV = numHeadsKV;
+  p.headDim = headDim;
+  p.causal = isCausal ? 1 : 0;
+  p.stream = static_cast<cudaStream_t>(stream);
+  ScoreFields f = {qStart, softcap, alibiSlopes, prefixLens, docIdsQ, docIdsKV, nullptr, nullptr, 0};
+  return score::dispatch(p, f, device);
+}

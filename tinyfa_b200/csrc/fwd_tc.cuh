@@ -36,6 +36,7 @@
 #include <type_traits>
 
 #include "ptx_sm100.cuh"
+#include "score.cuh"
 #include "tfa_common.cuh"
 
 namespace tfa_b200 {
@@ -76,6 +77,10 @@ struct TcPartParams : TcParams {
   float* partO;     // [parts][rows][headDim]
   float* partLse;   // [parts][rows]
 };
+
+// ... and of a call whose scores are capped, biased or masked by prefix or document (score.cuh), whole or cut into key ranges.
+struct TcScoreParams : TcParams, ScoreFields {};
+struct TcScorePartParams : TcPartParams, ScoreFields {};
 
 namespace tc {
 
@@ -262,7 +267,7 @@ struct WorkSlot {
   int qlo[2];
   int nblk[2];
   int nmax;
-  int part;        // key range (kModeFixedSplit)
+  int part;        // key range (kModeFixedSplit); first key block of the item (scored calls that are not cut)
 };
 
 struct Ctl {
@@ -345,6 +350,12 @@ __device__ __forceinline__ void spin_bar(uint32_t bar, uint32_t parity, const Wa
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -441,7 +452,8 @@ struct Work {
   int nblk[2];         // KV blocks each tile consumes
   int nmax;
 };
-// ... of a key range (kModeFixedSplit), whose first block is part * partBlocks
+// ... of a key range (kModeFixedSplit), whose first block is part * partBlocks; of a scored call that is not cut, whose first block
+// is `part`
 struct WorkPart : Work {
   int part;
 };
@@ -468,6 +480,9 @@ __device__ __forceinline__ void zero_v_tail(uint32_t tileAddr, int lane, int tai
   __syncwarp();
 }
 
+__device__ __forceinline__ int p_part_blocks(const TcParams&) { return 0; }
+__device__ __forceinline__ int p_part_blocks(const TcPartParams& p) { return p.partBlocks; }
+
 // Work item idx -> (query tile pair, Q head unit, batch entry).  Two orders.  Pair index fastest: CTAs running at the
 // same time work on the same head and share its K/V through L2 (all items cost the same when nothing is causal).
 // Causal: the cost of an item grows with its pair index, so inside a chunk of p.chunk consecutive (head unit, batch)
@@ -476,6 +491,7 @@ __device__ __forceinline__ void zero_v_tail(uint32_t tileAddr, int lane, int tai
 // group, which still share K/V, and the host sizes the chunk so that the K/V of its heads stay resident in L2.
 template <int NT, bool kVarlen, bool kSplit = false, class P = TcParams, class W = Work>
 __device__ __forceinline__ bool make_work(const P& p, int idx, W& w) {
+  constexpr bool kScored = std::is_base_of<ScoreFields, P>::value;
   int pr, rest;
   if constexpr (kSplit) {
     w.part = idx / p.numItems;
@@ -526,6 +542,41 @@ __device__ __forceinline__ bool make_work(const P& p, int idx, W& w) {
   if (seq0 >= w.sq || w.skv <= 0) return false;
   w.hkv = (w.unit << p.packShift) / p.group;
   const int nTotal = (w.skv + kBlockN - 1) / kBlockN;
+  if constexpr (kScored) {
+    // Key blocks that some row of a tile may see: [first, end), never empty, so that rows without a key are written too.  Both tiles
+    // of an item start at the earlier first block; what a tile does not see there is masked.
+    int first[2] = {nTotal, nTotal}, end[2] = {0, 0};
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      w.qlo[t] = seq0 + t * rows;
+      w.qhi[t] = min(w.qlo[t] + rows, w.sq);
+      if (t >= NT || w.qlo[t] >= w.sq) continue;
+      if (p.tileRange != nullptr) {
+        const int2 r = p.tileRange[(long long)b * p.tiles + w.qlo[t] / rows];
+        first[t] = r.x;
+        end[t] = r.y;
+      } else {
+        first[t] = 0;
+        end[t] = nTotal;
+        if (p.causal) {
+          int see = p.qStart + w.qhi[t];
+          if (p.prefix != nullptr) see = max(see, p.prefix[b]);
+          end[t] = min(nTotal, (see - 1) / kBlockN + 1);
+        }
+      }
+    }
+    if (end[1] > 0) end[1] = max(end[0], end[1]);  // the issuing threads take turns as if tile 1 had the longer way
+    const int lo = kSplit ? w.part * p_part_blocks(p) : min(first[0], first[1]);
+    if constexpr (!kSplit) w.part = lo;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      int n = max(0, end[t] - lo);
+      if constexpr (kSplit) n = min(n, p_part_blocks(p));
+      w.nblk[t] = n;
+      w.nmax = max(w.nmax, n);
+    }
+    return w.nmax > 0;
+  }
 #pragma unroll
   for (int t = 0; t < 2; t++) {
     w.qlo[t] = seq0 + t * rows;
@@ -544,9 +595,12 @@ __device__ __forceinline__ bool make_work(const P& p, int idx, W& w) {
 
 // Does a tile's whole key range fit its first part?  Such rows (the early ones of a causal problem) get their final output
 // straight away.
-__device__ __forceinline__ bool whole_tile(const TcPartParams& p, const Work& w, int t) {
+template <class P>
+__device__ __forceinline__ bool whole_tile(const P& p, const Work& w, int t) {
   int n = (w.skv + kBlockN - 1) / kBlockN;
-  if (p.causal) n = min(n, (min(w.qlo[t] + (kBlockM >> p.packShift), w.sq) + kBlockN - 1) / kBlockN);
+  int see = min(w.qlo[t] + (kBlockM >> p.packShift), w.sq);
+  if constexpr (std::is_base_of<ScoreFields, P>::value) see += p.qStart;
+  if (p.causal) n = min(n, (see + kBlockN - 1) / kBlockN);
   return n <= p.partBlocks;
 }
 // 32 columns of a row's partial result, normalised by the row sum of its key range
@@ -571,18 +625,123 @@ __device__ __forceinline__ void store_part(const TcPartParams& p, const WorkPart
 // Mode 3 is for calls that leave SMs idle otherwise: 2 x 8 query rows x 12289 keys, 32 heads over 8 of 128, 16 CTAs and 150
 // us whole, 144 CTAs and 36 us in nine ranges (19 us of key blocks, the rest launch, first loads and the combine kernel).
 constexpr int kModeFixed = 0, kModeVarlen = 1, kModeFixedNoMask = 2, kModeFixedSplit = 3;
-template <int kMode>
+template <int kMode, int kScore = 0>
 struct ParamsOf {
   using type = typename std::conditional<kMode == kModeFixedSplit, TcPartParams, TcParams>::type;
 };
+template <int kMode>
+struct ParamsOf<kMode, 1> {
+  using type = typename std::conditional<kMode == kModeFixedSplit, TcScorePartParams, TcScoreParams>::type;
+};
+// kScore: 0, or kScoreMask (masks by prefix, document and query offset) with kScoreCap and kScoreBias.  Instantiations of their own:
+// the cap is two more MUFU operations on every score, in kernels that the exponentials bound already.
+constexpr int kScoreMask = 1, kScoreCap = 2, kScoreBias = 4;
+// What a softmax thread keeps of its query row in a scored call.
+template <int kScore>
+struct ScoreRow {
+  int last;        // last key that the causal mask (with the prefix) leaves to the row
+  int seenByAll;   // ... to every row of the tile
+  int pos;         // position of the row
+  int doc;         // its document; below zero: none
+  float slope;     // log2(e) x slope of its head
+  float capArg, capLog2;
+  const int* docKV;
+  const int2* keyBlocks;
+
+  template <class P>
+  __device__ __forceinline__ void begin(const P& p, const Work& w, int qpos, int head, int qlo) {
+    pos = p.qStart + qpos;
+    last = pos;
+    seenByAll = p.qStart + qlo;
+    const int b = (p.prefix != nullptr || p.docKV != nullptr) ? (int)(w.qRow0 / w.sq) : 0;
+    if (p.prefix != nullptr) {
+      last = max(last, p.prefix[b] - 1);
+      seenByAll = max(seenByAll, p.prefix[b] - 1);
+    }
+    doc = -1;
+    if (p.docKV != nullptr) {
+      docKV = p.docKV + (long long)b * w.skv;
+      keyBlocks = p.keyBlocks + (long long)b * ((w.skv + kBlockN - 1) / kBlockN);
+      if (qpos < w.sq) doc = p.docQ[w.qRow0 + qpos];
+    }
+    if constexpr ((kScore & kScoreBias) != 0) slope = qpos < w.sq ? p.slopes[head] * 1.44269504f : 0.f;
+    if constexpr ((kScore & kScoreCap) != 0) {
+      capLog2 = p.cap * 1.44269504f;
+      capArg = 2.f * p.scaleLog2 / p.cap;
+    }
+  }
+
+  // Scores of a key block -> capped and biased, times log2(e).  c tanh(x) = c - 2 c / (e^2x + 1): off by about 2^-23 c whatever x is, which is
+  // what the exponential behind it sees.
+  template <class P>
+  __device__ __forceinline__ void transform(const P& p, uint32_t (&v)[4][32], int kbase) const {
+    if constexpr ((kScore & (kScoreCap | kScoreBias)) != 0) {
+      const float2 step = make_float2(2.f, 2.f);
+      float2 d = make_float2((float)(kbase - pos), (float)(kbase - pos + 1));  // key - position: exact up to 2^24
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float2 x = make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
+          if constexpr ((kScore & kScoreCap) != 0) {
+            x = fmul2(x, make_float2(capArg, capArg));
+            x.x = rcp(ex2(x.x) + 1.f);
+            x.y = rcp(ex2(x.y) + 1.f);
+            x = ffma2(x, make_float2(-2.f * capLog2, -2.f * capLog2), make_float2(capLog2, capLog2));
+          } else {
+            x = fmul2(x, make_float2(p.scaleLog2, p.scaleLog2));
+          }
+          if constexpr ((kScore & kScoreBias) != 0) {
+            x = ffma2(make_float2(fabsf(d.x), fabsf(d.y)), make_float2(-slope, -slope), x);
+            d = fadd2(d, step);
+          }
+          v[q][i] = __float_as_uint(x.x);
+          v[q][i + 1] = __float_as_uint(x.y);
+        }
+      }
+    }
+  }
+
+  // Keys of other documents.  Most blocks hold one document (smallest id = largest id) and are seen whole or not at all.
+  template <class P>
+  __device__ __forceinline__ void documents(const P& p, uint32_t (&v)[4][32], int kbase, int skv) const {
+    if (p.docKV == nullptr) return;
+    const int2 ids = keyBlocks[kbase / kBlockN];
+    const bool one = ids.x == ids.y;
+    if (__all_sync(0xffffffffu, one && doc >= 0 && ids.x == doc)) return;
+    uint32_t see[4] = {0u, 0u, 0u, 0u};
+    if (one) {
+      if (doc >= 0 && ids.x == doc) see[0] = see[1] = see[2] = see[3] = 0xffffffffu;
+    } else if (doc >= 0) {
+      const int n = min(kBlockN, skv - kbase);
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        uint32_t bits = 0u;
+#pragma unroll 8
+        for (int i = 0; i < 32; i++) {
+          if (q * 32 + i < n && docKV[kbase + q * 32 + i] == doc) bits |= 1u << i;
+        }
+        see[q] = bits;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+#pragma unroll
+      for (int i = 0; i < 32; i++) {
+        if ((see[q] >> i & 1u) == 0u) v[q][i] = 0xff800000u;
+      }
+    }
+  }
+};
+
 // kHD: the head dim the MMAs are shaped for.  The tiles in shared memory are always HDP wide (64-element slabs, TMA
 // zero-fills past the true head dim); with kHD < HDP (32 in the 64-wide kernel, 96 in the 128-wide one) Q.K^T stops
 // after kHD / 16 k-steps, P.V produces kHD output columns, and the rescale and output passes touch kHD columns.
 // kPair: the CTA-pair form of head dims 192 / 256 (CfgPair): launched as clusters of two, fixed-length input only.
-template <int HDP, bool kBf16, int kMode, bool kSolo = false, int kHD = HDP, bool kPair = false>
+template <int HDP, bool kBf16, int kMode, bool kSolo = false, int kHD = HDP, bool kPair = false, int kScore = 0>
 __global__ void __launch_bounds__(kSolo ? kThreadsSolo : kThreads, kSolo ? 2 : 1)
 fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-              const __grid_constant__ CUtensorMap tmV, const typename ParamsOf<kMode>::type p) {
+              const __grid_constant__ CUtensorMap tmV, const typename ParamsOf<kMode, (kScore != 0)>::type p) {
   static_assert(!kSolo || HDP == 64 || (HDP == 128 && kMode == kModeFixedSplit),
                 "the one-tile, two-CTAs-per-SM form exists for padded head dim 64, and at 128 for key ranges");
   static_assert(kHD == HDP || (HDP == 64 && kHD == 32) || (HDP == 128 && kHD == 96), "MMA head dim");
@@ -716,7 +875,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 
   // Every consumer of work items (8 softmax warps, 4 epilogue warps, 2 MMA threads) reads item k from slot k & 1
   // and frees the slot; a negative index ends the loop.
-  using WorkT = typename std::conditional<kSplit, WorkPart, Work>::type;
+  using WorkT = typename std::conditional<kSplit || kScore != 0, WorkPart, Work>::type;
   auto fetchWork = [&](int k, WorkT& w) -> int {
     wait_bar(bar(kBarWorkFull + (k & 1)), (k >> 1) & 1, wc, 20);
     // plain loads: the barrier wait above is an acquire and a compiler-level memory fence, and fields that a role
@@ -731,7 +890,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     w.nblk[0] = ws->nblk[0];
     w.nblk[1] = ws->nblk[1];
     w.nmax = ws->nmax;
-    if constexpr (kSplit) w.part = ws->part;
+    if constexpr (kSplit || kScore != 0) w.part = ws->part;
     return ws->idx;
   };
 
@@ -741,7 +900,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const int t = warp >> 2;
     const int r = threadIdx.x & 127;
     const uint32_t tRegion = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(t * C::kSRegion);
-    const float c = p.scaleLog2;
+    // scores that are capped or biased become multiples of log2(e) on the way, the others in the exponent
+    const float c = (kScore & (kScoreCap | kScoreBias)) != 0 ? 1.f : p.scaleLog2;
     int it = 0;      // blocks of this tile processed so far, over all work items (phase of the per-block barriers)
     int items = 0;   // work items in which this tile was active
     int ldBase = 0;  // K/V ring loads of all earlier items (packed variable-length input only, see below)
@@ -759,6 +919,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       const int qpos = w.qlo[t] + (r >> p.packShift);
       float m = -INFINITY, l = 0.f;
       const int n = w.nblk[t];
+      [[maybe_unused]] ScoreRow<kScore> row;
+      if constexpr (kScore != 0) row.begin(p, w, qpos, (w.unit << p.packShift) + (r & ((1 << p.packShift) - 1)), w.qlo[t]);
       for (int j = 0; j < n; j++, it++) {
         if constexpr (kRingSig) {  // ring order K0 | K1 V0 | K2 V1 | ...: K of block j is load 2 j - 1 of the item (K0: 0)
           const int g = ldItem + (j == 0 ? 0 : 2 * j - 1);
@@ -784,11 +946,14 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 
         int kbase = j * kBlockN;
         if constexpr (kSplit) kbase += w.part * p.partBlocks * kBlockN;
-        const bool needMask = (kMode != kModeFixedNoMask) &&
-                              ((kbase + kBlockN > w.skv) || (p.causal && (kbase + kBlockN - 1 > w.qlo[t])));
+        if constexpr (kScore != 0 && !kSplit) kbase += w.part * kBlockN;
+        if constexpr (kScore != 0) row.transform(p, v, kbase);
+        bool needMask = (kMode != kModeFixedNoMask) &&
+                        ((kbase + kBlockN > w.skv) || (p.causal && (kbase + kBlockN - 1 > (kScore != 0 ? row.seenByAll : w.qlo[t]))));
+        if constexpr (kScore != 0) row.documents(p, v, kbase, w.skv);
         if (needMask) {
           int lim = w.skv - kbase;                         // columns [0, lim) are real keys
-          if (p.causal) lim = min(lim, qpos - kbase + 1);  // ... that are not in the future
+          if (p.causal) lim = min(lim, (kScore != 0 ? row.last : qpos) - kbase + 1);  // ... that are not in the future
 #pragma unroll
           for (int q = 0; q < 4; q++) {
 #pragma unroll
@@ -921,6 +1086,12 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           ptx::tmem_ld_32x32b_x32(tO + ch * 32, o);
           ptx::tmem_wait_ld();
           ptx::tmem_ld_fence(o);
+          if constexpr (kScore != 0) {  // a row that sees no key is zero even where 0 times a value is not
+            if (l == 0.f) {
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] = 0u;
+            }
+          }
           if (ch == kHD / 32 - 1) {
             ptx::tc_fence_before();
             __syncwarp();
@@ -1003,6 +1174,12 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           ptx::tmem_ld_32x32b_x32(tO + ch * 32, o);
           ptx::tmem_wait_ld();
           ptx::tmem_ld_fence(o);
+          if constexpr (kScore != 0) {  // a row that sees no key is zero even where 0 times a value is not
+            if (l == 0.f) {
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] = 0u;
+            }
+          }
           if (ch == kHD / 32 - 1) {  // O is in registers: the next item's first P.V may overwrite the accumulator
             ptx::tc_fence_before();
             __syncwarp();
@@ -1330,7 +1507,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         ws->nblk[0] = w.nblk[0];
         ws->nblk[1] = w.nblk[1];
         ws->nmax = w.nmax;
-        if constexpr (kSplit) ws->part = w.part;
+        if constexpr (kSplit || kScore != 0) ws->part = w.part;
         ptx::mbar_arrive(bar(kBarWorkFull + (k & 1)));  // release: the stores above are visible to whoever waits
         return idx >= 0;
       };
@@ -1339,6 +1516,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       // and a key range that turns out empty - causal - takes its next index from the counter: both wait first.)
       bool early = !kVarlen;
       if constexpr (kSplit) early = !p.causal || p.numItems == p.numWork;
+      if constexpr (kScore != 0) early = early && p.prefix == nullptr && p.tileRange == nullptr;
       if (!early) ptx::grid_wait_previous();
       bool more = publish(0);
       if (early) ptx::grid_wait_previous();
@@ -1413,6 +1591,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           const CUtensorMap* tm = isV ? mapV : mapK;
           int row = w.kvRowTma + blkIdx * kBlockN;
           if constexpr (kSplit) row += w.part * p.partBlocks * kBlockN;
+          if constexpr (kScore != 0 && !kSplit) row += w.part * kBlockN;
           if constexpr (kPair) {
             // This CTA's half of the block, counted on rank 0's barrier together with the other half.
             // K: keys [64 rank, 64 rank + 64), all of the head dim (the K map's box is 64 rows high);

@@ -21,6 +21,8 @@ enum Status : int {
 // dtype codes follow the reference binding (reference csrc/binding/flash_attn_binding.cu:22).
 enum DType : int { kFp16 = 1, kBf16 = 2, kFp32 = 3 };
 
+struct ScoreFields;  // score.cuh
+
 // One attention-forward problem, fixed-length or packed variable-length.
 // Layouts (reference csrc/flash_attn/params.cuh:49-68, 97-116):
 //   fixed : Q,O [B,Sq,Hq,D]   K,V [B,Skv,Hkv,D]        cuQ == cuKV == nullptr
@@ -49,6 +51,7 @@ struct FwdProblem {
   const int* gate = nullptr;
   int gateEpoch = 0;
   bool overlap = false;  // launch with programmatic stream serialization (launch_kernel below); not under stream capture
+  const ScoreFields* score = nullptr;  // capped, biased or masked scores (fixed length)
 };
 
 // How the split-KV path cuts a call (fwd_decode.cu): `runs` equal runs over the key blocks of all batch entries, or, with
@@ -106,5 +109,6 @@ int validate_common(const void* Q, const void* K, const void* V, void* O, int dt
                     int hkv, int d);
 bool may_overlap(cudaStream_t stream);  // c_abi.cu: false under stream capture
 int check_device();  // current device must be compute capability 10.x
+int scratch_alloc(void** ptr, size_t bytes, int device, cudaStream_t stream);  // c_abi.cu: stream-ordered, from the library's pool; cudaFreeAsync
 
 }  // namespace tfa_b200
