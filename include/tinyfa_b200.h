@@ -118,6 +118,7 @@ int tfa_b200_device_status(int* site);
  *                      auto (head dim 256: non-causal, and causal from 1024 query rows; head dim 192: never, its
  *                      one-tile form measures as fast) / never / wherever it applies.  Results are bit-identical to
  *                      the one-tile form.
+ *   "cache_tc" -1/0/1  attention over the paged cache: tensor cores (tiles of 128 query rows) by size / never / always
  *   "work_order" -1/0/n  order in which the persistent kernel hands out (query tile pair, head, batch) items:
  *                      auto (causal: heaviest pairs first inside chunks of heads whose K/V fit a quarter of L2;
  *                      otherwise pair index fastest) / pair index fastest / heaviest first in chunks of n heads

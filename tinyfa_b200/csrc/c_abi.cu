@@ -90,6 +90,9 @@ int option_fp32_t8() { return g_optFp32T8.load(); }
 static std::atomic<int> g_optSplitTc{-1};  // tensor-core path, key ranges: -1 by size, 0 never, n > 0 exactly n
 static std::atomic<int> g_optFp32Tc{-1};  // fp32 on the tensor cores: -1 by size, 0 never, 1 wherever it applies
 
+static std::atomic<int> g_optCacheTc{-1};  // attention over the paged cache: tensor-core form -1 by size, 0 never, 1 always
+int option_cache_tc() { return g_optCacheTc.load(); }
+
 int next_epoch() { return (g_epoch.fetch_add(1) & 0x7FFFFF) + 1; }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -810,6 +813,10 @@ extern "C" int tfa_b200_set_option(const char* name, int value) {
   }
   if (strcmp(name, "fp32_tc") == 0) {
     g_optFp32Tc.store(value < 0 ? -1 : (value ? 1 : 0));
+    return kOk;
+  }
+  if (strcmp(name, "cache_tc") == 0) {
+    g_optCacheTc.store(value < 0 ? -1 : (value ? 1 : 0));
     return kOk;
   }
   if (strcmp(name, "pair_cta") == 0) {

@@ -25,6 +25,9 @@
 
 #include "../../include/tinyfa_b200.h"
 #include "build_config.cuh"
+#include "cache_codes.cuh"
+#include "cta_scan.cuh"
+#include "fwd_tc.cuh"
 #include "ptx_sm100.cuh"
 #include "tfa_common.cuh"
 
@@ -32,6 +35,35 @@ namespace tfa_b200 {
 
 int device_num_sms(int device);  // c_abi.cu
 int* device_join_counters(int device, cudaStream_t stream, int* rc);  // c_abi.cu
+int* device_status_word(int device);
+int next_epoch();
+int option_cache_tc();
+
+#define TFA_DECLARE_CACHE(HDP)                                                                              \
+  int launch_fwd_cache_hdp##HDP##_bf0(const TcCacheParams&, int, bool, int, cudaStream_t);                  \
+  int launch_fwd_cache_hdp##HDP##_bf1(const TcCacheParams&, int, bool, int, cudaStream_t);                  \
+  static inline int cache_call_hdp##HDP(const TcCacheParams& p, bool bf16, int ctas, bool overlap, int device, cudaStream_t s) { \
+    (void)p; (void)ctas; (void)overlap; (void)device; (void)s;                                              \
+    if (bf16) {                                                                                             \
+      if constexpr (TFA_HAVE_BF16) return launch_fwd_cache_hdp##HDP##_bf1(p, ctas, overlap, device, s);      \
+    } else {                                                                                                \
+      if constexpr (TFA_HAVE_FP16) return launch_fwd_cache_hdp##HDP##_bf0(p, ctas, overlap, device, s);      \
+    }                                                                                                       \
+    return kBadDtype;                                                                                       \
+  }
+#if TFA_HAVE_HDP64
+TFA_DECLARE_CACHE(64)
+#endif
+#if TFA_HAVE_HDP128
+TFA_DECLARE_CACHE(128)
+#endif
+#if TFA_HAVE_HDP192
+TFA_DECLARE_CACHE(192)
+#endif
+#if TFA_HAVE_HDP256
+TFA_DECLARE_CACHE(256)
+#endif
+#undef TFA_DECLARE_CACHE
 
 namespace cache {
 
@@ -122,21 +154,6 @@ __device__ __forceinline__ float rcp(float x) {
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
-}
-
-// Four codes of a word -> two pairs of halves, exactly.  int8: 0x6400 | (code ^ 0x80) is 1024 + 128 + code.
-template <bool kInt8>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (kInt8) {
-    w ^= 0x80808080u;
-    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  } else {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-  }
 }
 
 // kWords consecutive words of a lane from shared memory, in the widest loads that its alignment (kAlign bytes) allows.
@@ -396,7 +413,6 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
         qf[w][3] = validB ? b.y : 0u;
       }
       if constexpr (kBf16) {
-        // largest exponent of the row -> the power of two that brings its largest element into [2^13, 2^14)
         uint32_t ma = 0, mb = 0;
 #pragma unroll
         for (int w = 0; w < D / 16; w++) {
@@ -407,21 +423,17 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
         ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 2));
         mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
         mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
-        // exponent field e of the row's maximum: the factor is 2^(13 - (e - 127)); kept inside what a float's exponent holds
-        const int ea = min(max((int)(ma >> 7), 14), 253), eb = min(max((int)(mb >> 7), 14), 253);
-        const float upA = __int_as_float((267 - ea) << 23), upB = __int_as_float((267 - eb) << 23);  // 2^(140 - e), e - 127 = exponent
-        const float dnA = __int_as_float((ea - 13) << 23), dnB = __int_as_float((eb - 13) << 23);
+        float upA, upB, dnA, dnB;
+        row_scale(ma, upA, dnA);
+        row_scale(mb, upB, dnB);
         facA *= dnA;
         facB *= dnB;
-        auto conv = [](uint32_t x, float f) {
-          return half2_of(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xFFFF0000u) * f);
-        };
 #pragma unroll
         for (int w = 0; w < D / 16; w++) {
-          qf[w][0] = conv(qf[w][0], upA);
-          qf[w][1] = conv(qf[w][1], upB);
-          qf[w][2] = conv(qf[w][2], upA);
-          qf[w][3] = conv(qf[w][3], upB);
+          qf[w][0] = bf16_to_half2(qf[w][0], upA);
+          qf[w][1] = bf16_to_half2(qf[w][1], upB);
+          qf[w][2] = bf16_to_half2(qf[w][2], upA);
+          qf[w][3] = bf16_to_half2(qf[w][3], upB);
         }
       }
     }
@@ -772,6 +784,176 @@ int dispatch(Params& p, int headDim, bool int8, bool bf16, int runs, int device,
   }
 }
 
+// ------------------------------------------------------------------------------------------- many query rows: tensor cores
+struct UnitParams {
+  uint4* O;
+  const int* cuQ;
+  const int* lens;
+  int batch, capacity, totalQ, group, causal, unitRows, rowChunks;
+  int maxUnits;  // room for them: enough where cuQ does not decrease
+  int* numUnits;
+  int* unitBase;  // [batch + 1]
+  long long* unitStart;
+  int2* unitWhat;
+};
+
+// CTA 0: the units of a KV head (up to unitRows flat rows of a request each) and the key blocks ahead of each, by two prefix sums.  The
+// others: zeros in the rows that no unit has, those of a request without tokens (CTA b + 1) and of no request (the last).
+__global__ void __launch_bounds__(1024) cache_units_kernel(const UnitParams p) {
+  __shared__ long long sWarp[32];
+  ptx::grid_wait_previous();
+  ptx::grid_allow_next();
+  auto request = [&](int b, int& q0, int& nq, int& len) {
+    q0 = min(max(p.cuQ[b], 0), p.totalQ);
+    nq = min(max(p.cuQ[b + 1] - q0, 0), p.totalQ - q0);
+    len = min(max(p.lens[b], 0), p.capacity);
+  };
+  if (blockIdx.x > 0) {
+    const int b = (int)blockIdx.x - 1;
+    auto zero = [&](int r0, int r1) {
+      for (long long i = (long long)r0 * p.rowChunks + threadIdx.x; i < (long long)r1 * p.rowChunks; i += 1024) p.O[i] = make_uint4(0, 0, 0, 0);
+    };
+    if (b == p.batch) {
+      zero(0, min(max(p.cuQ[0], 0), p.totalQ));
+      zero(min(max(p.cuQ[p.batch], 0), p.totalQ), p.totalQ);
+    } else {
+      int q0, nq, len;
+      request(b, q0, nq, len);
+      if (len == 0) zero(q0, q0 + nq);
+    }
+    return;
+  }
+  long long units = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 1024) {
+    const int b = b0 + threadIdx.x;
+    int q0, nq = 0, len = 0;
+    if (b < p.batch) request(b, q0, nq, len);
+    const long long n = len > 0 ? ((long long)nq * p.group + p.unitRows - 1) / p.unitRows : 0;
+    long long sum;
+    const long long upto = cta_scan(n, sWarp, sum);
+    if (b < p.batch) p.unitBase[b] = (int)min(units + upto - n, (long long)p.maxUnits);
+    units += sum;
+  }
+  units = min(units, (long long)p.maxUnits);
+  if (threadIdx.x == 0) {
+    p.unitBase[p.batch] = (int)units;
+    *p.numUnits = (int)units;
+  }
+  __syncthreads();
+  long long blocks = 0;
+  for (long long u0 = 0; u0 < units; u0 += 1024) {
+    const long long u = u0 + threadIdx.x;
+    long long n = 0;
+    if (u < units) {
+      int lo = 0, hi = p.batch - 1;  // the request b with unitBase[b] <= u < unitBase[b + 1]
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (u < p.unitBase[mid + 1]) {
+          hi = mid;
+        } else {
+          lo = mid + 1;
+        }
+      }
+      int q0, nq, len;
+      request(lo, q0, nq, len);
+      const int flat = (int)(u - p.unitBase[lo]) * p.unitRows;
+      n = (len + tc::kBlockN - 1) / tc::kBlockN;
+      if (p.causal) {
+        const int last = (min(flat + p.unitRows, nq * p.group) - 1) / p.group;  // token of the unit's last row
+        n = min(n, (long long)max(1, (len - nq + last + tc::kBlockN) / tc::kBlockN));
+      }
+      p.unitWhat[u] = make_int2(lo, flat);
+    }
+    long long sum;
+    const long long upto = cta_scan(n, sWarp, sum);
+    if (u < units) p.unitStart[u] = blocks + upto - n;
+    blocks += sum;
+  }
+  if (threadIdx.x == 0) p.unitStart[units] = blocks;
+}
+
+int run_tc(const TcCacheParams& p, bool bf16, int ctas, bool overlap, int device, cudaStream_t s) {
+  switch (p.headDim) {
+#if TFA_HAVE_HDP64
+    case 32:
+    case 64: return cache_call_hdp64(p, bf16, ctas, overlap, device, s);
+#endif
+#if TFA_HAVE_HDP128
+    case 96:
+    case 128: return cache_call_hdp128(p, bf16, ctas, overlap, device, s);
+#endif
+#if TFA_HAVE_HDP192
+    case 192: return cache_call_hdp192(p, bf16, ctas, overlap, device, s);
+#endif
+#if TFA_HAVE_HDP256
+    case 256: return cache_call_hdp256(p, bf16, ctas, overlap, device, s);
+#endif
+    default: return kBadHeadDim;
+  }
+}
+
+int dispatch_tc(const Params& d, int headDim, bool int8, bool bf16, int device, cudaStream_t s) {
+  const int tiles = headDim <= 128 ? 2 : 1, unitRows = tiles * tc::kBlockM;
+  const int ctas = device_num_sms(device);
+  int rc = kOk;
+  TcCacheParams p = {};
+  p.join = device_join_counters(device, s, &rc);
+  if (p.join == nullptr) return rc;
+  const size_t maxUnits = (size_t)((long long)d.totalQ * d.group / unitRows) + d.batch;
+  const size_t parts = (size_t)ctas * 2 * tiles * tc::kBlockM;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  const size_t oBytes = up(parts * headDim * sizeof(float)), lseBytes = up(parts * sizeof(float)), startBytes = up((maxUnits + 1) * sizeof(long long)),
+               whatBytes = up((maxUnits + 1) * sizeof(int2)), baseBytes = up((size_t)(d.batch + 1) * sizeof(int));
+  void* scratch = nullptr;
+  rc = scratch_alloc(&scratch, oBytes + lseBytes + startBytes + whatBytes + baseBytes + 256, device, s);
+  if (rc != kOk) return rc;
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  p.partO = reinterpret_cast<float*>(at);
+  p.partLse = reinterpret_cast<float*>(at += oBytes);
+  long long* unitStart = reinterpret_cast<long long*>(at += lseBytes);
+  int2* unitWhat = reinterpret_cast<int2*>(at += startBytes);
+  int* unitBase = reinterpret_cast<int*>(at += whatBytes);
+  int* numUnits = reinterpret_cast<int*>(at += baseBytes);
+  UnitParams u = {static_cast<uint4*>(d.O), d.cuQ, d.lens, d.batch, d.width << d.blockShift, d.totalQ, d.group, d.causal, unitRows, d.headsQ * headDim / 8,
+                  (int)maxUnits, numUnits, unitBase, unitStart, unitWhat};
+  const bool overlap = may_overlap(s);
+  cudaError_t e = launch_kernel(cache_units_kernel, dim3((unsigned)d.batch + 2), 1024, 0, s, overlap, u);
+  if (e != cudaSuccess) {
+    set_error_string("cache unit kernel launch failed: %s", cudaGetErrorString(e));
+    rc = kCudaError;
+  }
+  if (rc == kOk) {
+    p.O = d.O;
+    p.Q = d.Q;
+    p.cuQ = d.cuQ;
+    p.seqLenQ = d.totalQ;
+    p.headsQ = d.headsQ;
+    p.headsKV = d.headsKV;
+    p.headDim = headDim;
+    p.group = d.group;
+    p.causal = d.causal;
+    p.scaleLog2 = d.scaleLog2;
+    p.status = device_status_word(device);
+    p.epoch = next_epoch();
+    p.cap = d.cap;
+    p.slopes = d.slopes;
+    p.codes[0] = d.kCodes, p.codes[1] = d.vCodes;
+    p.scales[0] = d.kScales, p.scales[1] = d.vScales;
+    p.table = d.table;
+    p.lens = d.lens;
+    p.width = d.width;
+    p.numBlocks = d.numBlocks;
+    p.blockShift = d.blockShift;
+    p.int8 = int8 ? 1 : 0;
+    p.numUnits = numUnits;
+    p.unitStart = unitStart;
+    p.unitWhat = unitWhat;
+    rc = p.status == nullptr ? kCudaError : run_tc(p, bf16, ctas, overlap, device, s);
+  }
+  cudaFreeAsync(scratch, s);
+  return rc;
+}
+
 }  // namespace cache
 }  // namespace tfa_b200
 
@@ -838,6 +1020,10 @@ extern "C" int tfa_b200_fwd_cache(const void* Q, void* O, const void* kCache, co
   p.totalQ = (int)totalQ;
   p.scaleLog2 = (float)(1.4426950408889634 / sqrt((double)headDim));
   p.cap = softcap;
+  const bool int8 = cacheType == TFA_B200_CACHE_INT8, bf16 = dtype == kBf16;
+  const int tcOption = option_cache_tc();
+  const long long rowsMost = (long long)maxSeqLenQ * p.group;  // query rows of a request that share a KV head
+  if (tcOption > 0 || (tcOption < 0 && rowsMost > 4 * kRows)) return dispatch_tc(p, headDim, int8, bf16, device, s);
   // as many runs as the GPU holds CTAs, and no more than there can be pairs of key blocks
   const long long slots = (long long)device_num_sms(device) * ctas_per_sm(headDim);
   const long long tiles = ((long long)(maxSeqLenQ > 0 ? maxSeqLenQ : 1) * p.group + kRows - 1) / kRows;
@@ -858,7 +1044,7 @@ extern "C" int tfa_b200_fwd_cache(const void* Q, void* O, const void* kCache, co
     p.partO = static_cast<float*>(scratch);
     p.partLse = p.partO + rows * headDim;
   }
-  rc = cache::dispatch(p, headDim, cacheType == TFA_B200_CACHE_INT8, dtype == kBf16, p.runs, device, s);
+  rc = cache::dispatch(p, headDim, int8, bf16, p.runs, device, s);
   if (scratch != nullptr) cudaFreeAsync(scratch, s);
   return rc;
 }

@@ -35,6 +35,7 @@
 
 #include <type_traits>
 
+#include "cache_codes.cuh"
 #include "ptx_sm100.cuh"
 #include "score.cuh"
 #include "tfa_common.cuh"
@@ -81,6 +82,24 @@ struct TcPartParams : TcParams {
 // ... and of a call whose scores are capped, biased or masked by prefix or document (score.cuh), whole or cut into key ranges.
 struct TcScoreParams : TcParams, ScoreFields {};
 struct TcScorePartParams : TcPartParams, ScoreFields {};
+
+// ... and of packed queries over the paged 8-bit cache.  cuQ: rows of the requests; group query heads of a KV head and the tokens of a
+// request together make flat rows, 128 to a tile, the tiles of a CTA to a unit.
+struct TcCacheParams : TcParams, ScoreFields {
+  const void* Q;
+  const uint8_t* codes[2];    // K, V [numBlocks][headsKV][1 << blockShift][headDim]
+  const float* scales[2];     // [numBlocks][headsKV]
+  const int* table;           // [batch][width]
+  const int* lens;            // [batch]
+  int width, numBlocks, blockShift, int8;
+  // the units of one KV head, in order (cache_units_kernel): how many, key blocks ahead of each, request and first flat row
+  const int* numUnits;
+  const long long* unitStart;  // [units + 1]
+  const int2* unitWhat;        // [units]
+  float* partO;                // [CTAs][2][tiles][headDim / 4][128] float4, normalised
+  float* partLse;              // [CTAs][2][tiles][128]
+  int* join;                   // [CTAs][2], zero
+};
 
 namespace tc {
 
@@ -576,7 +595,7 @@ __device__ __forceinline__ bool make_work(const P& p, int idx, W& w) {
       w.nmax = max(w.nmax, n);
     }
     return w.nmax > 0;
-  }
+  } else {
 #pragma unroll
   for (int t = 0; t < 2; t++) {
     w.qlo[t] = seq0 + t * rows;
@@ -591,6 +610,7 @@ __device__ __forceinline__ bool make_work(const P& p, int idx, W& w) {
   }
   if constexpr (kSplit) return w.nmax > 0;
   return true;
+  }
 }
 
 // Does a tile's whole key range fit its first part?  Such rows (the early ones of a causal problem) get their final output
@@ -624,10 +644,17 @@ __device__ __forceinline__ void store_part(const TcPartParams& p, const WorkPart
 // the 64 kernel), 3 fixed length with every item cut into key ranges (few query tiles, long keys).
 // Mode 3 is for calls that leave SMs idle otherwise: 2 x 8 query rows x 12289 keys, 32 heads over 8 of 128, 16 CTAs and 150
 // us whole, 144 CTAs and 36 us in nine ranges (19 us of key blocks, the rest launch, first loads and the combine kernel).
-constexpr int kModeFixed = 0, kModeVarlen = 1, kModeFixedNoMask = 2, kModeFixedSplit = 3;
+// 4: packed queries over the paged 8-bit cache.  The four epilogue warps (one tile per CTA: eight) turn pages into fp16 tiles in shared
+// memory where the loading thread issues TMA copies otherwise, the softmax warps write the output, and the work is cut statically into one
+// run of key blocks per CTA over all (head, unit) pairs.
+constexpr int kModeFixed = 0, kModeVarlen = 1, kModeFixedNoMask = 2, kModeFixedSplit = 3, kModeCache = 4;
 template <int kMode, int kScore = 0>
 struct ParamsOf {
   using type = typename std::conditional<kMode == kModeFixedSplit, TcPartParams, TcParams>::type;
+};
+template <>
+struct ParamsOf<kModeCache, 1> {
+  using type = TcCacheParams;
 };
 template <int kMode>
 struct ParamsOf<kMode, 1> {
@@ -702,6 +729,39 @@ struct ScoreRow {
     }
   }
 
+  // The same for codes: kf, by groups of 16 keys, is the scale of the keys x the row's factor (capped: of the argument 2 x log2(e)), and one
+  // from here on where the scores have been worked out.
+  __device__ __forceinline__ void cache_transform(uint32_t (&v)[4][32], int kbase, float (&kf)[8]) const {
+    if constexpr ((kScore & (kScoreCap | kScoreBias)) != 0) {
+      const float2 step = make_float2(2.f, 2.f);
+      float2 d = make_float2((float)(kbase - pos), (float)(kbase - pos + 1));
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float f = kf[q * 2 + i / 16];
+          float2 x = fmul2(make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1])), make_float2(f, f));
+          if constexpr ((kScore & kScoreCap) != 0) {
+            const bool gone0 = v[q][i] == 0xff800000u, gone1 = v[q][i + 1] == 0xff800000u;  // the key's block does not exist
+            x.x = rcp(ex2(x.x) + 1.f);
+            x.y = rcp(ex2(x.y) + 1.f);
+            x = ffma2(x, make_float2(-2.f * capLog2, -2.f * capLog2), make_float2(capLog2, capLog2));
+            if (gone0) x.x = -INFINITY;
+            if (gone1) x.y = -INFINITY;
+          }
+          if constexpr ((kScore & kScoreBias) != 0) {
+            x = ffma2(make_float2(fabsf(d.x), fabsf(d.y)), make_float2(-slope, -slope), x);
+            d = fadd2(d, step);
+          }
+          v[q][i] = __float_as_uint(x.x);
+          v[q][i + 1] = __float_as_uint(x.y);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) kf[i] = 1.f;
+    }
+  }
+
   // Keys of other documents.  Most blocks hold one document (smallest id = largest id) and are seen whole or not at all.
   template <class P>
   __device__ __forceinline__ void documents(const P& p, uint32_t (&v)[4][32], int kbase, int skv) const {
@@ -734,6 +794,105 @@ struct ScoreRow {
   }
 };
 
+// ---- kModeCache
+// Shared memory behind Ctl.  Scales of a key block stay in a ring of eight blocks, well past the ring of tiles; row factors in a ring of
+// four items: the Q tile of item k + 4 is written when Q.K^T of item k + 3 has finished, which follows P.V of item k + 1 at least, hence
+// the softmax of item k + 1.
+struct CacheSegment {  // what the loading thread publishes beside a WorkSlot
+  int b;           // request
+  int slot;        // 2 x CTA + (0: first segment of the CTA's run, 1: a later one)
+  int c0, c1;      // CTAs that share the unit
+  int at0;         // slot parity of the unit's part in c0
+};
+struct CacheCtl {
+  uint64_t scaleFull[8];
+  float scales[8][16];  // of the eight 16-key groups of a block: K (below zero: the block does not exist), V
+  float rowFactor[4][2][kBlockM];
+  CacheSegment seg[2];
+  int last[2];
+};
+constexpr int kCacheSmem = 5120;
+static_assert(sizeof(CacheCtl) <= kCacheSmem, "shared memory of the cache form");
+// Weights of V relative to the scale of V that O refers to, times 2^3: a weight is at most 2^8 (lazy rescale), scales at most 2^4 above the
+// reference, so fp16's 2^16 is not reached.
+constexpr float kCacheUp = 8.f, kCacheSlack = 16.f;
+
+// 32 columns of a row's output
+template <bool kBf16, class P, class W>
+__device__ __forceinline__ void cache_store(const P& p, const W& w, int flat, int ch, const uint32_t (&o)[32], float inv) {
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.O) +
+                                        ((w.qRow0 + flat / p.group) * p.headsQ + w.unit * p.group + flat % p.group) * (long long)p.headDim);
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    uint4 q;
+    q.x = pack2<kBf16>(__uint_as_float(o[g * 8 + 0]) * inv, __uint_as_float(o[g * 8 + 1]) * inv);
+    q.y = pack2<kBf16>(__uint_as_float(o[g * 8 + 2]) * inv, __uint_as_float(o[g * 8 + 3]) * inv);
+    q.z = pack2<kBf16>(__uint_as_float(o[g * 8 + 4]) * inv, __uint_as_float(o[g * 8 + 5]) * inv);
+    q.w = pack2<kBf16>(__uint_as_float(o[g * 8 + 6]) * inv, __uint_as_float(o[g * 8 + 7]) * inv);
+    dst[ch * 4 + g] = q;
+  }
+}
+
+// The four softmax warps of tile t have stored their part of the unit: if they are the last of the CTAs that share it, they put the parts
+// together, a row per thread (neighbouring rows lie next to one another in a part).
+template <int NT, int kHD, bool kBf16, class W>
+__device__ __forceinline__ void cache_join(const TcCacheParams& p, const W& w, const CacheSegment& seg, CacheCtl* cctl, int t, int r) {
+  __threadfence();
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+  if (r == 0) {
+    int* counter = p.join + 2 * seg.c0 + t;
+    const bool last = atomicAdd(counter, 1) == seg.c1 - seg.c0;
+    if (last) *counter = 0;  // for the next call
+    cctl->last[t] = last;
+    __threadfence();
+  }
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+  if (cctl->last[t] == 0) return;
+  const int flat = w.qlo[t] + r;
+  if (flat >= w.sq) return;
+  auto part = [&](int c) { return (2ll * c + (c == seg.c0 ? seg.at0 : 0)) * NT + t; };
+  float M = -INFINITY;
+  bool nan = false;
+#pragma unroll 4
+  for (int c = seg.c0; c <= seg.c1; c++) {
+    const float lse = __ldcg(p.partLse + part(c) * kBlockM + r);
+    nan = nan || lse != lse;
+    M = fmaxf(M, lse);
+  }
+  if (M == -INFINITY) M = 0.f;
+  if (nan) M = NAN;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int c = seg.c0; c <= seg.c1; c++) sum += ex2(__ldcg(p.partLse + part(c) * kBlockM + r) - M);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+  for (int ch = 0; ch < kHD / 32; ch++) {
+    float acc[32];
+#pragma unroll
+    for (int i = 0; i < 32; i++) acc[i] = 0.f;
+#pragma unroll 1
+    for (int c = seg.c0; c <= seg.c1; c++) {
+      const float wt = ex2(__ldcg(p.partLse + part(c) * kBlockM + r) - M);
+      if (wt == 0.f) continue;  // nothing there
+      const float4* src = reinterpret_cast<const float4*>(p.partO) + (part(c) * (kHD / 4) + ch * 8) * kBlockM + r;
+#pragma unroll
+      for (int g = 0; g < 8; g++) {
+        const float4 x = __ldcg(src + g * kBlockM);
+        acc[g * 4] = fmaf(wt, x.x, acc[g * 4]);
+        acc[g * 4 + 1] = fmaf(wt, x.y, acc[g * 4 + 1]);
+        acc[g * 4 + 2] = fmaf(wt, x.z, acc[g * 4 + 2]);
+        acc[g * 4 + 3] = fmaf(wt, x.w, acc[g * 4 + 3]);
+      }
+    }
+    uint32_t o[32];
+#pragma unroll
+    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(acc[i]);
+    cache_store<kBf16>(p, w, flat, ch, o, inv);
+  }
+}
+
+__device__ __forceinline__ int cache_run_of(long long u, long long total, int runs) { return (int)(((u + 1) * runs - 1) / total); }
+
 // kHD: the head dim the MMAs are shaped for.  The tiles in shared memory are always HDP wide (64-element slabs, TMA
 // zero-fills past the true head dim); with kHD < HDP (32 in the 64-wide kernel, 96 in the 128-wide one) Q.K^T stops
 // after kHD / 16 k-steps, P.V produces kHD output columns, and the rescale and output passes touch kHD columns.
@@ -751,7 +910,9 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                                                                 Cfg<HDP>>::type>::type;
   constexpr int NT = C::kNT;
   // warp roles: softmax warps [0, 4 * NT'), epilogue warps, the two MMA-issuing warps, the loading warp
-  constexpr int kSoftmaxWarps = kSolo ? 4 : 8;
+  constexpr bool kCache = (kMode == kModeCache);
+  static_assert(!kCache || (!kSolo && !kPair && kScore != 0), "cache form");
+  constexpr int kSoftmaxWarps = (kSolo || (kCache && NT == 1)) ? 4 : 8;
   constexpr int kEpilogueEnd = kSolo ? 4 : 12;  // epilogue warps are [kSoftmaxWarps, kEpilogueEnd): none in the solo form
   constexpr int kIssueWarpA = kSolo ? 4 : 12, kIssueWarpB = kSolo ? -1 : kIssuerB, kLoadWarp = kSolo ? 5 : 13;
   constexpr bool kVarlen = (kMode == kModeVarlen);
@@ -786,6 +947,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   const uint32_t sKV = tileAddr + NT * C::kQBufs * C::kTileBytes;
   Ctl* ctl = reinterpret_cast<Ctl*>(smem + NT * C::kQBufs * C::kTileBytes + NS * C::kStageBytes);
   const uint32_t barBase = ptx::smem_u32(&ctl->bars[0]);
+  [[maybe_unused]] CacheCtl* cctl = reinterpret_cast<CacheCtl*>((reinterpret_cast<uintptr_t>(ctl + 1) + 15) & ~(uintptr_t)15);
+  constexpr int kConvWarps = kEpilogueEnd - kSoftmaxWarps;  // cache form: the warps that fill the tiles
   auto bar = [&](int slot) { return barBase + 8u * (uint32_t)slot; };
 
   const int warp = threadIdx.x >> 5;
@@ -804,7 +967,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; t++) {
       for (int u = 0; u < 2; u++) {
-        ptx::mbar_init(bar(kBarQFull + 2 * t + u), 1);
+        ptx::mbar_init(bar(kBarQFull + 2 * t + u), kCache ? kConvWarps : 1);
         ptx::mbar_init(bar(kBarQEmpty + 2 * t + u), 1);
         // pair form: the softmax warps of both CTAs; packed input: the four softmax warps and the V-tail warp
         ptx::mbar_init(bar(kBarP0Ready + 2 * t + u), kPair ? 8 : (kVarlen ? 5 : 4));
@@ -823,8 +986,11 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     }
     ptx::mbar_init(bar(kBarOFreePair), 8);
     for (int s = 0; s < NS; s++) {
-      ptx::mbar_init(bar(kBarKvFull + s), 1);
+      ptx::mbar_init(bar(kBarKvFull + s), kCache ? kConvWarps : 1);
       ptx::mbar_init(bar(kBarKvEmpty + s), 2);  // one arrival per MMA-issuing thread
+    }
+    if constexpr (kCache) {
+      for (int s = 0; s < 8; s++) ptx::mbar_init(ptx::smem_u32(&cctl->scaleFull[s]), kConvWarps);
     }
     ctl->failed = 0;
     ptx::fence_barrier_init();
@@ -851,7 +1017,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     }
   }
   if (warp == kLoadWarp && lane == 0) {
-    if (kVarlen && p.devMaps != nullptr) {
+    if constexpr (kCache) {
+    } else if (kVarlen && p.devMaps != nullptr) {
       ptx::grid_wait_previous();  // the kernel that completes the maps
       ptx::tensormap_acquire(mapQ);
       ptx::tensormap_acquire(mapK);
@@ -901,13 +1068,16 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const int r = threadIdx.x & 127;
     const uint32_t tRegion = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(t * C::kSRegion);
     // scores that are capped or biased become multiples of log2(e) on the way, the others in the exponent
-    const float c = (kScore & (kScoreCap | kScoreBias)) != 0 ? 1.f : p.scaleLog2;
+    const float c = (kCache || (kScore & (kScoreCap | kScoreBias)) != 0) ? 1.f : p.scaleLog2;
     int it = 0;      // blocks of this tile processed so far, over all work items (phase of the per-block barriers)
     int items = 0;   // work items in which this tile was active
     int ldBase = 0;  // K/V ring loads of all earlier items (packed variable-length input only, see below)
+    [[maybe_unused]] int blkBase = 0;  // cache form: key blocks of all earlier items
     for (int k = 0;; k++) {
       WorkT w;
       const int idx = fetchWork(k, w);
+      [[maybe_unused]] CacheSegment seg;
+      if constexpr (kCache) seg = cctl->seg[k & 1];
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(kBarWorkEmpty + (k & 1)));
       if (idx < 0 || *wc.failed) break;
@@ -915,12 +1085,29 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       const int ldItem = ldBase;
       if constexpr (kRingSig) ldBase += 2 * w.nmax;
       (void)ldItem;
+      [[maybe_unused]] const int blkItem = blkBase;
+      if constexpr (kCache) {
+        blkBase += w.nmax;
+        if (t < NT && w.nblk[t] == 0 && w.qlo[t] < w.sq) {  // no keys for this tile in the segment, but a part that others count on
+          const long long part = ((long long)seg.slot * NT + t) * kBlockM + r;
+          __stcg(p.partLse + part, -INFINITY);
+          cache_join<NT, kHD, kBf16>(p, w, seg, cctl, t, r);
+        }
+      }
       if (t >= NT || w.nblk[t] == 0) continue;
-      const int qpos = w.qlo[t] + (r >> p.packShift);
+      const int qpos = kCache ? w.qlo[t] + r : w.qlo[t] + (r >> p.packShift);
       float m = -INFINITY, l = 0.f;
       const int n = w.nblk[t];
       [[maybe_unused]] ScoreRow<kScore> row;
-      if constexpr (kScore != 0) row.begin(p, w, qpos, (w.unit << p.packShift) + (r & ((1 << p.packShift) - 1)), w.qlo[t]);
+      [[maybe_unused]] float rowFactor = 0.f, vRef = 0.f, vInv = 0.f;  // cache form: scale of V that O refers to
+      if constexpr (kCache) {
+        const bool real = qpos < w.sq;
+        row.pos = w.skv - w.sq / p.group + (real ? qpos / p.group : 0);
+        row.last = row.pos;
+        row.seenByAll = w.skv - w.sq / p.group + w.qlo[t] / p.group;
+        if constexpr ((kScore & kScoreBias) != 0) row.slope = real ? p.slopes[w.unit * p.group + qpos % p.group] * 1.44269504f : 0.f;
+        if constexpr ((kScore & kScoreCap) != 0) row.capLog2 = p.cap * 1.44269504f;
+      } else if constexpr (kScore != 0) row.begin(p, w, qpos, (w.unit << p.packShift) + (r & ((1 << p.packShift) - 1)), w.qlo[t]);
       for (int j = 0; j < n; j++, it++) {
         if constexpr (kRingSig) {  // ring order K0 | K1 V0 | K2 V1 | ...: K of block j is load 2 j - 1 of the item (K0: 0)
           const int g = ldItem + (j == 0 ? 0 : 2 * j - 1);
@@ -947,10 +1134,46 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         int kbase = j * kBlockN;
         if constexpr (kSplit) kbase += w.part * p.partBlocks * kBlockN;
         if constexpr (kScore != 0 && !kSplit) kbase += w.part * kBlockN;
-        if constexpr (kScore != 0) row.transform(p, v, kbase);
+        [[maybe_unused]] float kf[8], vf[8];  // cache form: factors of the scores and of the weights, by groups of 16 keys
+        [[maybe_unused]] bool absent = false;
+        [[maybe_unused]] bool vGrow = false;
+        [[maybe_unused]] float vMax = 0.f;
+        if constexpr (kCache) {
+          const int g = blkItem + j;
+          wait_bar(ptx::smem_u32(&cctl->scaleFull[g & 7]), (g >> 3) & 1, wc, 32);
+          if (j == 0) {
+            rowFactor = cctl->rowFactor[k & 3][t][r] * p.scaleLog2;
+            if constexpr ((kScore & kScoreCap) != 0) rowFactor *= 2.f / p.cap;
+          }
+          const float4* sc = reinterpret_cast<const float4*>(cctl->scales[g & 7]);
+          const float4 k0 = sc[0], k1 = sc[1], v0 = sc[2], v1 = sc[3];
+          kf[0] = k0.x, kf[1] = k0.y, kf[2] = k0.z, kf[3] = k0.w, kf[4] = k1.x, kf[5] = k1.y, kf[6] = k1.z, kf[7] = k1.w;
+          vf[0] = v0.x, vf[1] = v0.y, vf[2] = v0.z, vf[3] = v0.w, vf[4] = v1.x, vf[5] = v1.y, vf[6] = v1.z, vf[7] = v1.w;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            absent = absent || kf[i] < 0.f;
+            vMax = fmaxf(vMax, vf[i]);
+          }
+          if (absent) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              if (kf[i] < 0.f) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) v[i >> 1][(i & 1) * 16 + e] = 0xff800000u;
+              }
+            }
+          }
+          // never zero: -inf in a block of zeros has to stay -inf
+#pragma unroll
+          for (int i = 0; i < 8; i++) kf[i] = fmaxf(fabsf(kf[i]) * rowFactor, 1.2e-38f);
+          row.cache_transform(v, kbase, kf);
+          vGrow = vMax > vRef * kCacheSlack;
+        } else if constexpr (kScore != 0) {
+          row.transform(p, v, kbase);
+        }
         bool needMask = (kMode != kModeFixedNoMask) &&
                         ((kbase + kBlockN > w.skv) || (p.causal && (kbase + kBlockN - 1 > (kScore != 0 ? row.seenByAll : w.qlo[t]))));
-        if constexpr (kScore != 0) row.documents(p, v, kbase, w.skv);
+        if constexpr (kScore != 0 && !kCache) row.documents(p, v, kbase, w.skv);
         if (needMask) {
           int lim = w.skv - kbase;                         // columns [0, lim) are real keys
           if (p.causal) lim = min(lim, (kScore != 0 ? row.last : qpos) - kbase + 1);  // ... that are not in the future
@@ -969,7 +1192,12 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             float2 x = make_float2(__uint_as_float(vq[i]), __uint_as_float(vq[i + 1]));
-            x = ffma2(x, c2, negMc2);
+            if constexpr (kCache) {
+              const float f = kf[quarter * 2 + i / 16];
+              x = ffma2(x, make_float2(f, f), negMc2);
+            } else {
+              x = ffma2(x, c2, negMc2);
+            }
             if (((quarter * 16 + (i >> 1)) % kEmuPeriod) < kEmuCount) {  // compile-time pattern: this pair goes to the FMA pipe
               x = ex2_fma2(x);
             } else {
@@ -977,7 +1205,13 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
               x.y = ex2(x.y);
             }
             sum = fadd2(sum, x);
-            dst[i >> 1] = pack2<kBf16>(x.x, x.y);
+            if constexpr (kCache) {
+              const float f = vf[quarter * 2 + i / 16];
+              x = fmul2(x, make_float2(f, f));
+              dst[i >> 1] = pack2<false>(x.x, x.y);
+            } else {
+              dst[i >> 1] = pack2<kBf16>(x.x, x.y);
+            }
           }
         };
         uint32_t pkA[16], pkB[16];
@@ -990,19 +1224,31 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
           for (int i = 2; i < 32; i += 2) mx4[q] = fmax3(mx4[q], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
         }
-        const float mx = fmax2(fmax2(mx4[0], mx4[1]), fmax2(mx4[2], mx4[3]));  // NaN if any score of the row is
+        float mx = fmax2(fmax2(mx4[0], mx4[1]), fmax2(mx4[2], mx4[3]));  // NaN if any score of the row is
+        if constexpr (kCache) {  // by groups, whose factors differ
+          mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const uint32_t(&vq)[32] = v[i >> 1];
+            float top = fmax2(__uint_as_float(vq[(i & 1) * 16]), __uint_as_float(vq[(i & 1) * 16 + 1]));
+#pragma unroll
+            for (int e = 2; e < 16; e += 2) top = fmax3(top, __uint_as_float(vq[(i & 1) * 16 + e]), __uint_as_float(vq[(i & 1) * 16 + e + 1]));
+            mx = fmax2(mx, top * kf[i]);
+          }
+        }
         // Lazy rescale: keep the old reference max while the new one exceeds it by less than kRescaleLog2 in
         // the exp2 domain (P then grows up to 2^kRescaleLog2, harmless in fp32 sums and 16-bit P); the
         // result is unchanged because O and the row sum stay relative to the same reference value.
         float mNew = fmaxf(m, mx);
         const bool grow = (m != -INFINITY) && ((mNew - m) * c > kRescaleLog2);
-        if (__any_sync(0xffffffffu, grow)) {
+        if (__any_sync(0xffffffffu, grow) || (kCache && vGrow && j > 0)) {
           // Rare: some row of this warp moves its reference max.  Rescale that row's O in tensor memory (rows
           // that keep their max multiply by 1) once the previous P.V has landed; P.V of this block waits for
           // the P0 arrival below, so it sees the rescaled accumulator.  (A parity wait is only meaningful for the
           // phase in progress or the one just completed: P.V of block it-2 finished before S of this block was
           // produced, and P.V of this block cannot start before this warp arrives.)
           const float scale = grow ? ex2((m - mNew) * c) : 1.f;
+          const float scaleO = (kCache && vGrow) ? scale * (vRef / vMax) : scale;
           if constexpr (kRingSig) {  // V of block j - 1 is load 2 j of the item (j >= 1 here: block 0 never rescales)
             const int g = ldItem + 2 * j;
             wait_bar(bar(kBarKvEmpty + g % NS), (g / NS) & 1, wc, 5);
@@ -1019,7 +1265,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             ptx::tmem_wait_ld();
             ptx::tmem_ld_fence(o);
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
+            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * scaleO);
             ptx::tmem_st_32x32b_x16(tO + ch * 16, o);
           }
           ptx::tmem_wait_st();
@@ -1028,6 +1274,14 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         if (m != -INFINITY && !grow) mNew = m;
         const float mUse = (mNew == -INFINITY) ? 0.f : mNew;
         m = mNew;
+        if constexpr (kCache) {
+          if (vGrow) {
+            vRef = vMax;
+            vInv = vMax > 0.f ? fminf(1.f / vMax, 3e38f) : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; i++) vf[i] = vf[i] * vInv * kCacheUp;
+        }
 
         // A NaN score makes every exponential of the row NaN (the pairs evaluated on the FMA pipe clamp their
         // argument and would turn a NaN of their own into 0), hence the row sum and the output row.
@@ -1062,6 +1316,53 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           const int head = (w.unit << p.packShift) + (r & ((1 << p.packShift) - 1));
           p.partLse[w.part * p.rows + (w.qRow0 + qpos) * p.headsQ + head] = (l == 0.f) ? -INFINITY : m * c + __log2f(l);
         }
+      }
+      if constexpr (kCache) {
+        // This warp is also the epilogue of its 32 rows: the output, or a part of it that the CTA that comes last puts together.
+        const int lastBlk = it - 1;
+        if constexpr (kRingSig) {
+          const int gLast = ldItem + 2 * w.nmax - 1;
+          wait_bar(bar(kBarKvEmpty + gLast % NS), (gLast / NS) & 1, wc, 7);
+        } else {
+          wait_bar(bar(kBarPvDone + 2 * t + (C::kTwoPos ? (lastBlk & 1) : 0)), (C::kTwoPos ? (lastBlk >> 1) : lastBlk) & 1, wc, 7);
+        }
+        ptx::tc_fence_after();
+        const float inv = l == 0.f ? 0.f : vRef * (1.f / kCacheUp) / l;  // NaN stays NaN
+        const bool whole = seg.c0 == seg.c1;
+        const uint32_t tO = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(C::kOCol0 + t * HDP);
+        const long long part = (long long)seg.slot * NT + t;
+#pragma unroll
+        for (int ch = 0; ch < kHD / 32; ch++) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32b_x32(tO + ch * 32, o);
+          ptx::tmem_wait_ld();
+          ptx::tmem_ld_fence(o);
+          if (l == 0.f) {
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = 0u;
+          }
+          if (ch == kHD / 32 - 1) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(kBarOFree + t));
+          }
+          if (whole) {
+            if (qpos < w.sq) cache_store<kBf16>(p, w, qpos, ch, o, inv);
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.partO) + (part * (kHD / 4) + ch * 8) * kBlockM + r;
+#pragma unroll
+            for (int g = 0; g < 8; g++) {
+              __stcg(dst + g * kBlockM, make_float4(__uint_as_float(o[g * 4]) * inv, __uint_as_float(o[g * 4 + 1]) * inv,
+                                                    __uint_as_float(o[g * 4 + 2]) * inv, __uint_as_float(o[g * 4 + 3]) * inv));
+            }
+          }
+        }
+        if (!whole) {
+          __stcg(p.partLse + part * kBlockM + r, l == 0.f ? -INFINITY : m + __log2f(l));
+          cache_join<NT, kHD, kBf16>(p, w, seg, cctl, t, r);
+        }
+        items++;
+        continue;
       }
       if constexpr (kSolo) {
         // This warp is also the epilogue of its 32 rows: wait for the last P.V of the item, read O, release the
@@ -1124,6 +1425,172 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(kBarScaleFull + t));
       items++;
+    }
+  } else if (kCache && warp < kEpilogueEnd) {
+    // ================================================================ cache form: pages and queries -> fp16 tiles in shared memory
+    ptx::setmaxnreg_dec<kRegsEpilogue>();
+    if constexpr (kCache) {
+      constexpr int kConv = kConvWarps * 32, kChunks = kHD / 16;    // 16-byte pieces of a cache row
+      constexpr int kPieces = kBlockN * kChunks / kConv;            // of a tile, per thread
+      static_assert(kBlockN * kChunks % kConv == 0, "pieces of a tile");
+      const int tid = threadIdx.x - kSoftmaxWarps * 32;
+      const int cw = warp - kSoftmaxWarps;
+      const long long headBytes = (long long)p.headDim << p.blockShift;
+      int ld = 0, blkBase = 0;
+      int qc[2] = {0, 0};
+      for (int k = 0;; k++) {
+        WorkT w;
+        const int idx = fetchWork(k, w);
+        const int b = cctl->seg[k & 1].b;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(kBarWorkEmpty + (k & 1)));
+        if (idx < 0 || *wc.failed) break;
+        if (w.nmax == 0) continue;
+        // a row per thread; rows past the request are zero
+        auto fillQ = [&](int t) {
+          if (t >= NT || w.nblk[t] == 0) return;
+          const int qb = qc[t] % C::kQBufs, qUse = qc[t] / C::kQBufs;
+          if (qUse > 0) wait_bar(bar(kBarQEmpty + 2 * t + qb), (qUse - 1) & 1, wc, 22);
+          if (tid < kBlockM) {
+            const int flat = w.qlo[t] + tid;
+            const uint32_t dst = sQ + (t * C::kQBufs + qb) * C::kTileBytes + tid * 128;
+            const bool real = flat < w.sq;
+            const uint4* src = reinterpret_cast<const uint4*>(
+                static_cast<const uint16_t*>(p.Q) +
+                ((w.qRow0 + (real ? flat / p.group : 0)) * p.headsQ + w.unit * p.group + (real ? flat % p.group : 0)) * (long long)p.headDim);
+            float up = 1.f, down = 1.f;
+            if constexpr (kBf16) {
+              uint32_t top = 0;
+#pragma unroll 4
+              for (int i = 0; i < kHD / 8; i++) {
+                const uint4 x = src[i];
+                top = max(top, max(max(max(x.x & 0x7F80u, x.x >> 16 & 0x7F80u), max(x.y & 0x7F80u, x.y >> 16 & 0x7F80u)),
+                                   max(max(x.z & 0x7F80u, x.z >> 16 & 0x7F80u), max(x.w & 0x7F80u, x.w >> 16 & 0x7F80u))));
+              }
+              row_scale(top, up, down);
+            }
+            cctl->rowFactor[k & 3][t][tid] = down;
+#pragma unroll 4
+            for (int i = 0; i < kHD / 8; i++) {
+              uint4 x = src[i];
+              if constexpr (kBf16) x = make_uint4(bf16_to_half2(x.x, up), bf16_to_half2(x.y, up), bf16_to_half2(x.z, up), bf16_to_half2(x.w, up));
+              if (!real) x = make_uint4(0, 0, 0, 0);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (i >> 3) * kSubTileBytes + (((i & 7) ^ (tid & 7)) << 4)),
+                           "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                           : "memory");
+            }
+          }
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(kBarQFull + 2 * t + qb));
+          qc[t]++;
+        };
+        // tile index (block x heads + head) of the 16-key group `lane` of a key block, -1: none
+        auto pageOf = [&](int blk) -> int {
+          const int key = blk * kBlockN + lane * 16;
+          int tile = -1;
+          if (lane < 8 && key < w.skv) {
+            const int page = p.table[(long long)b * p.width + (key >> p.blockShift)];
+            if (page >= 0 && page < p.numBlocks) tile = page;
+          }
+          return tile;
+        };
+        const int numLoads = 2 * w.nmax;
+        auto which = [&](int i, bool& isV, int& blk) {  // the ring's order
+          if constexpr (C::kTwoPos) {
+            isV = i != 0 && (i == numLoads - 1 || (i & 1) == 0);
+            blk = i == 0 ? 0 : i == numLoads - 1 ? w.nmax - 1 : isV ? (i - 2) / 2 : (i + 1) / 2;
+          } else {
+            isV = (i & 1) != 0;
+            blk = i >> 1;
+          }
+        };
+        bool isV;
+        int blk;
+        which(0, isV, blk);
+        int page = pageOf(w.part + blk);
+        fillQ(0);
+        for (int i = 0; i < numLoads; i++, ld++) {
+          const int key0 = (w.part + blk) * kBlockN;
+          const uint8_t* base = p.codes[isV ? 1 : 0];
+          uint4 d[kPieces];
+#pragma unroll
+          for (int e = 0; e < kPieces; e++) {
+            const int piece = tid + e * kConv, row = piece / kChunks;
+            const int pg = __shfl_sync(0xffffffffu, page, row >> 4);
+            d[e] = make_uint4(0, 0, 0, 0);
+            if (pg >= 0 && key0 + row < w.skv) {
+              d[e] = __ldg(reinterpret_cast<const uint4*>(base + ((long long)pg * p.headsKV + w.unit) * headBytes +
+                                                          (long long)((key0 + row) & ((1 << p.blockShift) - 1)) * kHD + (piece % kChunks) * 16));
+            }
+          }
+          float ks = -1.f, vs = 0.f;
+          if (!isV && cw == 0 && page >= 0) {
+            ks = __ldg(p.scales[0] + (long long)page * p.headsKV + w.unit);
+            vs = __ldg(p.scales[1] + (long long)page * p.headsKV + w.unit);
+          }
+          bool nextV = false;
+          int nextBlk = 0, nextPage = 0;
+          if (i + 1 < numLoads) {
+            which(i + 1, nextV, nextBlk);
+            nextPage = pageOf(w.part + nextBlk);
+          }
+          const int s = ld % NS;
+          if (ld >= NS) wait_bar(bar(kBarKvEmpty + s), ((ld / NS) - 1) & 1, wc, 14);
+          if (!isV) {  // scales and row factors first: the softmax warps look at them when the scores are there
+            const int g = (blkBase + blk) & 7;
+            if (cw == 0 && lane < 8) {
+              cctl->scales[g][lane] = ks;
+              cctl->scales[g][8 + lane] = vs;
+            }
+            __syncwarp();
+            if (blk > 0 && lane == 0) ptx::mbar_arrive(ptx::smem_u32(&cctl->scaleFull[g]));
+          }
+          const uint32_t dst = sKV + s * C::kStageBytes;
+          auto put = [&](auto int8) {
+#pragma unroll
+            for (int e = 0; e < kPieces; e++) {
+              const int piece = tid + e * kConv, row = piece / kChunks, c16 = piece % kChunks;
+              uint4 a, z;
+              widen<decltype(int8)::value>(d[e].x, a.x, a.y);
+              widen<decltype(int8)::value>(d[e].y, a.z, a.w);
+              widen<decltype(int8)::value>(d[e].z, z.x, z.y);
+              widen<decltype(int8)::value>(d[e].w, z.z, z.w);
+              // a slab's even pieces and the next slab's odd ones together: eight lanes, eight groups of banks
+              const bool swap = (c16 & 4) != 0;
+              const uint32_t at = dst + (c16 >> 2) * kSubTileBytes + row * 128;
+              const int c0 = 2 * (c16 & 3), sw = row & 7;
+              const uint32_t first = at + (((c0 + (swap ? 1 : 0)) ^ sw) << 4), second = at + (((c0 + (swap ? 0 : 1)) ^ sw) << 4);
+              const uint4 u = swap ? z : a, v2 = swap ? a : z;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(first), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(second), "r"(v2.x), "r"(v2.y), "r"(v2.z), "r"(v2.w) : "memory");
+            }
+          };
+          if (p.int8) {
+            put(std::integral_constant<bool, true>{});
+          } else {
+            put(std::integral_constant<bool, false>{});
+          }
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            ptx::mbar_arrive(bar(kBarKvFull + s));
+            if (cw == 0) {  // the stage-free arrival of every tile that will not touch this block
+#pragma unroll
+              for (int t = 0; t < 2; t++) {
+                if (t >= NT || blk >= w.nblk[t]) ptx::mbar_arrive(bar(kBarKvEmpty + s));
+              }
+            }
+          }
+          // the first block's: the row factors of both tiles belong to it
+          if (i == 0 && NT == 2) fillQ(1);
+          if (i == 0 && lane == 0) ptx::mbar_arrive(ptx::smem_u32(&cctl->scaleFull[blkBase & 7]));
+          isV = nextV;
+          blk = nextBlk;
+          page = nextPage;
+        }
+        blkBase += w.nmax;
+      }
     }
   } else if (warp < kEpilogueEnd) {
     // ================================================================ epilogue
@@ -1214,7 +1681,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     ptx::setmaxnreg_dec<kRegsIssue>();
     if ((warp == kIssueWarpA || warp == kIssueWarpB) && lane == 0) {
       // ============================================================== MMA issue
-      const int fmt = kBf16 ? 1 : 0;
+      const int fmt = (kBf16 && !kCache) ? 1 : 0;
       // pair form: M = 256 over the two CTAs
       const uint32_t idQK = ptx::instr_desc_f16(fmt, kPair ? 2 * kBlockM : kBlockM, kBlockN, 0, 0);
       const uint32_t idPV = ptx::instr_desc_f16(fmt, kPair ? 2 * kBlockM : kBlockM, kHD, 0, 1);
@@ -1444,8 +1911,80 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         it += n;
         if (n > 0) qc++;
       }
-    } else if (warp == kLoadWarp && lane == 0) {
+    } else if (kCache && warp == kLoadWarp && lane == 0) {
+      // ============================================================== cache form: the segments of this CTA's run
+      if constexpr (kCache) {
+        ptx::grid_wait_previous();
+        ptx::grid_allow_next();
+        const int units = *p.numUnits;
+        const long long perHead = p.unitStart[units], total = perHead * p.headsKV;
+        const int runs = (int)min((long long)gridDim.x, total);  // every run has a block
+        const int run = blockIdx.x;
+        long long at = 0, end = 0;
+        int h = 0, u = 0;
+        if (run < runs) {
+          at = total * run / runs;
+          end = total * (run + 1) / runs;
+          h = (int)(at / perHead);
+          const long long rem = at - (long long)h * perHead;
+          int hi = units - 1;  // the unit u with unitStart[u] <= rem < unitStart[u + 1]
+          while (u < hi) {
+            const int mid = (u + hi + 1) >> 1;
+            if (p.unitStart[mid] <= rem) {
+              u = mid;
+            } else {
+              hi = mid - 1;
+            }
+          }
+        }
+        for (int k = 0;; k++) {
+          if (k >= 2) wait_bar(bar(kBarWorkEmpty + (k & 1)), ((k >> 1) - 1) & 1, wc, 21);
+          volatile WorkSlot* ws = &ctl->work[k & 1];
+          volatile CacheSegment* cs = &cctl->seg[k & 1];
+          const bool more = at < end && !*reinterpret_cast<volatile int*>(&ctl->failed);
+          if (more) {
+            const long long start = p.unitStart[u];
+            const int blocks = (int)(p.unitStart[u + 1] - start);
+            const int2 what = p.unitWhat[u];
+            const int b = what.x;
+            const int q0 = min(max(p.cuQ[b], 0), p.seqLenQ), nq = min(max(p.cuQ[b + 1] - q0, 0), p.seqLenQ - q0);  // seqLenQ: rows of Q
+            const int len = min(max(p.lens[b], 0), p.width << p.blockShift);
+            const long long first = (long long)h * perHead + start;
+            const int blk0 = (int)(at - first), n = (int)min((long long)blocks - blk0, end - at);
+            int end0 = blocks;
+            if (NT == 2 && what.y + kBlockM < nq * p.group && p.causal) {  // two tiles, of which the first sees fewer keys
+              end0 = min(blocks, max(1, (len - nq + (what.y + kBlockM - 1) / p.group + kBlockN) / kBlockN));
+            }
+            ws->sq = nq * p.group;
+            ws->skv = len;
+            ws->unit = h;
+            ws->qRow0 = q0;
+            ws->qlo[0] = what.y;
+            ws->qlo[1] = what.y + kBlockM;
+            ws->nblk[0] = max(0, min(n, end0 - blk0));
+            ws->nblk[1] = (NT == 2 && what.y + kBlockM < nq * p.group) ? n : 0;
+            ws->nmax = n;
+            ws->part = blk0;
+            const int c0 = cache_run_of(first, total, runs), c1 = cache_run_of(first + blocks - 1, total, runs);
+            cs->b = b;
+            cs->slot = 2 * run + (k == 0 ? 0 : 1);
+            cs->c0 = c0;
+            cs->c1 = c1;
+            cs->at0 = total * c0 / runs == first ? 0 : 1;
+            at += n;
+            if (++u == units) {
+              u = 0;
+              h++;
+            }
+          }
+          ws->idx = more ? k : -1;
+          ptx::mbar_arrive(bar(kBarWorkFull + (k & 1)));
+          if (!more) break;
+        }
+      }
+    } else if (!kCache && warp == kLoadWarp && lane == 0) {
       // ============================================================== work distribution + TMA loads
+      if constexpr (!kCache) {
       const int gp = 1 << p.packShift;
       int ld = 0;            // KV-ring loads issued so far
       int qc[2] = {0, 0};    // Q loads issued so far per tile
@@ -1627,6 +2166,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         }
         if (!nextDone) more = publish(k + 1);
       }
+      }
     } else if (kVarlen && warp == kHelpWarp) {
       // ============================================================== packed input: V rows past a sequence's end
       int ldBase = 0;         // K/V ring loads of all earlier items
@@ -1678,7 +2218,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 
   ptx::tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (!kCache && threadIdx.x == 0) {
     // The last CTA to get here puts both counters back to zero for the next launch that uses them.  Every CTA's
     // fetches from the work counter precede its arrival on the done counter (same CTA, separated by the barrier above).
     __threadfence();

@@ -10,6 +10,7 @@
 
 #include "../../include/tinyfa_b200.h"
 #include "build_config.cuh"
+#include "cta_scan.cuh"
 #include "ptx_sm100.cuh"
 #include "tfa_common.cuh"
 
@@ -40,32 +41,6 @@ constexpr int kPlanThreads = 1024;
 __device__ __forceinline__ int blocks_of(long long tokens, int shift) { return (int)((tokens + (1 << shift) - 1) >> shift); }
 __device__ __forceinline__ long long length_before(const PlanParams& p, int b) {
   return min(max((long long)p.lens[b], 0ll), (long long)p.width << p.blockShift);
-}
-
-// Inclusive sum over the CTA; every thread gets the CTA's total as well.
-__device__ __forceinline__ long long cta_scan(long long v, long long* sWarp, long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, v, d);
-    if (lane >= d) v += o;
-  }
-  if (lane == 31) sWarp[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    long long w = lane < warps ? sWarp[lane] : 0;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, w, d);
-      if (lane >= d) w += o;
-    }
-    sWarp[lane] = w;
-  }
-  __syncthreads();
-  total = sWarp[31];
-  if (warp > 0) v += sWarp[warp - 1];
-  __syncthreads();  // sWarp is written again
-  return v;
 }
 
 // Cell of the cache for packed row `row`, -1 for a row of no request or of one that was not served.
