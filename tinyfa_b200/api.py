@@ -170,31 +170,41 @@ def flash_attn_varlen_forward(Q, K, V, cu_seqlens_q, cu_seqlens_kv, max_seqlen_q
 def _check_no_grad(*tensors):
     """These operators have no backward pass: better an error than gradients that are silently missing."""
     if torch.is_grad_enabled():
-        _check(not any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors),
-               "forward only: call under torch.no_grad(), or on tensors that do not require gradients")
+        for t in tensors:
+            _check(not (t is not None and t.requires_grad), "forward only: call under torch.no_grad(), or on tensors that do not require gradients")
+
+
+def _fits(x, dtype, shape, device):
+    """A contiguous CUDA tensor of this type, shape and device (an index)?  One look without messages; _check_aux says what is wrong."""
+    try:
+        return x.dtype is dtype and x.get_device() == device >= 0 and x.shape == shape and x.is_contiguous()
+    except AttributeError:
+        return False
 
 
 def _check_aux(x, name, dtype, shape, device):
-    """An optional tensor beside Q: its address, None where there is none."""
-    if x is None:
-        return None
     _check_input(x, name)
     _check(x.dtype == dtype, f"{name} must be {str(dtype).replace('torch.', '')}")
     _check(tuple(x.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
-    _check(x.get_device() == device, f"{name} must be on the device of Q")
+    _check(x.get_device() == device, f"{name} must be on the device of the other tensors")
+
+
+def _aux(x, name, dtype, shape, device):
+    """Address of a tensor beside the main ones."""
+    if not _fits(x, dtype, shape, device):
+        _check_aux(x, name, dtype, shape, device)
+        raise RuntimeError(f"{name}: unsupported input")
     return x.data_ptr()
 
 
 def _check_softcap(softcap):
-    softcap = float(softcap)
     _check(0.0 <= softcap < float("inf"), "softcap must be 0 (none) or a positive finite number")
-    return softcap
 
 
-def _run_scored(lib, device, Q, K, V, code, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv):
-    batch, seq_q, heads_q, head_dim = Q.shape
-    seq_kv, heads_kv = K.shape[1], K.shape[2]
-    O = torch.empty_like(Q) if (seq_kv > 0 and Q.numel() > 0) else torch.zeros_like(Q)
+def _run_scored(lib, device, Q, K, V, code, q_shape, kv_shape, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv):
+    batch, seq_q, heads_q, head_dim = q_shape
+    seq_kv, heads_kv = kv_shape[1], kv_shape[2]
+    O = torch.empty_like(Q) if (seq_kv > 0 and batch * seq_q > 0) else torch.zeros_like(Q)
     rc = lib.tfa_b200_fwd_scored(Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), code, batch, seq_q, seq_kv, heads_q, heads_kv,
                                  head_dim, 1 if is_causal else 0, q_start, softcap, slopes, prefix, docs_q, docs_kv, _raw_stream(device))
     if rc != 0:
@@ -212,25 +222,34 @@ def flash_attn_scored_forward(Q, K, V, is_causal=False, softcap=0.0, alibi_slope
     prefix_lens int32 [B] needs is_causal; doc_ids_q int32 [B,Sq] and doc_ids_kv int32 [B,Skv] are given together, negative ids are padding.
     A row that sees no key is zero.  Forward only.
     """
-    if not _usable(Q, K, V):
+    ok = _usable(Q, K, V)
+    if ok:
+        q_shape, kv_shape, dtype = Q.shape, K.shape, Q.dtype
+        code = _DTYPE_CODE.get(dtype)
+        ok = (code is not None and K.dtype == dtype and V.dtype == dtype and len(q_shape) == 4 and len(kv_shape) == 4
+              and V.shape == kv_shape and kv_shape[0] == q_shape[0] and kv_shape[3] == q_shape[3]
+              and kv_shape[2] > 0 and q_shape[2] % kv_shape[2] == 0)
+    if not ok:
         _check_fixed(Q, K, V)
-    q_shape, kv_shape = Q.shape, K.shape
-    _check_fixed(Q, K, V)
-    _check(kv_shape[0] == q_shape[0], "Batch sizes must match")
+        raise RuntimeError("flash_attn_scored_forward: unsupported input")
     _check_no_grad(Q, K, V, alibi_slopes)
     _check(isinstance(q_start, int) and q_start >= 0, "q_start must be an integer >= 0")
-    _check(prefix_lens is None or is_causal, "prefix_lens widens the causal mask: it needs is_causal")
-    _check((doc_ids_q is None) == (doc_ids_kv is None), "doc_ids_q and doc_ids_kv must be given together")
-    code, device, softcap = _DTYPE_CODE[Q.dtype], Q.get_device(), _check_softcap(softcap)
-    slopes = _check_aux(alibi_slopes, "alibi_slopes", torch.float32, (q_shape[2],), device)
-    prefix = _check_aux(prefix_lens, "prefix_lens", torch.int32, (q_shape[0],), device)
-    docs_q = _check_aux(doc_ids_q, "doc_ids_q", torch.int32, (q_shape[0], q_shape[1]), device)
-    docs_kv = _check_aux(doc_ids_kv, "doc_ids_kv", torch.int32, (q_shape[0], kv_shape[1]), device)
+    _check_softcap(softcap)
+    device, slopes, prefix, docs_q, docs_kv = Q.get_device(), None, None, None, None
+    if alibi_slopes is not None:
+        slopes = _aux(alibi_slopes, "alibi_slopes", torch.float32, (q_shape[2],), device)
+    if prefix_lens is not None:
+        _check(is_causal, "prefix_lens widens the causal mask: it needs is_causal")
+        prefix = _aux(prefix_lens, "prefix_lens", torch.int32, (q_shape[0],), device)
+    if doc_ids_q is not None or doc_ids_kv is not None:
+        _check(doc_ids_q is not None and doc_ids_kv is not None, "doc_ids_q and doc_ids_kv must be given together")
+        docs_q = _aux(doc_ids_q, "doc_ids_q", torch.int32, (q_shape[0], q_shape[1]), device)
+        docs_kv = _aux(doc_ids_kv, "doc_ids_kv", torch.int32, (q_shape[0], kv_shape[1]), device)
     lib = _lib.load()
     if _current_device() == device:
-        return _run_scored(lib, device, Q, K, V, code, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv)
+        return _run_scored(lib, device, Q, K, V, code, q_shape, kv_shape, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv)
     with torch.cuda.device(device):
-        return _run_scored(lib, device, Q, K, V, code, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv)
+        return _run_scored(lib, device, Q, K, V, code, q_shape, kv_shape, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv)
 
 
 def is_head_dim_compiled(head_dim):

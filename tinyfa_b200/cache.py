@@ -12,17 +12,11 @@ Checks, streams, devices and errors as in api.py; nothing is copied to the host.
 import torch
 
 from . import _lib
-from .api import _DTYPE_CODE, _check, _check_aux, _check_input, _check_no_grad, _check_softcap, _current_device, _dtype_code, _raw_stream
+from .api import (_aux, _check, _check_input, _check_no_grad, _check_softcap, _current_device, _dtype_code, _fits, _raw_stream)
 
 _CACHE_CODE = {torch.int8: 1, torch.float8_e4m3fn: 2}
 _BLOCK_TOKENS = (16, 32, 64, 128)
-
-
-def _on_device(device, call):
-    if _current_device() == device:
-        return call()
-    with torch.cuda.device(device):
-        return call()
+_QUERY_CODE = {torch.float16: 1, torch.bfloat16: 2}
 
 
 def _check_cache(k_cache, v_cache, k_scales, v_scales, device):
@@ -37,6 +31,38 @@ def _check_cache(k_cache, v_cache, k_scales, v_scales, device):
         _check(x.dtype == torch.float32 and x.shape == k_cache.shape[:2], f"{name} must be float32 [numBlocks, numHeadsKV]")
 
 
+def _table_shape(block_table):
+    if isinstance(block_table, torch.Tensor):
+        shape = block_table.shape
+        if len(shape) == 2 and _fits(block_table, torch.int32, shape, block_table.get_device()):
+            return shape
+    _check_input(block_table, "block_table")
+    raise RuntimeError("block_table must be int32 [batch, maxBlocks]")
+
+
+def _rows_shape(x, name, what):
+    """Shape, type and device of packed rows."""
+    if isinstance(x, torch.Tensor):
+        shape, dtype, device = x.shape, x.dtype, x.get_device()
+        if len(shape) == 3 and _fits(x, dtype, shape, device):
+            return shape, dtype, device
+    _check_input(x, name)
+    raise RuntimeError(f"{name} must be 3D {what}")
+
+
+def _cache_shape(k_cache, v_cache, k_scales, v_scales, device):
+    """[numBlocks, numHeadsKV, blockTokens, headDim] and the type code of a cache whose four tensors belong together."""
+    if isinstance(k_cache, torch.Tensor):
+        shape, dtype = k_cache.shape, k_cache.dtype
+        code, tiles = _CACHE_CODE.get(dtype), shape[:2]
+        if (code is not None and len(shape) == 4 and shape[2] in _BLOCK_TOKENS and _fits(k_cache, dtype, shape, device)
+                and _fits(v_cache, dtype, shape, device) and _fits(k_scales, torch.float32, tiles, device)
+                and _fits(v_scales, torch.float32, tiles, device)):
+            return shape, code
+    _check_cache(k_cache, v_cache, k_scales, v_scales, device)
+    raise RuntimeError("unsupported cache")
+
+
 def kv_cache_plan(block_table, seq_lens, new_lens, free_blocks, num_free, block_tokens, total_new, finished=None):
     """Block tables and slot maps from request lengths, on the GPU.
 
@@ -48,30 +74,35 @@ def kv_cache_plan(block_table, seq_lens, new_lens, free_blocks, num_free, block_
     A request that finds too few free blocks (counting what every request ahead of it asks for), or that would need more than maxBlocks,
     gets none: its length stays and its rows have slot -1.
     """
-    _check_input(block_table, "block_table")
-    _check(block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table must be int32 [batch, maxBlocks]")
-    _check(block_tokens in _BLOCK_TOKENS, f"blocks hold 16, 32, 64 or 128 tokens, got {block_tokens}")
+    table_shape = _table_shape(block_table)
+    if block_tokens not in _BLOCK_TOKENS:
+        raise RuntimeError(f"blocks hold 16, 32, 64 or 128 tokens, got {block_tokens}")
     _check(isinstance(total_new, int) and total_new >= 0, "total_new must be an integer >= 0")
-    device, (batch, width) = block_table.get_device(), block_table.shape
-    _check_input(free_blocks, "free_blocks")
-    _check(seq_lens is not None and new_lens is not None and num_free is not None, "seq_lens, new_lens and num_free must be tensors")
-    lens = _check_aux(seq_lens, "seq_lens", torch.int32, (batch,), device)
-    new = _check_aux(new_lens, "new_lens", torch.int32, (batch,), device)
-    free = _check_aux(free_blocks, "free_blocks", torch.int32, (free_blocks.numel(),), device)
-    have = _check_aux(num_free, "num_free", torch.int32, (1,), device)
-    done = _check_aux(finished, "finished", torch.bool, (batch,), device)
+    (batch, width), device = table_shape, block_table.get_device()
+    _check(isinstance(free_blocks, torch.Tensor) and free_blocks.dim() == 1, "free_blocks must be an int32 tensor of one dimension")
+    capacity = free_blocks.numel()
+    lens = _aux(seq_lens, "seq_lens", torch.int32, (batch,), device)
+    new = _aux(new_lens, "new_lens", torch.int32, (batch,), device)
+    free = _aux(free_blocks, "free_blocks", torch.int32, (capacity,), device)
+    have = _aux(num_free, "num_free", torch.int32, (1,), device)
+    done = _aux(finished, "finished", torch.bool, (batch,), device) if finished is not None else None
+    if _current_device() == device:
+        return _run_plan(block_table, lens, new, done, free, have, batch, width, capacity, block_tokens, total_new, device)
+    with torch.cuda.device(device):
+        return _run_plan(block_table, lens, new, done, free, have, batch, width, capacity, block_tokens, total_new, device)
 
-    def call():
-        # one allocation for the four results; slots first, so that they are aligned
-        out = torch.empty(2 * total_new + 2 * batch + 2, dtype=torch.int32, device=block_table.device)
-        slots, cu, after, left = out[:2 * total_new].view(torch.int64), out[2 * total_new:-batch - 1], out[-batch - 1:-1], out[-1:]
-        rc = _lib.load().tfa_b200_kv_cache_plan(block_table.data_ptr(), lens, new, done, free, have, slots.data_ptr(), cu.data_ptr(), after.data_ptr(),
-                                                left.data_ptr(), batch, width, free_blocks.numel(), block_tokens, total_new, _raw_stream(device))
-        if rc != 0:
-            _lib.check(rc, "kv_cache_plan")
-        return slots, cu, after, left
 
-    return _on_device(device, call)
+def _run_plan(block_table, lens, new, done, free, have, batch, width, capacity, block_tokens, total_new, device):
+    where = block_table.device
+    slots = torch.empty(total_new, dtype=torch.int64, device=where)
+    cu = torch.empty(batch + 1, dtype=torch.int32, device=where)
+    after = torch.empty(batch, dtype=torch.int32, device=where)
+    left = torch.empty(1, dtype=torch.int32, device=where)
+    rc = _lib.load().tfa_b200_kv_cache_plan(block_table.data_ptr(), lens, new, done, free, have, slots.data_ptr(), cu.data_ptr(), after.data_ptr(),
+                                            left.data_ptr(), batch, width, capacity, block_tokens, total_new, _raw_stream(device))
+    if rc != 0:
+        _lib.check(rc, "kv_cache_plan")
+    return slots, cu, after, left
 
 
 def kv_cache_store(K, V, k_cache, v_cache, k_scales, v_scales, slots):
@@ -81,26 +112,24 @@ def kv_cache_store(K, V, k_cache, v_cache, k_scales, v_scales, slots):
     block before are rounded anew.  Rows that begin at a block's first cell begin the block, whatever its scale was.  Infinities become the
     largest code and NaN zero.  The rows of one block follow one another and no slot comes twice, as kv_cache_plan gives them.
     """
-    _check_input(K, "K")
-    _check_input(V, "V")
-    _check(K.dim() == 3 and V.shape == K.shape, "K and V must be 3D [total, numHeadsKV, headDim] of the same shape")
-    _check(K.dtype == V.dtype, "K and V must have the same dtype")
-    code, device = _dtype_code(K, "kv_cache_store"), K.get_device()
-    _check(V.get_device() == device, "K and V must be on the same device")
-    _check_cache(k_cache, v_cache, k_scales, v_scales, device)
-    _check(k_cache.shape[1] == K.shape[1] and k_cache.shape[3] == K.shape[2], "cache and K must have the same heads and head dim")
-    _check(slots is not None, "slots must be a tensor")
+    shape, dtype, device = _rows_shape(K, "K", "[total, numHeadsKV, headDim]")
+    code = _dtype_code(K, "kv_cache_store")
+    v = _aux(V, "V", dtype, shape, device)
+    cache, kind = _cache_shape(k_cache, v_cache, k_scales, v_scales, device)
+    _check(cache[1] == shape[1] and cache[3] == shape[2], "cache and K must have the same heads and head dim")
     _check_no_grad(K, V)
-    where = _check_aux(slots, "slots", torch.int64, (K.shape[0],), device)
+    where = _aux(slots, "slots", torch.int64, (shape[0],), device)
+    if _current_device() == device:
+        return _run_store(K, v, k_cache, v_cache, k_scales, v_scales, where, code, kind, shape, cache, device)
+    with torch.cuda.device(device):
+        return _run_store(K, v, k_cache, v_cache, k_scales, v_scales, where, code, kind, shape, cache, device)
 
-    def call():
-        rc = _lib.load().tfa_b200_kv_cache_store(K.data_ptr(), V.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(),
-                                                 v_scales.data_ptr(), where, code, _CACHE_CODE[k_cache.dtype], K.shape[0], k_cache.shape[0],
-                                                 K.shape[1], K.shape[2], k_cache.shape[2], _raw_stream(device))
-        if rc != 0:
-            _lib.check(rc, "kv_cache_store")
 
-    _on_device(device, call)
+def _run_store(K, v, k_cache, v_cache, k_scales, v_scales, where, code, kind, shape, cache, device):
+    rc = _lib.load().tfa_b200_kv_cache_store(K.data_ptr(), v, k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), where, code,
+                                             kind, shape[0], cache[0], shape[1], shape[2], cache[2], _raw_stream(device))
+    if rc != 0:
+        _lib.check(rc, "kv_cache_store")
 
 
 def flash_attn_cache_forward(Q, k_cache, v_cache, k_scales, v_scales, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_kv,
@@ -111,34 +140,31 @@ def flash_attn_cache_forward(Q, k_cache, v_cache, k_scales, v_scales, block_tabl
     cu_seqlens_q int32 [B + 1]; max_seqlen_q / max_seqlen_kv only size the launch.  is_causal: a query sees keys up to its own position, else
     all of its request's.  softcap and alibi_slopes as in flash_attn_scored_forward.  Rows of no request and rows that see no key are zero.
     """
-    _check_input(Q, "Q")
-    _check(Q.dim() == 3, "Q must be 3D [totalQ, numHeadsQ, headDim]")
-    _check(Q.dtype in (torch.float16, torch.bfloat16), f"flash_attn_cache_forward only supports fp16 and bf16, got {Q.dtype}")
-    device = Q.get_device()
-    _check_cache(k_cache, v_cache, k_scales, v_scales, device)
-    total, heads_q, head_dim = Q.shape
-    blocks, heads_kv, block_tokens, _ = k_cache.shape
-    _check(k_cache.shape[3] == head_dim, "Head dims must match")
-    _check(heads_kv > 0 and heads_q % heads_kv == 0, "numHeadsQ must be divisible by numHeadsKV (GQA)")
-    _check_input(block_table, "block_table")
-    _check(block_table.dim() == 2, "block_table must be int32 [batch, maxBlocks]")
-    _check(seq_lens is not None and cu_seqlens_q is not None, "seq_lens and cu_seqlens_q must be tensors")
-    batch, width = block_table.shape
-    table = _check_aux(block_table, "block_table", torch.int32, (batch, width), device)
-    lens = _check_aux(seq_lens, "seq_lens", torch.int32, (batch,), device)
-    cu = _check_aux(cu_seqlens_q, "cu_seqlens_q", torch.int32, (batch + 1,), device)
-    slopes = _check_aux(alibi_slopes, "alibi_slopes", torch.float32, (heads_q,), device)
-    max_q, max_kv, softcap = int(max_seqlen_q), int(max_seqlen_kv), _check_softcap(softcap)
+    shape, dtype, device = _rows_shape(Q, "Q", "[totalQ, numHeadsQ, headDim]")
+    code = _QUERY_CODE.get(dtype)
+    if code is None:
+        raise RuntimeError(f"flash_attn_cache_forward only supports fp16 and bf16, got {dtype}")
+    cache, kind = _cache_shape(k_cache, v_cache, k_scales, v_scales, device)
+    _check(cache[3] == shape[2], "Head dims must match")
+    _check(cache[1] > 0 and shape[1] % cache[1] == 0, "numHeadsQ must be divisible by numHeadsKV (GQA)")
+    batch, width = table_shape = _table_shape(block_table)
+    table = _aux(block_table, "block_table", torch.int32, table_shape, device)
+    lens = _aux(seq_lens, "seq_lens", torch.int32, (batch,), device)
+    cu = _aux(cu_seqlens_q, "cu_seqlens_q", torch.int32, (batch + 1,), device)
+    slopes = _aux(alibi_slopes, "alibi_slopes", torch.float32, (shape[1],), device) if alibi_slopes is not None else None
+    _check_softcap(softcap)
     _check_no_grad(Q, alibi_slopes)
+    sizes = (batch, int(max_seqlen_q), int(max_seqlen_kv), shape[0], cache[0], width, cache[2], shape[1], cache[1], shape[2])
+    if _current_device() == device:
+        return _run_cache(Q, k_cache, v_cache, k_scales, v_scales, table, lens, cu, code, kind, sizes, is_causal, softcap, slopes, device)
+    with torch.cuda.device(device):
+        return _run_cache(Q, k_cache, v_cache, k_scales, v_scales, table, lens, cu, code, kind, sizes, is_causal, softcap, slopes, device)
 
-    def call():
-        O = torch.empty_like(Q)
-        rc = _lib.load().tfa_b200_fwd_cache(Q.data_ptr(), O.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(),
-                                            v_scales.data_ptr(), table, lens, cu, _DTYPE_CODE[Q.dtype], _CACHE_CODE[k_cache.dtype], batch, max_q,
-                                            max_kv, total, blocks, width, block_tokens, heads_q, heads_kv, head_dim, 1 if is_causal else 0,
-                                            softcap, slopes, _raw_stream(device))
-        if rc != 0:
-            _lib.check(rc, "flash_attn_cache_forward")
-        return O
 
-    return _on_device(device, call)
+def _run_cache(Q, k_cache, v_cache, k_scales, v_scales, table, lens, cu, code, kind, sizes, is_causal, softcap, slopes, device):
+    O = torch.empty_like(Q)
+    rc = _lib.load().tfa_b200_fwd_cache(Q.data_ptr(), O.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), table,
+                                        lens, cu, code, kind, *sizes, 1 if is_causal else 0, softcap, slopes, _raw_stream(device))
+    if rc != 0:
+        _lib.check(rc, "flash_attn_cache_forward")
+    return O

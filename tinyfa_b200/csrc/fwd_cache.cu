@@ -4,17 +4,20 @@
 //   O = sum_j exp(S_j) v_j / sum_j exp(S_j) over the keys j <= pos of a query at position pos (all keys without the causal mask)
 //
 // Bound by HBM: every code is read once per KV head, the products are a few per cent of the time.  So the kernel is a stream:
-//   * the query rows that share a KV head form tiles of 16 rows; the 64-key blocks of all (request, tile) units in a row are cut
+//   * the query rows that share a KV head form tiles of 8 (or 16) rows; the 64-key blocks of all (request, tile) units in a row are cut
 //     into equal runs, one CTA per run and KV head, whatever the lengths are - which only the device knows;
-//   * each of a CTA's four warps takes every fourth 16-key slice, with a ring of its own that cp.async fills several slices ahead,
-//     across the ends of requests, and a running maximum and sum of its own.  Nothing but the end of a unit synchronises the CTA;
+//   * each of a CTA's four warps takes every fourth 16-key slice, with a ring of its own that cp.async fills slices ahead, across the
+//     ends of requests, and a running reference value and sum of its own.  Nothing but the end of a unit synchronises the CTA;
 //   * codes become fp16 exactly (int8 and e4m3 both fit its 11 bits), so mma.sync sees the codes themselves: the scale of a block of
 //     keys multiplies the scores, the scale of a block of values the weights.  bf16 queries become fp16 with a power of two per row
 //     taken out, which loses only what lies 2^-31 below the row's largest element;
-//   * the contraction index of Q.K^T and the column index of P.V are permuted so that a lane's operands are 16 (D = 128) contiguous
-//     bytes of a cache row; P.V needs two byte permutes per four codes to bring two keys together;
-//   * weights are stored relative to the largest block scale of V seen so far and 2^10 up, so that the fp16 weights of a block
-//     whose scale is 2^-23 of the largest still have all their bits;
+//   * both products are transposed, S^T = K Q^T and O^T = V^T P^T, so that the 16 rows of an MMA are keys and head-dim elements and its
+//     8 columns the query rows, of which a decode step has few: half the MMAs, half the accumulators and half the exponentials of
+//     tiles of 16 query rows.  P^T becomes the other operand with two 8 x 8 transposes (movmatrix);
+//   * the contraction index of S^T and the row index of O^T are permuted so that a lane's codes are 16 (D = 128) contiguous bytes of a
+//     cache row; O^T needs two byte permutes per four codes to bring two keys together;
+//   * weights are stored relative to a scale of V that is at most 2^3 below the largest seen and 2^4 up, so that the fp16 weights of a
+//     block whose scale is 2^-18 of the largest still have all their bits;
 //   * a unit that several runs share is put together by the CTA that finishes last, which it learns from a counter.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -69,8 +72,10 @@ namespace cache {
 
 constexpr int kThreads = 128;
 constexpr int kBlockKeys = 64;  // unit of the partition: a slice of 16 keys for each warp
-constexpr int kRows = 16;       // query rows of a tile (MMA M)
-constexpr float kUp = 1024.f;   // weights are stored this much larger
+constexpr int kRows = 16;       // most query rows of a tile
+// A row's reference value follows its maximum when that is 2^8 ahead, the reference scale of V when a scale is 2^3 ahead; weights are stored
+// 2^4 larger: at most 2^15, within fp16.
+constexpr float kLag = 8.f, kScaleLag = 8.f, kUp = 16.f;
 
 struct Params {
   const void* Q;
@@ -90,8 +95,8 @@ struct Params {
   int totalQ;
   float scaleLog2;  // log2(e) / sqrt(D)
   float cap;        // 0: none
-  float* partO;     // [runs][headsKV][2][16][D] normalised
-  float* partLse;   // [runs][headsKV][2][16]
+  float* partO;     // [runs][headsKV][2][rows of a tile][D] normalised
+  float* partLse;   // [runs][headsKV][2][rows of a tile]
   int* join;        // [runs][headsKV], zero
 };
 
@@ -105,22 +110,29 @@ template <int D>
 constexpr int v_pitch() {
   return D + 16;
 }
-template <int D>
-constexpr int stages() {
-  return D <= 64 ? 6 : 4;
-}
 constexpr int kHeader = 16;  // scale of K, scale of V, whether the block exists
 template <int D>
 constexpr int stage_bytes() {
   return 16 * (k_pitch<D>() + v_pitch<D>()) + kHeader;
 }
-template <int D>
-constexpr int ring_bytes() {
-  return 4 * stages<D>() * stage_bytes<D>();
+// CTAs of an SM that registers allow (O^T and Q take 3 D / 8 a thread for 8 rows, twice that for 16), and slices in a warp's ring: what shared
+// memory holds then, three to six of them.
+template <int D, int NR>
+constexpr int ctas_per_sm() {
+  return D <= 64 ? (NR == 1 ? 5 : 4) : D <= 128 ? (NR == 1 ? 3 : 2) : NR == 1 ? 2 : 1;
 }
-template <int D>
+template <int D, int NR>
 constexpr int merge_bytes() {
-  return (kRows * (D + 8) + 8 * kRows) * (int)sizeof(float);
+  return (8 * NR * (D + 8) + 2 * 4 * 8 * NR) * (int)sizeof(float);
+}
+template <int D, int NR>
+constexpr int stages() {
+  constexpr int room = (227 * 1024 / ctas_per_sm<D, NR>() - 1536 - merge_bytes<D, NR>()) / (4 * stage_bytes<D>());
+  return room > 6 ? 6 : room;
+}
+template <int D, int NR>
+constexpr int ring_bytes() {
+  return 4 * stages<D, NR>() * stage_bytes<D>();
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -140,6 +152,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 8 x 8 matrix of 16-bit elements, a row per quad of lanes -> its transpose
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -189,26 +207,29 @@ struct Segment {
   int keyEnd;         // keys that some row of the tile sees
 };
 
-template <int D>
+template <int NR>
 __device__ __forceinline__ int tiles_of(int nq, int group) {
-  return (int)(((long long)nq * group + kRows - 1) / kRows);
+  return (int)(((long long)nq * group + 8 * NR - 1) / (8 * NR));
 }
 
 // Run that holds block u of `total` blocks, i.e. the c with total * c / runs <= u < total * (c + 1) / runs.
 __device__ __forceinline__ int run_of_block(long long u, long long total, int runs) { return (int)(((u + 1) * runs - 1) / total); }
 
-template <int D, bool kInt8, bool kBf16>
-__global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) {
-  constexpr int kS = stages<D>(), kStage = stage_bytes<D>(), KP = k_pitch<D>(), VP = v_pitch<D>();
-  constexpr int kNT = D / 8;   // 8-wide column tiles of O
-  constexpr int kLdO = D + 8;  // row pitch of the merge buffer
+// NR: tiles of 8 NR query rows.
+template <int D, bool kInt8, bool kBf16, int NR>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_kernel(const Params p) {
+  constexpr int kS = stages<D, NR>(), kStage = stage_bytes<D>(), KP = k_pitch<D>(), VP = v_pitch<D>();
+  static_assert(kS >= 2, "a slice to work on and one on its way");
+  constexpr int kTile = 8 * NR;  // query rows
+  constexpr int kMT = D / 16;    // 16-element row tiles of O^T
+  constexpr int kLdO = D + 8;    // row pitch of the merge buffer
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long sScan[kThreads / 32];
-  __shared__ long long sPlace[3];  // unit that holds the run's first block: request, unit's first block, 1 if found
+  __shared__ long long sPlace[2];  // unit that holds the run's first block: request, blocks ahead of the request
   __shared__ int sLast;
-  float* sO = reinterpret_cast<float*>(smem + ring_bytes<D>());  // [16][kLdO]
-  float* sM = sO + kRows * kLdO;                                 // [4][16]
-  float* sL = sM + 4 * kRows;                                    // [4][16]
+  float* sO = reinterpret_cast<float*>(smem + ring_bytes<D, NR>());  // [kTile][kLdO]
+  float* sM = sO + kTile * kLdO;                                     // [4][kTile]
+  float* sL = sM + 4 * kTile;                                        // [4][kTile]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, tig = lane & 3;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kS * kStage;
@@ -229,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
   auto blocks_of_request = [&](int b) -> long long {
     int q0, nq, len;
     request(b, q0, nq, len);
-    return (long long)tiles_of<D>(nq, p.group) * unit_blocks(len);
+    return (long long)tiles_of<NR>(nq, p.group) * unit_blocks(len);
   };
   // ---- the blocks of all requests, and where this run begins among them
   long long mine = 0, total = 0;
@@ -297,7 +318,7 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
   }
 
   auto finish = [&](Segment& s) {  // the fields that follow from the request and the tile
-    const int lastRow = min((s.tile + 1) * kRows, s.nq * p.group) - 1;
+    const int lastRow = min((s.tile + 1) * kTile, s.nq * p.group) - 1;
     s.keyEnd = p.causal ? min(s.len, s.len - s.nq + lastRow / p.group + 1) : s.len;
   };
   long long left;  // blocks of the run behind the segment
@@ -314,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
   };
   auto next_segment = [&](Segment& s, long long& rest) {  // rest > 0
     s.tile++;
-    if (s.tile >= tiles_of<D>(s.nq, p.group)) {
+    if (s.tile >= tiles_of<NR>(s.nq, p.group)) {
       s.tile = 0;
       do {  // ends: `rest` blocks are still to come
         s.b++;
@@ -354,17 +375,23 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
       const bool ok = ldPage >= 0 && ldPage < p.numBlocks;
       const long long tile = ok ? (long long)ldPage * p.headsKV + hkv : 0;
       const int rows = ok ? min(16, ls.len - ldKey) : 0;  // keys of the slice
-      const uint8_t* k = p.kCodes + tile * headBytes + (ldKey & ((1 << p.blockShift) - 1)) * D;
-      const uint8_t* v = p.vCodes + tile * headBytes + (ldKey & ((1 << p.blockShift) - 1)) * D;
+      const long long from = tile * headBytes + (ldKey & ((1 << p.blockShift) - 1)) * D + lane * 16;
+      const uint8_t* k = p.kCodes + from;
+      const uint8_t* v = p.vCodes + from;
+      if (rows == 16) {
 #pragma unroll
-      for (int i = 0; i < D / 32; i++) {
-        const int c = lane + i * 32, r = c / (D / 16), col = c % (D / 16) * 16;
-        cp_async16(st + r * KP + col, k + (r < rows ? c * 16 : 0), r < rows);
-      }
+        for (int i = 0; i < D / 32; i++) {
+          const int c = lane + i * 32, r = c / (D / 16), col = c % (D / 16) * 16;
+          cp_async16(st + r * KP + col, k + i * 512, true);
+          cp_async16(st + 16 * KP + r * VP + col, v + i * 512, true);
+        }
+      } else {  // what the request does not have is zero
 #pragma unroll
-      for (int i = 0; i < D / 32; i++) {
-        const int c = lane + i * 32, r = c / (D / 16), col = c % (D / 16) * 16;
-        cp_async16(st + 16 * KP + r * VP + col, v + (r < rows ? c * 16 : 0), r < rows);
+        for (int i = 0; i < D / 32; i++) {
+          const int c = lane + i * 32, r = c / (D / 16), col = c % (D / 16) * 16;
+          cp_async16(st + r * KP + col, r < rows ? k + i * 512 : p.kCodes, r < rows);
+          cp_async16(st + 16 * KP + r * VP + col, r < rows ? v + i * 512 : p.vCodes, r < rows);
+        }
       }
       const uint32_t head = st + 16 * (KP + VP);
       if (lane == 0) {
@@ -383,190 +410,190 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
   for (int i = 0; i < kS - 1; i++) issue();
 
   // ---- the units of the run
-  const int rowA = g, rowB = g + 8;
   Segment s;
   first_segment(s, left);
   bool firstSegment = true;
   int stage = 0;
   for (;;) {
-    const int nRows = min(s.nq * p.group - s.tile * kRows, kRows);
-    const int flatA = s.tile * kRows + rowA, flatB = s.tile * kRows + rowB;
-    const bool validA = rowA < nRows, validB = rowB < nRows;
-    const int tokA = validA ? flatA / p.group : 0, tokB = validB ? flatB / p.group : 0;
-    const int headA = hkv * p.group + (validA ? flatA % p.group : 0), headB = hkv * p.group + (validB ? flatB % p.group : 0);
-    const int posA = s.len - s.nq + tokA, posB = s.len - s.nq + tokB;
-    const float slopeA = p.slopes != nullptr ? p.slopes[headA] * 1.44269504f : 0.f;
-    const float slopeB = p.slopes != nullptr ? p.slopes[headB] * 1.44269504f : 0.f;
-    // Q fragments, permuted like the lanes' bytes of K; factors of the scores
-    uint32_t qf[D / 16][4];
-    float facA = p.scaleLog2, facB = p.scaleLog2;
-    {
-      const uint16_t* gQ = static_cast<const uint16_t*>(p.Q);
-      const uint16_t* qa = gQ + ((long long)(s.q0 + tokA) * p.headsQ + headA) * D;
-      const uint16_t* qb = gQ + ((long long)(s.q0 + tokB) * p.headsQ + headB) * D;
+    const int nRows = min(s.nq * p.group - s.tile * kTile, kTile);
+    // Q as the columns of S^T: row 8 nr + g of the tile, permuted like the lanes' bytes of K
+    uint32_t qf[D / 16][NR][2];
+    float rowDown[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+      const int row = nr * 8 + g, flat = s.tile * kTile + row;
+      const bool valid = row < nRows;
+      const uint16_t* q = static_cast<const uint16_t*>(p.Q) +
+                          ((long long)(s.q0 + (valid ? flat / p.group : 0)) * p.headsQ + hkv * p.group + (valid ? flat % p.group : 0)) * D;
 #pragma unroll
       for (int w = 0; w < D / 16; w++) {
-        const uint2 a = *reinterpret_cast<const uint2*>(qa + k_byte<D>(w, tig)), b = *reinterpret_cast<const uint2*>(qb + k_byte<D>(w, tig));
-        qf[w][0] = validA ? a.x : 0u;
-        qf[w][1] = validB ? b.x : 0u;
-        qf[w][2] = validA ? a.y : 0u;
-        qf[w][3] = validB ? b.y : 0u;
+        const uint2 x = *reinterpret_cast<const uint2*>(q + k_byte<D>(w, tig));
+        qf[w][nr][0] = valid ? x.x : 0u;
+        qf[w][nr][1] = valid ? x.y : 0u;
       }
-      if constexpr (kBf16) {
-        uint32_t ma = 0, mb = 0;
+      constexpr uint32_t kE = exponent_bits<kBf16>();
+      uint32_t top = 0;
 #pragma unroll
-        for (int w = 0; w < D / 16; w++) {
-          ma = max(max(ma, qf[w][0] & 0x7F80u), max(qf[w][0] >> 16 & 0x7F80u, max(qf[w][2] & 0x7F80u, qf[w][2] >> 16 & 0x7F80u)));
-          mb = max(max(mb, qf[w][1] & 0x7F80u), max(qf[w][1] >> 16 & 0x7F80u, max(qf[w][3] & 0x7F80u, qf[w][3] >> 16 & 0x7F80u)));
-        }
-        ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
-        ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 2));
-        mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
-        mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
-        float upA, upB, dnA, dnB;
-        row_scale(ma, upA, dnA);
-        row_scale(mb, upB, dnB);
-        facA *= dnA;
-        facB *= dnB;
+      for (int w = 0; w < D / 16; w++) {
+        top = max(max(top, qf[w][nr][0] & kE), max(qf[w][nr][0] >> 16 & kE, max(qf[w][nr][1] & kE, qf[w][nr][1] >> 16 & kE)));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      float up;
+      row_scale<kBf16>(top, up, rowDown[nr]);
 #pragma unroll
-        for (int w = 0; w < D / 16; w++) {
-          qf[w][0] = bf16_to_half2(qf[w][0], upA);
-          qf[w][1] = bf16_to_half2(qf[w][1], upB);
-          qf[w][2] = bf16_to_half2(qf[w][2], upA);
-          qf[w][3] = bf16_to_half2(qf[w][3], upB);
-        }
+      for (int w = 0; w < D / 16; w++) {
+        qf[w][nr][0] = scale_to_half2<kBf16>(qf[w][nr][0], up);
+        qf[w][nr][1] = scale_to_half2<kBf16>(qf[w][nr][1], up);
       }
     }
+    // this thread's columns of S^T and O^T: rows 8 nr + 2 tig + e
+    float fac[NR][2], slope[NR][2];
+    int pos[NR][2];
     const float capLog2 = p.cap * 1.44269504f;
-    if (p.cap > 0.f) {  // scores as arguments 2 log2(e) S / c of the exponential that gives the tanh
-      const float f = 2.f / p.cap;
-      facA *= f;
-      facB *= f;
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int row = nr * 8 + 2 * tig + e, flat = s.tile * kTile + (row < nRows ? row : 0);
+        // capped: scores as arguments 2 log2(e) S / c of the exponential that gives the tanh
+        fac[nr][e] = __shfl_sync(0xffffffffu, rowDown[nr], (2 * tig + e) * 4) * p.scaleLog2 * (p.cap > 0.f ? 2.f / p.cap : 1.f);
+        pos[nr][e] = s.len - s.nq + flat / p.group;
+        slope[nr][e] = p.slopes != nullptr ? p.slopes[hkv * p.group + flat % p.group] * 1.44269504f : 0.f;
+      }
     }
 
-    float o[kNT][4];
+    float o[kMT][NR][4];
 #pragma unroll
-    for (int i = 0; i < kNT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
-    float vRef = 0.f, vRefInv = 0.f;  // largest scale of V so far; O holds sums of 2^10 p v / vRef
+    for (int i = 0; i < kMT; i++) {
+#pragma unroll
+      for (int nr = 0; nr < NR; nr++) o[i][nr][0] = o[i][nr][1] = o[i][nr][2] = o[i][nr][3] = 0.f;
+    }
+    float ref[NR][2], limit[NR][2], l[NR][2];  // reference value (0 until a key is seen), score that moves it, sum of this thread's keys
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) ref[nr][0] = ref[nr][1] = l[nr][0] = l[nr][1] = 0.f, limit[nr][0] = limit[nr][1] = -INFINITY;
+    float vRef = 0.f, vUp = 0.f;  // scale of V that O refers to: O holds sums of 2^4 p v / vRef
 
-    const int keyStop = seg_key_end(s);
+    const int keyStop = seg_key_end(s), seenByAll = p.causal ? s.len - s.nq + s.tile * kTile / p.group : s.len - 1;
     for (int key0 = s.blk * kBlockKeys + warp * 16; key0 < keyStop; key0 += kBlockKeys) {
       cp_async_wait<kS - 2>();
-      __syncwarp();
+      __syncwarp();  // ... and every lane has read the stage of the slice before
+      if (kS == 2) issue();  // nothing else is on its way: D = 256, 64 x 4000 tokens 202 -> 176 us (and 99 -> 99.5 at 128, where two more are)
       const uint32_t st = ring + stage * kStage;
       float ks, vs;
       uint32_t there;
       asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks) : "r"(st + 16 * (KP + VP)));
       asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs) : "r"(st + 16 * (KP + VP) + 4));
       asm volatile("ld.shared.b32 %0, [%1];" : "=r"(there) : "r"(st + 16 * (KP + VP) + 8));
-      // ---- S = Q K^T for 16 rows x 16 keys
-      float sc[2][4];
+      // ---- S^T = K Q^T: 16 keys x 8 NR rows
+      float sc[NR][4], sd[NR][4];  // two chains of MMAs
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-        const uint32_t row = st + (n * 8 + g) * KP;
+      for (int nr = 0; nr < NR; nr++) {
+        sc[nr][0] = sc[nr][1] = sc[nr][2] = sc[nr][3] = 0.f;
+        sd[nr][0] = sd[nr][1] = sd[nr][2] = sd[nr][3] = 0.f;
+      }
+      const uint32_t k0 = st + g * KP, k1 = k0 + 8 * KP;
+      auto scores = [&](uint32_t w0, uint32_t w1, int step) {
+        uint32_t a[4];
+        widen<kInt8>(w0, a[0], a[2]);
+        widen<kInt8>(w1, a[1], a[3]);
 #pragma unroll
-        for (int c = 0; c < D / 64; c++) {
-          uint32_t w[4];
-          lds_words<4, 16>(row + c * 64 + tig * 16, w);
+        for (int nr = 0; nr < NR; nr++) mma_f16((step & 1) ? sd[nr] : sc[nr], a, qf[step][nr][0], qf[step][nr][1]);
+      };
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            uint32_t b0, b1;
-            widen<kInt8>(w[i], b0, b1);
-            mma_f16(sc[n], qf[c * 4 + i], b0, b1);
-          }
-        }
-        if constexpr (D % 64 != 0) {
-          uint32_t w[2];
-          lds_words<2, 8>(row + D / 64 * 64 + tig * 8, w);
+      for (int c = 0; c < D / 64; c++) {
+        uint32_t w0[4], w1[4];
+        lds_words<4, 16>(k0 + c * 64 + tig * 16, w0);
+        lds_words<4, 16>(k1 + c * 64 + tig * 16, w1);
 #pragma unroll
-          for (int i = 0; i < 2; i++) {
-            uint32_t b0, b1;
-            widen<kInt8>(w[i], b0, b1);
-            mma_f16(sc[n], qf[D / 64 * 4 + i], b0, b1);
-          }
-        }
+        for (int i = 0; i < 4; i++) scores(w0[i], w1[i], c * 4 + i);
+      }
+      if constexpr (D % 64 != 0) {
+        uint32_t w0[2], w1[2];
+        lds_words<2, 8>(k0 + D / 64 * 64 + tig * 8, w0);
+        lds_words<2, 8>(k1 + D / 64 * 64 + tig * 8, w1);
+#pragma unroll
+        for (int i = 0; i < 2; i++) scores(w0[i], w1[i], D / 64 * 4 + i);
       }
       // ---- scores in units of log2, capped, biased, masked
-      const float fA = facA * ks, fB = facB * ks;
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
+      for (int nr = 0; nr < NR; nr++) {
+        const float f0 = fac[nr][0] * ks, f1 = fac[nr][1] * ks;
 #pragma unroll
-        for (int e = 0; e < 4; e++) sc[n][e] *= e < 2 ? fA : fB;
-      }
-      if (p.cap > 0.f) {  // c tanh(x) = c - 2 c / (e^2x + 1)
+        for (int e = 0; e < 4; e++) sc[nr][e] = (sc[nr][e] + sd[nr][e]) * ((e & 1) ? f1 : f0);
+        if (p.cap > 0.f) {  // c tanh(x) = c - 2 c / (e^2x + 1)
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) sc[n][e] = fmaf(-2.f * capLog2, rcp(ex2(sc[n][e]) + 1.f), capLog2);
+          for (int e = 0; e < 4; e++) sc[nr][e] = fmaf(-2.f * capLog2, rcp(ex2(sc[nr][e]) + 1.f), capLog2);
         }
-      }
-      if (p.slopes != nullptr) {
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
+        if (p.slopes != nullptr) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const int key = key0 + n * 8 + 2 * tig + (e & 1);
-            sc[n][e] = fmaf(e < 2 ? -slopeA : -slopeB, fabsf((float)((e < 2 ? posA : posB) - key)), sc[n][e]);
+            sc[nr][e] = fmaf(-slope[nr][e & 1], fabsf((float)(pos[nr][e & 1] - (key0 + g + (e >> 1) * 8))), sc[nr][e]);
           }
         }
       }
-      if (!there || key0 + 16 > s.len || (p.causal && key0 + 15 > s.len - s.nq + s.tile * kRows / p.group)) {
-        const int limA = !there ? 0 : p.causal ? min(s.len, posA + 1) : s.len, limB = !there ? 0 : p.causal ? min(s.len, posB + 1) : s.len;
+      if (!there || key0 + 16 > s.len || key0 + 15 > seenByAll) {
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
+        for (int nr = 0; nr < NR; nr++) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            if (key0 + n * 8 + 2 * tig + (e & 1) >= (e < 2 ? limA : limB)) sc[n][e] = -INFINITY;
+            const int lim = !there ? 0 : p.causal ? min(s.len, pos[nr][e & 1] + 1) : s.len;
+            if (key0 + g + (e >> 1) * 8 >= lim) sc[nr][e] = -INFINITY;
           }
         }
       }
-      // ---- running maximum and sum for rows g (A) and g + 8 (B)
-      float mxA = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-      float mxB = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
-      mxA = fmaxf(mxA, __shfl_xor_sync(0xffffffffu, mxA, 1));
-      mxA = fmaxf(mxA, __shfl_xor_sync(0xffffffffu, mxA, 2));
-      mxB = fmaxf(mxB, __shfl_xor_sync(0xffffffffu, mxB, 1));
-      mxB = fmaxf(mxB, __shfl_xor_sync(0xffffffffu, mxB, 2));
-      const float mnA = fmaxf(mA, mxA), mnB = fmaxf(mB, mxB);
-      if (__any_sync(0xffffffffu, mnA > mA || mnB > mB || vs > vRef)) {
+      // ---- rows whose scores are far above their reference, or values far above theirs: rare
+      bool move = vs > vRef * kScaleLag;
+#pragma unroll
+      for (int nr = 0; nr < NR; nr++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) move = move || sc[nr][e] > limit[nr][e & 1];
+      }
+      if (__any_sync(0xffffffffu, move)) {
         const float vNew = fmaxf(vRef, vs);
         const float fv = vNew > vRef ? vRef / vNew : 1.f;
-        const float scA = mA == -INFINITY ? 0.f : ex2(mA - mnA), scB = mB == -INFINITY ? 0.f : ex2(mB - mnB);
-        lA *= scA;
-        lB *= scB;
-        const float oA = scA * fv, oB = scB * fv;
-#pragma unroll
-        for (int i = 0; i < kNT; i++) {
-          o[i][0] *= oA;
-          o[i][1] *= oA;
-          o[i][2] *= oB;
-          o[i][3] *= oB;
-        }
-        mA = mnA;
-        mB = mnB;
         vRef = vNew;
-        vRefInv = vNew > 0.f ? kUp / vNew : 0.f;
-      }
-      const float muA = mA == -INFINITY ? 0.f : mA, muB = mB == -INFINITY ? 0.f : mB;
-      const float wv = vs * vRefInv;
-      float pA[4], pB[4];
+        vUp = vNew > 0.f ? fminf(1.f / vNew, 1e37f) * kUp : 0.f;
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        pA[n * 2 + 0] = ex2(sc[n][0] - muA);
-        pA[n * 2 + 1] = ex2(sc[n][1] - muA);
-        pB[n * 2 + 0] = ex2(sc[n][2] - muB);
-        pB[n * 2 + 1] = ex2(sc[n][3] - muB);
+        for (int nr = 0; nr < NR; nr++) {
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float top = fmaxf(sc[nr][e], sc[nr][e + 2]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const bool none = limit[nr][e] == -INFINITY;  // no key so far
+            const float now = none ? top : fmaxf(ref[nr][e], top);
+            const float f = none ? 0.f : ex2(ref[nr][e] - now);
+            if (now != -INFINITY) {
+              ref[nr][e] = now;
+              limit[nr][e] = now + kLag;
+            }
+            l[nr][e] *= f;
+            const float fo = f * fv;
+#pragma unroll
+            for (int i = 0; i < kMT; i++) {
+              o[i][nr][e] *= fo;
+              o[i][nr][e + 2] *= fo;
+            }
+          }
+        }
       }
-      lA += (pA[0] + pA[1]) + (pA[2] + pA[3]);  // per-thread partial, reduced over the quad at the end
-      lB += (pB[0] + pB[1]) + (pB[2] + pB[3]);
-      uint32_t pf[4];  // weights to 11 bits: half a step is 2^-12 of a weight
-      pf[0] = half2_of(pA[0] * wv, pA[1] * wv);
-      pf[1] = half2_of(pB[0] * wv, pB[1] * wv);
-      pf[2] = half2_of(pA[2] * wv, pA[3] * wv);
-      pf[3] = half2_of(pB[2] * wv, pB[3] * wv);
-      // ---- O += P V: column n of tile j is head-dim element n * D / 8 + j, so that a lane's D / 8 codes of a key are contiguous
+      // ---- weights: 11 bits, half a step is 2^-12 of a weight
+      const float wv = vs * vUp;
+      uint32_t pf[NR][2];
+#pragma unroll
+      for (int nr = 0; nr < NR; nr++) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = ex2(sc[nr][e] - ref[nr][e & 1]);
+        l[nr][0] += w[0] + w[2];
+        l[nr][1] += w[1] + w[3];
+        pf[nr][0] = transpose8x8(half2_of(w[0] * wv, w[1] * wv));
+        pf[nr][1] = transpose8x8(half2_of(w[2] * wv, w[3] * wv));
+      }
+      // ---- O^T += V^T P^T: rows g and g + 8 of tile j are head-dim elements g D / 8 + 2 j and + 1, so that a lane's D / 8 codes of a key are
+      // contiguous
       constexpr int kAlign = (D / 8) % 16 == 0 ? 16 : (D / 8) % 8 == 0 ? 8 : 4;
       constexpr int kPiece = kAlign / 4;
       const uint32_t vr = st + 16 * KP + g * (D / 8);
@@ -577,50 +604,66 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
         for (int i = 0; i < 4; i++) lds_words<kPiece, kAlign>(vr + (2 * tig + (i & 1) + (i >> 1) * 8) * VP + c * 4, w[i]);
 #pragma unroll
         for (int i = 0; i < kPiece; i++) {
-          uint32_t b0[4], b1[4];
-          widen<kInt8>(__byte_perm(w[0][i], w[1][i], 0x5140), b0[0], b0[1]);
-          widen<kInt8>(__byte_perm(w[0][i], w[1][i], 0x7362), b0[2], b0[3]);
-          widen<kInt8>(__byte_perm(w[2][i], w[3][i], 0x5140), b1[0], b1[1]);
-          widen<kInt8>(__byte_perm(w[2][i], w[3][i], 0x7362), b1[2], b1[3]);
+          uint32_t lo[4], hi[4];  // by head-dim element: keys 2 tig, 2 tig + 1 and 2 tig + 8, 2 tig + 9
+          widen<kInt8>(__byte_perm(w[0][i], w[1][i], 0x5140), lo[0], lo[1]);
+          widen<kInt8>(__byte_perm(w[0][i], w[1][i], 0x7362), lo[2], lo[3]);
+          widen<kInt8>(__byte_perm(w[2][i], w[3][i], 0x5140), hi[0], hi[1]);
+          widen<kInt8>(__byte_perm(w[2][i], w[3][i], 0x7362), hi[2], hi[3]);
 #pragma unroll
-          for (int j = 0; j < 4; j++) mma_f16(o[(c + i) * 4 + j], pf, b0[j], b1[j]);
+          for (int j = 0; j < 2; j++) {
+            const uint32_t a[4] = {lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1]};
+#pragma unroll
+            for (int nr = 0; nr < NR; nr++) mma_f16(o[(c + i) * 2 + j][nr], a, pf[nr][0], pf[nr][1]);
+          }
         }
       }
-      __syncwarp();  // every lane has read the stage before the next issue overwrites it
       stage = stage + 1 == kS ? 0 : stage + 1;
-      issue();
+      if (kS > 2) {
+        __syncwarp();
+        issue();
+      }
     }
 
     // ---- the four warps' shares of the unit, one after the other
-    lA += __shfl_xor_sync(0xffffffffu, lA, 1);
-    lA += __shfl_xor_sync(0xffffffffu, lA, 2);
-    lB += __shfl_xor_sync(0xffffffffu, lB, 1);
-    lB += __shfl_xor_sync(0xffffffffu, lB, 2);
-    if (tig == 0) {
-      sM[warp * kRows + rowA] = mA;
-      sM[warp * kRows + rowB] = mB;
-      sL[warp * kRows + rowA] = lA;
-      sL[warp * kRows + rowB] = lB;
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        l[nr][e] += __shfl_xor_sync(0xffffffffu, l[nr][e], 4);
+        l[nr][e] += __shfl_xor_sync(0xffffffffu, l[nr][e], 8);
+        l[nr][e] += __shfl_xor_sync(0xffffffffu, l[nr][e], 16);
+        if (g == 0) {
+          sM[warp * kTile + nr * 8 + 2 * tig + e] = limit[nr][e] == -INFINITY ? -INFINITY : ref[nr][e];
+          sL[warp * kTile + nr * 8 + 2 * tig + e] = l[nr][e];
+        }
+      }
     }
     __syncthreads();
     {
-      float MA = -INFINITY, MB = -INFINITY;
+      float f[NR][2];
 #pragma unroll
-      for (int w = 0; w < 4; w++) {
-        MA = fmaxf(MA, sM[w * kRows + rowA]);
-        MB = fmaxf(MB, sM[w * kRows + rowB]);
+      for (int nr = 0; nr < NR; nr++) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float M = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < 4; w++) M = fmaxf(M, sM[w * kTile + nr * 8 + 2 * tig + e]);
+          f[nr][e] = (limit[nr][e] == -INFINITY ? 0.f : ex2(ref[nr][e] - M)) * vRef * (1.f / kUp);
+        }
       }
-      const float down = vRef * (1.f / kUp);
-      const float fA = (mA == -INFINITY ? 0.f : ex2(mA - MA)) * down, fB = (mB == -INFINITY ? 0.f : ex2(mB - MB)) * down;
 #pragma unroll 1
       for (int w = 0; w < 4; w++) {
         if (w == warp) {
 #pragma unroll
-          for (int j = 0; j < kNT; j++) {
+          for (int nr = 0; nr < NR; nr++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              float* at = sO + (e < 2 ? rowA : rowB) * kLdO + (2 * tig + (e & 1)) * (D / 8) + j;
-              *at = fmaf(o[j][e], e < 2 ? fA : fB, w == 0 ? 0.f : *at);
+            for (int e = 0; e < 2; e++) {
+              float2* at = reinterpret_cast<float2*>(sO + (nr * 8 + 2 * tig + e) * kLdO + g * (D / 8));
+#pragma unroll
+              for (int j = 0; j < kMT; j++) {
+                const float2 z = w == 0 ? make_float2(0.f, 0.f) : at[j];
+                at[j] = make_float2(fmaf(o[j][nr][e], f[nr][e], z.x), fmaf(o[j][nr][e + 2], f[nr][e], z.y));
+              }
             }
           }
         }
@@ -630,7 +673,7 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
     const bool whole = s.blk == 0 && s.end == s.blocks;
     const long long slot = ((long long)run * p.headsKV + hkv) * 2 + (firstSegment ? 0 : 1);
     auto store = [&](int r, int c4, float4 acc) {
-      const int flat = s.tile * kRows + r;
+      const int flat = s.tile * kTile + r;
       uint16_t* dst = static_cast<uint16_t*>(p.O) + ((long long)(s.q0 + flat / p.group) * p.headsQ + hkv * p.group + flat % p.group) * D + c4 * 4;
       uint2 out;
       if constexpr (kBf16) {
@@ -647,11 +690,11 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
       const int r = idx / (D / 4), c4 = idx % (D / 4);
       float m = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; w++) m = fmaxf(m, sM[w * kRows + r]);
+      for (int w = 0; w < 4; w++) m = fmaxf(m, sM[w * kTile + r]);
 #pragma unroll
       for (int w = 0; w < 4; w++) {
-        const float mw = sM[w * kRows + r];
-        l += sL[w * kRows + r] * (mw == -INFINITY ? 0.f : ex2(mw - m));
+        const float mw = sM[w * kTile + r];
+        l += sL[w * kTile + r] * (mw == -INFINITY ? 0.f : ex2(mw - m));
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
       float4 acc = *reinterpret_cast<const float4*>(sO + r * kLdO + c4 * 4);
@@ -662,8 +705,8 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
       if (whole) {
         store(r, c4, acc);
       } else {
-        __stcg(reinterpret_cast<float4*>(p.partO + (slot * kRows + r) * D + c4 * 4), acc);
-        if (c4 == 0) __stcg(p.partLse + slot * kRows + r, l == 0.f ? -INFINITY : m + log2f(l));
+        __stcg(reinterpret_cast<float4*>(p.partO + (slot * kTile + r) * D + c4 * 4), acc);
+        if (c4 == 0) __stcg(p.partLse + slot * kTile + r, l == 0.f ? -INFINITY : m + log2f(l));
       }
     }
     if (!whole) {
@@ -684,32 +727,73 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
         // the unit is the first segment of every run but possibly c0, which it begins in unless it begins the run
         const int at0 = total * c0 / runs == a ? 0 : 1;
         auto part = [&](int c) { return ((long long)c * p.headsKV + hkv) * 2 + (c == c0 ? at0 : 0); };
-        for (int idx = threadIdx.x; idx < nRows * (D / 4); idx += kThreads) {
-          const int r = idx / (D / 4), c4 = idx % (D / 4);
+        // largest log-sum-exp and sum of the weights of every row, a warp each
+        for (int r = warp; r < nRows; r += 4) {
           float M = -INFINITY;
           bool nan = false;
-#pragma unroll 8
-          for (int c = c0; c <= c1; c++) {
-            const float lse = __ldcg(p.partLse + part(c) * kRows + r);
+          for (int c = c0 + lane; c <= c1; c += 32) {
+            const float lse = __ldcg(p.partLse + part(c) * kTile + r);
             nan = nan || lse != lse;
             M = fmaxf(M, lse);
           }
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
           if (M == -INFINITY) M = 0.f;
-          if (nan) M = NAN;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (__any_sync(0xffffffffu, nan)) M = NAN;
           float sum = 0.f;
-#pragma unroll 4
-          for (int c = c0; c <= c1; c++) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partO + (part(c) * kRows + r) * D + c4 * 4));
-            const float w = ex2(__ldcg(p.partLse + part(c) * kRows + r) - M);
-            acc.x = fmaf(w, v.x, acc.x);
-            acc.y = fmaf(w, v.y, acc.y);
-            acc.z = fmaf(w, v.z, acc.z);
-            acc.w = fmaf(w, v.w, acc.w);
-            sum += w;
+          for (int c = c0 + lane; c <= c1; c += 32) sum += ex2(__ldcg(p.partLse + part(c) * kTile + r) - M);
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          if (lane == 0) {
+            sM[r] = M;
+            sL[r] = sum == 0.f ? 0.f : 1.f / sum;
           }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          store(r, c4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        }
+        __syncthreads();
+        // groups of D / 4 threads take turns over the parts, four rows of a part in flight at once
+        constexpr int kVec = D / 4, kGroups = kThreads / kVec < 4 ? kThreads / kVec : 4;
+        const int group = threadIdx.x / kVec, c4 = threadIdx.x % kVec;
+#pragma unroll 1
+        for (int r0 = 0; r0 < nRows; r0 += 4) {
+          float4 acc[4];
+#pragma unroll
+          for (int r = 0; r < 4; r++) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (group < kGroups) {
+#pragma unroll 2
+            for (int c = c0 + group; c <= c1; c += kGroups) {
+              const long long at = part(c) * kTile + r0;
+              const float4 lse = __ldcg(reinterpret_cast<const float4*>(p.partLse + at));
+              float4 v[4];
+#pragma unroll
+              for (int r = 0; r < 4; r++) v[r] = __ldcg(reinterpret_cast<const float4*>(p.partO + (at + r) * D + c4 * 4));
+              const float w[4] = {ex2(lse.x - sM[r0]), ex2(lse.y - sM[r0 + 1]), ex2(lse.z - sM[r0 + 2]), ex2(lse.w - sM[r0 + 3])};
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                acc[r].x = fmaf(w[r], v[r].x, acc[r].x);
+                acc[r].y = fmaf(w[r], v[r].y, acc[r].y);
+                acc[r].z = fmaf(w[r], v[r].z, acc[r].z);
+                acc[r].w = fmaf(w[r], v[r].w, acc[r].w);
+              }
+            }
+          }
+#pragma unroll 1
+          for (int i = 0; i < kGroups; i++) {  // (rows past nRows are rubbish that nobody reads)
+            if (i == group) {
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                float4* at = reinterpret_cast<float4*>(sO + (r0 + r) * kLdO + c4 * 4);
+                const float4 z = i == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
+                *at = make_float4(acc[r].x + z.x, acc[r].y + z.y, acc[r].z + z.z, acc[r].w + z.w);
+              }
+            }
+            __syncthreads();
+          }
+        }
+        for (int idx = threadIdx.x; idx < nRows * kVec; idx += kThreads) {
+          const int r = idx / kVec, c = idx % kVec;
+          const float inv = sL[r];
+          const float4 x = *reinterpret_cast<const float4*>(sO + r * kLdO + c * 4);
+          store(r, c, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
         }
       }
     }
@@ -721,14 +805,11 @@ __global__ void __launch_bounds__(kThreads) cache_decode_kernel(const Params p) 
   cp_async_wait<0>();
 }
 
-// CTAs of an SM: what shared memory and registers (255 a thread at most) hold.
-constexpr int ctas_per_sm(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
-
-template <int D, bool kInt8, bool kBf16>
-int launch(Params& p, int maxRuns, int device, cudaStream_t stream) {
-  constexpr int kSmem = ring_bytes<D>() + merge_bytes<D>();
+template <int D, bool kInt8, bool kBf16, int NR>
+int launch(const Params& p, int device, cudaStream_t stream) {
+  constexpr int kSmem = ring_bytes<D, NR>() + merge_bytes<D, NR>();
   static_assert(kSmem <= 227 * 1024, "shared memory");
-  auto kernel = cache_decode_kernel<D, kInt8, kBf16>;
+  auto kernel = cache_decode_kernel<D, kInt8, kBf16, NR>;
   static std::once_flag once[64];
   static cudaError_t attrErr[64];
   std::call_once(once[device], [&] {
@@ -741,7 +822,7 @@ int launch(Params& p, int maxRuns, int device, cudaStream_t stream) {
     set_error_string("cudaFuncSetAttribute(%d bytes): %s", kSmem, cudaGetErrorString(attrErr[device]));
     return kCudaError;
   }
-  const cudaError_t e = launch_kernel(kernel, dim3((unsigned)(maxRuns * p.headsKV)), kThreads, kSmem, stream, may_overlap(stream), p);
+  const cudaError_t e = launch_kernel(kernel, dim3((unsigned)(p.runs * p.headsKV)), kThreads, kSmem, stream, may_overlap(stream), p);
   if (e != cudaSuccess) {
     set_error_string("cache attention kernel launch failed: %s", cudaGetErrorString(e));
     return kCudaError;
@@ -749,36 +830,66 @@ int launch(Params& p, int maxRuns, int device, cudaStream_t stream) {
   return kOk;
 }
 
-template <int D>
-int launch_typed(Params& p, bool int8, bool bf16, int runs, int device, cudaStream_t stream) {
-  (void)p; (void)int8; (void)runs; (void)device; (void)stream;
+template <int D, int NR>
+int launch_typed(const Params& p, bool int8, bool bf16, int device, cudaStream_t stream) {
+  (void)p; (void)int8; (void)device; (void)stream;
   if (bf16) {
-    if constexpr (TFA_HAVE_BF16) return int8 ? launch<D, true, true>(p, runs, device, stream) : launch<D, false, true>(p, runs, device, stream);
+    if constexpr (TFA_HAVE_BF16) return int8 ? launch<D, true, true, NR>(p, device, stream) : launch<D, false, true, NR>(p, device, stream);
   } else {
-    if constexpr (TFA_HAVE_FP16) return int8 ? launch<D, true, false>(p, runs, device, stream) : launch<D, false, false>(p, runs, device, stream);
+    if constexpr (TFA_HAVE_FP16) return int8 ? launch<D, true, false, NR>(p, device, stream) : launch<D, false, false, NR>(p, device, stream);
   }
   return kBadDtype;
 }
 
-int dispatch(Params& p, int headDim, bool int8, bool bf16, int runs, int device, cudaStream_t stream) {
+// Tiles of 8 query rows where no request has more, else of 16.
+template <int D>
+int launch_stream(Params& p, long long rows, int maxSeqLenKV, bool int8, bool bf16, int device, cudaStream_t stream) {
+  const int nr = rows <= 8 ? 1 : 2;
+  // as many runs as the GPU holds CTAs, and no more than there can be pairs of key blocks
+  const long long slots = (long long)device_num_sms(device) * (nr == 1 ? ctas_per_sm<D, 1>() : ctas_per_sm<D, 2>());
+  const long long tiles = (rows + 8 * nr - 1) / (8 * nr);
+  const long long most = (tiles * ((maxSeqLenKV + kBlockKeys - 1) / kBlockKeys) * p.batch + 1) / 2;
+  long long runs = slots / p.headsKV;
+  if (runs > most) runs = most;
+  if (runs < 1) runs = 1;
+  p.runs = (int)runs;
+  p.partO = p.partLse = nullptr;
+  p.join = nullptr;
+  void* scratch = nullptr;
+  int rc = kOk;
+  if (runs > 1) {
+    p.join = device_join_counters(device, stream, &rc);
+    if (p.join == nullptr) return rc;
+    const size_t parts = (size_t)runs * p.headsKV * 2 * 8 * nr;
+    rc = scratch_alloc(&scratch, parts * (D + 1) * sizeof(float), device, stream);
+    if (rc != kOk) return rc;
+    p.partO = static_cast<float*>(scratch);
+    p.partLse = p.partO + parts * D;
+  }
+  rc = nr == 1 ? launch_typed<D, 1>(p, int8, bf16, device, stream) : launch_typed<D, 2>(p, int8, bf16, device, stream);
+  if (scratch != nullptr) cudaFreeAsync(scratch, stream);
+  return rc;
+}
+
+int dispatch_stream(Params& p, int headDim, long long rows, int maxSeqLenKV, bool int8, bool bf16, int device, cudaStream_t stream) {
   switch (headDim) {
 #if TFA_HAVE_HD32
-    case 32: return launch_typed<32>(p, int8, bf16, runs, device, stream);
+    case 32: return launch_stream<32>(p, rows, maxSeqLenKV, int8, bf16, device, stream);
 #endif
 #if TFA_HAVE_HD64
-    case 64: return launch_typed<64>(p, int8, bf16, runs, device, stream);
+    case 64: return launch_stream<64>(p, rows, maxSeqLenKV, int8, bf16, device, stream);
 #endif
 #if TFA_HAVE_HD96
-    case 96: return launch_typed<96>(p, int8, bf16, runs, device, stream);
+    case 96: return launch_stream<96>(p, rows, maxSeqLenKV, int8, bf16, device, stream);
 #endif
 #if TFA_HAVE_HD128
-    case 128: return launch_typed<128>(p, int8, bf16, runs, device, stream);
+    case 128: return launch_stream<128>(p, rows, maxSeqLenKV, int8, bf16, device, stream);
 #endif
 #if TFA_HAVE_HD192
-    case 192: return launch_typed<192>(p, int8, bf16, runs, device, stream);
+    case 192: return launch_stream<192>(p, rows, maxSeqLenKV, int8, bf16, device, stream);
 #endif
 #if TFA_HAVE_HD256
-    case 256: return launch_typed<256>(p, int8, bf16, runs, device, stream);
+    case 256: return launch_stream<256>(p, rows, maxSeqLenKV, int8, bf16, device, stream);
 #endif
     default: return kBadHeadDim;
   }
@@ -1024,27 +1135,5 @@ extern "C" int tfa_b200_fwd_cache(const void* Q, void* O, const void* kCache, co
   const int tcOption = option_cache_tc();
   const long long rowsMost = (long long)maxSeqLenQ * p.group;  // query rows of a request that share a KV head
   if (tcOption > 0 || (tcOption < 0 && rowsMost > 4 * kRows)) return dispatch_tc(p, headDim, int8, bf16, device, s);
-  // as many runs as the GPU holds CTAs, and no more than there can be pairs of key blocks
-  const long long slots = (long long)device_num_sms(device) * ctas_per_sm(headDim);
-  const long long tiles = ((long long)(maxSeqLenQ > 0 ? maxSeqLenQ : 1) * p.group + kRows - 1) / kRows;
-  const long long most = (tiles * ((maxSeqLenKV + kBlockKeys - 1) / kBlockKeys) * batchSize + 1) / 2;
-  long long runs = slots / numHeadsKV;
-  if (runs > most) runs = most;
-  if (runs < 1) runs = 1;
-  p.runs = (int)runs;
-  p.partO = p.partLse = nullptr;
-  p.join = nullptr;
-  void* scratch = nullptr;
-  if (runs > 1) {
-    p.join = device_join_counters(device, s, &rc);
-    if (p.join == nullptr) return rc;
-    const size_t rows = (size_t)runs * numHeadsKV * 2 * kRows;
-    rc = scratch_alloc(&scratch, rows * (headDim + 1) * sizeof(float), device, s);
-    if (rc != kOk) return rc;
-    p.partO = static_cast<float*>(scratch);
-    p.partLse = p.partO + rows * headDim;
-  }
-  rc = cache::dispatch(p, headDim, int8, bf16, p.runs, device, s);
-  if (scratch != nullptr) cudaFreeAsync(scratch, s);
-  return rc;
+  return dispatch_stream(p, headDim, rowsMost > 0 ? rowsMost : 1, maxSeqLenKV, int8, bf16, device, s);
 }

@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
       for (int r = 0; r < RPT; r++) {
         const int row = q0 + ty * RPT + r, pos = p.qStart + row;
         const int lim = p.causal ? min(skv, max(pos + 1, prefix)) : skv;
-        const int rowDoc = (p.docKV != nullptr && row < sq) ? p.docQ[qRow0 + row] : -1;
+        const int rowDoc = (p.docKV != nullptr && row < sq) ? p.docQ[qRow0 + row] : -1;  // (all keys by their ids: a few per thread)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           const int key = kbase + tx + 8 * i;

@@ -53,31 +53,44 @@ namespace score {
 constexpr int kWarps = 8;
 constexpr int kScoreTileRows = 64, kScoreBlockKeys = 64;  // of the fp32 kernel; the tensor-core kernel has 128 >> packShift and 128
 
-// Smallest and largest document of every key block, a warp each.
-__global__ void __launch_bounds__(kWarps * 32) key_blocks_kernel(const int* docKV, int2* out, int seqLenKV, int blockKeys, int blocks, long long all) {
+// Ascending order puts negative ids (no document) last.
+__device__ __forceinline__ int order_of(int id) { return id < 0 ? INT_MAX : id; }
+
+// Smallest and largest document of every key block, a warp each, and whether its keys and the one before it are in ascending order.
+__global__ void __launch_bounds__(kWarps * 32) key_blocks_kernel(const int* docKV, int2* out, unsigned char* sorted, int seqLenKV, int blockKeys, int blocks,
+                                                                 long long all) {
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
   const long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (i >= all) return;
   const long long b = i / blocks;
   const int k0 = (int)(i - b * blocks) * blockKeys, k1 = min(k0 + blockKeys, seqLenKV);
+  const int* ids = docKV + b * seqLenKV;
   int lo = INT_MAX, hi = INT_MIN;
+  bool ascends = true;
+#pragma unroll 4
   for (int k = k0 + (threadIdx.x & 31); k < k1; k += 32) {
-    const int d = docKV[b * seqLenKV + k];
+    const int d = ids[k], before = k > 0 ? ids[k - 1] : INT_MIN;
     lo = min(lo, d);
     hi = max(hi, d);
+    ascends = ascends && (k == 0 || order_of(before) <= order_of(d));
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
-  if ((threadIdx.x & 31) == 0) out[i] = make_int2(lo, hi);
+  ascends = __all_sync(0xffffffffu, ascends);
+  if ((threadIdx.x & 31) == 0) {
+    out[i] = make_int2(lo, hi);
+    sorted[i] = ascends ? 1 : 0;
+  }
 }
 
 // Key blocks [x, y) that some row of a query tile may see, a warp for each tile: from the first to the last block whose range of
 // documents meets the tile's (documents in ascending order: exactly those with a visible key), as far as the causal mask reaches.
-// Never empty: a tile that sees nothing gets one block, in which everything is masked, so that its rows are written.
-__global__ void __launch_bounds__(kWarps * 32) tile_range_kernel(const int* docQ, const int2* keyBlocks, const int* prefix, int2* out, int seqLenQ,
-                                                                 int seqLenKV, int tileRows, int tiles, int blockKeys, int blocks, int causal, int qStart,
-                                                                 long long all) {
+// Never empty: a tile that sees nothing gets one block, in which everything is masked, so that its rows are written.  Then the keys of every row's
+// document, by bisection among those blocks, where all blocks as far as the mask reaches are in ascending order.
+__global__ void __launch_bounds__(kWarps * 32) tile_range_kernel(const int* docQ, const int* docKV, const int2* keyBlocks, const unsigned char* sorted,
+                                                                 const int* prefix, int2* out, int2* rowKeys, int seqLenQ, int seqLenKV, int tileRows,
+                                                                 int tiles, int blockKeys, int blocks, int causal, int qStart, long long all) {
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
   const long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
@@ -86,6 +99,7 @@ __global__ void __launch_bounds__(kWarps * 32) tile_range_kernel(const int* docQ
   const long long b = i / tiles;
   const int r0 = (int)(i - b * tiles) * tileRows, r1 = min(r0 + tileRows, seqLenQ);
   int lo = INT_MAX, hi = INT_MIN;
+#pragma unroll 4
   for (int r = r0 + lane; r < r1; r += 32) {
     const int d = docQ[b * seqLenQ + r];
     if (d >= 0) {
@@ -102,8 +116,11 @@ __global__ void __launch_bounds__(kWarps * 32) tile_range_kernel(const int* docQ
     end = (int)min((long long)blocks, (see - 1) / blockKeys + 1);
   }
   int first = INT_MAX, last = -1;
+  bool ascends = true;
+#pragma unroll 4
   for (int k = lane; k < end; k += 32) {
     const int2 ids = keyBlocks[b * blocks + k];
+    ascends = ascends && sorted[b * blocks + k] != 0;
     if (ids.y >= lo && ids.x <= hi) {
       first = min(first, k);
       last = k;
@@ -111,7 +128,40 @@ __global__ void __launch_bounds__(kWarps * 32) tile_range_kernel(const int* docQ
   }
   first = __reduce_min_sync(0xffffffffu, first);
   last = __reduce_max_sync(0xffffffffu, last);
-  if (lane == 0) out[i] = last < 0 ? make_int2(0, 1) : make_int2(first, last + 1);
+  ascends = __all_sync(0xffffffffu, ascends);
+  if (last < 0) first = 0, last = 0;
+  if (lane == 0) out[i] = make_int2(first, last + 1);
+  const int* ids = docKV + b * seqLenKV;
+  const int k0 = first * blockKeys, k1 = min((last + 1) * blockKeys, seqLenKV);
+  for (int r = r0 + lane; r < r1; r += 32) {
+    const int d = docQ[b * seqLenQ + r];
+    int2 keys = make_int2(0, 0);
+    if (!ascends) {
+      keys = make_int2(-1, -1);
+    } else if (d >= 0) {
+      int from = k0, to = k1, from2 = k0, to2 = k1;  // first key not before the document, first behind it
+      while (from < to || from2 < to2) {
+        const int mid = (from + to) >> 1, mid2 = (from2 + to2) >> 1;
+        const int x = from < to ? order_of(ids[mid]) : 0, y = from2 < to2 ? order_of(ids[mid2]) : 0;
+        if (from < to) {
+          if (x < d) {
+            from = mid + 1;
+          } else {
+            to = mid;
+          }
+        }
+        if (from2 < to2) {
+          if (y <= d) {
+            from2 = mid2 + 1;
+          } else {
+            to2 = mid2;
+          }
+        }
+      }
+      keys = make_int2(from, from2);
+    }
+    rowKeys[b * seqLenQ + r] = keys;
+  }
 }
 
 int run_tc(const FwdProblem& p, int ps, const TcSplit& split) {
@@ -160,7 +210,7 @@ int dispatch(FwdProblem p, ScoreFields& f, int device) {
   const int tileRows = fp32 ? kScoreTileRows : 128 >> ps, blockKeys = fp32 ? kScoreBlockKeys : 128;
   const int blocks = (p.seqLenKV + blockKeys - 1) / blockKeys;
   f.tiles = (p.seqLenQ + tileRows - 1) / tileRows;
-  const size_t tableBytes = docs ? sizeof(int2) * (size_t)p.batch * (blocks + f.tiles) : 0;
+  const size_t tableBytes = docs ? (size_t)p.batch * (sizeof(int2) * ((size_t)blocks + f.tiles + p.seqLenQ) + blocks) : 0;
   void* scratch = nullptr;
   int rc = kOk;
   if (floats > 0 || tableBytes > 0) {
@@ -170,12 +220,14 @@ int dispatch(FwdProblem p, ScoreFields& f, int device) {
   if (docs) {
     int2* keyBlocks = static_cast<int2*>(scratch);
     int2* tileRange = keyBlocks + (size_t)p.batch * blocks;
+    int2* rowKeys = tileRange + (size_t)p.batch * f.tiles;
+    unsigned char* sorted = reinterpret_cast<unsigned char*>(rowKeys + (size_t)p.batch * p.seqLenQ);
     const long long allBlocks = (long long)p.batch * blocks, allTiles = (long long)p.batch * f.tiles;
     cudaError_t e = launch_kernel(key_blocks_kernel, dim3((unsigned)((allBlocks + kWarps - 1) / kWarps)), kWarps * 32, 0, p.stream, p.overlap, f.docKV,
-                                  keyBlocks, p.seqLenKV, blockKeys, blocks, allBlocks);
+                                  keyBlocks, sorted, p.seqLenKV, blockKeys, blocks, allBlocks);
     if (e == cudaSuccess) {
-      e = launch_kernel(tile_range_kernel, dim3((unsigned)((allTiles + kWarps - 1) / kWarps)), kWarps * 32, 0, p.stream, p.overlap, f.docQ, keyBlocks,
-                        f.prefix, tileRange, p.seqLenQ, p.seqLenKV, tileRows, f.tiles, blockKeys, blocks, p.causal, f.qStart, allTiles);
+      e = launch_kernel(tile_range_kernel, dim3((unsigned)((allTiles + kWarps - 1) / kWarps)), kWarps * 32, 0, p.stream, p.overlap, f.docQ, f.docKV, keyBlocks,
+                        sorted, f.prefix, tileRange, rowKeys, p.seqLenQ, p.seqLenKV, tileRows, f.tiles, blockKeys, blocks, p.causal, f.qStart, allTiles);
     }
     if (e != cudaSuccess) {
       set_error_string("document table kernel launch failed: %s", cudaGetErrorString(e));
@@ -183,6 +235,7 @@ int dispatch(FwdProblem p, ScoreFields& f, int device) {
     }
     f.keyBlocks = keyBlocks;
     f.tileRange = tileRange;
+    f.rowKeys = rowKeys;
   }
   if (rc == kOk) {
     if (fp32) {
@@ -250,6 +303,6 @@ extern "C" int tfa_b200_fwd_scored(const void* Q, const void* K, const void* V, 
   p.headDim = headDim;
   p.causal = isCausal ? 1 : 0;
   p.stream = static_cast<cudaStream_t>(stream);
-  ScoreFields f = {qStart, softcap, alibiSlopes, prefixLens, docIdsQ, docIdsKV, nullptr, nullptr, 0};
+  ScoreFields f = {qStart, softcap, alibiSlopes, prefixLens, docIdsQ, docIdsKV, nullptr, nullptr, nullptr, 0};
   return score::dispatch(p, f, device);
 }

@@ -385,6 +385,11 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float fmin3(float a, float b, float c) {  // NaN kept as well
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ float fmax2(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -660,6 +665,8 @@ template <int kMode>
 struct ParamsOf<kMode, 1> {
   using type = typename std::conditional<kMode == kModeFixedSplit, TcScorePartParams, TcScoreParams>::type;
 };
+// tanh(t) / t = c0 + c1 t^2 + c2 t^4 + c3 t^6 for |t| <= 1/2, fitted to the smallest largest error of the tanh (1.3e-7)
+constexpr float kTanh0 = 0.9999976754188538f, kTanh1 = -0.33320656418800354f, kTanh2 = 0.13145145773887634f, kTanh3 = -0.04337248206138611f;
 // kScore: 0, or kScoreMask (masks by prefix, document and query offset) with kScoreCap and kScoreBias.  Instantiations of their own:
 // the cap is two more MUFU operations on every score, in kernels that the exponentials bound already.
 constexpr int kScoreMask = 1, kScoreCap = 2, kScoreBias = 4;
@@ -669,9 +676,12 @@ struct ScoreRow {
   int last;        // last key that the causal mask (with the prefix) leaves to the row
   int seenByAll;   // ... to every row of the tile
   int pos;         // position of the row
+  int docLo, docHi;  // keys of its document where they lie side by side; docLo below zero: by their ids
   int doc;         // its document; below zero: none
   float slope;     // log2(e) x slope of its head
   float capArg, capLog2;
+  float small;     // capped: scores up to here take the polynomial
+  float tanhC[4];  // its coefficients
   const int* docKV;
   const int2* keyBlocks;
 
@@ -689,83 +699,135 @@ struct ScoreRow {
     if (p.docKV != nullptr) {
       docKV = p.docKV + (long long)b * w.skv;
       keyBlocks = p.keyBlocks + (long long)b * ((w.skv + kBlockN - 1) / kBlockN);
-      if (qpos < w.sq) doc = p.docQ[w.qRow0 + qpos];
+      docLo = docHi = 0;
+      if (qpos < w.sq) {
+        doc = p.docQ[w.qRow0 + qpos];
+        const int2 keys = p.rowKeys[w.qRow0 + qpos];
+        docLo = keys.x;
+        docHi = keys.y;
+      }
     }
     if constexpr ((kScore & kScoreBias) != 0) slope = qpos < w.sq ? p.slopes[head] * 1.44269504f : 0.f;
     if constexpr ((kScore & kScoreCap) != 0) {
-      capLog2 = p.cap * 1.44269504f;
       capArg = 2.f * p.scaleLog2 / p.cap;
+      begin_cap(p.cap, capArg * 0.34657359f);
     }
   }
-
-  // Scores of a key block -> capped and biased, times log2(e).  c tanh(x) = c - 2 c / (e^2x + 1): off by about 2^-23 c whatever x is, which is
-  // what the exponential behind it sees.
-  template <class P>
-  __device__ __forceinline__ void transform(const P& p, uint32_t (&v)[4][32], int kbase) const {
-    if constexpr ((kScore & (kScoreCap | kScoreBias)) != 0) {
-      const float2 step = make_float2(2.f, 2.f);
-      float2 d = make_float2((float)(kbase - pos), (float)(kbase - pos + 1));  // key - position: exact up to 2^24
+  // f: what a score is multiplied by to become the argument of the tanh
+  __device__ __forceinline__ void begin_cap(float cap, float f) {
+    capLog2 = cap * 1.44269504f;
+    const float f2 = f * f;
+    tanhC[0] = kTanh0 * capLog2 * f;
+    tanhC[1] = kTanh1 * capLog2 * f * f2;
+    tanhC[2] = kTanh2 * capLog2 * f * f2 * f2;
+    tanhC[3] = kTanh3 * capLog2 * f * f2 * f2 * f2;
+    small = (f < 1e4f && f > 1e-30f) ? 0.5f / f : -1.f;  // the coefficients are finite
+  }
+  // c tanh of all scores of a key block, times log2(e).  Arguments up to 1/2, which is where a cap is meant to leave scores, on the FMA pipe: an
+  // odd polynomial of degree 7, off by 1.6e-7 c at most; larger ones (of any row of the warp) with c - 2 c / (e^2x + 1), two more MUFU operations
+  // on every score, off by about as much.  arg: factor that makes a score the 2 x log2(e) of the latter.
+  // Causal B2 S4096 32 over 8 heads of 128, cap 50: TANH_MEASURED.
+  __device__ __forceinline__ void cap_scores(uint32_t (&v)[4][32], float arg) const {
+    float hi[4], lo[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      hi[q] = lo[q] = __uint_as_float(v[q][0]);
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        hi[q] = fmax3(hi[q], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
+        lo[q] = fmin3(lo[q], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
+      }
+    }
+    const float most = fmax3(fmax2(fmax2(hi[0], hi[1]), fmax2(hi[2], hi[3])), -lo[0], fmax3(-lo[1], -lo[2], -lo[3]));
+    if (__all_sync(0xffffffffu, most <= small)) {  // (a NaN is not)
 #pragma unroll
       for (int q = 0; q < 4; q++) {
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float2 x = make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
-          if constexpr ((kScore & kScoreCap) != 0) {
-            x = fmul2(x, make_float2(capArg, capArg));
-            x.x = rcp(ex2(x.x) + 1.f);
-            x.y = rcp(ex2(x.y) + 1.f);
-            x = ffma2(x, make_float2(-2.f * capLog2, -2.f * capLog2), make_float2(capLog2, capLog2));
-          } else {
-            x = fmul2(x, make_float2(p.scaleLog2, p.scaleLog2));
-          }
-          if constexpr ((kScore & kScoreBias) != 0) {
-            x = ffma2(make_float2(fabsf(d.x), fabsf(d.y)), make_float2(-slope, -slope), x);
-            d = fadd2(d, step);
-          }
-          v[q][i] = __float_as_uint(x.x);
-          v[q][i + 1] = __float_as_uint(x.y);
+          const float2 x = make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
+          const float2 u = fmul2(x, x);
+          float2 y = ffma2(u, make_float2(tanhC[3], tanhC[3]), make_float2(tanhC[2], tanhC[2]));
+          y = ffma2(y, u, make_float2(tanhC[1], tanhC[1]));
+          y = ffma2(y, u, make_float2(tanhC[0], tanhC[0]));
+          y = fmul2(y, x);
+          v[q][i] = __float_as_uint(y.x);
+          v[q][i + 1] = __float_as_uint(y.y);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+          const float x = __uint_as_float(v[q][i]);
+          v[q][i] = __float_as_uint(fmaf(-2.f * capLog2, rcp(ex2(x * arg) + 1.f), capLog2));
         }
       }
     }
   }
 
-  // The same for codes: kf, by groups of 16 keys, is the scale of the keys x the row's factor (capped: of the argument 2 x log2(e)), and one
-  // from here on where the scores have been worked out.
+  // The bias; `scale`: what a score still has to be multiplied by.
+  __device__ __forceinline__ void bias_scores(uint32_t (&v)[4][32], int kbase, float scale) const {
+    const float2 step = make_float2(2.f, 2.f);
+    float2 d = make_float2((float)(kbase - pos), (float)(kbase - pos + 1));  // key - position: exact up to 2^24
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        float2 x = make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
+        if constexpr ((kScore & kScoreCap) == 0) x = fmul2(x, make_float2(scale, scale));
+        x = ffma2(make_float2(fabsf(d.x), fabsf(d.y)), make_float2(-slope, -slope), x);
+        d = fadd2(d, step);
+        v[q][i] = __float_as_uint(x.x);
+        v[q][i + 1] = __float_as_uint(x.y);
+      }
+    }
+  }
+  // Scores of a key block -> capped and biased, times log2(e).
+  template <class P>
+  __device__ __forceinline__ void transform(const P& p, uint32_t (&v)[4][32], int kbase) const {
+    if constexpr ((kScore & kScoreCap) != 0) cap_scores(v, capArg);
+    if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, p.scaleLog2);
+  }
+
+  // The same for codes: kf, by groups of 16 keys, is the scale of the keys x the row's factor, and one from here on where the scores have been
+  // worked out.
   __device__ __forceinline__ void cache_transform(uint32_t (&v)[4][32], int kbase, float (&kf)[8]) const {
     if constexpr ((kScore & (kScoreCap | kScoreBias)) != 0) {
-      const float2 step = make_float2(2.f, 2.f);
-      float2 d = make_float2((float)(kbase - pos), (float)(kbase - pos + 1));
 #pragma unroll
       for (int q = 0; q < 4; q++) {
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const float f = kf[q * 2 + i / 16];
-          float2 x = fmul2(make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1])), make_float2(f, f));
-          if constexpr ((kScore & kScoreCap) != 0) {
-            const bool gone0 = v[q][i] == 0xff800000u, gone1 = v[q][i + 1] == 0xff800000u;  // the key's block does not exist
-            x.x = rcp(ex2(x.x) + 1.f);
-            x.y = rcp(ex2(x.y) + 1.f);
-            x = ffma2(x, make_float2(-2.f * capLog2, -2.f * capLog2), make_float2(capLog2, capLog2));
-            if (gone0) x.x = -INFINITY;
-            if (gone1) x.y = -INFINITY;
-          }
-          if constexpr ((kScore & kScoreBias) != 0) {
-            x = ffma2(make_float2(fabsf(d.x), fabsf(d.y)), make_float2(-slope, -slope), x);
-            d = fadd2(d, step);
-          }
+          const float2 x = fmul2(make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1])), make_float2(f, f));
           v[q][i] = __float_as_uint(x.x);
           v[q][i + 1] = __float_as_uint(x.y);
         }
       }
+      if constexpr ((kScore & kScoreCap) != 0) cap_scores(v, 1.f);
+      if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, 1.f);
 #pragma unroll
       for (int i = 0; i < 8; i++) kf[i] = 1.f;
     }
   }
 
-  // Keys of other documents.  Most blocks hold one document (smallest id = largest id) and are seen whole or not at all.
+  // Keys of other documents.  Documents in ascending order: their first and last key are known for every row.  Else by ids; blocks of one document
+  // (smallest id = largest id) are seen whole or not at all.
   template <class P>
   __device__ __forceinline__ void documents(const P& p, uint32_t (&v)[4][32], int kbase, int skv) const {
     if (p.docKV == nullptr) return;
+    const int lo = docLo - kbase, hi = docHi - kbase;
+    if (!__any_sync(0xffffffffu, lo > 0 || hi < kBlockN)) return;  // every row sees the whole block
+    if (!__any_sync(0xffffffffu, docLo < 0)) {
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+          if (q * 32 + i < lo || q * 32 + i >= hi) v[q][i] = 0xff800000u;
+        }
+      }
+      return;
+    }
     const int2 ids = keyBlocks[kbase / kBlockN];
     const bool one = ids.x == ids.y;
     if (__all_sync(0xffffffffu, one && doc >= 0 && ids.x == doc)) return;
@@ -1106,7 +1168,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         row.last = row.pos;
         row.seenByAll = w.skv - w.sq / p.group + w.qlo[t] / p.group;
         if constexpr ((kScore & kScoreBias) != 0) row.slope = real ? p.slopes[w.unit * p.group + qpos % p.group] * 1.44269504f : 0.f;
-        if constexpr ((kScore & kScoreCap) != 0) row.capLog2 = p.cap * 1.44269504f;
+        if constexpr ((kScore & kScoreCap) != 0) row.begin_cap(p.cap, 0.34657359f);  // of the scaled scores, 2 x log2(e)
       } else if constexpr (kScore != 0) row.begin(p, w, qpos, (w.unit << p.packShift) + (r & ((1 << p.packShift) - 1)), w.qlo[t]);
       for (int j = 0; j < n; j++, it++) {
         if constexpr (kRingSig) {  // ring order K0 | K1 V0 | K2 V1 | ...: K of block j is load 2 j - 1 of the item (K0: 0)
@@ -1135,7 +1197,6 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         if constexpr (kSplit) kbase += w.part * p.partBlocks * kBlockN;
         if constexpr (kScore != 0 && !kSplit) kbase += w.part * kBlockN;
         [[maybe_unused]] float kf[8], vf[8];  // cache form: factors of the scores and of the weights, by groups of 16 keys
-        [[maybe_unused]] bool absent = false;
         [[maybe_unused]] bool vGrow = false;
         [[maybe_unused]] float vMax = 0.f;
         if constexpr (kCache) {
@@ -1151,22 +1212,24 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           vf[0] = v0.x, vf[1] = v0.y, vf[2] = v0.z, vf[3] = v0.w, vf[4] = v1.x, vf[5] = v1.y, vf[6] = v1.z, vf[7] = v1.w;
 #pragma unroll
           for (int i = 0; i < 8; i++) {
-            absent = absent || kf[i] < 0.f;
             vMax = fmaxf(vMax, vf[i]);
           }
-          if (absent) {
+          uint32_t gone = 0;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            if (kf[i] < 0.f) gone |= 1u << i;
+            kf[i] = fmaxf(fabsf(kf[i]) * rowFactor, 1.2e-38f);  // never zero: -inf in a block of zeros has to stay -inf
+          }
+          row.cache_transform(v, kbase, kf);
+          if (gone != 0) {  // keys whose blocks do not exist
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-              if (kf[i] < 0.f) {
+              if (gone >> i & 1u) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) v[i >> 1][(i & 1) * 16 + e] = 0xff800000u;
               }
             }
           }
-          // never zero: -inf in a block of zeros has to stay -inf
-#pragma unroll
-          for (int i = 0; i < 8; i++) kf[i] = fmaxf(fabsf(kf[i]) * rowFactor, 1.2e-38f);
-          row.cache_transform(v, kbase, kf);
           vGrow = vMax > vRef * kCacheSlack;
         } else if constexpr (kScore != 0) {
           row.transform(p, v, kbase);
@@ -1458,22 +1521,20 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             const uint4* src = reinterpret_cast<const uint4*>(
                 static_cast<const uint16_t*>(p.Q) +
                 ((w.qRow0 + (real ? flat / p.group : 0)) * p.headsQ + w.unit * p.group + (real ? flat % p.group : 0)) * (long long)p.headDim);
-            float up = 1.f, down = 1.f;
-            if constexpr (kBf16) {
-              uint32_t top = 0;
+            constexpr uint32_t kE = exponent_bits<kBf16>();
+            float up, down;
+            uint32_t top = 0;
 #pragma unroll 4
-              for (int i = 0; i < kHD / 8; i++) {
-                const uint4 x = src[i];
-                top = max(top, max(max(max(x.x & 0x7F80u, x.x >> 16 & 0x7F80u), max(x.y & 0x7F80u, x.y >> 16 & 0x7F80u)),
-                                   max(max(x.z & 0x7F80u, x.z >> 16 & 0x7F80u), max(x.w & 0x7F80u, x.w >> 16 & 0x7F80u))));
-              }
-              row_scale(top, up, down);
+            for (int i = 0; i < kHD / 8; i++) {
+              const uint4 x = src[i];
+              top = max(top, max(max(max(x.x & kE, x.x >> 16 & kE), max(x.y & kE, x.y >> 16 & kE)), max(max(x.z & kE, x.z >> 16 & kE), max(x.w & kE, x.w >> 16 & kE))));
             }
+            row_scale<kBf16>(top, up, down);
             cctl->rowFactor[k & 3][t][tid] = down;
 #pragma unroll 4
             for (int i = 0; i < kHD / 8; i++) {
               uint4 x = src[i];
-              if constexpr (kBf16) x = make_uint4(bf16_to_half2(x.x, up), bf16_to_half2(x.y, up), bf16_to_half2(x.z, up), bf16_to_half2(x.w, up));
+              x = make_uint4(scale_to_half2<kBf16>(x.x, up), scale_to_half2<kBf16>(x.y, up), scale_to_half2<kBf16>(x.z, up), scale_to_half2<kBf16>(x.w, up));
               if (!real) x = make_uint4(0, 0, 0, 0);
               asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (i >> 3) * kSubTileBytes + (((i & 7) ^ (tid & 7)) << 4)),
                            "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)

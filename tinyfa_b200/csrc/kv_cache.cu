@@ -8,9 +8,10 @@
 #include <cuda_runtime.h>
 #include <float.h>
 
+#include <type_traits>
+
 #include "../../include/tinyfa_b200.h"
 #include "build_config.cuh"
-#include "cta_scan.cuh"
 #include "ptx_sm100.cuh"
 #include "tfa_common.cuh"
 
@@ -58,42 +59,82 @@ __device__ __forceinline__ long long slot_of_row(const PlanParams& p, long long 
   const long long before = (p.finished != nullptr && p.finished[lo] != 0) ? 0 : length_before(p, lo);
   if (p.lensAfter[lo] == before) return -1;  // the row exists, so its request asked for tokens: it was not served
   const long long place = before + (row - p.cu[lo]);
+  if (place < 0 || place >= (long long)p.width << p.blockShift) return -1;  // (rows of lengths whose sum does not fit 32 bits)
   const int block = p.table[(long long)lo * p.width + (place >> p.blockShift)];
   return block < 0 ? -1 : ((long long)block << p.blockShift) + (place & ((1 << p.blockShift) - 1));
 }
 
+// Inclusive sums of two values over the CTA.
+__device__ __forceinline__ void cta_scan2(int& a, long long& b, int (&sA)[32], long long (&sB)[32], int& totalA, long long& totalB) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, a, d);
+    const long long y = __shfl_up_sync(0xffffffffu, b, d);
+    if (lane >= d) {
+      a += x;
+      b += y;
+    }
+  }
+  if (lane == 31) {
+    sA[warp] = a;
+    sB[warp] = b;
+  }
+  __syncthreads();
+  totalA = 0;
+  totalB = 0;
+  int beforeA = 0;
+  long long beforeB = 0;
+  for (int w = 0; w < warps; w++) {
+    if (w == warp) {
+      beforeA = totalA;
+      beforeB = totalB;
+    }
+    totalA += sA[w];
+    totalB += sB[w];
+  }
+  a += beforeA;
+  b += beforeB;
+}
+
 // One CTA: two prefix sums over the requests (blocks given back, blocks and rows asked for), the stack and the tables; the slots
-// too where they are few.  Integers only; bound by latency of a handful of dependent reads.
+// too where they are few.  Integers only; bound by the latency of a handful of dependent reads, so requests are handed to the warps one by one
+// (PLAN_MEASURED).
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, bool withSlots) {
-  __shared__ long long sWarp[32];
-  const int lane = threadIdx.x & 31;
+  __shared__ int sA[2][32];
+  __shared__ long long sB[2][32];
+  __shared__ int sCount[kPlanThreads], sHeld[kPlanThreads];
+  __shared__ int sTop[kPlanThreads];
+  __shared__ int sTaken;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, threads = blockDim.x;
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
-  const long long free0 = min(max((long long)*p.numFree, 0ll), (long long)p.capacity);
+  if (threadIdx.x == 0) sTaken = 0;
+  const int free0 = min(max(*p.numFree, 0), p.capacity);
   // blocks of finished requests go on top of the stack, in the order of the requests
   long long returned = 0;
+  int turn = 0;  // which half of sA, sB: a warp may still read the other one
   if (p.finished != nullptr) {
-    for (int b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+    for (int b0 = 0; b0 < p.batch; b0 += threads, turn ^= 1) {
       const int b = b0 + threadIdx.x;
-      const int n = (b < p.batch && p.finished[b] != 0) ? blocks_of(length_before(p, b), p.blockShift) : 0;
-      long long sum;
-      const long long at = free0 + returned + cta_scan(n, sWarp, sum) - n;
-      for (unsigned todo = __ballot_sync(0xffffffffu, n > 0); todo != 0; todo &= todo - 1) {
-        const int who = __ffs(todo) - 1;
-        const int bw = __shfl_sync(0xffffffffu, b, who), nw = __shfl_sync(0xffffffffu, n, who);
-        const long long aw = __shfl_sync(0xffffffffu, at, who);
-        for (int i = lane; i < nw; i += 32) {
-          if (aw + i < p.capacity) p.freeBlocks[aw + i] = p.table[(long long)bw * p.width + i];
-        }
+      int n = (b < p.batch && p.finished[b] != 0) ? blocks_of(length_before(p, b), p.blockShift) : 0, none = 0;
+      sCount[threadIdx.x] = n;
+      long long upto = n, sum;
+      cta_scan2(none, upto, sA[turn], sB[turn], none, sum);
+      sTop[threadIdx.x] = (int)min(free0 + returned + upto - sCount[threadIdx.x], (long long)p.capacity);
+      __syncthreads();
+      for (int r = warp; r < min(threads, p.batch - b0); r += warps) {
+        const int count = sCount[r], at = sTop[r];
+        for (int i = lane; i < min(count, p.capacity - at); i += 32) p.freeBlocks[at + i] = p.table[(long long)(b0 + r) * p.width + i];
       }
       returned += sum;
+      __syncthreads();
     }
-    __syncthreads();
   }
-  const long long have = min(free0 + returned, (long long)p.capacity);
+  const int have = (int)min(free0 + returned, (long long)p.capacity);
   // every request takes its new blocks from the top; one that finds too few, or whose row of the table is too short, keeps its length
-  long long taken = 0, asked = 0, rows = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+  long long asked = 0, rows = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += threads, turn ^= 1) {
     const int b = b0 + threadIdx.x;
     long long before = 0, fresh = 0;
     int held = 0, need = 0;
@@ -105,34 +146,37 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, 
       fits = before + fresh <= ((long long)p.width << p.blockShift);
       need = fits ? blocks_of(before + fresh, p.blockShift) - held : 0;
     }
-    long long sum, sumRows, sumTaken;
-    const long long upto = asked + cta_scan(need, sWarp, sum);
-    const long long row = rows + cta_scan(fresh, sWarp, sumRows);
+    int sum, inclusive = need;
+    long long row = fresh, sumRows;
+    cta_scan2(inclusive, row, sA[turn], sB[turn], sum, sumRows);
+    const long long upto = asked + inclusive;
     const bool served = fits && (need == 0 || upto <= have);
-    cta_scan(served ? need : 0, sWarp, sumTaken);
     if (b < p.batch) {
-      p.cu[b + 1] = (int)row;
+      p.cu[b + 1] = (int)(rows + row);
       p.lensAfter[b] = (int)(served ? before + fresh : before);
     }
-    const int n = served ? need : 0;
-    const long long top = have - 1 - (upto - need);
-    for (unsigned todo = __ballot_sync(0xffffffffu, n > 0); todo != 0; todo &= todo - 1) {
-      const int who = __ffs(todo) - 1;
-      const int bw = __shfl_sync(0xffffffffu, b, who), nw = __shfl_sync(0xffffffffu, n, who), hw = __shfl_sync(0xffffffffu, held, who);
-      const long long tw = __shfl_sync(0xffffffffu, top, who);
-      for (int i = lane; i < nw; i += 32) p.table[(long long)bw * p.width + hw + i] = p.freeBlocks[tw - i];
+    sCount[threadIdx.x] = served ? need : 0;
+    sHeld[threadIdx.x] = held;
+    sTop[threadIdx.x] = (int)(served ? have - 1 - (upto - need) : 0);
+    if (served && need > 0) atomicMax(&sTaken, (int)upto);  // the served ones are those that ask for no more than there is
+    __syncthreads();
+    for (int r = warp; r < min(threads, p.batch - b0); r += warps) {
+      const int count = sCount[r], top = sTop[r];
+      int* row0 = p.table + (long long)(b0 + r) * p.width + sHeld[r];
+#pragma unroll 4
+      for (int i = lane; i < count; i += 32) row0[i] = p.freeBlocks[top - i];
     }
     asked += sum;
     rows += sumRows;
-    taken += sumTaken;
+    __syncthreads();
   }
   if (threadIdx.x == 0) {
     p.cu[0] = 0;
-    *p.numFreeAfter = (int)(have - taken);
+    *p.numFreeAfter = have - sTaken;
   }
   if (!withSlots) return;
   __syncthreads();
-  for (long long row = threadIdx.x; row < p.total; row += kPlanThreads) p.slots[row] = slot_of_row(p, row);
+  for (long long row = threadIdx.x; row < p.total; row += threads) p.slots[row] = slot_of_row(p, row);
 }
 
 __global__ void __launch_bounds__(256) slots_kernel(const PlanParams p) {
@@ -156,53 +200,71 @@ constexpr int kStoreThreads = 128;
 constexpr float kTinyScale = 1.17549435e-38f;  // 2^-126: the smallest scale of a block that holds anything but zeros
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(src);
-    const T* t = reinterpret_cast<const T*>(&a);
+struct Eight {  // eight elements as they come from memory
+  uint4 raw[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* src) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = static_cast<float>(t[i]);
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[i] = reinterpret_cast<const uint4*>(src)[i];
   }
-}
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+      v[0] = __uint_as_float(raw[0].x), v[1] = __uint_as_float(raw[0].y), v[2] = __uint_as_float(raw[0].z), v[3] = __uint_as_float(raw[0].w);
+      v[4] = __uint_as_float(raw[1].x), v[5] = __uint_as_float(raw[1].y), v[6] = __uint_as_float(raw[1].z), v[7] = __uint_as_float(raw[1].w);
+    } else {
+      const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float2 f;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+        } else {
+          f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        }
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  }
+};
 
 // x * num / den rounded to a code; beyond the largest code it is the largest code, a NaN is stored as zero.  The scale is den / num: given
 // as two numbers, because a scale max |x| / 448 that is rounded before the division would move quotients off the border between two
 // codes, where many lie.  (num x is exact for 16-bit x.)
 template <bool kInt8>
 __device__ __forceinline__ uint2 to_codes(const float (&x)[8], float num, float den) {
-  uint2 out;
-  uint8_t* c = reinterpret_cast<uint8_t*>(&out);
+  uint32_t word[2];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    float q[2];
+  for (int h = 0; h < 2; h++) {
+    float q[4];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < 4; j++) {
       const float top = kInt8 ? 127.f : 448.f;
-      q[j] = den > 0.f ? __fdiv_rn(x[i + j] * num, den) : 0.f;
+      q[j] = den > 0.f ? __fdiv_rn(x[h * 4 + j] * num, den) : 0.f;
       q[j] = (q[j] != q[j]) ? 0.f : fminf(fmaxf(q[j], -top), top);
     }
     if constexpr (kInt8) {
-      c[i] = (uint8_t)(int8_t)__float2int_rn(q[0]);
-      c[i + 1] = (uint8_t)(int8_t)__float2int_rn(q[1]);
+      uint32_t c[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) c[j] = (uint32_t)__float2int_rn(q[j]);
+      word[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     } else {
-      *reinterpret_cast<__nv_fp8x2_storage_t*>(c + i) = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
+      word[h] = lo | hi << 16;
     }
   }
-  return out;
+  return make_uint2(word[0], word[1]);
 }
 
 template <bool kInt8>
 __device__ __forceinline__ void from_codes(uint2 in, float (&x)[8]) {
-  const uint8_t* c = reinterpret_cast<const uint8_t*>(&in);
 #pragma unroll
   for (int i = 0; i < 8; i++) {
+    const uint32_t c = ((i < 4 ? in.x : in.y) >> (i % 4 * 8)) & 0xFFu;
     if constexpr (kInt8) {
-      x[i] = (float)(int8_t)c[i];
+      x[i] = (float)(int8_t)c;
     } else {
-      x[i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(c[i], __NV_E4M3)));
+      x[i] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
     }
   }
 }
@@ -212,61 +274,105 @@ __device__ __forceinline__ void from_codes(uint2 in, float (&x)[8]) {
 // and codes that were in the block before are rounded anew where the scale grew: code' = round(code * scale / scale').  A run that begins
 // at the block's first cell begins the block: what its scale was before says nothing.  Bound by memory (the rows once, the codes once;
 // the second look at the rows comes from L2 or nearer).  All quotients are IEEE divisions, so that codes do not depend on how they are computed.
-template <typename T, bool kInt8>
+template <typename T, bool kInt8, int D>
 __global__ void __launch_bounds__(kStoreThreads) store_kernel(const StoreParams p) {
-  __shared__ float sMax[kStoreThreads / 32];
+  constexpr int kChunks = D / 8, kWarps = kStoreThreads / 32;
+  constexpr int kKept = 8;  // eights of a run that a thread keeps between the two looks: 64 rows of 128 elements; longer runs are read again
+  __shared__ float sMax[kWarps];
+  __shared__ int sCells[kStoreThreads];  // cells of the run's rows
+  const int h = blockIdx.y, which = blockIdx.z, lane = threadIdx.x & 31;
+  const int blockTokens = 1 << p.blockShift;
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
-  const int h = blockIdx.y, which = blockIdx.z;
-  const T* x = static_cast<const T*>(p.x[which]) + (long long)h * p.headDim;
-  const long long rowStride = (long long)p.heads * p.headDim;
-  const int chunks = p.headDim / 8, blockTokens = 1 << p.blockShift;
-  auto block_of = [&](long long row) -> long long {  // -1: the row goes nowhere
+  const T* x = static_cast<const T*>(p.x[which]) + (long long)h * D;
+  const long long rowStride = (long long)p.heads * D;
+  auto block_of = [&](long long row) -> int {  // -1: the row goes nowhere
+    if (row < 0 || row >= p.rows) return -1;
     const long long s = p.slots[row];
-    return (s < 0 || s >= p.cells) ? -1 : s >> p.blockShift;
+    return (s < 0 || s >= p.cells) ? -1 : (int)(s >> p.blockShift);
   };
-  const long long r0 = (long long)blockIdx.x * p.rowsPerCta, r1 = min(r0 + p.rowsPerCta, p.rows);
-  long long before = r0 > 0 ? block_of(r0 - 1) : -1;
-  for (long long r = r0; r < r1; r++) {
-    const long long block = block_of(r);
-    const bool begins = block >= 0 && block != before;
-    before = block;
-    if (!begins) continue;
-    int n = 1;  // rows of the run; more than the block has cells only if a cell comes twice
-    while (r + n < p.rows && n < blockTokens && block_of(r + n) == block) n++;
-    const int first = (int)(p.slots[r] & (blockTokens - 1));
+  // which of the CTA's rows (16 at most) begin a run: every warp finds out for itself
+  const long long r0 = (long long)blockIdx.x * p.rowsPerCta;
+  const int mine = lane < p.rowsPerCta ? block_of(r0 + lane) : -1;
+  int before = __shfl_up_sync(0xffffffffu, mine, 1);
+  if (lane == 0) before = block_of(r0 - 1);
+  unsigned begins = __ballot_sync(0xffffffffu, mine >= 0 && mine != before);
+  for (; begins != 0; begins &= begins - 1) {
+    const int from = __ffs(begins) - 1;
+    const long long r = r0 + from;
+    const int block = __shfl_sync(0xffffffffu, mine, from);
+    // the run ends with the first row of another block; more rows than the block has cells only if a cell comes twice
+    __syncthreads();  // the run before may still read sCells and sMax
+    bool other = (int)threadIdx.x >= blockTokens;
+    if (!other) {
+      other = block_of(r + threadIdx.x) != block;
+      sCells[threadIdx.x] = other ? -1 : (int)(p.slots[r + threadIdx.x] & (blockTokens - 1));
+    }
+    // kStoreThreads rows are looked at, and a run has blockTokens <= kStoreThreads at most
+    const unsigned others = __ballot_sync(0xffffffffu, other);
+    if (lane == 0) sMax[threadIdx.x >> 5] = __int_as_float(others != 0 ? (int)(threadIdx.x & ~31) + __ffs(others) - 1 : kStoreThreads);
+    __syncthreads();
+    int n = kStoreThreads;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) n = min(n, __float_as_int(sMax[w]));
+    const int first = sCells[0], items = n * kChunks;
+    __syncthreads();  // sMax is written again
     float top = 0.f;
-    for (int i = threadIdx.x; i < n * chunks; i += kStoreThreads) {
+    auto look = [&](const Eight<T>& e) {
       float v[8];
-      load8(x + (r + i / chunks) * rowStride + (i % chunks) * 8, v);
+      e.values(v);
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const float a = fabsf(v[j]);
         if (a <= FLT_MAX) top = fmaxf(top, a);
       }
+    };
+    Eight<T> kept[kKept];
+#pragma unroll
+    for (int e = 0; e < kKept; e++) {
+      const int i = threadIdx.x + e * kStoreThreads;
+      if (i < items) kept[e].load(x + (r + i / kChunks) * rowStride + i % kChunks * 8);
+    }
+#pragma unroll
+    for (int e = 0; e < kKept; e++) {
+      if ((int)threadIdx.x + e * kStoreThreads < items) look(kept[e]);
+    }
+    for (int i = threadIdx.x + kKept * kStoreThreads; i < items; i += kStoreThreads) {
+      Eight<T> e;
+      e.load(x + (r + i / kChunks) * rowStride + i % kChunks * 8);
+      look(e);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    __syncthreads();  // the run before may still read sMax
-    if ((threadIdx.x & 31) == 0) sMax[threadIdx.x >> 5] = top;
+    if (lane == 0) sMax[threadIdx.x >> 5] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(sMax[0], sMax[1]), fmaxf(sMax[2], sMax[3]));
-    float* scaleAt = p.scales[which] + block * p.heads + h;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) top = fmaxf(top, sMax[w]);
+    float* scaleAt = p.scales[which] + (long long)block * p.heads + h;
     const float old = first == 0 ? 0.f : *scaleAt;
     const float need = top > 0.f ? fmaxf(__fdiv_rn(top, kInt8 ? 127.f : 448.f), kTinyScale) : 0.f;
     const float scale = fmaxf(old, need);
     // the scale is this run's (and not rounded up to a normal number, nor its numerator out of range)
     const bool fromRun = need >= old && need > kTinyScale && top <= 1e35f;
     const float num = fromRun ? (kInt8 ? 127.f : 448.f) : 1.f, den = fromRun ? top : scale;
-    uint8_t* tile = p.codes[which] + ((block * p.heads + h) << p.blockShift) * p.headDim;
-    for (int i = threadIdx.x; i < n * chunks; i += kStoreThreads) {
-      const int cell = (int)(p.slots[r + i / chunks] & (blockTokens - 1));
+    uint8_t* tile = p.codes[which] + (((long long)block * p.heads + h) << p.blockShift) * D;
+    auto put = [&](const Eight<T>& e, int i) {
       float v[8];
-      load8(x + (r + i / chunks) * rowStride + (i % chunks) * 8, v);
-      *reinterpret_cast<uint2*>(tile + (long long)cell * p.headDim + (i % chunks) * 8) = to_codes<kInt8>(v, num, den);
+      e.values(v);
+      *reinterpret_cast<uint2*>(tile + sCells[i / kChunks] * D + i % kChunks * 8) = to_codes<kInt8>(v, num, den);
+    };
+#pragma unroll
+    for (int e = 0; e < kKept; e++) {
+      const int i = threadIdx.x + e * kStoreThreads;
+      if (i < items) put(kept[e], i);
+    }
+    for (int i = threadIdx.x + kKept * kStoreThreads; i < items; i += kStoreThreads) {
+      Eight<T> e;
+      e.load(x + (r + i / kChunks) * rowStride + i % kChunks * 8);
+      put(e, i);
     }
     if (scale != old || first == 0) {
-      for (int i = threadIdx.x; i < first * chunks; i += kStoreThreads) {
+      for (int i = threadIdx.x; i < first * kChunks; i += kStoreThreads) {
         uint2* at = reinterpret_cast<uint2*>(tile + i * 8);
         float v[8];
         from_codes<kInt8>(*at, v);
@@ -280,10 +386,21 @@ __global__ void __launch_bounds__(kStoreThreads) store_kernel(const StoreParams 
   }
 }
 
+template <typename T, int D>
+cudaError_t launch_store(const StoreParams& p, bool int8, dim3 grid, cudaStream_t stream) {
+  auto kernel = int8 ? store_kernel<T, true, D> : store_kernel<T, false, D>;
+  return launch_kernel(kernel, grid, kStoreThreads, 0, stream, may_overlap(stream), p);
+}
 template <typename T>
 cudaError_t launch_store(const StoreParams& p, bool int8, dim3 grid, cudaStream_t stream) {
-  auto kernel = int8 ? store_kernel<T, true> : store_kernel<T, false>;
-  return launch_kernel(kernel, grid, kStoreThreads, 0, stream, may_overlap(stream), p);
+  switch (p.headDim) {
+    case 32: return launch_store<T, 32>(p, int8, grid, stream);
+    case 64: return launch_store<T, 64>(p, int8, grid, stream);
+    case 96: return launch_store<T, 96>(p, int8, grid, stream);
+    case 128: return launch_store<T, 128>(p, int8, grid, stream);
+    case 192: return launch_store<T, 192>(p, int8, grid, stream);
+    default: return launch_store<T, 256>(p, int8, grid, stream);
+  }
 }
 
 int block_shift(int blockTokens) {
@@ -330,7 +447,9 @@ extern "C" int tfa_b200_kv_cache_plan(int* blockTable, const int* seqLens, const
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool overlap = may_overlap(s);
   const bool few = totalNew <= kPlanThreads;  // more rows than the CTA has threads: a kernel of as many CTAs as they need
-  cudaError_t e = launch_kernel(plan_kernel, dim3(1), kPlanThreads, 0, s, overlap, p, few);
+  // a warp for every two requests or so: fewer to wait for
+  const int threads = batchSize <= 64 && few ? 256 : kPlanThreads;
+  cudaError_t e = launch_kernel(plan_kernel, dim3(1), threads, 0, s, overlap, p, few);
   if (e == cudaSuccess && !few) e = launch_kernel(slots_kernel, dim3((unsigned)((totalNew + 255) / 256)), 256, 0, s, overlap, p);
   if (e != cudaSuccess) {
     set_error_string("cache plan kernel launch failed: %s", cudaGetErrorString(e));

@@ -16,9 +16,11 @@ struct ScoreFields {
   const int* prefix;    // [batch] or null
   const int* docQ;      // [batch][seqLenQ] or null
   const int* docKV;     // [batch][seqLenKV]
-  // documents: smallest and largest id of every key block, and the key blocks [x, y) that some row of a query tile may see
+  // documents: smallest and largest id of every key block, the key blocks [x, y) that some row of a query tile may see, and the keys [x, y) of
+  // every row's document (x below zero where keys are not in ascending order of documents)
   const int2* keyBlocks;  // [batch][key blocks]
   const int2* tileRange;  // [batch][tiles]
+  const int2* rowKeys;    // [batch][seqLenQ]
   int tiles;
 };
 
