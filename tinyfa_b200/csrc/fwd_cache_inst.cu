@@ -40,13 +40,18 @@ int launch_one(const TcCacheParams& p, int ctas, bool overlap, int device, cudaS
   return kOk;
 }
 
+template <int kHD, int kCodes>
+int launch_codes(const TcCacheParams& p, int ctas, bool overlap, int device, cudaStream_t stream) {
+  constexpr int kBase = tc::kScoreMask | kCodes;
+  const bool cap = p.cap > 0.f, bias = p.slopes != nullptr;
+  if (cap && bias) return launch_one<kHD, kBase | tc::kScoreCap | tc::kScoreBias>(p, ctas, overlap, device, stream);
+  if (cap) return launch_one<kHD, kBase | tc::kScoreCap>(p, ctas, overlap, device, stream);
+  if (bias) return launch_one<kHD, kBase | tc::kScoreBias>(p, ctas, overlap, device, stream);
+  return launch_one<kHD, kBase>(p, ctas, overlap, device, stream);
+}
 template <int kHD>
 int launch_head_dim(const TcCacheParams& p, int ctas, bool overlap, int device, cudaStream_t stream) {
-  const bool cap = p.cap > 0.f, bias = p.slopes != nullptr;
-  if (cap && bias) return launch_one<kHD, tc::kScoreMask | tc::kScoreCap | tc::kScoreBias>(p, ctas, overlap, device, stream);
-  if (cap) return launch_one<kHD, tc::kScoreMask | tc::kScoreCap>(p, ctas, overlap, device, stream);
-  if (bias) return launch_one<kHD, tc::kScoreMask | tc::kScoreBias>(p, ctas, overlap, device, stream);
-  return launch_one<kHD, tc::kScoreMask>(p, ctas, overlap, device, stream);
+  return p.int8 ? launch_codes<kHD, tc::kScoreInt8>(p, ctas, overlap, device, stream) : launch_codes<kHD, 0>(p, ctas, overlap, device, stream);
 }
 
 }  // namespace

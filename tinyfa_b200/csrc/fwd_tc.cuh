@@ -670,11 +670,13 @@ constexpr float kTanh0 = 0.9999976754188538f, kTanh1 = -0.33320656418800354f, kT
 // kScore: 0, or kScoreMask (masks by prefix, document and query offset) with kScoreCap and kScoreBias.  Instantiations of their own:
 // the cap is two more MUFU operations on every score, in kernels that the exponentials bound already.
 constexpr int kScoreMask = 1, kScoreCap = 2, kScoreBias = 4;
+constexpr int kScoreInt8 = 8;  // kModeCache: codes are int8 rather than e4m3
 // What a softmax thread keeps of its query row in a scored call.
 template <int kScore>
 struct ScoreRow {
   int last;        // last key that the causal mask (with the prefix) leaves to the row
   int seenByAll;   // ... to every row of the tile
+  int seenByAllPos;  // position of the tile's first row
   int pos;         // position of the row
   int docLo, docHi;  // keys of its document where they lie side by side; docLo below zero: by their ids
   int doc;         // its document; below zero: none
@@ -689,7 +691,7 @@ struct ScoreRow {
   __device__ __forceinline__ void begin(const P& p, const Work& w, int qpos, int head, int qlo) {
     pos = p.qStart + qpos;
     last = pos;
-    seenByAll = p.qStart + qlo;
+    seenByAll = seenByAllPos = p.qStart + qlo;
     const int b = (p.prefix != nullptr || p.docKV != nullptr) ? (int)(w.qRow0 / w.sq) : 0;
     if (p.prefix != nullptr) {
       last = max(last, p.prefix[b] - 1);
@@ -766,8 +768,29 @@ struct ScoreRow {
     }
   }
 
-  // The bias; `scale`: what a score still has to be multiplied by.
-  __device__ __forceinline__ void bias_scores(uint32_t (&v)[4][32], int kbase, float scale) const {
+  // The bias; `scale`: what a score still has to be multiplied by (capped scores: nothing).  left: all keys that the row sees lie to its left,
+  // where the bias is linear in the key - 2 packed operations on a pair of scores instead of 3 and two absolute values.
+  __device__ __forceinline__ void bias_scores(uint32_t (&v)[4][32], int kbase, float scale, bool left) const {
+    if (left) {
+      const float2 step = make_float2(2.f * slope, 2.f * slope);
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        float2 d = make_float2(slope * (float)(kbase + q * 32 - pos), slope * (float)(kbase + q * 32 + 1 - pos));
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float2 x = make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
+          if constexpr ((kScore & kScoreCap) == 0) {
+            x = ffma2(x, make_float2(scale, scale), d);
+          } else {
+            x = fadd2(x, d);
+          }
+          d = fadd2(d, step);  // 16 times: off by 16 half steps of d at most
+          v[q][i] = __float_as_uint(x.x);
+          v[q][i + 1] = __float_as_uint(x.y);
+        }
+      }
+      return;
+    }
     const float2 step = make_float2(2.f, 2.f);
     float2 d = make_float2((float)(kbase - pos), (float)(kbase - pos + 1));  // key - position: exact up to 2^24
 #pragma unroll
@@ -787,27 +810,39 @@ struct ScoreRow {
   template <class P>
   __device__ __forceinline__ void transform(const P& p, uint32_t (&v)[4][32], int kbase) const {
     if constexpr ((kScore & kScoreCap) != 0) cap_scores(v, capArg);
-    if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, p.scaleLog2);
+    if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, p.scaleLog2, (p.causal && p.prefix == nullptr) || kbase + kBlockN - 1 <= seenByAllPos);
   }
 
-  // The same for codes: kf, by groups of 16 keys, is the scale of the keys x the row's factor, and one from here on where the scores have been
-  // worked out.
-  __device__ __forceinline__ void cache_transform(uint32_t (&v)[4][32], int kbase, float (&kf)[8]) const {
+  // The same for codes, whose scores are multiplied by kf (by groups of 16 keys: the scale of the keys x the row's factor) first.
+  // gone: groups whose block does not exist, as bits.
+  template <class F>
+  __device__ __forceinline__ void cache_transform(uint32_t (&v)[4][32], int kbase, F kf, bool left, uint32_t gone) const {
     if constexpr ((kScore & (kScoreCap | kScoreBias)) != 0) {
 #pragma unroll
       for (int q = 0; q < 4; q++) {
+        const float2 f2 = kf(q);
+        const float off0 = (gone >> (2 * q) & 1u) != 0 ? -INFINITY : 0.f, off1 = (gone >> (2 * q + 1) & 1u) != 0 ? -INFINITY : 0.f;
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          const float f = kf[q * 2 + i / 16];
-          const float2 x = fmul2(make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1])), make_float2(f, f));
+          const float f = i < 16 ? f2.x : f2.y, off = i < 16 ? off0 : off1;
+          const float2 x = ffma2(make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1])), make_float2(f, f), make_float2(off, off));
           v[q][i] = __float_as_uint(x.x);
           v[q][i + 1] = __float_as_uint(x.y);
         }
       }
-      if constexpr ((kScore & kScoreCap) != 0) cap_scores(v, 1.f);
-      if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, 1.f);
+      if constexpr ((kScore & kScoreCap) != 0) {
+        cap_scores(v, 1.f);
+        if (gone != 0) {  // minus infinity is -c by now
 #pragma unroll
-      for (int i = 0; i < 8; i++) kf[i] = 1.f;
+          for (int i = 0; i < 8; i++) {
+            if (gone >> i & 1u) {
+#pragma unroll
+              for (int e = 0; e < 16; e++) v[i >> 1][(i & 1) * 16 + e] = 0xff800000u;
+            }
+          }
+        }
+      }
+      if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, 1.f, left);
     }
   }
 
@@ -868,7 +903,8 @@ struct CacheSegment {  // what the loading thread publishes beside a WorkSlot
 };
 struct CacheCtl {
   uint64_t scaleFull[8];
-  float scales[8][16];  // of the eight 16-key groups of a block: K (below zero: the block does not exist), V
+  float scales[8][16];  // of the eight 16-key groups of a block: K, V
+  float2 summary[8];    // largest scale of V; groups whose block does not exist, as bits
   float rowFactor[4][2][kBlockM];
   CacheSegment seg[2];
   int last[2];
@@ -878,6 +914,25 @@ static_assert(sizeof(CacheCtl) <= kCacheSmem, "shared memory of the cache form")
 // Weights of V relative to the scale of V that O refers to, times 2^3: a weight is at most 2^8 (lazy rescale), scales at most 2^4 above the
 // reference, so fp16's 2^16 is not reached.
 constexpr float kCacheUp = 8.f, kCacheSlack = 16.f;
+
+// Loads under a predicate: nothing is read where it does not hold.
+__device__ __forceinline__ uint4 ldg_if(const uint4* at, bool ok) {
+  uint4 x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(x.x), "=&r"(x.y), "=&r"(x.z), "=&r"(x.w)
+      : "l"(at), "r"((int)ok));
+  return x;
+}
+__device__ __forceinline__ int ldg_if(const int* at, bool ok, int other) {
+  int x;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\tmov.b32 %0, %3;\n\t@p ld.global.nc.b32 %0, [%1];\n\t}" : "=&r"(x) : "l"(at), "r"((int)ok), "r"(other));
+  return x;
+}
+__device__ __forceinline__ float ldg_if(const float* at, bool ok, float other) {
+  return __int_as_float(ldg_if(reinterpret_cast<const int*>(at), ok, __float_as_int(other)));
+}
 
 // 32 columns of a row's output
 template <bool kBf16, class P, class W>
@@ -1196,9 +1251,16 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         int kbase = j * kBlockN;
         if constexpr (kSplit) kbase += w.part * p.partBlocks * kBlockN;
         if constexpr (kScore != 0 && !kSplit) kbase += w.part * kBlockN;
-        [[maybe_unused]] float kf[8], vf[8];  // cache form: factors of the scores and of the weights, by groups of 16 keys
         [[maybe_unused]] bool vGrow = false;
         [[maybe_unused]] float vMax = 0.f;
+        [[maybe_unused]] uint32_t gone = 0;  // groups whose block does not exist
+        [[maybe_unused]] const float* scales = nullptr;
+        // cache form: factors of the scores of quarter q, two groups of 16 keys - read again where they are used, because beside 128 scores there
+        // are no registers to keep them.  Never zero: -inf in a block of zeros has to stay -inf.
+        auto keyFactors = [&](int q) -> float2 {
+          const float2 k2 = *reinterpret_cast<const float2*>(scales + 2 * q);
+          return make_float2(fmaxf(k2.x * rowFactor, 1.2e-38f), fmaxf(k2.y * rowFactor, 1.2e-38f));
+        };
         if constexpr (kCache) {
           const int g = blkItem + j;
           wait_bar(ptx::smem_u32(&cctl->scaleFull[g & 7]), (g >> 3) & 1, wc, 32);
@@ -1206,30 +1268,11 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             rowFactor = cctl->rowFactor[k & 3][t][r] * p.scaleLog2;
             if constexpr ((kScore & kScoreCap) != 0) rowFactor *= 2.f / p.cap;
           }
-          const float4* sc = reinterpret_cast<const float4*>(cctl->scales[g & 7]);
-          const float4 k0 = sc[0], k1 = sc[1], v0 = sc[2], v1 = sc[3];
-          kf[0] = k0.x, kf[1] = k0.y, kf[2] = k0.z, kf[3] = k0.w, kf[4] = k1.x, kf[5] = k1.y, kf[6] = k1.z, kf[7] = k1.w;
-          vf[0] = v0.x, vf[1] = v0.y, vf[2] = v0.z, vf[3] = v0.w, vf[4] = v1.x, vf[5] = v1.y, vf[6] = v1.z, vf[7] = v1.w;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            vMax = fmaxf(vMax, vf[i]);
-          }
-          uint32_t gone = 0;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            if (kf[i] < 0.f) gone |= 1u << i;
-            kf[i] = fmaxf(fabsf(kf[i]) * rowFactor, 1.2e-38f);  // never zero: -inf in a block of zeros has to stay -inf
-          }
-          row.cache_transform(v, kbase, kf);
-          if (gone != 0) {  // keys whose blocks do not exist
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              if (gone >> i & 1u) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) v[i >> 1][(i & 1) * 16 + e] = 0xff800000u;
-              }
-            }
-          }
+          scales = cctl->scales[g & 7];
+          const float2 sum = cctl->summary[g & 7];
+          vMax = sum.x;
+          gone = __float_as_uint(sum.y);
+          row.cache_transform(v, kbase, keyFactors, p.causal || kbase + kBlockN - 1 <= row.seenByAll, gone);
           vGrow = vMax > vRef * kCacheSlack;
         } else if constexpr (kScore != 0) {
           row.transform(p, v, kbase);
@@ -1252,12 +1295,22 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         const float2 c2 = make_float2(c, c);
         auto expQuarter = [&](const uint32_t(&vq)[32], float negMc, uint32_t(&dst)[16], float2& sum, const int quarter) {
           const float2 negMc2 = make_float2(negMc, negMc);
+          [[maybe_unused]] float2 kf2, vf2;
+          [[maybe_unused]] float neg0, neg1;
+          if constexpr (kCache) {
+            kf2 = keyFactors(quarter);
+            neg0 = (gone >> (2 * quarter) & 1u) != 0 ? -INFINITY : negMc;
+            neg1 = (gone >> (2 * quarter + 1) & 1u) != 0 ? -INFINITY : negMc;
+            vf2 = *reinterpret_cast<const float2*>(scales + 8 + 2 * quarter);
+            vf2.x *= vInv;
+            vf2.y *= vInv;
+          }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             float2 x = make_float2(__uint_as_float(vq[i]), __uint_as_float(vq[i + 1]));
-            if constexpr (kCache) {
-              const float f = kf[quarter * 2 + i / 16];
-              x = ffma2(x, make_float2(f, f), negMc2);
+            if constexpr (kCache && (kScore & (kScoreCap | kScoreBias)) == 0) {
+              const float f = i < 16 ? kf2.x : kf2.y, n = i < 16 ? neg0 : neg1;
+              x = ffma2(x, make_float2(f, f), make_float2(n, n));
             } else {
               x = ffma2(x, c2, negMc2);
             }
@@ -1269,7 +1322,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             }
             sum = fadd2(sum, x);
             if constexpr (kCache) {
-              const float f = vf[quarter * 2 + i / 16];
+              const float f = i < 16 ? vf2.x : vf2.y;
               x = fmul2(x, make_float2(f, f));
               dst[i >> 1] = pack2<false>(x.x, x.y);
             } else {
@@ -1288,7 +1341,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           for (int i = 2; i < 32; i += 2) mx4[q] = fmax3(mx4[q], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
         }
         float mx = fmax2(fmax2(mx4[0], mx4[1]), fmax2(mx4[2], mx4[3]));  // NaN if any score of the row is
-        if constexpr (kCache) {  // by groups, whose factors differ
+        if constexpr (kCache && (kScore & (kScoreCap | kScoreBias)) == 0) {  // by groups, whose factors differ
           mx = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 8; i++) {
@@ -1296,7 +1349,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             float top = fmax2(__uint_as_float(vq[(i & 1) * 16]), __uint_as_float(vq[(i & 1) * 16 + 1]));
 #pragma unroll
             for (int e = 2; e < 16; e += 2) top = fmax3(top, __uint_as_float(vq[(i & 1) * 16 + e]), __uint_as_float(vq[(i & 1) * 16 + e + 1]));
-            mx = fmax2(mx, top * kf[i]);
+            const float2 f2 = keyFactors(i >> 1);
+            mx = fmax2(mx, (gone >> i & 1u) != 0 ? -INFINITY : top * ((i & 1) ? f2.y : f2.x));
           }
         }
         // Lazy rescale: keep the old reference max while the new one exceeds it by less than kRescaleLog2 in
@@ -1340,10 +1394,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         if constexpr (kCache) {
           if (vGrow) {
             vRef = vMax;
-            vInv = vMax > 0.f ? fminf(1.f / vMax, 3e38f) : 0.f;
+            vInv = vMax > 0.f ? fminf(1.f / vMax, 4e37f) * kCacheUp : 0.f;
           }
-#pragma unroll
-          for (int i = 0; i < 8; i++) vf[i] = vf[i] * vInv * kCacheUp;
         }
 
         // A NaN score makes every exponential of the row NaN (the pairs evaluated on the FMA pipe clamp their
@@ -1493,14 +1545,24 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     // ================================================================ cache form: pages and queries -> fp16 tiles in shared memory
     ptx::setmaxnreg_dec<kRegsEpilogue>();
     if constexpr (kCache) {
-      constexpr int kConv = kConvWarps * 32, kChunks = kHD / 16;    // 16-byte pieces of a cache row
-      constexpr int kPieces = kBlockN * kChunks / kConv;            // of a tile, per thread
-      static_assert(kBlockN * kChunks % kConv == 0, "pieces of a tile");
+      // A thread's 16-byte pieces of a tile: kPieces of them, kStepRows key rows apart, at one place of their rows.  Four threads take the 64
+      // codes of a row that go to one 64-wide slab, so that a quarter warp's stores (16 codes are two of the row's eight chunks) fall on eight
+      // groups of banks; head dims 32 and 96 end with half a slab, where two threads take 32.
+      constexpr int kConv = kConvWarps * 32, kFull = kHD / 64, kHalf = (kHD % 64) / 32;
+      constexpr int kSlabThreads = kConv / (kFull + kHalf) / 32 * 32;  // of a slab
+      constexpr int kStepRows = kSlabThreads / 4;                      // rows that they take at a time
+      constexpr int kPieces = kBlockN / kStepRows;
+      static_assert(kBlockN % kStepRows == 0, "rows of a tile");
       const int tid = threadIdx.x - kSoftmaxWarps * 32;
+      const int slab = tid / kSlabThreads, inSlab = tid % kSlabThreads;
+      const bool halfSlab = kHalf != 0 && slab == kFull;  // its threads take two rows a piece apart each where others take one
+      const int myRow = halfSlab ? inSlab / 2 : inSlab / 4, my16 = halfSlab ? inSlab % 2 : inSlab % 4;
+      const int stepRows = halfSlab ? 2 * kStepRows : kStepRows, myPieces = slab >= kFull + kHalf ? 0 : halfSlab ? kPieces / 2 : kPieces;
+      static_assert(kStepRows % 16 == 0 || kStepRows == 8, "a warp's piece lies in one group of 16 keys");
       const int cw = warp - kSoftmaxWarps;
       const long long headBytes = (long long)p.headDim << p.blockShift;
       int ld = 0, blkBase = 0;
-      int qc[2] = {0, 0};
+      int qc0 = 0, qc1 = 0;  // Q tiles filled
       for (int k = 0;; k++) {
         WorkT w;
         const int idx = fetchWork(k, w);
@@ -1511,8 +1573,9 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         if (w.nmax == 0) continue;
         // a row per thread; rows past the request are zero
         auto fillQ = [&](int t) {
-          if (t >= NT || w.nblk[t] == 0) return;
-          const int qb = qc[t] % C::kQBufs, qUse = qc[t] / C::kQBufs;
+          if (w.nblk[t] == 0) return;
+          const int use = t == 0 ? qc0 : qc1;
+          const int qb = use % C::kQBufs, qUse = use / C::kQBufs;
           if (qUse > 0) wait_bar(bar(kBarQEmpty + 2 * t + qb), (qUse - 1) & 1, wc, 22);
           if (tid < kBlockM) {
             const int flat = w.qlo[t] + tid;
@@ -1544,17 +1607,39 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(bar(kBarQFull + 2 * t + qb));
-          qc[t]++;
+          if (t == 0) {
+            qc0++;
+          } else {
+            qc1++;
+          }
         };
-        // tile index (block x heads + head) of the 16-key group `lane` of a key block, -1: none
+        // What is on its way is not looked at before it is needed: loads under a predicate rather than a branch, whose end would wait for them
+        // (with branches a tile took 4.6 k clocks, most of it such waits).
+        // block of the 16-key group `lane` of a key block, as the table has it; -1 past the request's end
         auto pageOf = [&](int blk) -> int {
           const int key = blk * kBlockN + lane * 16;
-          int tile = -1;
-          if (lane < 8 && key < w.skv) {
-            const int page = p.table[(long long)b * p.width + (key >> p.blockShift)];
-            if (page >= 0 && page < p.numBlocks) tile = page;
+          return ldg_if(p.table + (long long)b * p.width + (key >> p.blockShift), lane < 8 && key < w.skv, -1);
+        };
+        // this thread's pieces of a key block of K or V on their way into registers, and (K) the scales of lane's group; `page` as above
+        uint4 d[kPieces];
+        float ks = -1.f, vs = 0.f;
+        auto fetch = [&](bool isV, int blk, int page) {
+          const int key0 = blk * kBlockN;
+          const bool there = page >= 0 && page < p.numBlocks;
+          const long long tile = there ? (long long)page * p.headsKV + w.unit : 0;
+          const long long at = there ? tile * headBytes + (long long)((key0 + lane * 16) & ((1 << p.blockShift) - 1)) * kHD : -1;
+          if (!isV && cw == 0) {
+            ks = ldg_if(p.scales[0] + tile, there, -1.f);
+            vs = ldg_if(p.scales[1] + tile, there, 0.f);
           }
-          return tile;
+          const uint8_t* base = p.codes[isV ? 1 : 0] + (myRow & 15) * kHD + slab * 64 + my16 * 16;
+          const int tail = w.skv - key0;  // keys of the request in the block
+#pragma unroll
+          for (int e = 0; e < kPieces; e++) {
+            const int row = myRow + e * stepRows;
+            const long long from = __shfl_sync(0xffffffffu, at, (row >> 4) & 7);
+            d[e] = ldg_if(reinterpret_cast<const uint4*>(base + from), e < myPieces && from >= 0 && row < tail);
+          }
         };
         const int numLoads = 2 * w.nmax;
         auto which = [&](int i, bool& isV, int& blk) {  // the ring's order
@@ -1566,89 +1651,77 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             blk = i >> 1;
           }
         };
-        bool isV;
-        int blk;
+        bool isV, nextV = false;
+        int blk, nextBlk = 0;
         which(0, isV, blk);
-        int page = pageOf(w.part + blk);
-        fillQ(0);
+        fetch(isV, w.part + blk, pageOf(w.part + blk));
+        int page = -1;  // of the tile after the next
+        if (numLoads > 1) {
+          which(1, nextV, nextBlk);
+          page = pageOf(w.part + nextBlk);
+        }
+        fillQ(0);  // Q of tile 0 ahead of the first K block, Q of tile 1 behind it
         for (int i = 0; i < numLoads; i++, ld++) {
-          const int key0 = (w.part + blk) * kBlockN;
-          const uint8_t* base = p.codes[isV ? 1 : 0];
-          uint4 d[kPieces];
-#pragma unroll
-          for (int e = 0; e < kPieces; e++) {
-            const int piece = tid + e * kConv, row = piece / kChunks;
-            const int pg = __shfl_sync(0xffffffffu, page, row >> 4);
-            d[e] = make_uint4(0, 0, 0, 0);
-            if (pg >= 0 && key0 + row < w.skv) {
-              d[e] = __ldg(reinterpret_cast<const uint4*>(base + ((long long)pg * p.headsKV + w.unit) * headBytes +
-                                                          (long long)((key0 + row) & ((1 << p.blockShift) - 1)) * kHD + (piece % kChunks) * 16));
-            }
-          }
-          float ks = -1.f, vs = 0.f;
-          if (!isV && cw == 0 && page >= 0) {
-            ks = __ldg(p.scales[0] + (long long)page * p.headsKV + w.unit);
-            vs = __ldg(p.scales[1] + (long long)page * p.headsKV + w.unit);
-          }
-          bool nextV = false;
-          int nextBlk = 0, nextPage = 0;
-          if (i + 1 < numLoads) {
-            which(i + 1, nextV, nextBlk);
-            nextPage = pageOf(w.part + nextBlk);
-          }
           const int s = ld % NS;
           if (ld >= NS) wait_bar(bar(kBarKvEmpty + s), ((ld / NS) - 1) & 1, wc, 14);
-          if (!isV) {  // scales and row factors first: the softmax warps look at them when the scores are there
-            const int g = (blkBase + blk) & 7;
-            if (cw == 0 && lane < 8) {
+          const uint32_t dst = sKV + s * C::kStageBytes + slab * kSubTileBytes + myRow * 128;
+          const int sw = myRow & 7;  // steps are multiples of eight rows
+          const uint32_t at0 = dst + (((2 * my16) ^ sw) << 4), at1 = dst + (((2 * my16 + 1) ^ sw) << 4);
+#pragma unroll
+          for (int e = 0; e < kPieces; e++) {
+            constexpr bool kInt8 = (kScore & kScoreInt8) != 0;
+            uint4 a, z;
+            widen<kInt8>(d[e].x, a.x, a.y);
+            widen<kInt8>(d[e].y, a.z, a.w);
+            widen<kInt8>(d[e].z, z.x, z.y);
+            widen<kInt8>(d[e].w, z.z, z.w);
+            if (e < myPieces) {
+              const uint32_t step = (uint32_t)(e * stepRows * 128);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at0 + step), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w) : "memory");
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at1 + step), "r"(z.x), "r"(z.y), "r"(z.z), "r"(z.w) : "memory");
+            }
+          }
+          const int g = (blkBase + blk) & 7;
+          if (!isV && cw == 0) {
+            const bool there = ks >= 0.f || ks != ks;
+            float top = lane < 8 ? vs : 0.f;
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            const unsigned none = ~__ballot_sync(0xffffffffu, there) & 0xFFu;
+            if (lane < 8) {
               cctl->scales[g][lane] = ks;
               cctl->scales[g][8 + lane] = vs;
             }
-            __syncwarp();
-            if (blk > 0 && lane == 0) ptx::mbar_arrive(ptx::smem_u32(&cctl->scaleFull[g]));
+            if (lane == 0) cctl->summary[g] = make_float2(top, __uint_as_float(none));
           }
-          const uint32_t dst = sKV + s * C::kStageBytes;
-          auto put = [&](auto int8) {
-#pragma unroll
-            for (int e = 0; e < kPieces; e++) {
-              const int piece = tid + e * kConv, row = piece / kChunks, c16 = piece % kChunks;
-              uint4 a, z;
-              widen<decltype(int8)::value>(d[e].x, a.x, a.y);
-              widen<decltype(int8)::value>(d[e].y, a.z, a.w);
-              widen<decltype(int8)::value>(d[e].z, z.x, z.y);
-              widen<decltype(int8)::value>(d[e].w, z.z, z.w);
-              // a slab's even pieces and the next slab's odd ones together: eight lanes, eight groups of banks
-              const bool swap = (c16 & 4) != 0;
-              const uint32_t at = dst + (c16 >> 2) * kSubTileBytes + row * 128;
-              const int c0 = 2 * (c16 & 3), sw = row & 7;
-              const uint32_t first = at + (((c0 + (swap ? 1 : 0)) ^ sw) << 4), second = at + (((c0 + (swap ? 0 : 1)) ^ sw) << 4);
-              const uint4 u = swap ? z : a, v2 = swap ? a : z;
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(first), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(second), "r"(v2.x), "r"(v2.y), "r"(v2.z), "r"(v2.w) : "memory");
+          const bool wasV = isV;
+          const int wasBlk = blk;
+          if (i + 1 < numLoads) {  // the next tile is on its way while this one is handed over, and the pages of the one after it
+            isV = nextV;
+            blk = nextBlk;
+            fetch(isV, w.part + blk, page);
+            if (i + 2 < numLoads) {
+              which(i + 2, nextV, nextBlk);
+              page = pageOf(w.part + nextBlk);
             }
-          };
-          if (p.int8) {
-            put(std::integral_constant<bool, true>{});
-          } else {
-            put(std::integral_constant<bool, false>{});
           }
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
+            if (!wasV && wasBlk > 0) ptx::mbar_arrive(ptx::smem_u32(&cctl->scaleFull[g]));  // the scales: before the scores can be there
             ptx::mbar_arrive(bar(kBarKvFull + s));
             if (cw == 0) {  // the stage-free arrival of every tile that will not touch this block
 #pragma unroll
               for (int t = 0; t < 2; t++) {
-                if (t >= NT || blk >= w.nblk[t]) ptx::mbar_arrive(bar(kBarKvEmpty + s));
+                if (t >= NT || wasBlk >= w.nblk[t]) ptx::mbar_arrive(bar(kBarKvEmpty + s));
               }
             }
           }
-          // the first block's: the row factors of both tiles belong to it
-          if (i == 0 && NT == 2) fillQ(1);
-          if (i == 0 && lane == 0) ptx::mbar_arrive(ptx::smem_u32(&cctl->scaleFull[blkBase & 7]));
-          isV = nextV;
-          blk = nextBlk;
-          page = nextPage;
+          if (i == 0) {  // the row factors of both tiles belong to the first block
+            if (NT == 2) fillQ(1);
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&cctl->scaleFull[blkBase & 7]));
+          }
         }
         blkBase += w.nmax;
       }
