@@ -20,12 +20,12 @@ def _slopes(H):
     return torch.tensor([2.0 ** (-8.0 * (h + 1) / H) for h in range(H)], device="cuda")
 
 
-def _compare(got, Q, K, V, causal, cap=0.0, slopes=None, prefix=None, dq=None, dk=None, q_start=0):
+def _compare(got, Q, K, V, causal, cap=0.0, slopes=None, prefix=None, dq=None, dk=None, q_start=0, fp32_error=2.0 ** -21):
     for b in range(Q.shape[0]):
         see, dist = visible(Q.shape[1], K.shape[1], causal, q_start, None if prefix is None else int(prefix[b]), None if dq is None else dq[b],
                             None if dk is None else dk[b])
         o, off, a = attend(Q[b].double(), K[b].double(), V[b].double(), see, cap, slopes, dist,
-                            2.0 ** -21 if Q.dtype == torch.float32 else 8.6e-5)
+                            fp32_error if Q.dtype == torch.float32 else 8.6e-5)
         check(got[b], o, off, a, U[Q.dtype], K.shape[1] * 2.0 ** -25 * V[b].abs().max().item() if Q.dtype == torch.float16 else 0.0)
 
 
@@ -179,6 +179,104 @@ def test_nan_keys_and_values_in_places_nobody_sees(dtype):
     K[:, 200:] = math.nan  # the causal mask hides them from the rows before
     got = tfa.flash_attn_scored_forward(Q[:, :200].contiguous(), K, V, is_causal=True, doc_ids_q=docs[:, :200].contiguous(), doc_ids_kv=docs)
     assert torch.equal(got, want[:, :200])
+
+
+FP32_SHAPES = [  # B, Sq, Skv, Hq, Hkv: one key, tile edges, heads in one tile, several key ranges, more than one batch entry
+    (1, 1, 1, 1, 1), (2, 3, 1300, 8, 2), (1, 127, 129, 3, 1), (2, 129, 300, 4, 4), (1, 300, 1500, 2, 1), (3, 140, 131, 6, 2),
+]
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("shape", FP32_SHAPES, ids=lambda s: "-".join(map(str, s)))
+def test_both_fp32_forms(shape, D):
+    """CUDA cores and three bf16 parts per float.  The latter's scores: six passes of D/16 steps, each truncating once (2^-23 of the sum), and
+    the two products of 2^-24 that are left out: 0.75 D + 2 units of 2^-24, within plain64's D.  P V: the last pass of a block of 128 keys
+    truncates 8 times at full magnitude, 2^-20 A (the five before it at 2^-8 of that), blocks are added with 2^-24 each, and the parts
+    left out are 2^-23: with plain64's 2^-21 for the exponential together below 2^-19."""
+    B, Sq, Skv, Hq, Hkv = shape
+    Q, K, V = _inputs("fp32", *shape, D, 20)
+    prefix = torch.tensor([[0, Skv // 3 + 1, Skv + 500][b % 3] for b in range(B)], dtype=torch.int32, device="cuda")
+    docs = _documents(B, max(Sq, Skv), 70, 5)
+    mixed = _documents(B, max(Sq, Skv), 70, 5, shuffle=True)
+    slopes = _slopes(Hq)
+    calls = [
+        (dict(is_causal=True, softcap=2.5, alibi_slopes=slopes), dict(cap=2.5, slopes=slopes)),
+        (dict(is_causal=False, alibi_slopes=slopes), dict(slopes=slopes)),
+        (dict(is_causal=True, softcap=0.7, prefix_lens=prefix), dict(cap=0.7, prefix=prefix)),
+        (dict(is_causal=True, q_start=max(Skv - Sq, 0), alibi_slopes=slopes), dict(q_start=max(Skv - Sq, 0), slopes=slopes)),
+        (dict(is_causal=True, doc_ids_q=docs[:, :Sq].contiguous(), doc_ids_kv=docs[:, :Skv].contiguous()), dict(dq=docs[:, :Sq], dk=docs[:, :Skv])),
+        (dict(is_causal=False, doc_ids_q=docs[:, :Sq].contiguous(), doc_ids_kv=mixed[:, :Skv].contiguous(), alibi_slopes=slopes),
+         dict(dq=docs[:, :Sq], dk=mixed[:, :Skv], slopes=slopes)),
+    ]
+    for form, error in ((0, 2.0 ** -21), (1, 2.0 ** -19)):
+        tfa.set_option("fp32_tc", form)
+        try:
+            for args, plain in calls:
+                got = tfa.flash_attn_scored_forward(Q, K, V, **args)
+                _compare(got, Q, K, V, args["is_causal"], fp32_error=error, **plain)
+            tfa.device_status()
+        finally:
+            tfa.set_option("fp32_tc", -1)
+
+
+def test_fp32_values_outside_the_exact_range():
+    """Such calls are left to the CUDA cores, to the last bit; the document tables are then those of the other kernel's blocks."""
+    Q, K, V = _inputs("fp32", 2, 400, 400, 4, 2, 64, 21)
+    docs = _documents(2, 400, 90, 6)
+    K[0, 17, 1, 3] = 2.0 ** -110
+    args = dict(is_causal=True, softcap=3.0, alibi_slopes=_slopes(4), doc_ids_q=docs, doc_ids_kv=docs)
+    got = []
+    for form in (0, 1):
+        tfa.set_option("fp32_tc", form)
+        got.append(tfa.flash_attn_scored_forward(Q, K, V, **args))
+        tfa.set_option("fp32_tc", -1)
+    assert torch.equal(*got)
+    tfa.device_status()
+
+
+@pytest.mark.parametrize("dtype,B,Sq,Skv,Hq,Hkv,D", [
+    ("fp16", 2, 260, 260, 4, 2, 64), ("bf16", 1, 300, 300, 2, 1, 128), ("fp16", 1, 200, 200, 2, 2, 32), ("bf16", 1, 150, 150, 1, 1, 96), ("fp16", 1, 140, 140, 2, 1, 192),
+    ("bf16", 1, 140, 140, 2, 1, 256),  # tiles
+    ("fp16", 1, 64, 6000, 2, 1, 64), ("bf16", 1, 100, 4000, 2, 1, 256), ("bf16", 1, 40, 6000, 4, 1, 96), ("fp16", 1, 70, 6000, 4, 1, 128),  # key ranges
+    ("fp16", 3, 4, 700, 4, 1, 64), ("bf16", 1, 4, 9000, 8, 2, 128), ("bf16", 9, 2, 300, 16, 16, 96), ("fp16", 1, 3, 8000, 1, 1, 256),  # few rows
+    ("fp32", 2, 100, 130, 4, 2, 64), ("fp32", 1, 200, 260, 2, 1, 128), ("fp32", 1, 70, 200, 2, 1, 256),
+])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_values_that_a_mask_hides(dtype, B, Sq, Skv, Hq, Hkv, D, bad):
+    """V behind a row's own position may be anything: the row is as without it.  Rows that see it are what 0 x NaN and sums make of them."""
+    Q, K, V = _inputs(dtype, B, Sq, Skv, Hq, Hkv, D, 30)
+    q_start = Skv - Sq
+    slopes = _slopes(Hq)
+    first = q_start + Sq // 2  # the first key with a bad value
+    V2 = V.clone()
+    V2[:, first, :, 5] = bad
+    V2[:, first + 3:] = -bad
+    got = tfa.flash_attn_scored_forward(Q, K, V2, is_causal=True, softcap=3.0, alibi_slopes=slopes, q_start=q_start)
+    n = first - q_start  # rows before it
+    clean = V.clone()
+    clean[:, first:] = 0
+    _compare(got[:, :n], Q[:, :n], K, clean, True, 3.0, slopes, q_start=q_start, fp32_error=2.0 ** -19)
+    assert not torch.isfinite(got[:, n:, :, 5]).any()
+    if n + 3 <= Sq:
+        assert torch.isfinite(got[:, n:n + 3, :, 6:]).all()
+    tfa.device_status()
+
+
+@pytest.mark.parametrize("dtype,S,D", [("fp16", 300, 64), ("bf16", 500, 128), ("fp32", 300, 64), ("fp16", 200, 256)])
+@pytest.mark.parametrize("shuffle", [False, True])
+def test_values_of_other_documents_and_padding(dtype, S, D, shuffle):
+    Q, K, V = _inputs(dtype, 2, S, S, 2, 1, D, 31)
+    docs = _documents(2, S, 40, 7, shuffle=shuffle)
+    V2, K2 = V.clone(), K.clone()
+    V2[docs < 0] = math.nan
+    K2[docs < 0] = math.nan
+    V2[docs == 4] = math.inf
+    got = tfa.flash_attn_scored_forward(Q, K2, V2, is_causal=False, doc_ids_q=docs, doc_ids_kv=docs)
+    want = tfa.flash_attn_scored_forward(Q, K, V, is_causal=False, doc_ids_q=docs, doc_ids_kv=docs)
+    assert (docs == 4).any() and not torch.isfinite(got[docs == 4]).any()
+    got[docs == 4] = want[docs == 4]
+    _compare(got, Q, K, V, False, dq=docs, dk=docs, fp32_error=2.0 ** -19)
+    tfa.device_status()
 
 
 def test_refusals():

@@ -431,14 +431,19 @@ static int dispatch_splitkv(const FwdProblem& p, const SplitPlan& plan) {
 // on the CUDA cores, as before there were tensor-core kernels: a graph that allocates cannot be cloned or instantiated twice at
 // a time, and graphs of these calls could.  (The split-KV path has always allocated under capture.)  So a captured call and an
 // eager one may differ in the last bits of their sums.
-static int dispatch_fp32(const FwdProblem& p) {
+bool fp32_on_tensor_cores(const FwdProblem& p) {
   const int opt = g_optFp32Tc.load();
   // an explicit choice of the CUDA-core form (option "fp32_t8") is kept
-  if (opt == 0 || (opt < 0 && g_optFp32T8.load() != 1)) return launch_fwd_fp32(p);
+  if (opt == 0 || (opt < 0 && g_optFp32T8.load() != 1)) return false;
   int device = 0;
-  if (!p.overlap || cudaGetDevice(&device) != cudaSuccess) return launch_fwd_fp32(p);  // under capture
+  if (!p.overlap || cudaGetDevice(&device) != cudaSuccess) return false;  // under capture
+  return fp32tc_applicable(p, pick_pack_shift(p), device_num_sms(device), opt);
+}
+
+int dispatch_fp32(const FwdProblem& p, bool tensorCores) {
+  int device = 0;
+  if (!tensorCores || cudaGetDevice(&device) != cudaSuccess) return launch_fwd_fp32(p);
   const int ps = pick_pack_shift(p);
-  if (!fp32tc_applicable(p, ps, device_num_sms(device), opt)) return launch_fwd_fp32(p);
   cudaMemPool_t pool = scratch_pool(device);
   void* ws = nullptr;
   // A workspace beyond what the pool keeps would be taken from the driver and given back around every synchronisation, at
@@ -602,7 +607,7 @@ bool may_overlap(cudaStream_t stream) {
 
 static int dispatch(FwdProblem p) {
   p.overlap = may_overlap(p.stream);
-  if (p.dtype == kFp32) return dispatch_fp32(p);
+  if (p.dtype == kFp32) return dispatch_fp32(p, fp32_on_tensor_cores(p));
   const int optSplit = g_optSplitKv.load();
   if (optSplit != 0 && p.totalQ >= 0 && splitkv_applicable(p)) {
     return dispatch_splitkv(p, splitkv_plan(p, num_sms(), optSplit));

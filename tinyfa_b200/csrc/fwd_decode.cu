@@ -26,11 +26,13 @@
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/tinyfa_b200.h"
 #include "build_config.cuh"
 #include "ptx_sm100.cuh"
 #include "score.cuh"
+#include "score_row.cuh"
 #include "tfa_common.cuh"
 
 namespace tfa_b200 {
@@ -43,6 +45,9 @@ constexpr int kThreads = 128;
 constexpr int kBlockKeys = 64;
 constexpr int kStages = 3;
 constexpr int kRows = 16;  // query rows per CTA (MMA M)
+
+template <bool kBf16>
+using Element = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
 
 struct Params {
   const void* Q;
@@ -331,6 +336,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
       }
       __syncthreads();
     }
+    [[maybe_unused]] uint32_t spoilt = 0;  // rows with a value that is not finite, though their weights are
     for (int idx = threadIdx.x; idx < nRows * (D / 4); idx += kThreads) {
       const int r = idx / (D / 4), c4 = idx % (D / 4);
       float m = -INFINITY;
@@ -363,10 +369,20 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
         out.x = pack2<kBf16>(acc.x, acc.y);
         out.y = pack2<kBf16>(acc.z, acc.w);
         *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.O) + orow * D + c4 * 4) = out;
+        if (kScore && l > 0.f && l < INFINITY && !(fabsf(acc.x + acc.y + acc.z + acc.w) < INFINITY)) spoilt |= 1u << r;
       } else {
         const long long prow = (long long)part * p.totalQ * p.headsQ + orow;
         *reinterpret_cast<float4*>(p.partO + prow * D + c4 * 4) = acc;
         if (c4 == 0) p.partLse[prow] = (l == 0.f) ? -INFINITY : (m * c + log2f(l));  // NaN stays NaN
+      }
+    }
+    if constexpr (kScore) {
+      __syncwarp();
+      spoilt = __reduce_or_sync(0xffffffffu, spoilt);
+#pragma unroll 1
+      for (; spoilt != 0u; spoilt &= spoilt - 1) {
+        const int r = __ffs(spoilt) - 1;
+        score::exact_row<Element<kBf16>, D>(p, qRow0 + r / p.group, hkv * p.group + r % p.group, p.O);
       }
     }
   };
@@ -547,13 +563,17 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
 // Packed input: the grid is that of the split kernel with the rows of a tile in place of the splits, so that exactly the rows
 // that have partials are stored - none before cu_seqlens_q[0], past the last sequence or past a tile's sixteen.
 constexpr int kCombineThreads = 128;
-template <int D, bool kBf16>
+struct NoFields {};
+// kScore: rows that V has spoilt from a masked place are computed again
+template <int D, bool kBf16, bool kScore = false>
 __global__ void __launch_bounds__(kCombineThreads)
 combine_kernel(const float* partO, const float* partLse, void* O, long long rows /* totalQ * Hq */, int splits, const int* cuQ,
-               const int* cuKV, int headsQ, int group, int runs, int blocksPerEntry, long long totalBlocks, int seqLenQ) {
+               const int* cuKV, int headsQ, int group, int runs, int blocksPerEntry, long long totalBlocks, int seqLenQ,
+               const typename std::conditional<kScore, ScoreFields, NoFields>::type fields) {
   constexpr int kVec = D / 4, kGroups = kCombineThreads / kVec;
   __shared__ float4 sAcc[kGroups][kVec];
   __shared__ float sSum[kGroups];
+  [[maybe_unused]] __shared__ bool sBad[kScore ? kVec : 1];
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
   int r = 0, nRows = 1;  // rows of this CTA: r, r + gridDim.x, ... (packed input), one (fixed length)
@@ -612,6 +632,15 @@ combine_kernel(const float* partO, const float* partLse, void* O, long long rows
       out.x = pack2<kBf16>(acc.x * inv, acc.y * inv);
       out.y = pack2<kBf16>(acc.z * inv, acc.w * inv);
       *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(O) + row * D + threadIdx.x * 4) = out;
+      if constexpr (kScore) sBad[threadIdx.x] = wsum > 0.f && wsum < INFINITY && !(fabsf(acc.x + acc.y + acc.z + acc.w) < INFINITY);
+    }
+    if constexpr (kScore) {
+      __syncthreads();
+      if (threadIdx.x < 32) {
+        bool bad = false;
+        for (int i = threadIdx.x; i < kVec; i += 32) bad |= sBad[i];
+        if (__any_sync(0xffffffffu, bad)) score::exact_row<Element<kBf16>, D>(fields, row / headsQ, (int)(row % headsQ), O);
+      }
     }
     if (r + (int)gridDim.x < nRows) __syncthreads();  // sAcc is written again
   }
@@ -619,62 +648,73 @@ combine_kernel(const float* partO, const float* partLse, void* O, long long rows
 
 // Partial results of the tensor-core kernel's key ranges (kModeFixedSplit), many rows and few ranges: D / 4 threads per
 // row, several rows per CTA.
-template <int D, bool kBf16>
+template <int D, bool kBf16, bool kScore = false>
 __global__ void __launch_bounds__(kCombineThreads)
 combine_parts_kernel(const float* partO, const float* partLse, void* O, long long rows, int partBlocks,
-                     int seqLenQ, int seqLenKV, int headsQ, int causal, int rowsPerTile, int qStart) {
+                     int seqLenQ, int seqLenKV, int headsQ, int causal, int rowsPerTile,
+                     const typename std::conditional<kScore, ScoreFields, NoFields>::type fields) {
   constexpr int kVec = D / 4, kGroups = kCombineThreads / kVec;
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
   const int g = threadIdx.x / kVec, c4 = threadIdx.x % kVec;
   const long long row = (long long)blockIdx.x * kGroups + g;
-  if (g >= kGroups || row >= rows) return;
+  bool on = g < kGroups && row < rows, bad = false;
+  if (!kScore && !on) return;
   int blocks = (seqLenKV + 127) / 128;
   if (causal) {  // key blocks of this row's query tile, as in make_work
+    int qStart = 0;
+    if constexpr (kScore) qStart = fields.qStart;
     const int tile = (int)(row / headsQ % seqLenQ) / rowsPerTile;
     blocks = min(blocks, (qStart + min((tile + 1) * rowsPerTile, seqLenQ) + 127) / 128);
   }
   const int parts = (blocks + partBlocks - 1) / partBlocks;
-  if (parts == 1) return;  // the attention kernel has written the output
-  float M = -INFINITY;
+  if (parts == 1) on = false;  // the attention kernel has written the output
+  if (!kScore && !on) return;
+  if (on) {
+    float M = -INFINITY;
 #pragma unroll 8
-  for (int s = 0; s < parts; s++) M = fmax_nan(M, __ldcg(partLse + s * rows + row));
-  if (M == -INFINITY) M = 0.f;  // no score above -inf: all weights and the row are 0, as in the unsplit kernel
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float wsum = 0.f;
+    for (int s = 0; s < parts; s++) M = fmax_nan(M, __ldcg(partLse + s * rows + row));
+    if (M == -INFINITY) M = 0.f;  // no score above -inf: all weights and the row are 0, as in the unsplit kernel
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float wsum = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < parts; s++) {
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(partO + (s * rows + row) * D + c4 * 4));
-    const float w = exp2f(__ldcg(partLse + s * rows + row) - M);
-    acc.x += w * v.x;
-    acc.y += w * v.y;
-    acc.z += w * v.z;
-    acc.w += w * v.w;
-    wsum += w;
+    for (int s = 0; s < parts; s++) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(partO + (s * rows + row) * D + c4 * 4));
+      const float w = exp2f(__ldcg(partLse + s * rows + row) - M);
+      acc.x += w * v.x;
+      acc.y += w * v.y;
+      acc.z += w * v.z;
+      acc.w += w * v.w;
+      wsum += w;
+    }
+    const float inv = (wsum == 0.f) ? 0.f : (1.f / wsum);  // NaN stays NaN
+    uint2 out;
+    out.x = pack2<kBf16>(acc.x * inv, acc.y * inv);
+    out.y = pack2<kBf16>(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(O) + row * D + c4 * 4) = out;
+    if (kScore) bad = wsum > 0.f && wsum < INFINITY && !(fabsf(acc.x + acc.y + acc.z + acc.w) < INFINITY);
   }
-  const float inv = (wsum == 0.f) ? 0.f : (1.f / wsum);  // NaN stays NaN
-  uint2 out;
-  out.x = pack2<kBf16>(acc.x * inv, acc.y * inv);
-  out.y = pack2<kBf16>(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(O) + row * D + c4 * 4) = out;
+  if constexpr (kScore) score::exact_rows<Element<kBf16>, D>(fields, bad, row / headsQ, (int)(row % headsQ), O);
 }
 
-template <int D, bool kBf16>
+template <int D, bool kBf16, bool kScore = false>
 int launch_combine(const FwdProblem& p, int packShift, const TcSplit& split) {
   constexpr int kGroups = kCombineThreads / (D / 4);
   const long long rows = p.totalQ * p.headsQ;
+  typename std::conditional<kScore, ScoreFields, NoFields>::type fields;
+  if constexpr (kScore) fields = *p.score;
   cudaError_t e;
   if (!p.causal && (rows <= 1024 || (rows <= 3072 && split.parts >= 12))) {
     // Few rows: one CTA per row, whose threads read the ranges side by side (without the mask every tile has all ranges).  us a call
     // at head dim 128, the kernel below -> this one, with 3, 6, 12 ranges: 512 rows 15.4 -> 14.7, 16.8 -> 15.1, 17.7 -> 15.8; 1024 16.7 -> 16.2,
     // 17.9 -> 16.5, 19.2 -> 17.4; 3072 17.4 -> 18.8, 24.8 -> 23.7, 38.7 -> 37.6; 4096 and 4, 6, 8 ranges 22.7 -> 20.6, 24.3 -> 26.0, 24.1 ->
     // 26.6; 8192 25.9 -> 29.4, 44.0 -> 45.9, 46.6 -> 50.6.
-    e = launch_kernel(combine_kernel<D, kBf16>, dim3((unsigned)rows), kCombineThreads, 0, p.stream, p.overlap, split.partO,
-                      split.partLse, p.O, rows, split.parts, nullptr, nullptr, p.headsQ, 1, 0, 0, 0ll, p.seqLenQ);
+    e = launch_kernel(combine_kernel<D, kBf16, kScore>, dim3((unsigned)rows), kCombineThreads, 0, p.stream, p.overlap, split.partO,
+                      split.partLse, p.O, rows, split.parts, nullptr, nullptr, p.headsQ, 1, 0, 0, 0ll, p.seqLenQ, fields);
   } else {
-    e = launch_kernel(combine_parts_kernel<D, kBf16>, dim3((unsigned)((rows + kGroups - 1) / kGroups)), kCombineThreads, 0, p.stream,
+    e = launch_kernel(combine_parts_kernel<D, kBf16, kScore>, dim3((unsigned)((rows + kGroups - 1) / kGroups)), kCombineThreads, 0, p.stream,
                       p.overlap, split.partO, split.partLse, p.O, rows, split.partBlocks, p.seqLenQ, p.seqLenKV, p.headsQ, p.causal,
-                      128 >> packShift, p.score != nullptr ? p.score->qStart : 0);
+                      128 >> packShift, fields);
   }
   if (e != cudaSuccess) {
     set_error_string("combine kernel launch failed: %s", cudaGetErrorString(e));
@@ -775,8 +815,10 @@ int launch(const FwdProblem& pr, const SplitPlan& plan, float* partO, float* par
     const long long rows = pr.totalQ * pr.headsQ;
     const int tileRows = pr.seqLenQ * p.group;  // a longer sequence than the caller's maximum: the CTAs take turns
     const dim3 combineGrid = pr.cuQ != nullptr ? dim3((unsigned)tileRows, (unsigned)pr.headsKV, (unsigned)pr.batch) : dim3((unsigned)rows);
-    e = launch_kernel(combine_kernel<D, kBf16>, combineGrid, kCombineThreads, 0, pr.stream, pr.overlap, partO, partLse, pr.O, rows,
-                      plan.splits, pr.cuQ, pr.cuKV, pr.headsQ, p.group, p.runs, p.blocksPerEntry, p.totalBlocks, pr.seqLenQ);
+    typename std::conditional<kScore, ScoreFields, NoFields>::type fields;
+    if constexpr (kScore) fields = *pr.score;
+    e = launch_kernel(combine_kernel<D, kBf16, kScore>, combineGrid, kCombineThreads, 0, pr.stream, pr.overlap, partO, partLse, pr.O, rows,
+                      plan.splits, pr.cuQ, pr.cuKV, pr.headsQ, p.group, p.runs, p.blocksPerEntry, p.totalBlocks, pr.seqLenQ, fields);
   }
   if (e != cudaSuccess) {
     set_error_string("split-KV kernel launch failed: %s", cudaGetErrorString(e));
@@ -862,9 +904,15 @@ int launch_combine_parts(const FwdProblem& p, int packShift, const TcSplit& spli
 #define TFA_COMBINE_CASE(D)                                                                    \
   case D:                                                                                      \
     if (bf) {                                                                                  \
-      if constexpr (TFA_HAVE_BF16) return decode::launch_combine<D, true>(p, packShift, split);  \
+      if constexpr (TFA_HAVE_BF16) {                                                           \
+        return p.score != nullptr ? decode::launch_combine<D, true, true>(p, packShift, split)  \
+                                  : decode::launch_combine<D, true>(p, packShift, split);       \
+      }                                                                                        \
     } else {                                                                                   \
-      if constexpr (TFA_HAVE_FP16) return decode::launch_combine<D, false>(p, packShift, split); \
+      if constexpr (TFA_HAVE_FP16) {                                                           \
+        return p.score != nullptr ? decode::launch_combine<D, false, true>(p, packShift, split) \
+                                  : decode::launch_combine<D, false>(p, packShift, split);      \
+      }                                                                                        \
     }                                                                                          \
     return kBadDtype;
   (void)bf;

@@ -19,6 +19,7 @@
 #include "build_config.cuh"
 #include "ptx_sm100.cuh"
 #include "score.cuh"
+#include "score_row.cuh"
 #include "tfa_common.cuh"
 
 namespace tfa_b200 {
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
   if constexpr (kScore) {
     nblk = (skv + kBC - 1) / kBC;
     if (p.prefix != nullptr) prefix = p.prefix[b];
-    if (p.tileRange != nullptr) {
+    if (p.tileRange != nullptr && p.blockKeys == kBC) {  // else they are the tensor-core kernel's, which has left the call to this one
       const int2 range = p.tileRange[(long long)b * p.tiles + tileIdx];
       blk0 = range.x;
       nblk = range.y;
@@ -379,6 +380,7 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
     sum += __shfl_xor_sync(0xffffffffu, sum, 4);
     const float inv = (sum > 0.f) ? (1.f / sum) : 0.f;
     const int qpos = q0 + ty * RPT + r;
+    [[maybe_unused]] float spoilt = 0.f;  // NaN where a value of the row is not finite
     if (qpos < sq) {
       float* dst = p.O + (qRow0 + qpos) * qStride + (long long)h * D;
 #pragma unroll
@@ -389,9 +391,11 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
         v.z = o[r][i][2] * inv;
         v.w = o[r][i][3] * inv;
         if (kScore && sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);  // sees no key: zero even where 0 times a value is not
+        if constexpr (kScore) spoilt = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, spoilt))));
         *reinterpret_cast<float4*>(dst + (tx + 8 * i) * 4) = v;
       }
     }
+    if constexpr (kScore) score::exact_rows<float, D>(p, qpos < sq && spoilt != 0.f && sum > 0.f && sum < INFINITY, qRow0 + qpos, h, p.O);
   }
 }
 
@@ -944,18 +948,15 @@ template <int D, int BR, bool kScore = false>
 int launch(const FwdProblem& pr) {
   constexpr int LD = D + 4;
   constexpr int kSmem = (BR * LD + 2 * kBC * LD + BR * (kBC + 4)) * (int)sizeof(float);
-  auto kernel = fwd_fp32_kernel<D, BR, false, kScore>;
-  if constexpr (!kScore) {
-    if (pr.gate != nullptr) kernel = fwd_fp32_kernel<D, BR, true>;
-  }
+  auto kernel = pr.gate != nullptr ? fwd_fp32_kernel<D, BR, true, kScore> : fwd_fp32_kernel<D, BR, false, kScore>;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kCudaError;
   static std::once_flag once[64];
   static cudaError_t attrErr[64];
   std::call_once(once[device], [&] {
     attrErr[device] = cudaFuncSetAttribute(fwd_fp32_kernel<D, BR, false, kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (!kScore && attrErr[device] == cudaSuccess) {
-      attrErr[device] = cudaFuncSetAttribute(fwd_fp32_kernel<D, BR, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (attrErr[device] == cudaSuccess) {
+      attrErr[device] = cudaFuncSetAttribute(fwd_fp32_kernel<D, BR, true, kScore>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     }
   });
   if (attrErr[device] != cudaSuccess) {

@@ -37,6 +37,7 @@
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "build_config.cuh"
 #include "fwd_tc.cuh"
@@ -74,6 +75,12 @@ struct SplitParams {
   int batches;
   int* flag;            // set to epoch when a value is outside the exact range
   int epoch;
+  // What nobody sees is taken as zero, whatever it holds: rows of no document (ids of Q's and of K's and V's rows, or null), and keys that the
+  // causal mask leaves to no row: those from reach on, where the prefix (or null) is no longer.
+  const int* doc[3];
+  const int* prefix;
+  int reach[3];
+  int seqLen[3];
 };
 
 // x = p0 + p1 + p2 for two values at once, each part packed as bf16x2 (first value in the low half)
@@ -90,6 +97,7 @@ __device__ __forceinline__ bool outside(float x) {
 }
 
 // Bound by memory: 4 bytes read and 6 written per element.  Eight elements per thread and step.
+template <bool kScore>
 __global__ void __launch_bounds__(kSplitThreads) split_kernel(const SplitParams p) {
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
@@ -110,7 +118,16 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const SplitParams 
     for (long long i = (long long)blockIdx.x * kSplitThreads + threadIdx.x; i < n8; i += (long long)gridDim.x * kSplitThreads) {
       const long long at = gap8 == 0 ? i : i + i / w8 * gap8;
       float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
-      if (i >= first && i < end) {
+      bool take = i >= first && i < end;
+      if constexpr (kScore) {
+        const long long row = i / w8;
+        if (p.doc[t] != nullptr) take = p.doc[t][row] >= 0;
+        if (p.reach[t] < p.seqLen[t]) {
+          const int b = (int)(row / p.seqLen[t]), at = (int)(row - (long long)b * p.seqLen[t]);
+          take = take && (at < p.reach[t] || (p.prefix != nullptr && at < p.prefix[b]));
+        }
+      }
+      if (take) {
         u = src[2 * at];
         v = src[2 * at + 1];
       }
@@ -159,8 +176,9 @@ struct Ctl {
 };
 static_assert(sizeof(Ctl) <= 3072, "control block");
 
-struct Params {
-  TcParams w;        // work description (make_work), output, mask, scale, status word
+template <class W>
+struct ParamsT {
+  W w;               // work description (make_work), output, mask, scale, status word
   int batches;       // batch entries of the tensor maps (1 for packed input): part i of entry b is entry i * batches + b
   const int* flag;   // inputs outside the exact range: leave the call to the CUDA-core kernel
   // Key ranges (fixed-length input with few tiles): blockIdx.y is the range, partBlocks key blocks of the tile.  Partial
@@ -171,15 +189,78 @@ struct Params {
   float* partM;    // [ranges][rows]
   float* partL;    // [ranges][rows]
 };
+using Params = ParamsT<TcParams>;
+using ScoreParams = ParamsT<TcScoreParams>;  // scores capped, biased or masked by prefix or document (score.cuh)
+template <bool kScore>
+struct ParamsOf {
+  using type = Params;
+};
+template <>
+struct ParamsOf<true> {
+  using type = ScoreParams;
+};
 
-template <int HDP, int kHD, bool kVarlen>
+// A query row of a scored call: masks as in the 16-bit kernels, cap and bias in full fp32 (tanhf, and distances that are exact).  Capped or
+// biased scores are multiples of log2(e) afterwards, the others in the exponent.
+struct ScoredRow {
+  tc::ScoreRow<tc::kScoreMask> row;
+  float scale, slope, cap, capInv;
+  bool bias;
+
+  __device__ __forceinline__ float begin(const ScoreParams& p, const tc::Work& w, int qpos, int head) {
+    row.begin(p.w, w, qpos, head, w.qlo[0]);
+    cap = p.w.cap;
+    bias = p.w.slopes != nullptr;
+    slope = bias && qpos < w.sq ? p.w.slopes[head] * 1.44269504f : 0.f;
+    scale = p.w.scaleLog2;
+    capInv = cap > 0.f ? p.w.scaleLog2 / (cap * 1.44269504f) : 0.f;
+    return cap > 0.f || bias ? 1.f : p.w.scaleLog2;
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t v, int key) const {
+    float x = __uint_as_float(v);
+    if (cap > 0.f) {
+      x = cap * 1.44269504f * tanhf(x * capInv);
+    } else if (bias) {
+      x *= scale;
+    }
+    if (bias) x = fmaf(-slope, fabsf((float)(row.pos - key)), x);
+    return __float_as_uint(x);
+  }
+  __device__ __forceinline__ bool changes() const { return cap > 0.f || bias; }
+  // keys of other documents among n scores from key kbase on
+  template <int N>
+  __device__ __forceinline__ void documents(const ScoreParams& p, uint32_t (&v)[N], int kbase, int skv) const {
+    if (p.w.docKV == nullptr) return;
+    if (!__any_sync(0xffffffffu, row.docLo > kbase || row.docHi < kbase + N)) return;  // every row sees all of them
+    if (row.docLo >= 0) {  // rows behind the last one too, in a warp whose other rows go by ids
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        if (kbase + i < row.docLo || kbase + i >= row.docHi) v[i] = 0xff800000u;
+      }
+    } else {
+      uint32_t see = 0;
+      for (int i = 0; i < N; i++) {
+        if (row.doc >= 0 && kbase + i < skv && row.docKV[kbase + i] == row.doc) see |= 1u << i;
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        if ((see >> i & 1u) == 0u) v[i] = 0xff800000u;
+      }
+    }
+  }
+};
+
+template <int HDP, int kHD, bool kVarlen, bool kScore = false>
 __global__ void __launch_bounds__(kThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-           const __grid_constant__ CUtensorMap tmV, const Params p) {
+           const __grid_constant__ CUtensorMap tmV, const typename ParamsOf<kScore>::type p) {
   using C = Cfg<HDP>;
   constexpr int NS = C::kStages;
   if constexpr (kVarlen) ptx::grid_wait_previous();  // the lengths are in global memory
-  tc::Work w;
+  if constexpr (kScore) {
+    if (p.w.prefix != nullptr || p.w.tileRange != nullptr) ptx::grid_wait_previous();  // and so are these
+  }
+  typename std::conditional<kScore, tc::WorkPart, tc::Work>::type w;
   if (!tc::make_work<1, kVarlen>(p.w, (int)blockIdx.x, w)) return;
   int n = w.nblk[0], j0 = 0;  // key blocks of this CTA and the first of them
   bool whole = true;
@@ -193,6 +274,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       return;
     }
   }
+  if constexpr (kScore) j0 += w.part;  // documents: the first block that the tile sees
 
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sQ = ptx::smem_u32(smem);
@@ -350,7 +432,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     const int r = threadIdx.x & 127;
     const uint32_t laneOff = (uint32_t)((warp & 3) * 32) << 16;
     const int qpos = w.qlo[0] + (r >> p.w.packShift);
-    const float c = p.w.scaleLog2;
+    float c = p.w.scaleLog2;
+    [[maybe_unused]] ScoredRow row;
+    if constexpr (kScore) c = row.begin(p, w, qpos, (w.unit << p.w.packShift) + (r & ((1 << p.w.packShift) - 1)));
     float m = -INFINITY, l = 0.f;
     for (int j = 0; j < n; j++) {
       tc::wait_bar(bar(kBarSFull + (j & 1)), (j >> 1) & 1, wc, 46);
@@ -363,9 +447,20 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
 #pragma unroll
       for (int q = 0; q < 4; q++) ptx::tmem_ld_fence(v[q]);
       const int kbase = (j0 + j) * kBlockN;
-      if ((kbase + kBlockN > w.skv) || (p.w.causal && (kbase + kBlockN - 1 > w.qlo[0]))) {
+      if constexpr (kScore) {
+        if (row.changes()) {
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+#pragma unroll
+            for (int i = 0; i < 32; i++) v[q][i] = row(v[q][i], kbase + q * 32 + i);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) row.documents(p, v[q], kbase + q * 32, w.skv);
+      }
+      if ((kbase + kBlockN > w.skv) || (p.w.causal && (kbase + kBlockN - 1 > (kScore ? row.row.seenByAll : w.qlo[0])))) {
         int lim = w.skv - kbase;
-        if (p.w.causal) lim = min(lim, qpos - kbase + 1);
+        if (p.w.causal) lim = min(lim, (kScore ? row.row.last : qpos) - kbase + 1);
 #pragma unroll
         for (int q = 0; q < 4; q++) {
 #pragma unroll
@@ -506,14 +601,17 @@ constexpr int kThreadsWide = 512;
 constexpr int kRegsIssueW = 64, kRegsSoftmaxW = 96, kRegsOutW = 176;
 static_assert(kRegsIssueW + kRegsSoftmaxW + 2 * kRegsOutW <= 4 * ((65536 / kThreadsWide) / 8 * 8), "register budget");
 
-template <int kHD, bool kVarlen>
+template <int kHD, bool kVarlen, bool kScore = false>
 __global__ void __launch_bounds__(kThreadsWide, 1)
 fwd_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, const Params p) {
+                const __grid_constant__ CUtensorMap tmV, const typename ParamsOf<kScore>::type p) {
   using C = CfgWide<kHD>;
   constexpr int NS = C::kStages;
   if constexpr (kVarlen) ptx::grid_wait_previous();  // the lengths are in global memory
-  tc::Work w;
+  if constexpr (kScore) {
+    if (p.w.prefix != nullptr || p.w.tileRange != nullptr) ptx::grid_wait_previous();  // and so are these
+  }
+  typename std::conditional<kScore, tc::WorkPart, tc::Work>::type w;
   if (!tc::make_work<1, kVarlen>(p.w, (int)blockIdx.x, w)) return;
   int n = w.nblk[0], j0 = 0;  // key blocks of this CTA and the first of them
   bool whole = true;
@@ -526,6 +624,7 @@ fwd_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       return;
     }
   }
+  if constexpr (kScore) j0 += w.part;  // documents: the first block that the tile sees
 
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sQ = ptx::smem_u32(smem);
@@ -685,16 +784,18 @@ fwd_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const int r = threadIdx.x & 127;
     const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const int qpos = w.qlo[0] + (r >> p.w.packShift);
-    const float c = p.w.scaleLog2;
+    float c = p.w.scaleLog2;
+    [[maybe_unused]] ScoredRow row;
+    if constexpr (kScore) c = row.begin(p, w, qpos, (w.unit << p.w.packShift) + (r & ((1 << p.w.packShift) - 1)));
     float m = -INFINITY, l = 0.f;
     for (int j = 0; j < n; j++) {
       tc::wait_bar(bar(kBarSFull), j & 1, wc, 46);
       ptx::tc_fence_after();
       const int kbase = (j0 + j) * kBlockN;
       int lim = kBlockN;  // columns [0, lim) are real keys that are not in the future
-      if ((kbase + kBlockN > w.skv) || (p.w.causal && (kbase + kBlockN - 1 > w.qlo[0]))) {
+      if ((kbase + kBlockN > w.skv) || (p.w.causal && (kbase + kBlockN - 1 > (kScore ? row.row.seenByAll : w.qlo[0])))) {
         lim = w.skv - kbase;
-        if (p.w.causal) lim = min(lim, qpos - kbase + 1);
+        if (p.w.causal) lim = min(lim, (kScore ? row.row.last : qpos) - kbase + 1);
       }
       float mNew = m;
 #pragma unroll
@@ -707,6 +808,13 @@ fwd_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         ptx::tmem_ld_fence(v2);
 #pragma unroll
         for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(v2[i]));
+        if constexpr (kScore) {
+          if (row.changes()) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = row(v[i], kbase + q * 16 + i);
+          }
+          row.documents(p, v, kbase + q * 16, w.skv);
+        }
         if (lim < q * 16 + 16) {
 #pragma unroll
           for (int i = 0; i < 16; i++) {
@@ -828,8 +936,9 @@ fwd_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 
 // Adds up the key ranges of the tiles that have several: D / 4 threads per row.
 constexpr int kMergeThreads = 128;
-template <int kHD>
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
+// qStart: position of query row 0.  scale: of maxima that are not multiples of log2(e) yet.
+template <int kHD, class P>
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const P p, int qStart, float scale) {
   constexpr int kVec = kHD / 4, kGroups = kMergeThreads / kVec;
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
@@ -840,7 +949,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
   if (p.w.causal) {  // key blocks of this row's query tile, as in make_work
     const int rowsPerTile = kBlockM >> p.w.packShift;
     const int tile = (int)(row / p.w.headsQ % p.w.seqLenQ) / rowsPerTile;
-    blocks = min(blocks, (min((tile + 1) * rowsPerTile, p.w.seqLenQ) + kBlockN - 1) / kBlockN);
+    blocks = min(blocks, (qStart + min((tile + 1) * rowsPerTile, p.w.seqLenQ) + kBlockN - 1) / kBlockN);
   }
   const int parts = (blocks + p.partBlocks - 1) / p.partBlocks;
   if (parts == 1) return;  // the attention kernel has written the output
@@ -854,7 +963,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
   for (int s = 0; s < parts; s++) {
     const long long i = s * p.rows + row;
     const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partO + i * kHD + c4 * 4));
-    const float f = tc::ex2((__ldcg(p.partM + i) - M) * p.w.scaleLog2);
+    const float f = tc::ex2((__ldcg(p.partM + i) - M) * scale);
     l = fmaf(__ldcg(p.partL + i), f, l);
     acc.x = fmaf(v.x, f, acc.x);
     acc.y = fmaf(v.y, f, acc.y);
@@ -895,9 +1004,11 @@ struct Ranges {
 static Ranges plan_ranges(const FwdProblem& pr, const Fp32Piece& piece, int packShift, int numSMs) {
   Ranges r;
   if (pr.cuQ != nullptr || piece.heads != pr.headsKV) return r;
+  if (pr.score != nullptr && (pr.score->prefix != nullptr || pr.score->docKV != nullptr)) return r;  // blocks that only the device knows
   const int rows = kBlockM >> packShift;
   const long long tiles = (long long)((pr.seqLenQ + rows - 1) / rows) * (pr.headsQ >> packShift) * piece.batches;
-  const int seen = pr.causal && pr.seqLenQ < pr.seqLenKV ? pr.seqLenQ : pr.seqLenKV;
+  const int reach = pr.seqLenQ + (pr.score != nullptr ? pr.score->qStart : 0);
+  const int seen = pr.causal && reach < pr.seqLenKV ? reach : pr.seqLenKV;
   const int n = (seen + kBlockN - 1) / kBlockN;
   long long parts = numSMs / tiles;
   if (parts > n / 2) parts = n / 2;
@@ -931,29 +1042,32 @@ static Layout layout(const FwdProblem& pr, const Fp32Piece& piece, const Ranges&
 }
 
 // The kernel of a head dim: two 128-row K / V rings up to 128, the wide form above.
-template <int kHD, bool kVarlen>
+template <int kHD, bool kVarlen, bool kScore = false>
 constexpr auto kernel_of() {
   if constexpr (kHD > 128) {
-    return fwd_wide_kernel<kHD, kVarlen>;
+    return fwd_wide_kernel<kHD, kVarlen, kScore>;
   } else {
-    return fwd_kernel<(kHD <= 64 ? 64 : 128), kHD, kVarlen>;
+    return fwd_kernel<(kHD <= 64 ? 64 : 128), kHD, kVarlen, kScore>;
   }
 }
 
-template <int kHD>
+template <int kHD, bool kScore = false>
 int launch(const FwdProblem& pr, const Fp32Piece& piece, int packShift, uint8_t* ws, int epoch) {
   constexpr int kSmem = kHD > 128 ? CfgWide<(kHD > 128 ? kHD : 256)>::kSmemBytes : Cfg<(kHD <= 64 ? 64 : 128)>::kSmemBytes;
   constexpr int threads = kHD > 128 ? kThreadsWide : kThreads;
   const bool varlen = (pr.cuQ != nullptr);
-  auto kernel = varlen ? kernel_of<kHD, true>() : kernel_of<kHD, false>();
+  auto kernel = kernel_of<kHD, false, kScore>();
+  if constexpr (!kScore) {
+    if (varlen) kernel = kernel_of<kHD, true>();
+  }
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kCudaError;
   static std::once_flag once[64];
   static cudaError_t attrErr[64];
   std::call_once(once[device], [&] {
-    attrErr[device] = cudaFuncSetAttribute(kernel_of<kHD, true>(), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (attrErr[device] == cudaSuccess) {
-      attrErr[device] = cudaFuncSetAttribute(kernel_of<kHD, false>(), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    attrErr[device] = cudaFuncSetAttribute(kernel_of<kHD, false, kScore>(), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (!kScore && attrErr[device] == cudaSuccess) {
+      attrErr[device] = cudaFuncSetAttribute(kernel_of<kHD, true>(), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     }
   });
   if (attrErr[device] != cudaSuccess) {
@@ -974,7 +1088,24 @@ int launch(const FwdProblem& pr, const Fp32Piece& piece, int packShift, uint8_t*
   if ((rc = make_map(&tmK, ws + lay.k, nb, rowsKV, piece.heads, pr.headDim, 1, kBlockN)) != kOk) return rc;
   if ((rc = make_map(&tmV, ws + lay.v, nb, rowsKV, piece.heads, pr.headDim, 1, kBlockN)) != kOk) return rc;
 
-  Params p = {};
+  typename ParamsOf<kScore>::type p = {};
+  float mergeScale = (float)(1.4426950408889634 / sqrt((double)pr.headDim));
+  int qStart = 0;
+  if constexpr (kScore) {
+    ScoreFields& f = p.w;
+    f = *pr.score;
+    qStart = f.qStart;
+    if (f.cap > 0.f || f.slopes != nullptr) mergeScale = 1.f;
+    if (f.slopes != nullptr) f.slopes += piece.head0 * group;
+    if (f.prefix != nullptr) f.prefix += piece.batch0;
+    if (f.docKV != nullptr) {
+      f.docQ += (long long)piece.batch0 * pr.seqLenQ;
+      f.docKV += (long long)piece.batch0 * pr.seqLenKV;
+      f.rowKeys += (long long)piece.batch0 * pr.seqLenQ;
+      f.tileRange += (long long)piece.batch0 * f.tiles;
+      f.keyBlocks += (long long)piece.batch0 * ((pr.seqLenKV + kBlockN - 1) / kBlockN);
+    }
+  }
   p.w.O = static_cast<float*>(pr.O) + skipQ;
   p.w.cuQ = pr.cuQ;
   p.w.cuKV = pr.cuKV;
@@ -1030,13 +1161,25 @@ int launch(const FwdProblem& pr, const Fp32Piece& piece, int packShift, uint8_t*
   sp.batches = pr.batch;
   sp.count[0] = rows_q(pr, piece) * sp.width[0];
   sp.count[1] = sp.count[2] = rows_kv(pr, piece) * sp.width[1];
+  sp.prefix = nullptr;
+  for (int t = 0; t < 3; t++) {
+    sp.doc[t] = nullptr;
+    sp.reach[t] = sp.seqLen[t] = t == 0 ? pr.seqLenQ : pr.seqLenKV;
+  }
+  if constexpr (kScore) {
+    sp.doc[0] = p.w.docQ;
+    sp.doc[1] = sp.doc[2] = p.w.docKV;
+    sp.prefix = p.w.prefix;
+    if (pr.causal) sp.reach[1] = sp.reach[2] = qStart + pr.seqLenQ;
+  }
   sp.flag = reinterpret_cast<int*>(ws);
   sp.epoch = epoch;
-  cudaError_t e = launch_kernel(split_kernel, dim3(8u * (unsigned)device_num_sms(device)), kSplitThreads, 0, pr.stream, pr.overlap, sp);
+  cudaError_t e = launch_kernel(split_kernel<kScore>, dim3(8u * (unsigned)device_num_sms(device)), kSplitThreads, 0, pr.stream, pr.overlap, sp);
   if (e == cudaSuccess) e = launch_kernel(kernel, dim3((unsigned)numWork, (unsigned)ranges.parts), threads, kSmem, pr.stream, pr.overlap, tmQ, tmK, tmV, p);
   if (e == cudaSuccess && ranges.parts > 1) {
     constexpr int kGroups = kMergeThreads / (kHD / 4);
-    e = launch_kernel(merge_kernel<kHD>, dim3((unsigned)((p.rows + kGroups - 1) / kGroups)), kMergeThreads, 0, pr.stream, pr.overlap, p);
+    e = launch_kernel(merge_kernel<kHD, typename ParamsOf<kScore>::type>, dim3((unsigned)((p.rows + kGroups - 1) / kGroups)), kMergeThreads, 0, pr.stream,
+                      pr.overlap, p, qStart, mergeScale);
   }
   if (e != cudaSuccess) {
     set_error_string("fp32 tensor-core kernel launch failed: %s", cudaGetErrorString(e));
@@ -1062,7 +1205,9 @@ static double mean_blocks(double sq, double skv, bool causal, int block) {
 // call (CUDA cores, tensor cores): B512 S64 8 heads of 64 125, 348; B512 S49 12 heads of 32 111, 405; 2 x 100 x 3000 causal 8 heads of
 // 128 18.6, 32.8; B4 4096 x 16 8 heads of 64 61, 88; on the other side B64 S256 8 heads of 64 213, 137; B4 4096 x 77 113, 89.
 // Below the first line the launches decide: S128 4 heads of 64 11.7, 13.6; S128 4 heads of 128 18.6, 15.4; S256 4 heads of 64 21.2, 15.7.
-bool fp32tc_applicable(const FwdProblem& p, int packShift, int numSMs, int option) {
+bool fp32tc_applicable(const FwdProblem& call, int packShift, int numSMs, int option) {
+  FwdProblem p = call;
+  if (p.score != nullptr && (p.score->qStart > 0 || p.score->prefix != nullptr)) p.causal = 0;  // rows that see keys ahead of their own: about all of them
   if (!TFA_HAVE_FP32 || p.dtype != kFp32 || p.totalQ < 0 || p.totalKV < 0) return false;
   const bool packed = p.cuQ != nullptr;
   const int rows = fp32tc::kBlockM >> packShift;
@@ -1101,27 +1246,27 @@ int launch_fwd_fp32tc(const FwdProblem& p, const Fp32Piece& piece, int packShift
   switch (p.headDim) {
 #if TFA_HAVE_HD32
     case 32:
-      return fp32tc::launch<32>(p, piece, packShift, w, epoch);
+      return p.score != nullptr ? fp32tc::launch<32, true>(p, piece, packShift, w, epoch) : fp32tc::launch<32>(p, piece, packShift, w, epoch);
 #endif
 #if TFA_HAVE_HD64
     case 64:
-      return fp32tc::launch<64>(p, piece, packShift, w, epoch);
+      return p.score != nullptr ? fp32tc::launch<64, true>(p, piece, packShift, w, epoch) : fp32tc::launch<64>(p, piece, packShift, w, epoch);
 #endif
 #if TFA_HAVE_HD96
     case 96:
-      return fp32tc::launch<96>(p, piece, packShift, w, epoch);
+      return p.score != nullptr ? fp32tc::launch<96, true>(p, piece, packShift, w, epoch) : fp32tc::launch<96>(p, piece, packShift, w, epoch);
 #endif
 #if TFA_HAVE_HD128
     case 128:
-      return fp32tc::launch<128>(p, piece, packShift, w, epoch);
+      return p.score != nullptr ? fp32tc::launch<128, true>(p, piece, packShift, w, epoch) : fp32tc::launch<128>(p, piece, packShift, w, epoch);
 #endif
 #if TFA_HAVE_HD192
     case 192:
-      return fp32tc::launch<192>(p, piece, packShift, w, epoch);
+      return p.score != nullptr ? fp32tc::launch<192, true>(p, piece, packShift, w, epoch) : fp32tc::launch<192>(p, piece, packShift, w, epoch);
 #endif
 #if TFA_HAVE_HD256
     case 256:
-      return fp32tc::launch<256>(p, piece, packShift, w, epoch);
+      return p.score != nullptr ? fp32tc::launch<256, true>(p, piece, packShift, w, epoch) : fp32tc::launch<256>(p, piece, packShift, w, epoch);
 #endif
     default:
       break;

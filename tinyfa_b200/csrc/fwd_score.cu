@@ -15,6 +15,8 @@ namespace tfa_b200 {
 int device_num_sms(int device);  // c_abi.cu
 int pack_shift_of(const FwdProblem& p);
 int split_kv_option();
+bool fp32_on_tensor_cores(const FwdProblem& p);
+int dispatch_fp32(const FwdProblem& p, bool tensorCores);
 TcSplit tc_split_of(const FwdProblem& p, int packShift, int qStart);
 bool splitkv_applicable(const FwdProblem& p);  // fwd_decode.cu
 SplitPlan splitkv_plan(const FwdProblem& p, int numSMs, int forced);
@@ -207,7 +209,9 @@ int dispatch(FwdProblem p, ScoreFields& f, int device) {
     if (!docs && f.prefix == nullptr) split = tc_split_of(p, ps, f.qStart);
     if (split.parts > 1) floats = (size_t)split.parts * p.totalQ * p.headsQ * (p.headDim + 1);
   }
-  const int tileRows = fp32 ? kScoreTileRows : 128 >> ps, blockKeys = fp32 ? kScoreBlockKeys : 128;
+  const bool cores = fp32 && !fp32_on_tensor_cores(p);
+  if (fp32) ps = pack_shift_of(p);
+  const int tileRows = cores ? kScoreTileRows : 128 >> ps, blockKeys = f.blockKeys = cores ? kScoreBlockKeys : 128;
   const int blocks = (p.seqLenKV + blockKeys - 1) / blockKeys;
   f.tiles = (p.seqLenQ + tileRows - 1) / tileRows;
   const size_t tableBytes = docs ? (size_t)p.batch * (sizeof(int2) * ((size_t)blocks + f.tiles + p.seqLenQ) + blocks) : 0;
@@ -239,7 +243,7 @@ int dispatch(FwdProblem p, ScoreFields& f, int device) {
   }
   if (rc == kOk) {
     if (fp32) {
-      rc = launch_fwd_fp32(p);
+      rc = dispatch_fp32(p, !cores);
     } else if (rows) {
       rc = launch_fwd_splitkv(p, plan, static_cast<float*>(scratch));
     } else {
@@ -303,6 +307,7 @@ extern "C" int tfa_b200_fwd_scored(const void* Q, const void* K, const void* V, 
   p.headDim = headDim;
   p.causal = isCausal ? 1 : 0;
   p.stream = static_cast<cudaStream_t>(stream);
-  ScoreFields f = {qStart, softcap, alibiSlopes, prefixLens, docIdsQ, docIdsKV, nullptr, nullptr, nullptr, 0};
+  ScoreFields f = {qStart, softcap, alibiSlopes, prefixLens, docIdsQ, docIdsKV, nullptr, nullptr, nullptr, 0, 0,
+                   {Q, K, V, seqLenQ, seqLenKV, numHeadsQ, numHeadsKV, p.causal}};
   return score::dispatch(p, f, device);
 }

@@ -38,6 +38,7 @@
 #include "cache_codes.cuh"
 #include "ptx_sm100.cuh"
 #include "score.cuh"
+#include "score_row.cuh"
 #include "tfa_common.cuh"
 
 namespace tfa_b200 {
@@ -703,7 +704,7 @@ struct ScoreRow {
       keyBlocks = p.keyBlocks + (long long)b * ((w.skv + kBlockN - 1) / kBlockN);
       docLo = docHi = 0;
       if (qpos < w.sq) {
-        doc = p.docQ[w.qRow0 + qpos];
+        doc = p.docQ[w.qRow0 + qpos];  // (qRow0: first row of the batch entry among the call's, or the piece's of it)
         const int2 keys = p.rowKeys[w.qRow0 + qpos];
         docLo = keys.x;
         docHi = keys.y;
@@ -890,6 +891,15 @@ struct ScoreRow {
     }
   }
 };
+
+// Rows of a tile that V has spoilt from a masked place.  Partial results: the kernel that joins them looks.
+template <bool kBf16, int kHD, class P, class W>
+__device__ __forceinline__ void exact_rows_of_tile(const P& p, const W& w, int t, bool bad, int qpos, int head) {
+  if constexpr (std::is_base_of<TcPartParams, P>::value) {
+    if (!whole_tile(p, w, t)) return;
+  }
+  score::exact_rows<typename std::conditional<kBf16, __nv_bfloat16, __half>::type, kHD>(p, bad, w.qRow0 + qpos, head, p.O);
+}
 
 // ---- kModeCache
 // Shared memory behind Ctl.  Scales of a key block stay in a ring of eight blocks, well past the ring of tiles; row factors in a ring of
@@ -1496,6 +1506,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.O) +
                                               ((w.qRow0 + qpos) * p.headsQ + head) * (long long)p.headDim);
         const uint32_t tO = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(C::kOCol0 + t * HDP);
+        [[maybe_unused]] float spoilt = 0.f;  // NaN where a value of the row is not finite
 #pragma unroll
         for (int ch = 0; ch < kHD / 32; ch++) {
           uint32_t o[32];
@@ -1507,6 +1518,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
               for (int i = 0; i < 32; i++) o[i] = 0u;
             }
+#pragma unroll
+            for (int i = 0; i < 32; i++) spoilt = fmaf(__uint_as_float(o[i]), 0.f, spoilt);
           }
           if (ch == kHD / 32 - 1) {
             ptx::tc_fence_before();
@@ -1531,6 +1544,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             }
           }
         }
+        if constexpr (kScore != 0) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head);
         items++;
         continue;
       }
@@ -1769,6 +1783,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.O) +
                                               ((w.qRow0 + qpos) * p.headsQ + head) * (long long)p.headDim);
         const uint32_t tO = tmem + laneOff + (uint32_t)(C::kOCol0 + t * HDP);
+        [[maybe_unused]] float spoilt = 0.f;  // NaN where a value of the row is not finite
 #pragma unroll
         for (int ch = 0; ch < kHD / 32; ch++) {
           uint32_t o[32];
@@ -1780,6 +1795,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
               for (int i = 0; i < 32; i++) o[i] = 0u;
             }
+#pragma unroll
+            for (int i = 0; i < 32; i++) spoilt = fmaf(__uint_as_float(o[i]), 0.f, spoilt);
           }
           if (ch == kHD / 32 - 1) {  // O is in registers: the next item's first P.V may overwrite the accumulator
             ptx::tc_fence_before();
@@ -1808,6 +1825,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             }
           }
         }
+        if constexpr (kScore != 0 && !kCache) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head);
         items[t]++;
       }
     }

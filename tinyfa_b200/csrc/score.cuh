@@ -9,6 +9,11 @@
 
 namespace tfa_b200 {
 
+struct ScoreSource {  // the call's tensors, for rows that are computed one by one (score_row.cuh)
+  const void *q, *k, *v;
+  int seqLenQ, seqLenKV, headsQ, headsKV, causal;
+};
+
 struct ScoreFields {
   int qStart;           // position of query row 0
   float cap;            // 0: none
@@ -22,6 +27,8 @@ struct ScoreFields {
   const int2* tileRange;  // [batch][tiles]
   const int2* rowKeys;    // [batch][seqLenQ]
   int tiles;
+  int blockKeys;  // keys of a block in those tables
+  ScoreSource src;
 };
 
 }  // namespace tfa_b200
