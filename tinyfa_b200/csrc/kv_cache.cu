@@ -44,27 +44,28 @@ __device__ __forceinline__ long long length_before(const PlanParams& p, int b) {
   return min(max((long long)p.lens[b], 0ll), (long long)p.width << p.blockShift);
 }
 
-// Cell of the cache for packed row `row`, -1 for a row of no request or of one that was not served.
-__device__ __forceinline__ long long slot_of_row(const PlanParams& p, long long row) {
-  if (row >= p.cu[p.batch]) return -1;
+// Cell of the cache for packed row `row`, -1 for a row of no request or of one that was not served.  cu: p.cu or a copy of it.
+__device__ __forceinline__ long long slot_of_row(const PlanParams& p, const int* cu, long long row) {
+  if (row >= cu[p.batch]) return -1;
   int lo = 0, hi = p.batch - 1;  // the request b with cu[b] <= row < cu[b + 1]
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (row < p.cu[mid + 1]) {
+    if (row < cu[mid + 1]) {
       hi = mid;
     } else {
       lo = mid + 1;
     }
   }
-  const long long before = (p.finished != nullptr && p.finished[lo] != 0) ? 0 : length_before(p, lo);
-  if (p.lensAfter[lo] == before) return -1;  // the row exists, so its request asked for tokens: it was not served
-  const long long place = before + (row - p.cu[lo]);
+  const int after = p.lensAfter[lo];
+  const long long length = length_before(p, lo), before = (p.finished != nullptr && p.finished[lo] != 0) ? 0 : length;
+  if (after == before) return -1;  // the row exists, so its request asked for tokens: it was not served
+  const long long place = before + (row - cu[lo]);
   if (place < 0 || place >= (long long)p.width << p.blockShift) return -1;  // (rows of lengths whose sum does not fit 32 bits)
   const int block = p.table[(long long)lo * p.width + (place >> p.blockShift)];
   return block < 0 ? -1 : ((long long)block << p.blockShift) + (place & ((1 << p.blockShift) - 1));
 }
 
-// Inclusive sums of two values over the CTA.
+// Inclusive sums of two values over the CTA, whose first threads have values other than zero.
 __device__ __forceinline__ void cta_scan2(int& a, long long& b, int (&sA)[32], long long (&sB)[32], int& totalA, long long& totalB) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
@@ -81,50 +82,65 @@ __device__ __forceinline__ void cta_scan2(int& a, long long& b, int (&sA)[32], l
     sB[warp] = b;
   }
   __syncthreads();
-  totalA = 0;
-  totalB = 0;
-  int beforeA = 0;
-  long long beforeB = 0;
-  for (int w = 0; w < warps; w++) {
-    if (w == warp) {
-      beforeA = totalA;
-      beforeB = totalB;
+  int wa = lane < warps ? sA[lane] : 0;  // every warp sums the warps' totals for itself
+  long long wb = lane < warps ? sB[lane] : 0;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, wa, d);
+    const long long y = __shfl_up_sync(0xffffffffu, wb, d);
+    if (lane >= d) {
+      wa += x;
+      wb += y;
     }
-    totalA += sA[w];
-    totalB += sB[w];
   }
-  a += beforeA;
-  b += beforeB;
+  totalA = __shfl_sync(0xffffffffu, wa, 31);
+  totalB = __shfl_sync(0xffffffffu, wb, 31);
+  const int beforeA = __shfl_sync(0xffffffffu, wa, (warp + 31) & 31);
+  const long long beforeB = __shfl_sync(0xffffffffu, wb, (warp + 31) & 31);
+  if (warp > 0) {
+    a += beforeA;
+    b += beforeB;
+  }
 }
 
 // One CTA: two prefix sums over the requests (blocks given back, blocks and rows asked for), the stack and the tables; the slots
-// too where they are few.  Integers only; bound by the latency of a handful of dependent reads, so requests are handed to the warps one by one
-// (PLAN_MEASURED).
+// too where they are few.  Integers only; bound by the latency of a handful of dependent reads: what does not depend on another read is asked for at
+// once, a request's first new block is its thread's, further ones a warp's, and rows look for their request in shared memory.
+// PLAN_MEASURED
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, bool withSlots) {
   __shared__ int sA[2][32];
   __shared__ long long sB[2][32];
   __shared__ int sCount[kPlanThreads], sHeld[kPlanThreads];
   __shared__ int sTop[kPlanThreads];
+  __shared__ int sCu[kPlanThreads + 1];
   __shared__ int sTaken;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, threads = blockDim.x;
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
   if (threadIdx.x == 0) sTaken = 0;
   const int free0 = min(max(*p.numFree, 0), p.capacity);
+  // the thread's request of the first round
+  const bool mine = (int)threadIdx.x < p.batch;
+  const long long length0 = mine ? length_before(p, threadIdx.x) : 0;
+  const int fresh0 = mine ? max(p.newLens[threadIdx.x], 0) : 0;
+  const bool finished0 = mine && p.finished != nullptr && p.finished[threadIdx.x] != 0;
   // blocks of finished requests go on top of the stack, in the order of the requests
   long long returned = 0;
   int turn = 0;  // which half of sA, sB: a warp may still read the other one
-  if (p.finished != nullptr) {
+  if (p.finished != nullptr && __syncthreads_or(finished0 || p.batch > threads)) {
     for (int b0 = 0; b0 < p.batch; b0 += threads, turn ^= 1) {
       const int b = b0 + threadIdx.x;
-      int n = (b < p.batch && p.finished[b] != 0) ? blocks_of(length_before(p, b), p.blockShift) : 0, none = 0;
+      const bool ended = b0 == 0 ? finished0 : b < p.batch && p.finished[b] != 0;
+      int n = ended ? blocks_of(b0 == 0 ? length0 : length_before(p, b), p.blockShift) : 0, none = 0;
       sCount[threadIdx.x] = n;
       long long upto = n, sum;
       cta_scan2(none, upto, sA[turn], sB[turn], none, sum);
       sTop[threadIdx.x] = (int)min(free0 + returned + upto - sCount[threadIdx.x], (long long)p.capacity);
       __syncthreads();
-      for (int r = warp; r < min(threads, p.batch - b0); r += warps) {
-        const int count = sCount[r], at = sTop[r];
+      // requests warp, warp + warps, ... are this warp's
+      for (unsigned some = __ballot_sync(0xffffffffu, sCount[warp + lane * warps] > 0); some != 0; some &= some - 1) {
+        const int r = warp + (__ffs(some) - 1) * warps, count = sCount[r], at = sTop[r];
+#pragma unroll 4
         for (int i = lane; i < min(count, p.capacity - at); i += 32) p.freeBlocks[at + i] = p.table[(long long)(b0 + r) * p.width + i];
       }
       returned += sum;
@@ -140,8 +156,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, 
     int held = 0, need = 0;
     bool fits = true;
     if (b < p.batch) {
-      before = (p.finished != nullptr && p.finished[b] != 0) ? 0 : length_before(p, b);
-      fresh = max(p.newLens[b], 0);
+      if (b0 == 0) {
+        before = finished0 ? 0 : length0;
+        fresh = fresh0;
+      } else {
+        before = (p.finished != nullptr && p.finished[b] != 0) ? 0 : length_before(p, b);
+        fresh = max(p.newLens[b], 0);
+      }
       held = blocks_of(before, p.blockShift);
       fits = before + fresh <= ((long long)p.width << p.blockShift);
       need = fits ? blocks_of(before + fresh, p.blockShift) - held : 0;
@@ -151,39 +172,53 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, 
     cta_scan2(inclusive, row, sA[turn], sB[turn], sum, sumRows);
     const long long upto = asked + inclusive;
     const bool served = fits && (need == 0 || upto <= have);
+    const int top = (int)(served ? have - 1 - (upto - need) : 0);
     if (b < p.batch) {
-      p.cu[b + 1] = (int)(rows + row);
+      const int end = (int)(rows + row);
+      p.cu[b + 1] = end;
+      if (b0 == 0) sCu[b + 1] = end;
       p.lensAfter[b] = (int)(served ? before + fresh : before);
+      if (served && need > 0) {
+        p.table[(long long)b * p.width + held] = p.freeBlocks[top];
+        atomicMax(&sTaken, (int)upto);  // the served ones are those that ask for no more than there is
+      }
     }
     sCount[threadIdx.x] = served ? need : 0;
     sHeld[threadIdx.x] = held;
-    sTop[threadIdx.x] = (int)(served ? have - 1 - (upto - need) : 0);
-    if (served && need > 0) atomicMax(&sTaken, (int)upto);  // the served ones are those that ask for no more than there is
-    __syncthreads();
-    for (int r = warp; r < min(threads, p.batch - b0); r += warps) {
-      const int count = sCount[r], top = sTop[r];
-      int* row0 = p.table + (long long)(b0 + r) * p.width + sHeld[r];
+    sTop[threadIdx.x] = top;
+    if (__syncthreads_or(served && need > 1)) {
+      for (unsigned some = __ballot_sync(0xffffffffu, sCount[warp + lane * warps] > 1); some != 0; some &= some - 1) {
+        const int r = warp + (__ffs(some) - 1) * warps, count = sCount[r], first = sTop[r];
+        int* row0 = p.table + (long long)(b0 + r) * p.width + sHeld[r];
 #pragma unroll 4
-      for (int i = lane; i < count; i += 32) row0[i] = p.freeBlocks[top - i];
+        for (int i = 1 + lane; i < count; i += 32) row0[i] = p.freeBlocks[first - i];
+      }
     }
     asked += sum;
     rows += sumRows;
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    p.cu[0] = 0;
+    p.cu[0] = sCu[0] = 0;
     *p.numFreeAfter = have - sTaken;
   }
   if (!withSlots) return;
   __syncthreads();
-  for (long long row = threadIdx.x; row < p.total; row += threads) p.slots[row] = slot_of_row(p, row);
+  const int* cu = p.batch <= threads ? sCu : p.cu;
+  for (long long row = threadIdx.x; row < p.total; row += threads) p.slots[row] = slot_of_row(p, cu, row);
 }
 
 __global__ void __launch_bounds__(256) slots_kernel(const PlanParams p) {
+  __shared__ int sCu[kPlanThreads + 1];
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
+  const bool few = p.batch <= kPlanThreads;
+  if (few) {
+    for (int i = threadIdx.x; i <= p.batch; i += 256) sCu[i] = p.cu[i];
+    __syncthreads();
+  }
   const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (row < p.total) p.slots[row] = slot_of_row(p, row);
+  if (row < p.total) p.slots[row] = slot_of_row(p, few ? sCu : p.cu, row);
 }
 
 // ------------------------------------------------------------------------------------------------------------ store
@@ -256,6 +291,45 @@ __device__ __forceinline__ uint2 to_codes(const float (&x)[8], float num, float 
   return make_uint2(word[0], word[1]);
 }
 
+// The same codes by multiplication: q = x * inv is within 5 x 2^-24 of the quotient, so a code that does not change within 2^-21 of q is the
+// quotient's.  False where one of the eight is that near the border between two codes (about one in 10^4 eights of random values); x is finite.
+template <bool kInt8>
+__device__ __forceinline__ bool quick_codes(const float (&x)[8], float inv, uint2& out) {
+  uint32_t word[2];
+  bool certain = true;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    float q[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) q[j] = x[h * 4 + j] * inv;
+    if constexpr (kInt8) {
+      constexpr float kRound = 12582912.f;  // 1.5 x 2^23: added, it leaves the nearest integer in the low bits
+      uint32_t c[4];
+      float far = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float r = __fadd_rn(q[j], kRound);
+        c[j] = __float_as_uint(r);
+        far = fmaxf(far, fabsf(q[j] - __fsub_rn(r, kRound)));
+      }
+      certain = certain && far < 0.4999f;  // 127 x 2^-21 from the border at least
+      word[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    } else {
+      constexpr float kLess = 1.f - 0x1p-21f, kMore = 1.f + 0x1p-21f;
+      uint32_t both[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const uint32_t less = __nv_cvt_float2_to_fp8x2(make_float2(q[2 * j] * kLess, q[2 * j + 1] * kLess), __NV_SATFINITE, __NV_E4M3);
+        both[j] = __nv_cvt_float2_to_fp8x2(make_float2(q[2 * j] * kMore, q[2 * j + 1] * kMore), __NV_SATFINITE, __NV_E4M3);
+        certain = certain && less == both[j];
+      }
+      word[h] = both[0] | both[1] << 16;
+    }
+  }
+  out = make_uint2(word[0], word[1]);
+  return certain;
+}
+
 template <bool kInt8>
 __device__ __forceinline__ void from_codes(uint2 in, float (&x)[8]) {
 #pragma unroll
@@ -268,6 +342,42 @@ __device__ __forceinline__ void from_codes(uint2 in, float (&x)[8]) {
     }
   }
 }
+
+// Largest |x| of elements as they come; +inf where one is not finite.
+template <typename T>
+struct Largest {
+  float top = 0.f;
+  __device__ __forceinline__ void add(const Eight<T>& e) {
+    float v[8];
+    e.values(v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = fabsf(v[j]) <= FLT_MAX ? fmaxf(top, fabsf(v[j])) : INFINITY;
+  }
+  __device__ __forceinline__ float get() const { return top; }
+};
+template <typename T2, typename T>
+struct LargestPair {  // 16-bit types: two at a time, NaN stays
+  T2 top;
+  __device__ __forceinline__ LargestPair() {
+    const uint32_t zero = 0;
+    top = *reinterpret_cast<const T2*>(&zero);
+  }
+  __device__ __forceinline__ void add(const Eight<T>& e) {
+    const uint32_t w[4] = {e.raw[0].x, e.raw[0].y, e.raw[0].z, e.raw[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const T2*>(&w[i])));
+  }
+  __device__ __forceinline__ float get() const {
+    const float a = to_float(top.x), b = to_float(top.y);
+    return a <= FLT_MAX && b <= FLT_MAX ? fmaxf(a, b) : INFINITY;
+  }
+  static __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+  static __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+};
+template <>
+struct Largest<__half> : LargestPair<__half2, __half> {};
+template <>
+struct Largest<__nv_bfloat16> : LargestPair<__nv_bfloat162, __nv_bfloat16> {};
 
 // One head of K or V (blockIdx.z) and rowsPerCta rows; the CTA that has the first row of a run of rows in one block does the run.
 //   need = max |x| / largest code over the run's finite values;  scale' = max(scale before, need);  code = round(x / scale'),
@@ -284,14 +394,15 @@ __global__ void __launch_bounds__(kStoreThreads) store_kernel(const StoreParams 
   const int blockTokens = 1 << p.blockShift;
   ptx::grid_wait_previous();
   ptx::grid_allow_next();
-  const T* x = static_cast<const T*>(p.x[which]) + (long long)h * D;
+  const bool second = which != 0;  // (indexing the parameters by it would copy them to local memory)
+  const T* x = static_cast<const T*>(second ? p.x[1] : p.x[0]) + (long long)h * D;
   const long long rowStride = (long long)p.heads * D;
   auto block_of = [&](long long row) -> int {  // -1: the row goes nowhere
     if (row < 0 || row >= p.rows) return -1;
     const long long s = p.slots[row];
     return (s < 0 || s >= p.cells) ? -1 : (int)(s >> p.blockShift);
   };
-  // which of the CTA's rows (16 at most) begin a run: every warp finds out for itself
+  // which of the CTA's rows (32 at most) begin a run: every warp finds out for itself
   const long long r0 = (long long)blockIdx.x * p.rowsPerCta;
   const int mine = lane < p.rowsPerCta ? block_of(r0 + lane) : -1;
   int before = __shfl_up_sync(0xffffffffu, mine, 1);
@@ -317,68 +428,106 @@ __global__ void __launch_bounds__(kStoreThreads) store_kernel(const StoreParams 
     for (int w = 0; w < kWarps; w++) n = min(n, __float_as_int(sMax[w]));
     const int first = sCells[0], items = n * kChunks;
     __syncthreads();  // sMax is written again
-    float top = 0.f;
-    auto look = [&](const Eight<T>& e) {
-      float v[8];
-      e.values(v);
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float a = fabsf(v[j]);
-        if (a <= FLT_MAX) top = fmaxf(top, a);
-      }
-    };
     Eight<T> kept[kKept];
+    auto at = [&](int i) { return x + (r + i / kChunks) * rowStride + i % kChunks * 8; };
+    // maximum over the CTA's threads of a number that is not negative
+    auto cta_max = [&](float v) {
+      const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+      if (lane == 0) sMax[threadIdx.x >> 5] = __uint_as_float(m);
+      __syncthreads();
+      float all = sMax[0];
+#pragma unroll
+      for (int w = 1; w < kWarps; w++) all = fmaxf(all, sMax[w]);
+      return all;
+    };
+    Largest<T> largest;
 #pragma unroll
     for (int e = 0; e < kKept; e++) {
       const int i = threadIdx.x + e * kStoreThreads;
-      if (i < items) kept[e].load(x + (r + i / kChunks) * rowStride + i % kChunks * 8);
+      if (i < items) kept[e].load(at(i));
     }
 #pragma unroll
     for (int e = 0; e < kKept; e++) {
-      if ((int)threadIdx.x + e * kStoreThreads < items) look(kept[e]);
+      if ((int)threadIdx.x + e * kStoreThreads < items) largest.add(kept[e]);
     }
+#pragma unroll 4
     for (int i = threadIdx.x + kKept * kStoreThreads; i < items; i += kStoreThreads) {
       Eight<T> e;
-      e.load(x + (r + i / kChunks) * rowStride + i % kChunks * 8);
-      look(e);
+      e.load(at(i));
+      largest.add(e);
     }
+    float top = cta_max(largest.get());
+    const bool clean = top <= FLT_MAX;
+    if (!clean) {  // the largest finite one
+      top = 0.f;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < items; i += kStoreThreads) {
+        Eight<T> e;
+        e.load(at(i));
+        float v[8];
+        e.values(v);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (lane == 0) sMax[threadIdx.x >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) top = fmaxf(top, sMax[w]);
-    float* scaleAt = p.scales[which] + (long long)block * p.heads + h;
+        for (int j = 0; j < 8; j++) {
+          if (fabsf(v[j]) <= FLT_MAX) top = fmaxf(top, fabsf(v[j]));
+        }
+      }
+      __syncthreads();  // sMax is written again
+      top = cta_max(top);
+    }
+    float* scaleAt = (second ? p.scales[1] : p.scales[0]) + (long long)block * p.heads + h;
     const float old = first == 0 ? 0.f : *scaleAt;
     const float need = top > 0.f ? fmaxf(__fdiv_rn(top, kInt8 ? 127.f : 448.f), kTinyScale) : 0.f;
     const float scale = fmaxf(old, need);
     // the scale is this run's (and not rounded up to a normal number, nor its numerator out of range)
     const bool fromRun = need >= old && need > kTinyScale && top <= 1e35f;
     const float num = fromRun ? (kInt8 ? 127.f : 448.f) : 1.f, den = fromRun ? top : scale;
-    uint8_t* tile = p.codes[which] + (((long long)block * p.heads + h) << p.blockShift) * D;
-    auto put = [&](const Eight<T>& e, int i) {
-      float v[8];
-      e.values(v);
-      *reinterpret_cast<uint2*>(tile + sCells[i / kChunks] * D + i % kChunks * 8) = to_codes<kInt8>(v, num, den);
-    };
-#pragma unroll
-    for (int e = 0; e < kKept; e++) {
-      const int i = threadIdx.x + e * kStoreThreads;
-      if (i < items) put(kept[e], i);
-    }
-    for (int i = threadIdx.x + kKept * kStoreThreads; i < items; i += kStoreThreads) {
+    uint8_t* tile = (second ? p.codes[1] : p.codes[0]) + (((long long)block * p.heads + h) << p.blockShift) * D;
+    auto put = [&](int i, uint2 codes) { *reinterpret_cast<uint2*>(tile + sCells[i / kChunks] * D + i % kChunks * 8) = codes; };
+    auto divide = [&](int i) {
       Eight<T> e;
-      e.load(x + (r + i / kChunks) * rowStride + i % kChunks * 8);
-      put(e, i);
+      float v[8];
+      e.load(at(i));
+      e.values(v);
+      put(i, to_codes<kInt8>(v, num, den));
+    };
+    const float inv = __fdiv_rn(num, den);
+    if (clean && inv > 1e-30f && inv < 1e30f) {
+      unsigned again = 0;  // eights that are divided
+#pragma unroll
+      for (int e = 0; e < kKept; e++) {
+        const int i = threadIdx.x + e * kStoreThreads;
+        if (i < items) {
+          float v[8];
+          uint2 codes;
+          kept[e].values(v);
+          if (!quick_codes<kInt8>(v, inv, codes)) again |= 1u << e;
+          put(i, codes);
+        }
+      }
+#pragma unroll 1
+      for (; again != 0; again &= again - 1) divide(threadIdx.x + (__ffs(again) - 1) * kStoreThreads);
+#pragma unroll 4
+      for (int i = threadIdx.x + kKept * kStoreThreads; i < items; i += kStoreThreads) {
+        Eight<T> e;
+        float v[8];
+        uint2 codes;
+        e.load(at(i));
+        e.values(v);
+        if (!quick_codes<kInt8>(v, inv, codes)) codes = to_codes<kInt8>(v, num, den);
+        put(i, codes);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = threadIdx.x; i < items; i += kStoreThreads) divide(i);
     }
     if (scale != old || first == 0) {
       for (int i = threadIdx.x; i < first * kChunks; i += kStoreThreads) {
-        uint2* at = reinterpret_cast<uint2*>(tile + i * 8);
+        uint2* cell = reinterpret_cast<uint2*>(tile + i * 8);
         float v[8];
-        from_codes<kInt8>(*at, v);
+        from_codes<kInt8>(*cell, v);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] *= old;
-        *at = to_codes<kInt8>(v, num, den);
+        *cell = to_codes<kInt8>(v, num, den);
       }
       __syncthreads();  // every thread has read the scale
       if (threadIdx.x == 0) *scaleAt = scale;
@@ -447,8 +596,7 @@ extern "C" int tfa_b200_kv_cache_plan(int* blockTable, const int* seqLens, const
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool overlap = may_overlap(s);
   const bool few = totalNew <= kPlanThreads;  // more rows than the CTA has threads: a kernel of as many CTAs as they need
-  // a warp for every two requests or so: fewer to wait for
-  const int threads = batchSize <= 64 && few ? 256 : kPlanThreads;
+  const int threads = batchSize <= 256 && totalNew <= 256 ? 256 : kPlanThreads;  // fewer warps to wait for
   cudaError_t e = launch_kernel(plan_kernel, dim3(1), threads, 0, s, overlap, p, few);
   if (e == cudaSuccess && !few) e = launch_kernel(slots_kernel, dim3((unsigned)((totalNew + 255) / 256)), 256, 0, s, overlap, p);
   if (e != cudaSuccess) {
@@ -498,8 +646,9 @@ extern "C" int tfa_b200_kv_cache_store(const void* K, const void* V, void* kCach
   p.heads = numHeadsKV;
   p.headDim = headDim;
   p.blockShift = shift;
-  // Few rows are mostly runs of one row (a decode step), a CTA each; of many, sixteen rows hold the beginning of one run or two.
-  p.rowsPerCta = totalNew <= 512 ? 1 : 16;
+  // Few rows are mostly runs of one row (a decode step), a CTA each; of many, sixteen (blocks of 64 or more: 32) rows hold the beginning of one
+  // run or two.
+  p.rowsPerCta = totalNew <= 512 ? 1 : shift >= 6 ? 32 : 16;
   const dim3 grid((unsigned)((totalNew + p.rowsPerCta - 1) / p.rowsPerCta), (unsigned)numHeadsKV, 2);
   const bool int8 = cacheType == TFA_B200_CACHE_INT8;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
