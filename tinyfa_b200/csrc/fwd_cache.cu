@@ -212,8 +212,19 @@ __device__ __forceinline__ int tiles_of(int nq, int group) {
   return (int)(((long long)nq * group + 8 * NR - 1) / (8 * NR));
 }
 
-// Run that holds block u of `total` blocks, i.e. the c with total * c / runs <= u < total * (c + 1) / runs.
-__device__ __forceinline__ int run_of_block(long long u, long long total, int runs) { return (int)(((u + 1) * runs - 1) / total); }
+// The blocks of all units, in order, cut into runs of equal length.  A cut within `snap` blocks of a unit's end is moved there: two blocks more
+// for one run cost less than parts of a unit that have to be put together (64 requests of 300 tokens: SNAP_MEASURED).
+struct Cuts {
+  int total, base, extra, snap;
+  __device__ __forceinline__ Cuts(int blocks, int runs) : total(blocks), base(blocks / runs), extra(blocks - base * runs), snap(min(2, base / 3)) {}
+  __device__ __forceinline__ int begin(int c) const { return c * base + min(c, extra); }
+  __device__ __forceinline__ int run_of(int u) const {  // the c with begin(c) <= u < begin(c + 1)
+    const int longer = extra * (base + 1);
+    return u < longer ? u / (base + 1) : extra + (u - longer) / base;
+  }
+  // how far a cut moves that is blk blocks into a unit of `blocks`
+  __device__ __forceinline__ int move(int blk, int blocks) const { return blk <= snap ? -blk : blocks - blk <= snap ? blocks - blk : 0; }
+};
 
 // NR: tiles of 8 NR query rows.
 template <int D, bool kInt8, bool kBf16, int NR>
@@ -224,8 +235,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
   constexpr int kMT = D / 16;    // 16-element row tiles of O^T
   constexpr int kLdO = D + 8;    // row pitch of the merge buffer
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long sScan[kThreads / 32];
-  __shared__ long long sPlace[2];  // unit that holds the run's first block: request, blocks ahead of the request
+  __shared__ long long sScan[2][kThreads / 32];
+  __shared__ int sPlace[2][5];  // request that holds the run's first block, and the one behind its last: number, blocks ahead of it, q0, nq, len
   __shared__ int sLast;
   float* sO = reinterpret_cast<float*>(smem + ring_bytes<D, NR>());  // [kTile][kLdO]
   float* sM = sO + kTile * kLdO;                                     // [4][kTile]
@@ -247,24 +258,45 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
     len = min(max(p.lens[b], 0), capacity);
   };
   auto unit_blocks = [&](int len) { return (len + kBlockKeys - 1) / kBlockKeys; };
-  auto blocks_of_request = [&](int b) -> long long {
-    int q0, nq, len;
-    request(b, q0, nq, len);
-    return (long long)tiles_of<NR>(nq, p.group) * unit_blocks(len);
-  };
-  // ---- the blocks of all requests, and where this run begins among them
-  long long mine = 0, total = 0;
-  for (int b = threadIdx.x; b < p.batch; b += kThreads) mine += blocks_of_request(b);
+  auto blocks_of = [&](int nq, int len) { return (long long)tiles_of<NR>(nq, p.group) * unit_blocks(len); };
+  // ---- the blocks of all requests; the first kThreads requests stay in registers
+  int q0 = 0, nq = 0, len = 0;
+  if ((int)threadIdx.x < p.batch) request(threadIdx.x, q0, nq, len);
+  const long long mine = blocks_of(nq, len);
+  long long upto = mine, more = 0;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  if (lane == 0) sScan[warp] = mine;
-  __syncthreads();
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += o;
+  }
+  for (int b = threadIdx.x + kThreads; b < p.batch; b += kThreads) {
+    int a, n, m;
+    request(b, a, n, m);
+    more += blocks_of(n, m);
+  }
+  if (p.batch > kThreads) {
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; w++) total += sScan[w];
+    for (int d = 16; d > 0; d >>= 1) more += __shfl_xor_sync(0xffffffffu, more, d);
+  }
+  if (lane == 31) {
+    sScan[0][warp] = upto;
+    sScan[1][warp] = more;
+  }
   __syncthreads();
+  long long sum = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; w++) {
+    if (w < warp) upto += sScan[0][w];
+    sum += sScan[0][w];
+    all += sScan[1][w];
+  }
+  all += sum;
+  if (all > 0x7FFFFFFFll) return;  // offsets that are not ascending: the host has checked what rows and blocks can give
+  const int total = (int)all;
+  int carry = (int)sum;
 
   // ---- rows that no unit has: those of no request, and those of requests without a token; a share for every CTA
-  {
+  auto zero_rest = [&]() {
     uint16_t* O = static_cast<uint16_t*>(p.O);
     auto zero_rows = [&](int r0, int r1) {  // this head's part of them
       constexpr int kVec = D / 8;
@@ -283,57 +315,59 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
       request(b, q0, nq, len);
       if (len == 0) zero_rows(q0, q0 + nq);
     }
+  };
+  // The host sized the grid for the largest lengths: with fewer blocks, fewer runs of at least two blocks.
+  const int runs = min(p.runs, (total + 1) / 2);
+  if (run >= runs) {
+    zero_rest();
+    return;
   }
-  // The host sized the grid for the largest lengths: with fewer blocks, fewer runs of at least two blocks.  (Every run has to have a
-  // block: the parts of a unit are counted by the runs between its first block's and its last one's.)
-  const int runs = (int)min((long long)p.runs, (total + 1) / 2);
-  if (run >= runs) return;
-  const long long u0 = total * run / runs, u1 = total * (run + 1) / runs;
-  long long carry = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+  const Cuts cuts(total, runs);
+  int u0 = cuts.begin(run), u1 = cuts.begin(run + 1);
+  auto place = [&](int b, int ahead, int n, int a, int rows, int tokens) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int u = i == 0 ? u0 : u1;
+      if (u >= ahead && u < ahead + n) {
+        sPlace[i][0] = b;
+        sPlace[i][1] = ahead;
+        sPlace[i][2] = a;
+        sPlace[i][3] = rows;
+        sPlace[i][4] = tokens;
+      }
+    }
+  };
+  place(threadIdx.x, (int)(upto - mine), (int)mine, q0, nq, len);
+  for (int b0 = kThreads; b0 < p.batch && carry <= u1; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
-    const long long n = b < p.batch ? blocks_of_request(b) : 0;
-    long long v = n;
+    int a = 0, n = 0, m = 0;
+    if (b < p.batch) request(b, a, n, m);
+    const int blocks = (int)blocks_of(n, m);
+    int v = blocks;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, v, d);
+      const int o = __shfl_up_sync(0xffffffffu, v, d);
       if (lane >= d) v += o;
     }
-    if (lane == 31) sScan[warp] = v;
+    __syncthreads();  // sScan has been read
+    if (lane == 31) sScan[0][warp] = v;
     __syncthreads();
-    long long sum = 0;
+    int here = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; w++) {
-      if (w < warp) v += sScan[w];
-      sum += sScan[w];
+      if (w < warp) v += (int)sScan[0][w];
+      here += (int)sScan[0][w];
     }
-    v += carry - n;  // blocks ahead of request b
-    if (u0 >= v && u0 < v + n) {
-      sPlace[0] = b;
-      sPlace[1] = v;
-    }
-    carry += sum;
-    __syncthreads();
-    if (carry > u0) break;
+    place(b, carry + v - blocks, blocks, a, n, m);
+    carry += here;
   }
+  __syncthreads();
 
   auto finish = [&](Segment& s) {  // the fields that follow from the request and the tile
     const int lastRow = min((s.tile + 1) * kTile, s.nq * p.group) - 1;
     s.keyEnd = p.causal ? min(s.len, s.len - s.nq + lastRow / p.group + 1) : s.len;
   };
-  long long left;  // blocks of the run behind the segment
-  auto first_segment = [&](Segment& s, long long& rest) {
-    s.b = (int)sPlace[0];
-    request(s.b, s.q0, s.nq, s.len);
-    s.blocks = unit_blocks(s.len);
-    const long long at = u0 - sPlace[1];
-    s.tile = (int)(at / s.blocks);
-    s.blk = (int)(at - (long long)s.tile * s.blocks);
-    s.end = (int)min((long long)s.blocks, s.blk + (u1 - u0));
-    rest = (u1 - u0) - (s.end - s.blk);
-    finish(s);
-  };
-  auto next_segment = [&](Segment& s, long long& rest) {  // rest > 0
+  auto next_segment = [&](Segment& s, int& rest) {  // rest > 0
     s.tile++;
     if (s.tile >= tiles_of<NR>(s.nq, p.group)) {
       s.tile = 0;
@@ -344,19 +378,47 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
       s.blocks = unit_blocks(s.len);
     }
     s.blk = 0;
-    s.end = (int)min((long long)s.blocks, rest);
+    s.end = min(s.blocks, rest);
     rest -= s.end;
     finish(s);
   };
 
   // ---- the loads: a cursor of its own, kS - 1 slices ahead
   Segment ls;
-  long long lsRest;
-  first_segment(ls, lsRest);
+  ls.b = sPlace[0][0];
+  ls.q0 = sPlace[0][2];
+  ls.nq = sPlace[0][3];
+  ls.len = sPlace[0][4];
+  ls.blocks = unit_blocks(ls.len);
+  ls.tile = (u0 - sPlace[0][1]) / ls.blocks;
+  ls.blk = u0 - sPlace[0][1] - ls.tile * ls.blocks;
+  const int moved = cuts.move(ls.blk, ls.blocks);
+  u0 += moved;
+  if (u1 < total) {
+    const int blocks = unit_blocks(sPlace[1][4]);
+    u1 += cuts.move((u1 - sPlace[1][1]) % blocks, blocks);
+  }
+  if (u0 >= u1) {
+    zero_rest();
+    return;
+  }
+  int left = u1 - u0;  // blocks of the run behind the segment
+  if (moved > 0) {
+    next_segment(ls, left);
+  } else {
+    ls.blk += moved;
+    ls.end = min(ls.blocks, ls.blk + left);
+    left -= ls.end - ls.blk;
+    finish(ls);
+  }
+  Segment s = ls;
+  int lsRest = left;
   bool loading = true;
   int ldKey = ls.blk * kBlockKeys + warp * 16, ldStage = 0;
   const long long headBytes = (long long)D << p.blockShift;
   auto seg_key_end = [&](const Segment& s) { return min(s.end * kBlockKeys, s.keyEnd); };
+  // Pages of the next 32 slices of the segment, one to a lane: asked for together, and a slice ahead of their use.
+  int ldPages = 0, ldTurn = 32;
   auto settle = [&]() {  // on to the next slice that exists
     while (loading && ldKey >= seg_key_end(ls)) {
       if (lsRest == 0) {
@@ -364,14 +426,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
       } else {
         next_segment(ls, lsRest);
         ldKey = warp * 16;
+        ldTurn = 32;
       }
+    }
+    if (loading && ldTurn == 32) {
+      const int key = ldKey + lane * kBlockKeys;
+      ldPages = key < seg_key_end(ls) ? p.table[(long long)ls.b * p.width + (key >> p.blockShift)] : -1;
+      ldTurn = 0;
     }
   };
   settle();
-  int ldPage = loading ? p.table[(long long)ls.b * p.width + (ldKey >> p.blockShift)] : 0;
   auto issue = [&]() {
     if (loading) {
       const uint32_t st = ring + ldStage * kStage;
+      const int ldPage = __shfl_sync(0xffffffffu, ldPages, ldTurn);
+      ldTurn++;
       const bool ok = ldPage >= 0 && ldPage < p.numBlocks;
       const long long tile = ok ? (long long)ldPage * p.headsKV + hkv : 0;
       const int rows = ok ? min(16, ls.len - ldKey) : 0;  // keys of the slice
@@ -402,39 +471,56 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
       ldStage = ldStage + 1 == kS ? 0 : ldStage + 1;
       ldKey += kBlockKeys;
       settle();
-      if (loading) ldPage = p.table[(long long)ls.b * p.width + (ldKey >> p.blockShift)];
     }
     cp_async_commit();
   };
-#pragma unroll
-  for (int i = 0; i < kS - 1; i++) issue();
-
   // ---- the units of the run
-  Segment s;
-  first_segment(s, left);
-  bool firstSegment = true;
   int stage = 0;
+  bool started = false;
   for (;;) {
     const int nRows = min(s.nq * p.group - s.tile * kTile, kTile);
+    // rows of the tile: row 0 is head `head0` of query `query0`.  (x + 1/2) / group in 32 bits: exact for the few rows of a tile
+    const int query0 = s.tile * kTile / p.group, head0 = s.tile * kTile - query0 * p.group;
+    const float byGroup = 1.f / (float)p.group;
+    auto query_of = [&](int row) { return (int)(((float)(head0 + row) + 0.5f) * byGroup); };
     // Q as the columns of S^T: row 8 nr + g of the tile, permuted like the lanes' bytes of K
     uint32_t qf[D / 16][NR][2];
-    float rowDown[NR];
+    float rowDown[NR], slope[NR][2];
+    int pos[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; nr++) {
-      const int row = nr * 8 + g, flat = s.tile * kTile + row;
-      const bool valid = row < nRows;
+      const int row = nr * 8 + g < nRows ? nr * 8 + g : 0, query = query_of(row);
       const uint16_t* q = static_cast<const uint16_t*>(p.Q) +
-                          ((long long)(s.q0 + (valid ? flat / p.group : 0)) * p.headsQ + hkv * p.group + (valid ? flat % p.group : 0)) * D;
+                          ((long long)(s.q0 + query0 + query) * p.headsQ + hkv * p.group + head0 + row - query * p.group) * D;
 #pragma unroll
       for (int w = 0; w < D / 16; w++) {
         const uint2 x = *reinterpret_cast<const uint2*>(q + k_byte<D>(w, tig));
-        qf[w][nr][0] = valid ? x.x : 0u;
-        qf[w][nr][1] = valid ? x.y : 0u;
+        qf[w][nr][0] = x.x;
+        qf[w][nr][1] = x.y;
       }
+      // this thread's columns of S^T and O^T: rows 8 nr + 2 tig + e
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int col = nr * 8 + 2 * tig + e < nRows ? nr * 8 + 2 * tig + e : 0, query = query_of(col);
+        pos[nr][e] = s.len - s.nq + query0 + query;
+        slope[nr][e] = p.slopes != nullptr ? p.slopes[hkv * p.group + head0 + col - query * p.group] * 1.44269504f : 0.f;
+      }
+    }
+    if (!started) {  // the first slices, while Q is on its way
+#pragma unroll 1
+      for (int i = 0; i < kS - 1; i++) issue();
+      zero_rest();
+      started = true;
+    }
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+      const bool valid = nr * 8 + g < nRows;
       constexpr uint32_t kE = exponent_bits<kBf16>();
       uint32_t top = 0;
 #pragma unroll
       for (int w = 0; w < D / 16; w++) {
+        qf[w][nr][0] = valid ? qf[w][nr][0] : 0u;
+        qf[w][nr][1] = valid ? qf[w][nr][1] : 0u;
         top = max(max(top, qf[w][nr][0] & kE), max(qf[w][nr][0] >> 16 & kE, max(qf[w][nr][1] & kE, qf[w][nr][1] >> 16 & kE)));
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -447,20 +533,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
         qf[w][nr][1] = scale_to_half2<kBf16>(qf[w][nr][1], up);
       }
     }
-    // this thread's columns of S^T and O^T: rows 8 nr + 2 tig + e
-    float fac[NR][2], slope[NR][2];
-    int pos[NR][2];
-    const float capLog2 = p.cap * 1.44269504f;
+    // capped: scores as arguments 2 log2(e) S / c of the exponential that gives the tanh
+    float fac[NR][2];
+    const float capLog2 = p.cap * 1.44269504f, unit = p.scaleLog2 * (p.cap > 0.f ? 2.f / p.cap : 1.f);
 #pragma unroll
     for (int nr = 0; nr < NR; nr++) {
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const int row = nr * 8 + 2 * tig + e, flat = s.tile * kTile + (row < nRows ? row : 0);
-        // capped: scores as arguments 2 log2(e) S / c of the exponential that gives the tanh
-        fac[nr][e] = __shfl_sync(0xffffffffu, rowDown[nr], (2 * tig + e) * 4) * p.scaleLog2 * (p.cap > 0.f ? 2.f / p.cap : 1.f);
-        pos[nr][e] = s.len - s.nq + flat / p.group;
-        slope[nr][e] = p.slopes != nullptr ? p.slopes[hkv * p.group + flat % p.group] * 1.44269504f : 0.f;
-      }
+      for (int e = 0; e < 2; e++) fac[nr][e] = __shfl_sync(0xffffffffu, rowDown[nr], (2 * tig + e) * 4) * unit;
     }
 
     float o[kMT][NR][4];
@@ -474,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
     for (int nr = 0; nr < NR; nr++) ref[nr][0] = ref[nr][1] = l[nr][0] = l[nr][1] = 0.f, limit[nr][0] = limit[nr][1] = -INFINITY;
     float vRef = 0.f, vUp = 0.f;  // scale of V that O refers to: O holds sums of 2^4 p v / vRef
 
-    const int keyStop = seg_key_end(s), seenByAll = p.causal ? s.len - s.nq + s.tile * kTile / p.group : s.len - 1;
+    const int keyStop = seg_key_end(s), seenByAll = p.causal ? s.len - s.nq + query0 : s.len - 1;
     for (int key0 = s.blk * kBlockKeys + warp * 16; key0 < keyStop; key0 += kBlockKeys) {
       cp_async_wait<kS - 2>();
       __syncwarp();  // ... and every lane has read the stage of the slice before
@@ -658,11 +737,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
           for (int nr = 0; nr < NR; nr++) {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              float2* at = reinterpret_cast<float2*>(sO + (nr * 8 + 2 * tig + e) * kLdO + g * (D / 8));
+              // elements g D / 8 + 2 j and + 1 of the row stand at 16 j + 2 g: the lanes of an access on different banks
+              float2* at = reinterpret_cast<float2*>(sO + (nr * 8 + 2 * tig + e) * kLdO + 2 * g);
 #pragma unroll
               for (int j = 0; j < kMT; j++) {
-                const float2 z = w == 0 ? make_float2(0.f, 0.f) : at[j];
-                at[j] = make_float2(fmaf(o[j][nr][e], f[nr][e], z.x), fmaf(o[j][nr][e + 2], f[nr][e], z.y));
+                const float2 z = w == 0 ? make_float2(0.f, 0.f) : at[j * 8];
+                at[j * 8] = make_float2(fmaf(o[j][nr][e], f[nr][e], z.x), fmaf(o[j][nr][e + 2], f[nr][e], z.y));
               }
             }
           }
@@ -671,10 +751,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
       }
     }
     const bool whole = s.blk == 0 && s.end == s.blocks;
-    const long long slot = ((long long)run * p.headsKV + hkv) * 2 + (firstSegment ? 0 : 1);
+    // parts of a run: of the unit that it begins and does not end, of the one that it does not begin
+    const long long slot = ((long long)run * p.headsKV + hkv) * 2 + (s.blk == 0 ? 0 : 1);
     auto store = [&](int r, int c4, float4 acc) {
-      const int flat = s.tile * kTile + r;
-      uint16_t* dst = static_cast<uint16_t*>(p.O) + ((long long)(s.q0 + flat / p.group) * p.headsQ + hkv * p.group + flat % p.group) * D + c4 * 4;
+      const int query = query_of(r);
+      uint16_t* dst = static_cast<uint16_t*>(p.O) + ((long long)(s.q0 + query0 + query) * p.headsQ + hkv * p.group + head0 + r - query * p.group) * D + c4 * 4;
       uint2 out;
       if constexpr (kBf16) {
         __nv_bfloat162 x = __floats2bfloat162_rn(acc.x, acc.y), y = __floats2bfloat162_rn(acc.z, acc.w);
@@ -697,7 +778,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
         l += sL[w * kTile + r] * (mw == -INFINITY ? 0.f : ex2(mw - m));
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
-      float4 acc = *reinterpret_cast<const float4*>(sO + r * kLdO + c4 * 4);
+      const float* from = sO + r * kLdO + c4 * 4 % (D / 8) * 8 + c4 * 4 / (D / 8) * 2;
+      const float2 lo = *reinterpret_cast<const float2*>(from), hi = *reinterpret_cast<const float2*>(from + 16);
+      float4 acc = make_float4(lo.x, lo.y, hi.x, hi.y);
       acc.x *= inv;
       acc.y *= inv;
       acc.z *= inv;
@@ -711,70 +794,87 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
     }
     if (!whole) {
       // ---- the unit is shared by runs c0 .. c1: whoever comes last puts the parts together
-      const long long a = (u1 - left) - s.end;  // the unit's first block (u1 - left: the block behind the segment)
-      const int c0 = run_of_block(a, total, runs), c1 = run_of_block(a + s.blocks - 1, total, runs);
-      __threadfence();
+      const int a = (u1 - left) - s.end;  // the unit's first block (u1 - left: the block behind the segment)
+      const int c0 = cuts.run_of(a + cuts.snap), c1 = cuts.run_of(a + s.blocks - 1 - cuts.snap);
       __syncthreads();
-      if (threadIdx.x == 0) {
+      if (threadIdx.x == 0) {  // releases what the CTA has stored before the barrier, acquires what the others' have
         int* counter = p.join + (long long)c0 * p.headsKV + hkv;
-        const bool last = atomicAdd(counter, 1) == c1 - c0;
+        int seen;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(counter) : "memory");
+        const bool last = seen == c1 - c0;
         if (last) *counter = 0;  // for the next call
         sLast = last;
-        __threadfence();
       }
       __syncthreads();
       if (sLast) {
-        // the unit is the first segment of every run but possibly c0, which it begins in unless it begins the run
-        const int at0 = total * c0 / runs == a ? 0 : 1;
-        auto part = [&](int c) { return ((long long)c * p.headsKV + hkv) * 2 + (c == c0 ? at0 : 0); };
-        // largest log-sum-exp and sum of the weights of every row, a warp each
-        for (int r = warp; r < nRows; r += 4) {
-          float M = -INFINITY;
-          bool nan = false;
-          for (int c = c0 + lane; c <= c1; c += 32) {
-            const float lse = __ldcg(p.partLse + part(c) * kTile + r);
-            nan = nan || lse != lse;
-            M = fmaxf(M, lse);
-          }
-#pragma unroll
-          for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-          if (M == -INFINITY) M = 0.f;
-          if (__any_sync(0xffffffffu, nan)) M = NAN;
-          float sum = 0.f;
-          for (int c = c0 + lane; c <= c1; c += 32) sum += ex2(__ldcg(p.partLse + part(c) * kTile + r) - M);
-#pragma unroll
-          for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-          if (lane == 0) {
-            sM[r] = M;
-            sL[r] = sum == 0.f ? 0.f : 1.f / sum;
-          }
-        }
-        __syncthreads();
-        // groups of D / 4 threads take turns over the parts, four rows of a part in flight at once
-        constexpr int kVec = D / 4, kGroups = kThreads / kVec < 4 ? kThreads / kVec : 4;
+        auto part = [&](int c) { return ((long long)c * p.headsKV + hkv) * 2 + (c == c0 ? 0 : 1); };
+        // Groups of D / 4 threads take turns over the parts, four rows of kAhead parts in flight at once: sums relative to the largest
+        // log-sum-exp so far; then the groups' sums.
+        constexpr int kVec = D / 4, kGroups = kThreads / kVec < 4 ? kThreads / kVec : 4, kAhead = D <= 64 ? 2 : 4;
         const int group = threadIdx.x / kVec, c4 = threadIdx.x % kVec;
 #pragma unroll 1
         for (int r0 = 0; r0 < nRows; r0 += 4) {
           float4 acc[4];
+          float M[4], sum[4];
 #pragma unroll
-          for (int r = 0; r < 4; r++) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int r = 0; r < 4; r++) {
+            acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+            M[r] = -INFINITY;
+            sum[r] = 0.f;
+          }
           if (group < kGroups) {
-#pragma unroll 2
-            for (int c = c0 + group; c <= c1; c += kGroups) {
-              const long long at = part(c) * kTile + r0;
-              const float4 lse = __ldcg(reinterpret_cast<const float4*>(p.partLse + at));
-              float4 v[4];
+#pragma unroll 1
+            for (int c = c0 + group; c <= c1; c += kGroups * kAhead) {
+              float lse[kAhead][4];
+              float4 v[kAhead][4];
 #pragma unroll
-              for (int r = 0; r < 4; r++) v[r] = __ldcg(reinterpret_cast<const float4*>(p.partO + (at + r) * D + c4 * 4));
-              const float w[4] = {ex2(lse.x - sM[r0]), ex2(lse.y - sM[r0 + 1]), ex2(lse.z - sM[r0 + 2]), ex2(lse.w - sM[r0 + 3])};
+              for (int u = 0; u < kAhead; u++) {
+                const bool there = c + u * kGroups <= c1;
+                const long long at = part(there ? c + u * kGroups : c) * kTile + r0;
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(p.partLse + at));
+                lse[u][0] = there ? x.x : -INFINITY;
+                lse[u][1] = there ? x.y : -INFINITY;
+                lse[u][2] = there ? x.z : -INFINITY;
+                lse[u][3] = there ? x.w : -INFINITY;
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[u][r] = __ldcg(reinterpret_cast<const float4*>(p.partO + (at + r) * D + c4 * 4));
+              }
 #pragma unroll
               for (int r = 0; r < 4; r++) {
-                acc[r].x = fmaf(w[r], v[r].x, acc[r].x);
-                acc[r].y = fmaf(w[r], v[r].y, acc[r].y);
-                acc[r].z = fmaf(w[r], v[r].z, acc[r].z);
-                acc[r].w = fmaf(w[r], v[r].w, acc[r].w);
+                float top = M[r];
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) top = fmaxf(top, lse[u][r]);
+                const float ref = top == -INFINITY ? 0.f : top, f = ex2(M[r] - ref);
+                M[r] = top;
+                sum[r] *= f;
+                acc[r] = make_float4(acc[r].x * f, acc[r].y * f, acc[r].z * f, acc[r].w * f);
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) {
+                  const float w = ex2(lse[u][r] - ref);  // NaN stays NaN
+                  sum[r] += w;
+                  acc[r].x = fmaf(w, v[u][r].x, acc[r].x);
+                  acc[r].y = fmaf(w, v[u][r].y, acc[r].y);
+                  acc[r].z = fmaf(w, v[u][r].z, acc[r].z);
+                  acc[r].w = fmaf(w, v[u][r].w, acc[r].w);
+                }
               }
             }
+            if (c4 == 0) {
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                sM[group * 4 + r] = M[r];
+                sL[group * 4 + r] = sum[r];
+              }
+            }
+          }
+          __syncthreads();
+          float all[4];
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            all[r] = sM[r];
+#pragma unroll
+            for (int i = 1; i < kGroups; i++) all[r] = fmaxf(all[r], sM[i * 4 + r]);
+            if (all[r] == -INFINITY) all[r] = 0.f;
           }
 #pragma unroll 1
           for (int i = 0; i < kGroups; i++) {  // (rows past nRows are rubbish that nobody reads)
@@ -783,23 +883,30 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
               for (int r = 0; r < 4; r++) {
                 float4* at = reinterpret_cast<float4*>(sO + (r0 + r) * kLdO + c4 * 4);
                 const float4 z = i == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
-                *at = make_float4(acc[r].x + z.x, acc[r].y + z.y, acc[r].z + z.z, acc[r].w + z.w);
+                const float f = ex2(M[r] - all[r]);
+                *at = make_float4(fmaf(f, acc[r].x, z.x), fmaf(f, acc[r].y, z.y), fmaf(f, acc[r].z, z.z), fmaf(f, acc[r].w, z.w));
               }
             }
             __syncthreads();
           }
-        }
-        for (int idx = threadIdx.x; idx < nRows * kVec; idx += kThreads) {
-          const int r = idx / kVec, c = idx % kVec;
-          const float inv = sL[r];
-          const float4 x = *reinterpret_cast<const float4*>(sO + r * kLdO + c * 4);
-          store(r, c, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+          for (int idx = threadIdx.x; idx < min(4, nRows - r0) * kVec; idx += kThreads) {
+            const int r = idx / kVec, c = idx % kVec;
+            float top = sM[r], total = 0.f;
+#pragma unroll
+            for (int i = 1; i < kGroups; i++) top = fmaxf(top, sM[i * 4 + r]);
+            if (top == -INFINITY) top = 0.f;
+#pragma unroll
+            for (int i = 0; i < kGroups; i++) total += sL[i * 4 + r] * ex2(sM[i * 4 + r] - top);
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            const float4 x = *reinterpret_cast<const float4*>(sO + (r0 + r) * kLdO + c * 4);
+            store(r0 + r, c, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+          }
+          if (r0 + 4 < nRows) __syncthreads();  // sM and sL are written again
         }
       }
     }
     if (left == 0) break;
     next_segment(s, left);
-    firstSegment = false;
     __syncthreads();  // the merge buffer is written again
   }
   cp_async_wait<0>();
@@ -848,6 +955,11 @@ int launch_stream(Params& p, long long rows, int maxSeqLenKV, bool int8, bool bf
   // as many runs as the GPU holds CTAs, and no more than there can be pairs of key blocks
   const long long slots = (long long)device_num_sms(device) * (nr == 1 ? ctas_per_sm<D, 1>() : ctas_per_sm<D, 2>());
   const long long tiles = (rows + 8 * nr - 1) / (8 * nr);
+  const long long allTiles = ((long long)p.totalQ * p.group) / (8 * nr) + p.batch;  // of all requests, at most
+  if (allTiles * ((((long long)p.width << p.blockShift) + kBlockKeys - 1) / kBlockKeys) > 0x7FFFFFFFll) {
+    set_error_string("more than 2^31 - 1 tiles of query rows and 64 keys (%d rows of Q, block table for %lld tokens)", p.totalQ, (long long)p.width << p.blockShift);
+    return kTooLarge;
+  }
   const long long most = (tiles * ((maxSeqLenKV + kBlockKeys - 1) / kBlockKeys) * p.batch + 1) / 2;
   long long runs = slots / p.headsKV;
   if (runs > most) runs = most;
