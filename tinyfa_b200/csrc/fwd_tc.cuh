@@ -386,9 +386,9 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ float fmin3(float a, float b, float c) {  // NaN kept as well
+__device__ __forceinline__ float fmax3_abs(float a, float b, float c) {  // largest magnitude
   float d;
-  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 __device__ __forceinline__ float fmax2(float a, float b) {
@@ -731,18 +731,15 @@ struct ScoreRow {
   // on every score, off by about as much.  arg: factor that makes a score the 2 x log2(e) of the latter.
   // Causal B2 S4096 32 over 8 heads of 128, cap 50: TANH_MEASURED.
   __device__ __forceinline__ void cap_scores(uint32_t (&v)[4][32], float arg) const {
-    float hi[4], lo[4];
+    float top[4];
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-      hi[q] = lo[q] = __uint_as_float(v[q][0]);
+      top[q] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        hi[q] = fmax3(hi[q], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
-        lo[q] = fmin3(lo[q], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
-      }
+      for (int i = 0; i < 32; i += 2) top[q] = fmax3_abs(top[q], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
     }
-    const float most = fmax3(fmax2(fmax2(hi[0], hi[1]), fmax2(hi[2], hi[3])), -lo[0], fmax3(-lo[1], -lo[2], -lo[3]));
-    if (__all_sync(0xffffffffu, most <= small)) {  // (a NaN is not)
+    const float most = fmax2(fmax2(top[0], top[1]), fmax2(top[2], top[3]));
+    if (__all_sync(0xffffffffu, most <= small)) {  // (a NaN stays one on either way)
 #pragma unroll
       for (int q = 0; q < 4; q++) {
 #pragma unroll
