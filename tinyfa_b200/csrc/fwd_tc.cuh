@@ -739,7 +739,7 @@ struct ScoreRow {
       for (int i = 0; i < 32; i += 2) top[q] = fmax3_abs(top[q], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
     }
     const float most = fmax2(fmax2(top[0], top[1]), fmax2(top[2], top[3]));
-    if (__all_sync(0xffffffffu, most <= small)) {  // (a NaN stays one on either way)
+    if (__builtin_expect(__all_sync(0xffffffffu, most <= small), 1)) {  // (a NaN stays one on either way)
 #pragma unroll
       for (int q = 0; q < 4; q++) {
 #pragma unroll
@@ -769,7 +769,7 @@ struct ScoreRow {
   // The bias; `scale`: what a score still has to be multiplied by (capped scores: nothing).  left: all keys that the row sees lie to its left,
   // where the bias is linear in the key - 2 packed operations on a pair of scores instead of 3 and two absolute values.
   __device__ __forceinline__ void bias_scores(uint32_t (&v)[4][32], int kbase, float scale, bool left) const {
-    if (left) {
+    if (__builtin_expect(left, 1)) {
       const float2 step = make_float2(2.f * slope, 2.f * slope);
 #pragma unroll
       for (int q = 0; q < 4; q++) {
@@ -815,6 +815,29 @@ struct ScoreRow {
   // gone: groups whose block does not exist, as bits.
   template <class F>
   __device__ __forceinline__ void cache_transform(uint32_t (&v)[4][32], int kbase, F kf, bool left, uint32_t gone) const {
+    if constexpr ((kScore & (kScoreCap | kScoreBias)) == kScoreBias) {
+      if (__builtin_expect(left, 1)) {  // scale and bias in one step, as in bias_scores
+        const float2 step = make_float2(2.f * slope, 2.f * slope);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const float2 f2 = kf(q);
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const float f = h == 0 ? f2.x : f2.y, off = (gone >> (2 * q + h) & 1u) != 0 ? -INFINITY : 0.f;
+            const float first = fmaf(slope, (float)(kbase + q * 32 + h * 16 - pos), off);
+            float2 d = make_float2(first, first + slope);
+#pragma unroll
+            for (int i = h * 16; i < h * 16 + 16; i += 2) {
+              const float2 x = ffma2(make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1])), make_float2(f, f), d);
+              d = fadd2(d, step);
+              v[q][i] = __float_as_uint(x.x);
+              v[q][i + 1] = __float_as_uint(x.y);
+            }
+          }
+        }
+        return;
+      }
+    }
     if constexpr ((kScore & (kScoreCap | kScoreBias)) != 0) {
 #pragma unroll
       for (int q = 0; q < 4; q++) {
@@ -1287,7 +1310,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         bool needMask = (kMode != kModeFixedNoMask) &&
                         ((kbase + kBlockN > w.skv) || (p.causal && (kbase + kBlockN - 1 > (kScore != 0 ? row.seenByAll : w.qlo[t]))));
         if constexpr (kScore != 0 && !kCache) row.documents(p, v, kbase, w.skv);
-        if (needMask) {
+        if (kScore != 0 ? __builtin_expect(needMask, 0) : needMask) {  // (scored: out of the way of the other blocks' instructions)
           int lim = w.skv - kbase;                         // columns [0, lim) are real keys
           if (p.causal) lim = min(lim, (kScore != 0 ? row.last : qpos) - kbase + 1);  // ... that are not in the future
 #pragma unroll
