@@ -1096,6 +1096,62 @@ __global__ void __launch_bounds__(1024) cache_units_kernel(const UnitParams p) {
   if (threadIdx.x == 0) p.unitStart[units] = blocks;
 }
 
+// Units that several CTAs share: O = sum 2^(lse_c - M) O_c / sum 2^(lse_c - M) over their parts, which are [D / 4][128 rows] float4 each.  CTA
+// (x, y): sixteen rows of every 128 of the unit that attention CTA x begins, 32 threads to a row; four parts in flight, relative to the
+// largest log-sum-exp so far.  Bound by latency and the reads from L2; against the CTA that finishes a unit last doing it alone: one request of
+// 16000 tokens, 64 rows a KV head, 8 heads of 128 (18 parts): 82 -> 44 us for the call; 2 heads of 256 (74 parts): 373 -> 58.
+constexpr int kJoinRows = 16, kJoinThreads = 32 * kJoinRows, kJoinShares = tc::kBlockM / kJoinRows;
+template <bool kBf16>
+__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(const TcCacheJoin* joins, const float* partO, const float* partLse, uint16_t* O, int headsQ,
+                                                                  int group, int headDim, int tiles) {
+  ptx::grid_wait_previous();
+  ptx::grid_allow_next();
+  const int c0 = (int)blockIdx.x;
+  const TcCacheJoin join = joins[c0];
+  if (join.last < 0) return;
+  const int r = (int)blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, chunks = headDim / 4;
+  for (int i = threadIdx.x / kJoinRows; i < tiles * chunks; i += 32) {
+    const int t = i / chunks, c4 = i - t * chunks, flat = join.flat + t * tc::kBlockM + r;
+    if (flat >= join.rows) break;
+    constexpr int kAhead = 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -INFINITY, sum = 0.f;
+    for (int c = c0; c <= join.last; c += kAhead) {
+      float lse[kAhead];
+      float4 x[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        const bool there = c + u <= join.last;
+        const long long part = (2ll * (there ? c + u : c) + (c + u == c0 ? join.first : 0)) * tiles + t;
+        const float v = __ldcg(partLse + part * tc::kBlockM + r);
+        lse[u] = there ? v : -INFINITY;
+        x[u] = __ldcg(reinterpret_cast<const float4*>(partO) + (part * chunks + c4) * tc::kBlockM + r);
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) top = fmaxf(top, lse[u]);
+      const float ref = top == -INFINITY ? 0.f : top, f = ex2(M - ref);
+      M = top;
+      sum *= f;
+      acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        const float w = ex2(lse[u] - ref);  // NaN stays NaN
+        sum += w;
+        if (w != 0.f) {  // (a part without a key is not written)
+          acc.x = fmaf(w, x[u].x, acc.x);
+          acc.y = fmaf(w, x[u].y, acc.y);
+          acc.z = fmaf(w, x[u].z, acc.z);
+          acc.w = fmaf(w, x[u].w, acc.w);
+        }
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint16_t* dst = O + ((long long)(join.row0 + flat / group) * headsQ + join.head * group + flat % group) * headDim + c4 * 4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(tc::pack2<kBf16>(acc.x * inv, acc.y * inv), tc::pack2<kBf16>(acc.z * inv, acc.w * inv));
+  }
+}
+
 int run_tc(const TcCacheParams& p, bool bf16, int ctas, bool overlap, int device, cudaStream_t s) {
   switch (p.headDim) {
 #if TFA_HAVE_HDP64
@@ -1121,15 +1177,14 @@ int dispatch_tc(const Params& d, int headDim, bool int8, bool bf16, int device, 
   const int ctas = device_num_sms(device);
   int rc = kOk;
   TcCacheParams p = {};
-  p.join = device_join_counters(device, s, &rc);
-  if (p.join == nullptr) return rc;
   const size_t maxUnits = (size_t)((long long)d.totalQ * d.group / unitRows) + d.batch;
   const size_t parts = (size_t)ctas * 2 * tiles * tc::kBlockM;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const size_t oBytes = up(parts * headDim * sizeof(float)), lseBytes = up(parts * sizeof(float)), startBytes = up((maxUnits + 1) * sizeof(long long)),
-               whatBytes = up((maxUnits + 1) * sizeof(int2)), baseBytes = up((size_t)(d.batch + 1) * sizeof(int));
+               whatBytes = up((maxUnits + 1) * sizeof(int2)), baseBytes = up((size_t)(d.batch + 1) * sizeof(int)),
+               joinBytes = up((size_t)ctas * sizeof(TcCacheJoin));
   void* scratch = nullptr;
-  rc = scratch_alloc(&scratch, oBytes + lseBytes + startBytes + whatBytes + baseBytes + 256, device, s);
+  rc = scratch_alloc(&scratch, oBytes + lseBytes + startBytes + whatBytes + baseBytes + joinBytes + 256, device, s);
   if (rc != kOk) return rc;
   uint8_t* at = static_cast<uint8_t*>(scratch);
   p.partO = reinterpret_cast<float*>(at);
@@ -1137,7 +1192,8 @@ int dispatch_tc(const Params& d, int headDim, bool int8, bool bf16, int device, 
   long long* unitStart = reinterpret_cast<long long*>(at += lseBytes);
   int2* unitWhat = reinterpret_cast<int2*>(at += startBytes);
   int* unitBase = reinterpret_cast<int*>(at += whatBytes);
-  int* numUnits = reinterpret_cast<int*>(at += baseBytes);
+  p.joins = reinterpret_cast<TcCacheJoin*>(at += baseBytes);
+  int* numUnits = reinterpret_cast<int*>(at += joinBytes);
   UnitParams u = {static_cast<uint4*>(d.O), d.cuQ, d.lens, d.batch, d.width << d.blockShift, d.totalQ, d.group, d.causal, unitRows, d.headsQ * headDim / 8,
                   (int)maxUnits, numUnits, unitBase, unitStart, unitWhat};
   const bool overlap = may_overlap(s);
@@ -1173,6 +1229,17 @@ int dispatch_tc(const Params& d, int headDim, bool int8, bool bf16, int device, 
     p.unitStart = unitStart;
     p.unitWhat = unitWhat;
     rc = p.status == nullptr ? kCudaError : run_tc(p, bf16, ctas, overlap, device, s);
+  }
+  if (rc == kOk) {
+    auto join = [&](auto kernel) {
+      return launch_kernel(kernel, dim3((unsigned)ctas, kJoinShares), kJoinThreads, 0, s, overlap, p.joins, p.partO, p.partLse,
+                           static_cast<uint16_t*>(d.O), d.headsQ, d.group, headDim, tiles);
+    };
+    e = bf16 ? join(cache_join_kernel<true>) : join(cache_join_kernel<false>);
+    if (e != cudaSuccess) {
+      set_error_string("cache join kernel launch failed: %s", cudaGetErrorString(e));
+      rc = kCudaError;
+    }
   }
   cudaFreeAsync(scratch, s);
   return rc;
@@ -1245,6 +1312,10 @@ extern "C" int tfa_b200_fwd_cache(const void* Q, void* O, const void* kCache, co
   p.scaleLog2 = (float)(1.4426950408889634 / sqrt((double)headDim));
   p.cap = softcap;
   const bool int8 = cacheType == TFA_B200_CACHE_INT8, bf16 = dtype == kBf16;
+  // Few query rows for a KV head: the stream kernel, whose time grows with every 16 of them; many: tensor-core tiles of 128, which cost the same for one
+  // row as for all.  They meet near 64 rows.  us of stream / tensor form at 48, 64, 96 and 256 rows (8 KV heads of 128, e4m3): 4 x 4000 tokens
+  // 40/42, 45/43, 56/44, 114/63; 16 x 2000 57/66, 73/68, 99/72, 228/106; 64 x 1000 113/140, 146/143, 207/152, 507/207; one of 16000 40/44, 46/44,
+  // 57/45, 110/67; one of 1000 (launch and latency) 19/22, 19/22, 20/23, 24/32.  16 heads of 64, 16 x 2000: 66/84, 84/86, 116/89 at 96.
   const int tcOption = option_cache_tc();
   const long long rowsMost = (long long)maxSeqLenQ * p.group;  // query rows of a request that share a KV head
   if (tcOption > 0 || (tcOption < 0 && rowsMost > 4 * kRows)) return dispatch_tc(p, headDim, int8, bf16, device, s);

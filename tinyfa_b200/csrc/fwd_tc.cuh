@@ -86,6 +86,15 @@ struct TcScorePartParams : TcPartParams, ScoreFields {};
 
 // ... and of packed queries over the paged 8-bit cache.  cuQ: rows of the requests; group query heads of a KV head and the tokens of a
 // request together make flat rows, 128 to a tile, the tiles of a CTA to a unit.
+// The unit that a CTA begins and others go on with, for the kernel that joins its parts (cache_join_kernel).
+struct TcCacheJoin {
+  int last;   // the last of those CTAs; below zero: there is no such unit
+  int first;  // part of the first CTA: 0 where the unit begins its run, else 1; the others': 0
+  int head;   // KV head
+  int row0;   // first row of Q of the request
+  int flat;   // first flat row of the unit,
+  int rows;   // flat rows of the request
+};
 struct TcCacheParams : TcParams, ScoreFields {
   const void* Q;
   const uint8_t* codes[2];    // K, V [numBlocks][headsKV][1 << blockShift][headDim]
@@ -99,7 +108,7 @@ struct TcCacheParams : TcParams, ScoreFields {
   const int2* unitWhat;        // [units]
   float* partO;                // [CTAs][2][tiles][headDim / 4][128] float4, normalised
   float* partLse;              // [CTAs][2][tiles][128]
-  int* join;                   // [CTAs][2], zero
+  TcCacheJoin* joins;          // [CTAs]
 };
 
 namespace tc {
@@ -729,7 +738,7 @@ struct ScoreRow {
   // c tanh of all scores of a key block, times log2(e).  Arguments up to 1/2, which is where a cap is meant to leave scores, on the FMA pipe: an
   // odd polynomial of degree 7, off by 1.6e-7 c at most; larger ones (of any row of the warp) with c - 2 c / (e^2x + 1), two more MUFU operations
   // on every score, off by about as much.  arg: factor that makes a score the 2 x log2(e) of the latter.
-  // Causal B2 S4096 32 over 8 heads of 128, cap 50: TANH_MEASURED.
+  // Causal B2 S4096 32 over 8 heads of 128, cap 50: 506 us with the latter for all scores, 384 so.
   __device__ __forceinline__ void cap_scores(uint32_t (&v)[4][32], float arg) const {
     float top[4];
 #pragma unroll
@@ -928,8 +937,7 @@ __device__ __forceinline__ void exact_rows_of_tile(const P& p, const W& w, int t
 struct CacheSegment {  // what the loading thread publishes beside a WorkSlot
   int b;           // request
   int slot;        // 2 x CTA + (0: first segment of the CTA's run, 1: a later one)
-  int c0, c1;      // CTAs that share the unit
-  int at0;         // slot parity of the unit's part in c0
+  int whole;       // no other CTA has a part of the unit
 };
 struct CacheCtl {
   uint64_t scaleFull[8];
@@ -937,7 +945,6 @@ struct CacheCtl {
   float2 summary[8];    // largest scale of V; groups whose block does not exist, as bits
   float rowFactor[4][2][kBlockM];
   CacheSegment seg[2];
-  int last[2];
 };
 constexpr int kCacheSmem = 5120;
 static_assert(sizeof(CacheCtl) <= kCacheSmem, "shared memory of the cache form");
@@ -977,64 +984,6 @@ __device__ __forceinline__ void cache_store(const P& p, const W& w, int flat, in
     q.z = pack2<kBf16>(__uint_as_float(o[g * 8 + 4]) * inv, __uint_as_float(o[g * 8 + 5]) * inv);
     q.w = pack2<kBf16>(__uint_as_float(o[g * 8 + 6]) * inv, __uint_as_float(o[g * 8 + 7]) * inv);
     dst[ch * 4 + g] = q;
-  }
-}
-
-// The four softmax warps of tile t have stored their part of the unit: if they are the last of the CTAs that share it, they put the parts
-// together, a row per thread (neighbouring rows lie next to one another in a part).
-template <int NT, int kHD, bool kBf16, class W>
-__device__ __forceinline__ void cache_join(const TcCacheParams& p, const W& w, const CacheSegment& seg, CacheCtl* cctl, int t, int r) {
-  __threadfence();
-  asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
-  if (r == 0) {
-    int* counter = p.join + 2 * seg.c0 + t;
-    const bool last = atomicAdd(counter, 1) == seg.c1 - seg.c0;
-    if (last) *counter = 0;  // for the next call
-    cctl->last[t] = last;
-    __threadfence();
-  }
-  asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
-  if (cctl->last[t] == 0) return;
-  const int flat = w.qlo[t] + r;
-  if (flat >= w.sq) return;
-  auto part = [&](int c) { return (2ll * c + (c == seg.c0 ? seg.at0 : 0)) * NT + t; };
-  float M = -INFINITY;
-  bool nan = false;
-#pragma unroll 4
-  for (int c = seg.c0; c <= seg.c1; c++) {
-    const float lse = __ldcg(p.partLse + part(c) * kBlockM + r);
-    nan = nan || lse != lse;
-    M = fmaxf(M, lse);
-  }
-  if (M == -INFINITY) M = 0.f;
-  if (nan) M = NAN;
-  float sum = 0.f;
-#pragma unroll 4
-  for (int c = seg.c0; c <= seg.c1; c++) sum += ex2(__ldcg(p.partLse + part(c) * kBlockM + r) - M);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll 1
-  for (int ch = 0; ch < kHD / 32; ch++) {
-    float acc[32];
-#pragma unroll
-    for (int i = 0; i < 32; i++) acc[i] = 0.f;
-#pragma unroll 1
-    for (int c = seg.c0; c <= seg.c1; c++) {
-      const float wt = ex2(__ldcg(p.partLse + part(c) * kBlockM + r) - M);
-      if (wt == 0.f) continue;  // nothing there
-      const float4* src = reinterpret_cast<const float4*>(p.partO) + (part(c) * (kHD / 4) + ch * 8) * kBlockM + r;
-#pragma unroll
-      for (int g = 0; g < 8; g++) {
-        const float4 x = __ldcg(src + g * kBlockM);
-        acc[g * 4] = fmaf(wt, x.x, acc[g * 4]);
-        acc[g * 4 + 1] = fmaf(wt, x.y, acc[g * 4 + 1]);
-        acc[g * 4 + 2] = fmaf(wt, x.z, acc[g * 4 + 2]);
-        acc[g * 4 + 3] = fmaf(wt, x.w, acc[g * 4 + 3]);
-      }
-    }
-    uint32_t o[32];
-#pragma unroll
-    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(acc[i]);
-    cache_store<kBf16>(p, w, flat, ch, o, inv);
   }
 }
 
@@ -1238,7 +1187,6 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         if (t < NT && w.nblk[t] == 0 && w.qlo[t] < w.sq) {  // no keys for this tile in the segment, but a part that others count on
           const long long part = ((long long)seg.slot * NT + t) * kBlockM + r;
           __stcg(p.partLse + part, -INFINITY);
-          cache_join<NT, kHD, kBf16>(p, w, seg, cctl, t, r);
         }
       }
       if (t >= NT || w.nblk[t] == 0) continue;
@@ -1463,7 +1411,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         }
       }
       if constexpr (kCache) {
-        // This warp is also the epilogue of its 32 rows: the output, or a part of it that the CTA that comes last puts together.
+        // This warp is also the epilogue of its 32 rows: the output, or a part of it for cache_join_kernel.
         const int lastBlk = it - 1;
         if constexpr (kRingSig) {
           const int gLast = ldItem + 2 * w.nmax - 1;
@@ -1473,7 +1421,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         }
         ptx::tc_fence_after();
         const float inv = l == 0.f ? 0.f : vRef * (1.f / kCacheUp) / l;  // NaN stays NaN
-        const bool whole = seg.c0 == seg.c1;
+        const bool whole = seg.whole != 0;
         const uint32_t tO = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(C::kOCol0 + t * HDP);
         const long long part = (long long)seg.slot * NT + t;
 #pragma unroll
@@ -1504,7 +1452,6 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         }
         if (!whole) {
           __stcg(p.partLse + part * kBlockM + r, l == 0.f ? -INFINITY : m + __log2f(l));
-          cache_join<NT, kHD, kBf16>(p, w, seg, cctl, t, r);
         }
         items++;
         continue;
@@ -2109,6 +2056,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             }
           }
         }
+        TcCacheJoin join = {-1, 0, 0, 0, 0, 0};
         for (int k = 0;; k++) {
           if (k >= 2) wait_bar(bar(kBarWorkEmpty + (k & 1)), ((k >> 1) - 1) & 1, wc, 21);
           volatile WorkSlot* ws = &ctl->work[k & 1];
@@ -2140,9 +2088,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             const int c0 = cache_run_of(first, total, runs), c1 = cache_run_of(first + blocks - 1, total, runs);
             cs->b = b;
             cs->slot = 2 * run + (k == 0 ? 0 : 1);
-            cs->c0 = c0;
-            cs->c1 = c1;
-            cs->at0 = total * c0 / runs == first ? 0 : 1;
+            cs->whole = c0 == c1;
+            if (c0 == run && c1 > run) join = {c1, k == 0 ? 0 : 1, h, q0, what.y, nq * p.group};
             at += n;
             if (++u == units) {
               u = 0;
@@ -2153,6 +2100,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           ptx::mbar_arrive(bar(kBarWorkFull + (k & 1)));
           if (!more) break;
         }
+        p.joins[run] = join;
       }
     } else if (!kCache && warp == kLoadWarp && lane == 0) {
       // ============================================================== work distribution + TMA loads
