@@ -110,6 +110,67 @@ def test_block_scales_that_differ_by_orders_of_magnitude(form):
         _expect(got, Q, cache, [400, 600], [20, 20])
 
 
+def test_caps_far_above_all_scores(form):
+    """c tanh(s / c) is s within s^3 / 3 c^2 < 1e-7, and within 2.4e-6 |s| as it is computed, which the exponential's bound leaves room for."""
+    for code, dtype, lens, new, cap in (("int8", "fp16", [400, 70], [1, 2], 1e5), ("e4m3", "bf16", [300], [90], 1e35)):
+        cache = _cache(code, lens, 2, 64, 16, 6, spread=0.3)
+        Q = (torch.randn(sum(new), 4, 64, device="cuda") * 0.3).to(DT[dtype])
+        cu = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32, device="cuda")
+        got = tfa.flash_attn_cache_forward(Q, *cache, torch.tensor(lens, dtype=torch.int32, device="cuda"), cu, max(new), max(lens), softcap=cap)
+        _expect(got, Q, cache, lens, new)
+
+
+def test_nan_in_cells_and_blocks_that_no_request_has(form):
+    cache = _cache("e4m3", [100, 37, 64], 2, 128, 16, 9)
+    kc, vc, ks, vs, table = cache
+    used = {int(i) for row, n in zip(table.tolist(), (100, 37, 64)) for i in row[:-(-n // 16)]}
+    for c, s in ((kc, ks), (vc, vs)):
+        raw = c.view(torch.uint8)
+        for i in range(kc.shape[0]):
+            if i not in used:
+                raw[i] = 0x7F
+                s[i] = math.nan
+        raw[int(table[0, 6]), :, 4:] = 0x7F  # behind token 99
+        raw[int(table[1, 2]), :, 5:] = 0xFF  # behind token 36
+    cu = torch.tensor([0, 1, 20, 84], dtype=torch.int32, device="cuda")
+    Q = torch.randn(84, 4, 128, device="cuda").half()
+    got = tfa.flash_attn_cache_forward(Q, *cache, torch.tensor([100, 37, 64], dtype=torch.int32, device="cuda"), cu, 64, 100)
+    _expect(got, Q, cache, [100, 37, 64], [1, 19, 64])
+
+
+def test_calls_on_streams_and_graphs_at_once(form):
+    """Arrival counters and parts belong to a stream or a captured call: eager calls on two streams and two graphs of one call side by side."""
+    cache = _cache("int8", [9000, 2500, 40], 2, 128, 64, 10)
+    lens = torch.tensor([9000, 2500, 40], dtype=torch.int32, device="cuda")
+    jobs = []
+    for n, new in enumerate(([1, 1, 1], [40, 3, 20])):
+        cu = torch.tensor([0, new[0], new[0] + new[1], sum(new)], dtype=torch.int32, device="cuda")
+        Q = torch.randn(sum(new), 8, 128, device="cuda").half()
+        jobs.append((Q, *cache, lens, cu, max(new), 9000))
+    want = [tfa.flash_attn_cache_forward(*j) for j in jobs]
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append([tfa.flash_attn_cache_forward(*j) for j in jobs])
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for k in range(10):
+        for s, graph in zip(streams[:2], graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        for n, s in enumerate(streams[2:]):
+            with torch.cuda.stream(s):
+                got.append((n, tfa.flash_attn_cache_forward(*jobs[n])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[n]) for n, x in got)
+    for outs in held:
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
+    tfa.device_status()
+
+
 def test_queries_of_any_magnitude(form):
     """bf16 queries become fp16 with a power of two per row taken out."""
     cache = _cache("int8", [300], 1, 128, 16, 4)

@@ -181,6 +181,54 @@ def test_nan_keys_and_values_in_places_nobody_sees(dtype):
     assert torch.equal(got, want[:, :200])
 
 
+@pytest.mark.parametrize("dtype,B,Sq,Skv,Hq,Hkv,D", [("fp16", 1, 200, 300, 2, 1, 64), ("bf16", 1, 150, 150, 2, 2, 128), ("fp16", 2, 2, 900, 4, 2, 64),
+                                                      ("bf16", 1, 1, 5000, 8, 2, 128), ("fp32", 1, 150, 200, 2, 1, 64), ("fp32", 1, 40, 50, 2, 1, 128)])
+@pytest.mark.parametrize("cap", [1e5, 1e35])
+def test_caps_far_above_all_scores(dtype, B, Sq, Skv, Hq, Hkv, D, cap):
+    """c tanh(s / c) is s within s^3 / 3 c^2 < 1e-8, and within 2.4e-6 |s| as it is computed: 2 x 2.4e-6 x 8 < 4e-5 of A, inside the
+    exponential's 8.6e-5, of which these calls use a part; fp32 has an exact tanh."""
+    Q, K, V = _inputs(dtype, B, Sq, Skv, Hq, Hkv, D, 40)
+    got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, softcap=cap, q_start=Skv - Sq)
+    _compare(got, Q, K, V, True, q_start=Skv - Sq, fp32_error=2.0 ** -19)
+    tiny = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, softcap=1e-36, q_start=Skv - Sq)  # all scores are zero: means of V
+    _compare(tiny, Q * 0, K, V, True, q_start=Skv - Sq, fp32_error=2.0 ** -19)
+
+
+def test_calls_on_streams_and_threads_at_once():
+    """Partial results, document tables and work counters belong to a call, whatever runs beside it."""
+    import threading
+
+    shapes = [("bf16", 1, 3, 6000, 8, 2, 128), ("fp16", 1, 100, 4000, 2, 1, 64), ("bf16", 2, 600, 600, 4, 2, 96), ("fp32", 1, 300, 900, 2, 1, 64)]
+    jobs = []
+    for n, shape in enumerate(shapes):
+        Q, K, V = _inputs(*shape, 50 + n)
+        kw = dict(is_causal=True, softcap=5.0, q_start=shape[3] - shape[2])
+        if n == 2:
+            docs = _documents(2, 600, 100, 8)
+            kw.update(doc_ids_q=docs, doc_ids_kv=docs)
+        jobs.append((Q, K, V, kw, tfa.flash_attn_scored_forward(Q, K, V, **kw)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for k in range(12):
+                Q, K, V, kw, want = jobs[(i + k) % len(jobs)]
+                got = tfa.flash_attn_scored_forward(Q, K, V, **kw)
+                if not torch.equal(got, want):
+                    wrong.append((i, k))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    tfa.device_status()
+
+
 FP32_SHAPES = [  # B, Sq, Skv, Hq, Hkv: one key, tile edges, heads in one tile, several key ranges, more than one batch entry
     (1, 1, 1, 1, 1), (2, 3, 1300, 8, 2), (1, 127, 129, 3, 1), (2, 129, 300, 4, 4), (1, 300, 1500, 2, 1), (3, 140, 131, 6, 2),
 ]

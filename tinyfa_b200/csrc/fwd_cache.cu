@@ -164,11 +164,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
@@ -601,10 +596,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
         const float f0 = fac[nr][0] * ks, f1 = fac[nr][1] * ks;
 #pragma unroll
         for (int e = 0; e < 4; e++) sc[nr][e] = (sc[nr][e] + sd[nr][e]) * ((e & 1) ? f1 : f0);
-        if (p.cap > 0.f) {  // c tanh(x) = c - 2 c / (e^2x + 1)
-#pragma unroll
-          for (int e = 0; e < 4; e++) sc[nr][e] = fmaf(-2.f * capLog2, rcp(ex2(sc[nr][e]) + 1.f), capLog2);
-        }
+        if (p.cap > 0.f) score::cap_few(sc[nr], capLog2);
         if (p.slopes != nullptr) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
@@ -1310,7 +1302,7 @@ extern "C" int tfa_b200_fwd_cache(const void* Q, void* O, const void* kCache, co
   p.causal = isCausal ? 1 : 0;
   p.totalQ = (int)totalQ;
   p.scaleLog2 = (float)(1.4426950408889634 / sqrt((double)headDim));
-  p.cap = softcap;
+  p.cap = score::usable_cap(softcap);
   const bool int8 = cacheType == TFA_B200_CACHE_INT8, bf16 = dtype == kBf16;
   // Few query rows for a KV head: the stream kernel, whose time grows with every 16 of them; many: tensor-core tiles of 128, which cost the same for one
   // row as for all.  They meet near 64 rows.  us of stream / tensor form at 48, 64, 96 and 256 rows (8 KV heads of 128, e4m3): 4 x 4000 tokens

@@ -123,11 +123,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float fmax_nan(float a, float b) {  // NaN is kept
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -439,7 +434,6 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
         mma16816<kBf16>(sc[1], qf[ks], kf[2], kf[3]);
       }
       if constexpr (kScore) {
-        // c tanh(x) = c - 2 c / (e^2x + 1): off by about 2^-23 c whatever x is, which is what the exponential behind it sees
         const float capLog2 = p.cap * 1.44269504f, factor = p.cap > 0.f ? 2.f * p.scaleLog2 / p.cap : p.scaleLog2;
         const int posA = p.qStart + qposA, posB = p.qStart + qposB;
         int limA = keyEnd, limB = keyEnd;
@@ -453,25 +447,17 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
           slopeA = validA ? p.slopes[hkv * p.group + rowA % p.group] * 1.44269504f : 0.f;
           slopeB = validB ? p.slopes[hkv * p.group + rowB % p.group] * 1.44269504f : 0.f;
         }
-        int docA = -1, docB = -1;
-        if (p.docKV != nullptr) {
-          docA = validA ? p.docQ[qRow0 + qposA] : -1;
-          docB = validB ? p.docQ[qRow0 + qposB] : -1;
-        }
 #pragma unroll
         for (int n = 0; n < 2; n++) {
 #pragma unroll
+          for (int e = 0; e < 4; e++) sc[n][e] *= factor;
+          if (p.cap > 0.f) score::cap_few(sc[n], capLog2);
+#pragma unroll
           for (int e = 0; e < 4; e++) {
             const int key = kb + n * 8 + 2 * tig + (e & 1);
-            float x = sc[n][e] * factor;
-            if (p.cap > 0.f) x = fmaf(-2.f * capLog2, rcp(ex2(x) + 1.f), capLog2);
+            float x = sc[n][e];
             if (p.slopes != nullptr) x = fmaf(e < 2 ? -slopeA : -slopeB, fabsf((float)((e < 2 ? posA : posB) - key)), x);
-            bool see = key < (e < 2 ? limA : limB);
-            if (p.docKV != nullptr) {
-              const int doc = e < 2 ? docA : docB;
-              see = see && doc >= 0 && p.docKV[(long long)b * skv + key] == doc;
-            }
-            sc[n][e] = see ? x : -INFINITY;
+            sc[n][e] = key < (e < 2 ? limA : limB) ? x : -INFINITY;
           }
         }
       }

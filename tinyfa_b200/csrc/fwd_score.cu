@@ -307,7 +307,7 @@ extern "C" int tfa_b200_fwd_scored(const void* Q, const void* K, const void* V, 
   p.headDim = headDim;
   p.causal = isCausal ? 1 : 0;
   p.stream = static_cast<cudaStream_t>(stream);
-  ScoreFields f = {qStart, softcap, alibiSlopes, prefixLens, docIdsQ, docIdsKV, nullptr, nullptr, nullptr, 0, 0,
+  ScoreFields f = {qStart, score::usable_cap(softcap), alibiSlopes, prefixLens, docIdsQ, docIdsKV, nullptr, nullptr, nullptr, 0, 0,
                    {Q, K, V, seqLenQ, seqLenKV, numHeadsQ, numHeadsKV, p.causal}};
   return score::dispatch(p, f, device);
 }

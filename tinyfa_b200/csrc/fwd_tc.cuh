@@ -675,8 +675,6 @@ template <int kMode>
 struct ParamsOf<kMode, 1> {
   using type = typename std::conditional<kMode == kModeFixedSplit, TcScorePartParams, TcScoreParams>::type;
 };
-// tanh(t) / t = c0 + c1 t^2 + c2 t^4 + c3 t^6 for |t| <= 1/2, fitted to the smallest largest error of the tanh (1.3e-7)
-constexpr float kTanh0 = 0.9999976754188538f, kTanh1 = -0.33320656418800354f, kTanh2 = 0.13145145773887634f, kTanh3 = -0.04337248206138611f;
 // kScore: 0, or kScoreMask (masks by prefix, document and query offset) with kScoreCap and kScoreBias.  Instantiations of their own:
 // the cap is two more MUFU operations on every score, in kernels that the exponentials bound already.
 constexpr int kScoreMask = 1, kScoreCap = 2, kScoreBias = 4;
@@ -729,10 +727,10 @@ struct ScoreRow {
   __device__ __forceinline__ void begin_cap(float cap, float f) {
     capLog2 = cap * 1.44269504f;
     const float f2 = f * f;
-    tanhC[0] = kTanh0 * capLog2 * f;
-    tanhC[1] = kTanh1 * capLog2 * f * f2;
-    tanhC[2] = kTanh2 * capLog2 * f * f2 * f2;
-    tanhC[3] = kTanh3 * capLog2 * f * f2 * f2 * f2;
+    tanhC[0] = score::kTanh0 * capLog2 * f;
+    tanhC[1] = score::kTanh1 * capLog2 * f * f2;
+    tanhC[2] = score::kTanh2 * capLog2 * f * f2 * f2;
+    tanhC[3] = score::kTanh3 * capLog2 * f * f2 * f2 * f2;
     small = (f < 1e4f && f > 1e-30f) ? 0.5f / f : -1.f;  // the coefficients are finite
   }
   // c tanh of all scores of a key block, times log2(e).  Arguments up to 1/2, which is where a cap is meant to leave scores, on the FMA pipe: an
@@ -855,14 +853,19 @@ struct ScoreRow {
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const float f = i < 16 ? f2.x : f2.y, off = i < 16 ? off0 : off1;
-          const float2 x = ffma2(make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1])), make_float2(f, f), make_float2(off, off));
+          float2 x = make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
+          if constexpr ((kScore & kScoreCap) == 0) {
+            x = ffma2(x, make_float2(f, f), make_float2(off, off));
+          } else {
+            x = fmul2(x, make_float2(f, f));
+          }
           v[q][i] = __float_as_uint(x.x);
           v[q][i + 1] = __float_as_uint(x.y);
         }
       }
       if constexpr ((kScore & kScoreCap) != 0) {
         cap_scores(v, 1.f);
-        if (gone != 0) {  // minus infinity is -c by now
+        if (gone != 0) {  // (minus infinity before would be -c by now)
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             if (gone >> i & 1u) {

@@ -31,4 +31,37 @@ struct ScoreFields {
   ScoreSource src;
 };
 
+namespace score {
+
+// tanh(t) / t = c0 + c1 t^2 + c2 t^4 + c3 t^6 for |t| <= 1/2, fitted to the smallest largest error of the tanh (1.3e-7)
+constexpr float kTanh0 = 0.9999976754188538f, kTanh1 = -0.33320656418800354f, kTanh2 = 0.13145145773887634f, kTanh3 = -0.04337248206138611f;
+
+// A cap stays where products with it neither overflow nor vanish; beyond, it changes no result (scores within 1e-30, or no cap at all).
+inline float usable_cap(float cap) { return cap > 0.f ? (cap < 1e-30f ? 1e-30f : cap > 1e28f ? 1e28f : cap) : 0.f; }
+
+// c tanh of a few scores, times log2(e); x: 2 log2(e) S / c.  Scores up to c / 2 (of the whole warp) by the polynomial; else c - 2 c / (e^2x + 1), which
+// is off by 2^-22 c: no more than 2^-21 of the largest score then, but everything where c is far above all scores.
+template <int N>
+__device__ __forceinline__ void cap_few(float (&x)[N], float capLog2) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i++) top = fmaxf(top, fabsf(x[i]));
+  if (__all_sync(0xffffffffu, top <= 1.44269504f)) {  // (a NaN stays one on either way)
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float t = x[i] * 0.34657359f, u = t * t;
+      x[i] = capLog2 * t * fmaf(fmaf(fmaf(kTanh3, u, kTanh2), u, kTanh1), u, kTanh0);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      float e, r;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x[i]));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.f));
+      x[i] = fmaf(-2.f * capLog2, r, capLog2);
+    }
+  }
+}
+
+}  // namespace score
 }  // namespace tfa_b200
