@@ -267,6 +267,22 @@ def test_both_fp32_forms(shape, D):
             tfa.set_option("fp32_tc", -1)
 
 
+def test_fp32_call_in_pieces():
+    """A workspace beyond what the pool keeps: fewer batch entries at a time, each with its part of the tables, slopes and prefixes."""
+    B, S, H, D = 260, 520, 16, 64
+    g = torch.Generator(device="cuda").manual_seed(60)
+    Q, K, V = (torch.randn(B, S, H, D, device="cuda", generator=g) for _ in range(3))
+    docs, slopes = _documents(B, S, 200, 9), _slopes(H)
+    prefix = torch.arange(B, dtype=torch.int32, device="cuda")
+    for kw in (dict(doc_ids_q=docs, doc_ids_kv=docs), dict(prefix_lens=prefix)):
+        got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, softcap=4.0, alibi_slopes=slopes, **kw)
+        for b in (0, B // 2 - 1, B // 2, B - 1):
+            one = slice(b, b + 1)
+            more = dict(dq=docs[one], dk=docs[one]) if "doc_ids_q" in kw else dict(prefix=prefix[one])
+            _compare(got[one], Q[one], K[one], V[one], True, 4.0, slopes, fp32_error=2.0 ** -19, **more)
+    tfa.device_status()
+
+
 def test_fp32_values_outside_the_exact_range():
     """Such calls are left to the CUDA cores, to the last bit; the document tables are then those of the other kernel's blocks."""
     Q, K, V = _inputs("fp32", 2, 400, 400, 4, 2, 64, 21)

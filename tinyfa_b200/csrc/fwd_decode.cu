@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
       }
     }
     if constexpr (kScore) {
-      __syncwarp();
+      if (__syncthreads_or(spoilt != 0u) == 0) spoilt = 0u;  // (a row's columns may be two warps')
       spoilt = __reduce_or_sync(0xffffffffu, spoilt);
 #pragma unroll 1
       for (; spoilt != 0u; spoilt &= spoilt - 1) {
@@ -680,7 +680,9 @@ combine_parts_kernel(const float* partO, const float* partLse, void* O, long lon
     *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(O) + row * D + c4 * 4) = out;
     if (kScore) bad = wsum > 0.f && wsum < INFINITY && !(fabsf(acc.x + acc.y + acc.z + acc.w) < INFINITY);
   }
-  if constexpr (kScore) score::exact_rows<Element<kBf16>, D>(fields, bad, row / headsQ, (int)(row % headsQ), O);
+  if constexpr (kScore) {
+    if (__syncthreads_or(bad)) score::exact_rows<Element<kBf16>, D>(fields, bad, row / headsQ, (int)(row % headsQ), O);
+  }
 }
 
 template <int D, bool kBf16, bool kScore = false>

@@ -53,10 +53,12 @@ int launch_one(const FwdProblem& pr, int packShift, const TcSplit& split, int de
     p.partO = split.partO;
     p.partLse = split.partLse;
   }
+  // keys behind the last row's position are nobody's (a prefix may reach further): zeros, whatever they hold
+  const long long reach = (long long)p.qStart + pr.seqLenQ, readable = pr.causal && p.prefix == nullptr && reach < pr.seqLenKV ? reach : pr.seqLenKV;
   CUtensorMap tmQ, tmK, tmV;
   if ((rc = make_map(&tmQ, pr.Q, pr.batch, pr.seqLenQ, pr.headsQ, pr.headDim, 1 << packShift, tc::kBlockM >> packShift)) != kOk) return rc;
-  if ((rc = make_map(&tmK, pr.K, pr.batch, pr.seqLenKV, pr.headsKV, pr.headDim, 1, tc::kBlockN)) != kOk) return rc;
-  if ((rc = make_map(&tmV, pr.V, pr.batch, pr.seqLenKV, pr.headsKV, pr.headDim, 1, tc::kBlockN)) != kOk) return rc;
+  if ((rc = make_map(&tmK, pr.K, pr.batch, pr.seqLenKV, pr.headsKV, pr.headDim, 1, tc::kBlockN, readable)) != kOk) return rc;
+  if ((rc = make_map(&tmV, pr.V, pr.batch, pr.seqLenKV, pr.headsKV, pr.headDim, 1, tc::kBlockN, readable)) != kOk) return rc;
   rc = kCudaError;
   p.workCounter = device_work_counter(device, pr.stream, &rc, nullptr);
   if (p.workCounter == nullptr) return rc;

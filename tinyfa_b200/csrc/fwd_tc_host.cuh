@@ -25,10 +25,10 @@ int option_pair_cta();                // c_abi.cu: head dims 192 / 256 in cluste
 // [batches, rows, heads, headDim] tensor, 16-bit elements (packed varlen: batches = 1, rows = total);
 // box = 64 elements x boxHeads x boxRows x 1, 128-byte swizzle; out-of-range elements read as zero.
 static int make_map(CUtensorMap* m, const void* base, long long batches, long long rows, int heads, int headDim,
-                    int boxHeads, int boxRows) {
+                    int boxHeads, int boxRows, long long readable = -1 /* rows of an entry that are read; zeros behind them */) {
   EncodeTiledFn enc = get_encode_tiled();
   if (enc == nullptr) return kCudaError;
-  cuuint64_t dims[4] = {(cuuint64_t)headDim, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)batches};
+  cuuint64_t dims[4] = {(cuuint64_t)headDim, (cuuint64_t)heads, (cuuint64_t)(readable > 0 ? readable : rows), (cuuint64_t)batches};
   cuuint64_t strides[3] = {(cuuint64_t)headDim * 2, (cuuint64_t)heads * headDim * 2,
                            (cuuint64_t)rows * heads * headDim * 2};
   cuuint32_t box[4] = {64, (cuuint32_t)boxHeads, (cuuint32_t)boxRows, 1};
