@@ -264,6 +264,17 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
   const int qposA = rowA / p.group, qposB = rowB / p.group;
   const bool validA = rowA < nRows, validB = rowB < nRows;
   const float c = kScore ? 1.f : p.scaleLog2;
+  [[maybe_unused]] float slopeA = 0.f, slopeB = 0.f, capLog2 = 0.f, factor = p.scaleLog2;
+  if constexpr (kScore) {
+    if (p.slopes != nullptr) {
+      slopeA = validA ? p.slopes[hkv * p.group + rowA % p.group] * 1.44269504f : 0.f;
+      slopeB = validB ? p.slopes[hkv * p.group + rowB % p.group] * 1.44269504f : 0.f;
+    }
+    if (p.cap > 0.f) {
+      capLog2 = p.cap * 1.44269504f;
+      factor *= 2.f / p.cap;
+    }
+  }
 
   float o[kNT][4];
   float mA, mB, lA, lB;
@@ -434,18 +445,12 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
         mma16816<kBf16>(sc[1], qf[ks], kf[2], kf[3]);
       }
       if constexpr (kScore) {
-        const float capLog2 = p.cap * 1.44269504f, factor = p.cap > 0.f ? 2.f * p.scaleLog2 / p.cap : p.scaleLog2;
         const int posA = p.qStart + qposA, posB = p.qStart + qposB;
         int limA = keyEnd, limB = keyEnd;
         if (p.causal) {
           const int prefix = p.prefix != nullptr ? p.prefix[b] : 0;
           limA = min(limA, max(posA + 1, prefix));
           limB = min(limB, max(posB + 1, prefix));
-        }
-        float slopeA = 0.f, slopeB = 0.f;
-        if (p.slopes != nullptr) {
-          slopeA = validA ? p.slopes[hkv * p.group + rowA % p.group] * 1.44269504f : 0.f;
-          slopeB = validB ? p.slopes[hkv * p.group + rowB % p.group] * 1.44269504f : 0.f;
         }
 #pragma unroll
         for (int n = 0; n < 2; n++) {
