@@ -137,6 +137,13 @@ constexpr int kRegsIssue = 64;
 constexpr int kRegsAtLaunch = (65536 / kThreads) / 8 * 8;
 static_assert(8 * kRegsSoftmax + 4 * kRegsEpilogue + 4 * kRegsIssue <= (kThreads / 32) * kRegsAtLaunch,
               "register budget: the CTA's launch allocation must cover every role's setmaxnreg value");
+// Cache form: converter warps in the place of the epilogue's, eight (and four softmax warps) where a CTA has one tile.  512 queries behind 8192
+// tokens, e4m3, 32 over 8 heads of 128, without and with a bias, softmax / converter / issue: 176 / 96 / 64 391 and 507 us, 176 / 104 / 56 376 and 502,
+// 168 / 112 / 64 384 and 550, 176 / 112 / 48 444 and 569, 192 / 80 / 48 603 and 613.
+constexpr int kRegsConvert = 104, kRegsIssueCache = 56, kRegsConvertOneTile = 128;
+static_assert(8 * kRegsSoftmax + 4 * kRegsConvert + 4 * kRegsIssueCache <= (kThreads / 32) * kRegsAtLaunch &&
+                  4 * kRegsSoftmax + 8 * kRegsConvertOneTile + 4 * kRegsIssue <= (kThreads / 32) * kRegsAtLaunch,
+              "register budget of the cache form");
 // Lazy-rescale threshold, log2 units.  Price in accuracy, measured on the benchmark shapes against fp64: the mean
 // output error is 3-4 % above that of exact running maxima (and of the reference kernels), the maximum error within one
 // unit in the last place of the output type.  With the exact maximum the largest weights of a row sit just below 1.0,
@@ -1527,7 +1534,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     }
   } else if (kCache && warp < kEpilogueEnd) {
     // ================================================================ cache form: pages and queries -> fp16 tiles in shared memory
-    ptx::setmaxnreg_dec<kRegsEpilogue>();
+    ptx::setmaxnreg_dec<NT == 2 ? kRegsConvert : kRegsConvertOneTile>();
     if constexpr (kCache) {
       // A thread's 16-byte pieces of a tile: kPieces of them, kStepRows key rows apart, at one place of their rows.  Four threads take the 64
       // codes of a row that go to one 64-wide slab, so that a quarter warp's stores (16 codes are two of the row's eight chunks) fall on eight
@@ -1800,7 +1807,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       }
     }
   } else {
-    ptx::setmaxnreg_dec<kRegsIssue>();
+    ptx::setmaxnreg_dec<kCache && NT == 2 ? kRegsIssueCache : kRegsIssue>();
     if ((warp == kIssueWarpA || warp == kIssueWarpB) && lane == 0) {
       // ============================================================== MMA issue
       const int fmt = (kBf16 && !kCache) ? 1 : 0;
