@@ -163,7 +163,8 @@ int tfa_b200_fwd_decode_noalloc(const void* Q, const void* K, const void* V, voi
  * prefixLens int32 [batchSize] (with isCausal only); docIdsQ int32 [batchSize, seqLenQ], docIdsKV int32 [batchSize, seqLenKV]: both or
  * neither; negative ids belong to no document (padding): such a key is seen by no row and such a row sees no key.  Ids may come in any
  * order; keys outside the range of blocks that a 128-row tile of queries can see are not read, so runs of equal ids in ascending order
- * are fast.  A row that sees no key is zero.  softcap 0 and null pointers switch a part off.
+ * are fast.  A row that sees no key is zero.  What a row does not see has no effect on it, NaN and infinities included.  softcap 0 and
+ * null pointers switch a part off.
  */
 int tfa_b200_fwd_scored(const void* Q, const void* K, const void* V, void* O, int dtype, int batchSize, int seqLenQ, int seqLenKV,
                         int numHeadsQ, int numHeadsKV, int headDim, int isCausal, int qStart, float softcap, const float* alibiSlopes,
@@ -209,7 +210,8 @@ int tfa_b200_kv_cache_store(const void* K, const void* V, void* kCache, void* vC
  * int32 [batchSize]: tokens of each request, those of its queries included - they are its last positions.  isCausal: a query sees the
  * keys up to its own position, else all of the request's.  softcap and alibiSlopes as in tfa_b200_fwd_scored.  maxSeqLenQ / maxSeqLenKV
  * only size the launch.  Every row of O is written: rows of no request, of a request without tokens and rows in front of its first position
- * are zero.  Keys in blocks whose id is outside [0, numBlocks) are not seen.  The first call on a device allocates 16 MB of counters: not
+ * are zero.  Keys in blocks whose id is outside [0, numBlocks) are not seen;
+ * cells behind a request's last token may hold anything.  The first call on a device allocates 16 MB of counters: not
  * under stream capture.  Captured calls allocate their partial results in the graph.
  */
 int tfa_b200_fwd_cache(const void* Q, void* O, const void* kCache, const void* vCache, const float* kScales, const float* vScales,

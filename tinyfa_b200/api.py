@@ -220,7 +220,7 @@ def flash_attn_scored_forward(Q, K, V, is_causal=False, softcap=0.0, alibi_slope
       s = q.k / sqrt(D);  softcap > 0: s = softcap * tanh(s / softcap);  alibi_slopes (float32 [Hq]): s -= slope * |p - j|
     Row i sees key j if (not is_causal, or j <= p, or j < prefix_lens[b]) and (no documents, or doc_ids_q[b,i] == doc_ids_kv[b,j] >= 0).
     prefix_lens int32 [B] needs is_causal; doc_ids_q int32 [B,Sq] and doc_ids_kv int32 [B,Skv] are given together, negative ids are padding.
-    A row that sees no key is zero.  Forward only.
+    A row that sees no key is zero; what a row does not see has no effect on it, NaN and infinities included.  Forward only.
     """
     ok = _usable(Q, K, V)
     if ok:
