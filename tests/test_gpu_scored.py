@@ -326,6 +326,20 @@ def test_values_that_a_mask_hides(dtype, B, Sq, Skv, Hq, Hkv, D, bad):
     tfa.device_status()
 
 
+@pytest.mark.parametrize("dtype,Sq,Hq,Hkv,D", [("fp16", 1, 4, 1, 64), ("bf16", 3, 8, 4, 128), ("fp16", 200, 2, 2, 64), ("fp32", 150, 2, 1, 64)])
+def test_values_far_behind_a_prefix(dtype, Sq, Hq, Hkv, D):
+    """With a prefix the decode kernel reads every key, however far behind the rows."""
+    B, Skv, q_start = 2, 3000, 500
+    Q, K, V = _inputs(dtype, B, Sq, Skv, Hq, Hkv, D, 32)
+    prefix = torch.tensor([400, 900], dtype=torch.int32, device="cuda")
+    V2, K2 = V.clone(), K.clone()
+    V2[:, 1500:] = math.nan
+    K2[:, 2000:] = math.inf
+    got = tfa.flash_attn_scored_forward(Q, K2, V2, is_causal=True, prefix_lens=prefix, q_start=q_start)
+    _compare(got, Q, K, V, True, prefix=prefix, q_start=q_start, fp32_error=2.0 ** -19)
+    tfa.device_status()
+
+
 @pytest.mark.parametrize("dtype,S,D", [("fp16", 300, 64), ("bf16", 500, 128), ("fp32", 300, 64), ("fp16", 200, 256)])
 @pytest.mark.parametrize("shuffle", [False, True])
 def test_values_of_other_documents_and_padding(dtype, S, D, shuffle):

@@ -69,7 +69,8 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
   if (s.causal) end = min(end, max(pos, f.prefix != nullptr ? f.prefix[b] - 1 : -1) + 1);
   if (!docs) {
     bool hidden = false;
-    const int stop = min(f.prefix != nullptr ? s.seqLenKV : min(s.seqLenKV, f.qStart + s.seqLenQ), end + 256);
+    // (with a prefix, whose length only the device knows, the decode kernel reads all keys)
+    const int stop = f.prefix != nullptr ? s.seqLenKV : min(min(s.seqLenKV, f.qStart + s.seqLenQ), end + 256);
 #pragma unroll 1
     for (int k0 = end; k0 < stop; k0 += 8) {
       float x[8][kCols];
