@@ -535,6 +535,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
         storeSegment(entryDone && segStart == 0);
         if (blk + 1 < count) {  // on to the next batch entry, whose blocks are already on their way
           qRow0 += sq;
+          if constexpr (kScore) b++;  // whose prefix it is
           segStart = kbase = 0;
           part = 0;
           startSegment();
