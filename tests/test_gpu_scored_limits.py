@@ -32,3 +32,28 @@ def test_prefixes_of_entries_that_one_run_reads(dtype, B, n, Skv, Hq, Hkv, D, q_
         prefix = torch.tensor([[0, Skv, Skv // 2 + 1, 130][(b + turn) % 4] for b in range(B)], dtype=torch.int32, device="cuda")
         got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, prefix_lens=prefix, softcap=8.0, q_start=q_start)
         _compare(got, Q, K, V, True, 8.0, prefix=prefix, q_start=q_start)
+
+
+def test_prefixes_at_the_ends_of_their_type(call):
+    dtype, Sq, Skv, Hq, Hkv, D = call
+    values = [LARGEST, LARGEST - 62, LARGEST - 63, SMALLEST, SMALLEST + 1, -1]
+    Q, K, V = _inputs(dtype, len(values), Sq, Skv, Hq, Hkv, D, 1)
+    prefix = torch.tensor(values, dtype=torch.int32, device="cuda")
+    for slopes in (None, _slopes(Hq)):
+        got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=True, prefix_lens=prefix, alibi_slopes=slopes)
+        _compare(got, Q, K, V, True, slopes=slopes, prefix=prefix, fp32_error=2.0 ** -19)
+    tfa.device_status()
+
+
+def test_lowest_prefix_and_values_that_the_mask_hides(call):
+    """A row that is computed again from what it sees: no key of a prefix below zero."""
+    dtype, Sq, Skv, Hq, Hkv, D = call
+    Q, K, V = _inputs(dtype, 2, Sq, Skv, Hq, Hkv, D, 2)
+    prefix = torch.tensor([SMALLEST, LARGEST], dtype=torch.int32, device="cuda")
+    V2 = V.clone()
+    first = Sq // 2
+    V2[0, first:] = math.nan
+    got = tfa.flash_attn_scored_forward(Q, K, V2, is_causal=True, prefix_lens=prefix)
+    _compare(got[:1, :first], Q[:1, :first], K[:1], V[:1], True, prefix=prefix[:1], fp32_error=2.0 ** -19)
+    _compare(got[1:], Q[1:], K[1:], V[1:], True, prefix=prefix[1:], fp32_error=2.0 ** -19)
+    tfa.device_status()

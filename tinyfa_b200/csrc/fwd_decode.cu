@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
         const int posA = p.qStart + qposA, posB = p.qStart + qposB;
         int limA = keyEnd, limB = keyEnd;
         if (p.causal) {
-          const int prefix = p.prefix != nullptr ? p.prefix[b] : 0;
+          const int prefix = p.prefix != nullptr ? score::prefix_of(p, b, p.seqLenKV) : 0;
           limA = min(limA, max(posA + 1, prefix));
           limB = min(limB, max(posB + 1, prefix));
         }

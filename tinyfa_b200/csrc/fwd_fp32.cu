@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
   int blk0 = 0;
   [[maybe_unused]] int prefix = 0;
   if constexpr (kScore) {
-    if (p.prefix != nullptr) prefix = p.prefix[b];
+    if (p.prefix != nullptr) prefix = score::prefix_of(p, b, skv);
     if (p.causal) skv = min(skv, max(p.qStart + sq, prefix));  // what is behind is nobody's
     nblk = (skv + kBC - 1) / kBC;
     if (p.tileRange != nullptr && p.blockKeys == kBC) {  // else they are the tensor-core kernel's, which has left the call to this one

@@ -601,7 +601,7 @@ __device__ __forceinline__ bool make_work(const P& p, int idx, W& w) {
         end[t] = nTotal;
         if (p.causal) {
           int see = p.qStart + w.qhi[t];
-          if (p.prefix != nullptr) see = max(see, p.prefix[b]);
+          if (p.prefix != nullptr) see = max(see, score::prefix_of(p, b, w.skv));
           end[t] = min(nTotal, (see - 1) / kBlockN + 1);
         }
       }
@@ -709,8 +709,9 @@ struct ScoreRow {
     seenByAll = seenByAllPos = p.qStart + qlo;
     const int b = (p.prefix != nullptr || p.docKV != nullptr) ? (int)(w.qRow0 / w.sq) : 0;
     if (p.prefix != nullptr) {
-      last = max(last, p.prefix[b] - 1);
-      seenByAll = max(seenByAll, p.prefix[b] - 1);
+      const int prefix = score::prefix_of(p, b, w.skv);
+      last = max(last, prefix - 1);
+      seenByAll = max(seenByAll, prefix - 1);
     }
     doc = -1;
     if (p.docKV != nullptr) {

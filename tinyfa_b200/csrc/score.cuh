@@ -33,6 +33,10 @@ struct ScoreFields {
 
 namespace score {
 
+// Prefix of batch entry b.  Any int may stand there: lengths below zero are none and those past the keys are all of them, which also keeps sums
+// with it inside 32 bits.
+__device__ __forceinline__ int prefix_of(const ScoreFields& f, long long b, int seqLenKV) { return min(max(f.prefix[b], 0), seqLenKV); }
+
 // tanh(t) / t = c0 + c1 t^2 + c2 t^4 + c3 t^6 for |t| <= 1/2, fitted to the smallest largest error of the tanh (1.3e-7)
 constexpr float kTanh0 = 0.9999976754188538f, kTanh1 = -0.33320656418800354f, kTanh2 = 0.13145145773887634f, kTanh3 = -0.04337248206138611f;
 

@@ -66,7 +66,7 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
     if (!finite(to_float(out[32 * i]))) spoilt |= 1u << i;
   }
   int end = s.seqLenKV;
-  if (s.causal) end = min(end, max(pos, f.prefix != nullptr ? f.prefix[b] - 1 : -1) + 1);
+  if (s.causal) end = min(end, max(pos, f.prefix != nullptr ? prefix_of(f, b, s.seqLenKV) - 1 : -1) + 1);
   if (!docs) {
     bool hidden = false;
     // (with a prefix, whose length only the device knows, the decode kernel reads all keys)
