@@ -57,3 +57,22 @@ def test_lowest_prefix_and_values_that_the_mask_hides(call):
     _compare(got[:1, :first], Q[:1, :first], K[:1], V[:1], True, prefix=prefix[:1], fp32_error=2.0 ** -19)
     _compare(got[1:], Q[1:], K[1:], V[1:], True, prefix=prefix[1:], fp32_error=2.0 ** -19)
     tfa.device_status()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,S,Hq,Hkv,D,fp32_tc", [("fp16", 300, 4, 2, 64, -1), ("bf16", 200, 2, 1, 128, -1), ("bf16", 140, 2, 1, 256, -1), ("fp32", 200, 2, 1, 64, 0),
+                                                       ("fp32", 200, 2, 1, 64, 1), ("fp32", 200, 1, 1, 256, 1)])
+def test_largest_document_id_beside_padding(dtype, S, Hq, Hkv, D, fp32_tc, causal):
+    """Padding belongs to no document, to the one with the largest id as little as to another."""
+    Q, K, V = _inputs(dtype, 3, S, S, Hq, Hkv, D, 3)
+    docs = torch.full((3, S), -1, dtype=torch.int32, device="cuda")
+    docs[0, : S // 2], docs[1, : S // 3], docs[1, S // 3: S // 2] = LARGEST, LARGEST - 1, LARGEST
+    docs[2, : S // 2], docs[2, S // 2 + 9:] = LARGEST, SMALLEST
+    tfa.set_option("fp32_tc", fp32_tc)
+    try:
+        got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=causal, doc_ids_q=docs, doc_ids_kv=docs)
+    finally:
+        tfa.set_option("fp32_tc", -1)
+    _compare(got, Q, K, V, causal, dq=docs, dk=docs, fp32_error=2.0 ** -19)
+    assert (got[docs < 0] == 0).all()
+    tfa.device_status()

@@ -55,8 +55,8 @@ namespace score {
 constexpr int kWarps = 8;
 constexpr int kScoreTileRows = 64, kScoreBlockKeys = 64;  // of the fp32 kernel; the tensor-core kernel has 128 >> packShift and 128
 
-// Ascending order puts negative ids (no document) last.
-__device__ __forceinline__ int order_of(int id) { return id < 0 ? INT_MAX : id; }
+// Ascending order puts negative ids (no document) last, behind the largest id that a document can have.
+__device__ __forceinline__ unsigned order_of(int id) { return id < 0 ? UINT_MAX : (unsigned)id; }
 
 // Smallest and largest document of every key block, a warp each, and whether its keys and the one before it are in ascending order.
 __global__ void __launch_bounds__(kWarps * 32) key_blocks_kernel(const int* docKV, int2* out, unsigned char* sorted, int seqLenKV, int blockKeys, int blocks,
@@ -144,16 +144,16 @@ __global__ void __launch_bounds__(kWarps * 32) tile_range_kernel(const int* docQ
       int from = k0, to = k1, from2 = k0, to2 = k1;  // first key not before the document, first behind it
       while (from < to || from2 < to2) {
         const int mid = (from + to) >> 1, mid2 = (from2 + to2) >> 1;
-        const int x = from < to ? order_of(ids[mid]) : 0, y = from2 < to2 ? order_of(ids[mid2]) : 0;
+        const unsigned x = from < to ? order_of(ids[mid]) : 0u, y = from2 < to2 ? order_of(ids[mid2]) : 0u;
         if (from < to) {
-          if (x < d) {
+          if (x < (unsigned)d) {
             from = mid + 1;
           } else {
             to = mid;
           }
         }
         if (from2 < to2) {
-          if (y <= d) {
+          if (y <= (unsigned)d) {
             from2 = mid2 + 1;
           } else {
             to2 = mid2;
