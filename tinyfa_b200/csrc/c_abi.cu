@@ -142,15 +142,29 @@ static int g_capturePairsUsed[64] = {0};
 // host does not know the packed tensors' row totals (patch_varlen_maps below).  Same sharing rule as the counters.
 static CUtensorMap* g_mapBlock[64] = {nullptr};
 
+// Device memory of zeros that kernels on any stream may use as soon as this returns.  cudaMemset would clear it on the default stream, behind
+// whatever is queued there, and streams that do not wait for that one could count with it before; so a stream of its own clears it and is
+// waited for.
+static int* zeroed_block(size_t bytes, const char* what) {
+  int* p = nullptr;
+  cudaStream_t s = nullptr;
+  cudaError_t e = cudaMalloc(&p, bytes);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, bytes, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (s != nullptr) cudaStreamDestroy(s);
+  if (e == cudaSuccess) return p;
+  set_error_string("could not allocate %s: %s", what, cudaGetErrorString(e));
+  (void)cudaGetLastError();
+  cudaFree(p);
+  return nullptr;
+}
+
 static int* device_block_locked(int device) {
   if (device < 0 || device >= 64) return nullptr;
   if (g_statusWord[device] == nullptr) {
-    int* p = nullptr;
-    const size_t bytes = sizeof(int) * (1 + 2 * (kStreamPairs + kCapturePairs));
-    if (cudaMalloc(&p, bytes) != cudaSuccess || cudaMemset(p, 0, bytes) != cudaSuccess) {
-      set_error_string("could not allocate the device status word: %s", cudaGetErrorString(cudaGetLastError()));
-      return nullptr;
-    }
+    int* p = zeroed_block(sizeof(int) * (1 + 2 * (kStreamPairs + kCapturePairs)), "the device status word");
+    if (p == nullptr) return nullptr;
     CUtensorMap* maps = nullptr;
     if (cudaMalloc(&maps, sizeof(CUtensorMap) * 3 * (kStreamPairs + kCapturePairs)) != cudaSuccess) {
       set_error_string("could not allocate the device tensor-map block: %s", cudaGetErrorString(cudaGetLastError()));
@@ -217,10 +231,8 @@ int* device_join_counters(int device, cudaStream_t stream, int* rc) {
   if (pair == nullptr) return nullptr;
   std::lock_guard<std::mutex> lock(g_devMutex);
   if (g_joinBlock[device] == nullptr) {
-    const size_t bytes = sizeof(int) * kJoinCounters * (kStreamPairs + kCapturePairs);
-    int* p = nullptr;
-    if (cudaMalloc(&p, bytes) != cudaSuccess || cudaMemset(p, 0, bytes) != cudaSuccess) {
-      set_error_string("could not allocate the arrival counters: %s", cudaGetErrorString(cudaGetLastError()));
+    int* p = zeroed_block(sizeof(int) * kJoinCounters * (kStreamPairs + kCapturePairs), "the arrival counters");
+    if (p == nullptr) {
       *rc = kCudaError;
       return nullptr;
     }
