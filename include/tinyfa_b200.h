@@ -211,8 +211,8 @@ int tfa_b200_kv_cache_store(const void* K, const void* V, void* kCache, void* vC
  * keys up to its own position, else all of the request's.  softcap and alibiSlopes as in tfa_b200_fwd_scored.  maxSeqLenQ / maxSeqLenKV
  * only size the launch.  Every row of O is written: rows of no request, of a request without tokens and rows in front of its first position
  * are zero.  Keys in blocks whose id is outside [0, numBlocks) are not seen;
- * cells behind a request's last token may hold anything.  The first call on a device allocates 16 MB of counters: not
- * under stream capture.  Captured calls allocate their partial results in the graph.
+ * cells behind a request's last token may hold anything.  Every stream and every captured call has arrival counters of its own, 4 KB that are
+ * allocated when they are needed first, under stream capture too.  Captured calls allocate their partial results in the graph.
  */
 int tfa_b200_fwd_cache(const void* Q, void* O, const void* kCache, const void* vCache, const float* kScales, const float* vScales,
                        const int* blockTable, const int* seqLens, const int* cuSeqLensQ, int dtype, int cacheType, int batchSize,

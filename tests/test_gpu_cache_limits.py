@@ -64,3 +64,37 @@ want = tfa.flash_attn_forward(Q, K, V, True)
 assert all(torch.equal(x, want) for x in got)
 tfa.device_status()
 """)
+
+
+@pytest.mark.parametrize("form", [0, 1])
+def test_first_call_of_a_process_under_capture(form):  # noqa: F811
+    _run(FIRST_USE.split("side = ")[0] + f"tfa.set_option('cache_tc', {form})" + """
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = tfa.flash_attn_cache_forward(*args)
+for _ in range(3):
+    got.zero_()
+    graph.replay()
+    want = tfa.flash_attn_cache_forward(*args)
+    assert want.abs().sum() > 0 and torch.equal(got, want)
+""")
+
+
+def test_more_captured_calls_than_the_work_counters_have_room_for():
+    """A decode graph for each batch size of a server and each layer of a model."""
+    cache = _cache("int8", [2500, 40], 2, 64, 64, 11)
+    lens, cu = torch.tensor([2500, 40], dtype=torch.int32, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda")
+    Q = torch.randn(2, 8, 64, device="cuda").half()
+    want = tfa.flash_attn_cache_forward(Q, *cache, lens, cu, 1, 2500)
+    graphs, held = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append([tfa.flash_attn_cache_forward(Q, *cache, lens, cu, 1, 2500) for _ in range(1700)])
+        graphs.append(graph)
+    for graph, outs in zip(graphs, held):
+        for _ in range(2):
+            graph.replay()
+        assert all(torch.equal(x, want) for x in outs)
+    assert torch.equal(tfa.flash_attn_cache_forward(Q, *cache, lens, cu, 1, 2500), want)
+    tfa.device_status()

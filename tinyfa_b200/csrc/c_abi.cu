@@ -16,6 +16,7 @@
 #include <mutex>
 #include <thread>
 #include <unordered_map>
+#include <vector>
 
 #include "../../include/tinyfa_b200.h"
 #include "build_config.cuh"
@@ -142,10 +143,18 @@ static int g_capturePairsUsed[64] = {0};
 // host does not know the packed tensors' row totals (patch_varlen_maps below).  Same sharing rule as the counters.
 static CUtensorMap* g_mapBlock[64] = {nullptr};
 
+// Allocations that take no part in a capture which this or another thread has under way.
+struct OutsideCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // Device memory of zeros that kernels on any stream may use as soon as this returns.  cudaMemset would clear it on the default stream, behind
 // whatever is queued there, and streams that do not wait for that one could count with it before; so a stream of its own clears it and is
 // waited for.
 static int* zeroed_block(size_t bytes, const char* what) {
+  const OutsideCapture outside;
   int* p = nullptr;
   cudaStream_t s = nullptr;
   cudaError_t e = cudaMalloc(&p, bytes);
@@ -166,6 +175,7 @@ static int* device_block_locked(int device) {
     int* p = zeroed_block(sizeof(int) * (1 + 2 * (kStreamPairs + kCapturePairs)), "the device status word");
     if (p == nullptr) return nullptr;
     CUtensorMap* maps = nullptr;
+    const OutsideCapture outside;
     if (cudaMalloc(&maps, sizeof(CUtensorMap) * 3 * (kStreamPairs + kCapturePairs)) != cudaSuccess) {
       set_error_string("could not allocate the device tensor-map block: %s", cudaGetErrorString(cudaGetLastError()));
       cudaFree(p);
@@ -222,24 +232,40 @@ int* device_work_counter(int device, cudaStream_t stream, int* rc, CUtensorMap**
 }
 
 // Arrival counters of the cache attention kernel, by which the parts of a unit that several runs share find out who comes last:
-// zero between launches (the last one puts its counter back), and never shared by launches that can run at the same time - a slot
-// of kJoinCounters for every counter pair above, with the same rule.
-constexpr int kJoinCounters = 1024;
-static int* g_joinBlock[64] = {nullptr};
+// zero between launches (the last one puts its counter back), and never shared by launches that can run at the same time - kJoinCounters of
+// them, more than a launch has CTAs, for every stream and for every captured call.  A server captures a decode graph for each batch size, with a
+// call for each layer: blocks of counters are added as they are needed, under capture too.
+constexpr int kJoinCounters = 1024, kJoinSlots = 64;  // of a call; calls' counters in a block
+static std::vector<int*> g_joinBlocks[64];
+static int g_joinUsed[64] = {0};
+static std::unordered_map<StreamKey, int, StreamKeyHash> g_streamJoin[64];
 int* device_join_counters(int device, cudaStream_t stream, int* rc) {
-  int* pair = device_work_counter(device, stream, rc, nullptr);
-  if (pair == nullptr) return nullptr;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &cap) != cudaSuccess) {
+    set_error_string("cudaStreamIsCapturing: %s", cudaGetErrorString(cudaGetLastError()));
+    *rc = kCudaError;
+    return nullptr;
+  }
+  const StreamKey key{stream, stream == cudaStreamPerThread ? std::this_thread::get_id() : std::thread::id()};
   std::lock_guard<std::mutex> lock(g_devMutex);
-  if (g_joinBlock[device] == nullptr) {
-    int* p = zeroed_block(sizeof(int) * kJoinCounters * (kStreamPairs + kCapturePairs), "the arrival counters");
+  int slot = g_joinUsed[device];
+  if (cap == cudaStreamCaptureStatusNone) {
+    const auto it = g_streamJoin[device].find(key);
+    if (it != g_streamJoin[device].end()) slot = it->second;
+  }
+  if (slot == (int)g_joinBlocks[device].size() * kJoinSlots) {
+    int* p = zeroed_block(sizeof(int) * kJoinCounters * kJoinSlots, "arrival counters");
     if (p == nullptr) {
       *rc = kCudaError;
       return nullptr;
     }
-    g_joinBlock[device] = p;
+    g_joinBlocks[device].push_back(p);
   }
-  const long long slot = (pair - (g_statusWord[device] + 1)) / 2;
-  return g_joinBlock[device] + slot * kJoinCounters;
+  if (slot == g_joinUsed[device]) {
+    g_joinUsed[device]++;
+    if (cap == cudaStreamCaptureStatusNone) g_streamJoin[device].emplace(key, slot);
+  }
+  return g_joinBlocks[device][slot / kJoinSlots] + slot % kJoinSlots * kJoinCounters;
 }
 
 // Completes the tensor maps of a packed variable-length launch on the device: the three maps arrive as kernel
@@ -315,6 +341,7 @@ static cudaMemPool_t scratch_pool(int device) {
     props.location.type = cudaMemLocationTypeDevice;
     props.location.id = device;
     cudaMemPool_t pool = nullptr;
+    const OutsideCapture outside;
     if (cudaMemPoolCreate(&pool, &props) != cudaSuccess) {
       cudaGetLastError();
       return nullptr;
