@@ -197,9 +197,10 @@ int tfa_b200_kv_cache_plan(int* blockTable, const int* seqLens, const int* newLe
  * Rows of K and V [totalNew, numHeadsKV, headDim] (dtype code) -> their slots of the cache.  A block's scale grows to what its new
  * rows need: scale <- max(scale, max |x| / 127 or / 448), codes = round(x / scale) with a new scale taken before it is rounded to the fp32
  * that is stored, and codes that were there before are rounded anew when it
- * grows; rows that begin at a block's first cell begin it, whatever its scale was.  Infinities become the largest code and NaN zero, and
- * neither counts for the scale.  Slots below 0 or past the cache are skipped.  The rows of one block have to follow one another, and no slot
- * may come twice (as tfa_b200_kv_cache_plan gives them): what such a call leaves in that block is undefined.
+ * grows; rows of which one goes to a block's first cell begin it, whatever its scale was, and what lies behind a call's first cell of a block is
+ * taken to be the call's.  Infinities become the largest code and NaN zero, and neither counts for the scale.  Slots below 0 or past the cache are
+ * skipped.  The rows of one block have to follow one another, in any order of their cells, and no slot may come twice (as
+ * tfa_b200_kv_cache_plan gives them): what another call leaves in that block is undefined.
  */
 int tfa_b200_kv_cache_store(const void* K, const void* V, void* kCache, void* vCache, float* kScales, float* vScales, const long long* slots,
                             int dtype, int cacheType, long long totalNew, int numBlocks, int numHeadsKV, int headDim, int blockTokens,

@@ -98,3 +98,30 @@ def test_more_captured_calls_than_the_work_counters_have_room_for():
         assert all(torch.equal(x, want) for x in outs)
     assert torch.equal(tfa.flash_attn_cache_forward(Q, *cache, lens, cu, 1, 2500), want)
     tfa.device_status()
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("what", ["begins", "grows"])
+def test_rows_of_a_block_in_any_order(code, what):
+    """Rows of a block follow one another, in whatever order of their cells: as if they came in ascending order."""
+    g = torch.Generator().manual_seed(13)
+    for block, D, dtype in ((16, 64, torch.float16), (128, 256, torch.float32), (64, 128, torch.bfloat16)):
+        n, Hkv = 40, 2
+        kc = torch.randint(-100, 101, (n, Hkv, block, D), device="cuda").float().to(CODE[code][0])
+        ks = torch.full((n, Hkv), 50.0 if what == "begins" else 1e-3, device="cuda")
+        runs = []
+        for blk in torch.randperm(n, generator=g).tolist()[:30]:
+            first = 0 if what == "begins" else int(torch.randint(1, block - 3, (1,), generator=g))
+            cells = torch.arange(first, int(torch.randint(first + 1, block + 1, (1,), generator=g)))
+            cells = cells[torch.randperm(len(cells), generator=g)]
+            if what == "begins" and len(cells) > 1 and cells[0] == 0:
+                cells = cells.flip(0)
+            runs.append(blk * block + cells)
+        slots = torch.cat(runs).cuda()
+        rise = torch.cat([r.argsort() + sum(map(len, runs[:i])) for i, r in enumerate(runs)]).cuda()
+        K = torch.randn(len(slots), Hkv, D, device="cuda").to(dtype)
+        want = _store_by_hand(K[rise], kc, ks, slots[rise], code)
+        vc, vs = kc.clone(), ks.clone()
+        tfa.kv_cache_store(K, K.clone(), kc, vc, ks, vs, slots)
+        assert torch.equal(ks.cpu(), want[1]) and torch.equal(kc.float().cpu(), want[0])
+        assert torch.equal(kc.view(torch.uint8), vc.view(torch.uint8)) and torch.equal(ks, vs)

@@ -109,8 +109,9 @@ def kv_cache_store(K, V, k_cache, v_cache, k_scales, v_scales, slots):
     """Writes rows of K and V [total, Hkv, D] (fp16, bf16, fp32) into their slots (int64 [total], -1: nowhere) of the cache, in place.
 
     The scale of a block and head grows to what its new rows need, max |x| / 127 (int8) or / 448 (e4m3); when it grows, codes that were in the
-    block before are rounded anew.  Rows that begin at a block's first cell begin the block, whatever its scale was.  Infinities become the
-    largest code and NaN zero.  The rows of one block follow one another and no slot comes twice, as kv_cache_plan gives them.
+    block before - in front of the first cell that the call writes - are rounded anew.  Rows of which one goes to a block's first cell begin the
+    block, whatever its scale was.  Infinities become the largest code and NaN zero.  The rows of one block follow one another, in any order
+    of their cells, and no slot comes twice, as kv_cache_plan gives them.
     """
     shape, dtype, device = _rows_shape(K, "K", "[total, numHeadsKV, headDim]")
     code = _dtype_code(K, "kv_cache_store")

@@ -380,7 +380,8 @@ struct Largest<__half> : LargestPair<__half2, __half> {};
 template <>
 struct Largest<__nv_bfloat16> : LargestPair<__nv_bfloat162, __nv_bfloat16> {};
 
-// One head of K or V (blockIdx.z) and rowsPerCta rows; the CTA that has the first row of a run of rows in one block does the run.
+// One head of K or V (blockIdx.z) and rowsPerCta rows; the CTA that has the first row of a run of rows in one block does the run, whose cells may
+// come in any order; what is below the lowest of them was in the block before.
 //   need = max |x| / largest code over the run's finite values;  scale' = max(scale before, need);  code = round(x / scale'),
 // and codes that were in the block before are rounded anew where the scale grew: code' = round(code * scale / scale').  A run that begins
 // at the block's first cell begins the block: what its scale was before says nothing.  Bound by memory (the rows once, the codes once;
@@ -391,6 +392,7 @@ __global__ void __launch_bounds__(kStoreThreads) store_kernel(const StoreParams 
   constexpr int kChunks = D / 8, kWarps = kStoreThreads / 32;
   constexpr int kKept = 8;  // eights of a run that a thread keeps between the two looks: 64 rows of 128 elements; longer runs are read again
   __shared__ float sMax[kWarps];
+  __shared__ int sEnd[kWarps], sLowest[kWarps];
   __shared__ int sCells[kStoreThreads];  // cells of the run's rows
   const int h = blockIdx.y, which = blockIdx.z, lane = threadIdx.x & 31;
   const int blockTokens = 1 << p.blockShift;
@@ -415,21 +417,29 @@ __global__ void __launch_bounds__(kStoreThreads) store_kernel(const StoreParams 
     const long long r = r0 + from;
     const int block = __shfl_sync(0xffffffffu, mine, from);
     // the run ends with the first row of another block; more rows than the block has cells only if a cell comes twice
-    __syncthreads();  // the run before may still read sCells and sMax
+    __syncthreads();  // the run before may still read sCells, sEnd and sMax
     bool other = (int)threadIdx.x >= blockTokens;
+    int cell = blockTokens;
     if (!other) {
       other = block_of(r + threadIdx.x) != block;
-      sCells[threadIdx.x] = other ? -1 : (int)(p.slots[r + threadIdx.x] & (blockTokens - 1));
+      cell = other ? -1 : (int)(p.slots[r + threadIdx.x] & (blockTokens - 1));
+      sCells[threadIdx.x] = cell;
     }
     // kStoreThreads rows are looked at, and a run has blockTokens <= kStoreThreads at most
     const unsigned others = __ballot_sync(0xffffffffu, other);
-    if (lane == 0) sMax[threadIdx.x >> 5] = __int_as_float(others != 0 ? (int)(threadIdx.x & ~31) + __ffs(others) - 1 : kStoreThreads);
+    const int mineEnd = others != 0 ? __ffs(others) - 1 : 32;  // lanes of the run, where it gets as far as this warp
+    const int lowest = __reduce_min_sync(0xffffffffu, lane < mineEnd ? cell : blockTokens);
+    if (lane == 0) {
+      sEnd[threadIdx.x >> 5] = others != 0 ? (int)(threadIdx.x & ~31) + mineEnd : kStoreThreads;
+      sLowest[threadIdx.x >> 5] = lowest;
+    }
     __syncthreads();
-    int n = kStoreThreads;
+    int n = kStoreThreads, first = blockTokens;  // rows of the run and its first cell: rows may come in any order of their cells
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) n = min(n, __float_as_int(sMax[w]));
-    const int first = sCells[0], items = n * kChunks;
-    __syncthreads();  // sMax is written again
+    for (int w = 0; w < kWarps; w++) n = min(n, sEnd[w]);
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) first = w * 32 < n ? min(first, sLowest[w]) : first;
+    const int items = n * kChunks;
     Eight<T> kept[kKept];
     auto at = [&](int i) { return x + (r + i / kChunks) * rowStride + i % kChunks * 8; };
     // maximum over the CTA's threads of a number that is not negative
