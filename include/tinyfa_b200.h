@@ -186,7 +186,7 @@ int tfa_b200_fwd_scored(const void* Q, const void* K, const void* V, void* O, in
  * blocks would not all be there, counting every request ahead of it, or that would need more than maxBlocks, gets none: its length stays
  * and its rows have slot -1.  blockTable and freeBlocks are updated in place; written are
  *   cuSeqLens [batchSize + 1]: prefix sums of newLens;  slots int64 [totalNew]: the slot of every packed row, -1 behind the last request;
- *   seqLensAfter [batchSize];  *numFreeAfter.
+ *   seqLensAfter [batchSize], which may not overlap seqLens;  *numFreeAfter.
  * totalNew is the row count of the packed tensors, at least the sum of newLens (rows past it get no slot).
  */
 int tfa_b200_kv_cache_plan(int* blockTable, const int* seqLens, const int* newLens, const unsigned char* finished, int* freeBlocks,

@@ -7,6 +7,7 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <float.h>
+#include <stdint.h>
 
 #include <type_traits>
 
@@ -599,6 +600,12 @@ extern "C" int tfa_b200_kv_cache_plan(int* blockTable, const int* seqLens, const
       (batchSize > 0 && (seqLens == nullptr || newLens == nullptr || seqLensAfter == nullptr)) ||
       (batchSize > 0 && maxBlocks > 0 && blockTable == nullptr) || (freeCapacity > 0 && freeBlocks == nullptr)) {
     set_error_string("null pointer");
+    return kBadArgument;
+  }
+  // slots are worked out from the lengths before and after
+  const uintptr_t before = reinterpret_cast<uintptr_t>(seqLens), after = reinterpret_cast<uintptr_t>(seqLensAfter), bytes = sizeof(int) * (uintptr_t)batchSize;
+  if (batchSize > 0 && before < after + bytes && after < before + bytes) {
+    set_error_string("seqLens and seqLensAfter overlap");
     return kBadArgument;
   }
   int rc = check_device();
