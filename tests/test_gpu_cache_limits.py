@@ -101,6 +101,24 @@ def test_more_captured_calls_than_the_work_counters_have_room_for():
 
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_smallest_scales(code, form):  # noqa: F811
+    """Scales that kv_cache_store writes for the smallest values, alone, and beside blocks of zeros and of 2^-120."""
+    lens, new = [400, 90, 300], [3, 1, 70]
+    for kind in ("alone", "mixed"):
+        cache = _cache(code, lens, 2, 64, 16, 12)
+        vs = cache[3]
+        vs.fill_(2.0 ** -126)
+        if kind == "mixed":
+            vs[::3] = 2.0 ** -120
+            vs[1::5] = 0.0
+        Q = torch.randn(sum(new), 4, 64, device="cuda").bfloat16()
+        cu = torch.tensor([0, 3, 4, 74], dtype=torch.int32, device="cuda")
+        got = tfa.flash_attn_cache_forward(Q, *cache, torch.tensor(lens, dtype=torch.int32, device="cuda"), cu, 70, 400)
+        _expect(got, Q, cache, lens, new)
+    tfa.device_status()
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("what", ["begins", "grows"])
 def test_rows_of_a_block_in_any_order(code, what):
     """Rows of a block follow one another, in whatever order of their cells: as if they came in ascending order."""

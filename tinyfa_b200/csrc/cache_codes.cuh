@@ -24,6 +24,10 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
   }
 }
+// Sums over V refer to a scale of V that is no smaller than this: 2^4 times its reciprocal is a float, and 2^-4 of it almost a normal one (scales go
+// down to 2^-126).
+constexpr float kSmallestVRef = 1e-37f;
+
 // Rows of queries become fp16 with a power of two taken out, which brings the row's largest element into [2^13, 2^14): what is lost lies
 // 2^-31 below that element.  `largest`: exponent bits of the largest element, in place; the factors stay
 // inside what a float's exponent holds.

@@ -622,10 +622,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NR>()) cache_decode_k
         for (int e = 0; e < 4; e++) move = move || sc[nr][e] > limit[nr][e & 1];
       }
       if (__any_sync(0xffffffffu, move)) {
-        const float vNew = fmaxf(vRef, vs);
+        const float vNew = fmaxf(fmaxf(vRef, vs), kSmallestVRef);
         const float fv = vNew > vRef ? vRef / vNew : 1.f;
         vRef = vNew;
-        vUp = vNew > 0.f ? fminf(1.f / vNew, 1e37f) * kUp : 0.f;
+        vUp = 1.f / vNew * kUp;
 #pragma unroll
         for (int nr = 0; nr < NR; nr++) {
 #pragma unroll

@@ -1382,8 +1382,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         m = mNew;
         if constexpr (kCache) {
           if (vGrow) {
-            vRef = vMax;
-            vInv = vMax > 0.f ? fminf(1.f / vMax, 4e37f) * kCacheUp : 0.f;
+            vRef = fmaxf(vMax, kSmallestVRef);
+            vInv = 1.f / vRef * kCacheUp;
           }
         }
 
