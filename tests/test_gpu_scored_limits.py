@@ -76,3 +76,11 @@ def test_largest_document_id_beside_padding(dtype, S, Hq, Hkv, D, fp32_tc, causa
     _compare(got, Q, K, V, causal, dq=docs, dk=docs, fp32_error=2.0 ** -19)
     assert (got[docs < 0] == 0).all()
     tfa.device_status()
+
+
+def test_positions_that_a_c_int_does_not_hold():
+    Q, K, V = _inputs("fp16", 1, 8, 20, 2, 1, 64, 5)
+    f = tfa.flash_attn_scored_forward
+    for q_start in (2 ** 31, 2 ** 32 + 5, 2 ** 64 + 3):
+        with pytest.raises(RuntimeError, match="q_start"):
+            f(Q, K, V, is_causal=True, q_start=q_start)

@@ -233,7 +233,7 @@ def flash_attn_scored_forward(Q, K, V, is_causal=False, softcap=0.0, alibi_slope
         _check_fixed(Q, K, V)
         raise RuntimeError("flash_attn_scored_forward: unsupported input")
     _check_no_grad(Q, K, V, alibi_slopes)
-    _check(isinstance(q_start, int) and q_start >= 0, "q_start must be an integer >= 0")
+    _check(isinstance(q_start, int) and 0 <= q_start < 2 ** 31, "q_start must be an integer >= 0 and below 2^31")  # (a C int would keep its low bits)
     _check_softcap(softcap)
     device, slopes, prefix, docs_q, docs_kv = Q.get_device(), None, None, None, None
     if alibi_slopes is not None:

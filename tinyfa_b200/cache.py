@@ -155,7 +155,8 @@ def flash_attn_cache_forward(Q, k_cache, v_cache, k_scales, v_scales, block_tabl
     slopes = _aux(alibi_slopes, "alibi_slopes", torch.float32, (shape[1],), device) if alibi_slopes is not None else None
     _check_softcap(softcap)
     _check_no_grad(Q, alibi_slopes)
-    sizes = (batch, int(max_seqlen_q), int(max_seqlen_kv), shape[0], cache[0], width, cache[2], shape[1], cache[1], shape[2])
+    most_q, most_kv = min(int(max_seqlen_q), 2 ** 31 - 1), min(int(max_seqlen_kv), 2 ** 31 - 1)  # (a C int would keep their low bits)
+    sizes = (batch, most_q, most_kv, shape[0], cache[0], width, cache[2], shape[1], cache[1], shape[2])
     if _current_device() == device:
         return _run_cache(Q, k_cache, v_cache, k_scales, v_scales, table, lens, cu, code, kind, sizes, is_causal, softcap, slopes, device)
     with torch.cuda.device(device):
