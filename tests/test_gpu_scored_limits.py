@@ -84,3 +84,13 @@ def test_positions_that_a_c_int_does_not_hold():
     for q_start in (2 ** 31, 2 ** 32 + 5, 2 ** 64 + 3):
         with pytest.raises(RuntimeError, match="q_start"):
             f(Q, K, V, is_causal=True, q_start=q_start)
+
+
+def test_caps_below_and_above_what_fp32_holds(call):
+    """A cap of next to nothing leaves all scores equal, one far above them leaves them as they are."""
+    dtype, Sq, Skv, Hq, Hkv, D = call
+    Q, K, V = _inputs(dtype, 2, Sq, Skv, Hq, Hkv, D, 6)
+    got = tfa.flash_attn_scored_forward(Q, K, V, softcap=1e-60)
+    _compare(got, Q * 0, K, V, False, fp32_error=2.0 ** -19)
+    got = tfa.flash_attn_scored_forward(Q, K, V, softcap=1e60)
+    _compare(got, Q, K, V, False, fp32_error=2.0 ** -19)

@@ -197,8 +197,10 @@ def _aux(x, name, dtype, shape, device):
     return x.data_ptr()
 
 
-def _check_softcap(softcap):
+def _usable_softcap(softcap):
+    """A cap that fp32 holds: 1e-50 would become 0, which is none, and 1e50 infinite.  Beyond these bounds a cap changes no result."""
     _check(0.0 <= softcap < float("inf"), "softcap must be 0 (none) or a positive finite number")
+    return min(max(float(softcap), 1e-30), 1e30) if softcap > 0 else 0.0
 
 
 def _run_scored(lib, device, Q, K, V, code, q_shape, kv_shape, is_causal, q_start, softcap, slopes, prefix, docs_q, docs_kv):
@@ -234,7 +236,7 @@ def flash_attn_scored_forward(Q, K, V, is_causal=False, softcap=0.0, alibi_slope
         raise RuntimeError("flash_attn_scored_forward: unsupported input")
     _check_no_grad(Q, K, V, alibi_slopes)
     _check(isinstance(q_start, int) and 0 <= q_start < 2 ** 31, "q_start must be an integer >= 0 and below 2^31")  # (a C int would keep its low bits)
-    _check_softcap(softcap)
+    softcap = _usable_softcap(softcap)
     device, slopes, prefix, docs_q, docs_kv = Q.get_device(), None, None, None, None
     if alibi_slopes is not None:
         slopes = _aux(alibi_slopes, "alibi_slopes", torch.float32, (q_shape[2],), device)

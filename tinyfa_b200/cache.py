@@ -12,7 +12,7 @@ Checks, streams, devices and errors as in api.py; nothing is copied to the host.
 import torch
 
 from . import _lib
-from .api import (_aux, _check, _check_input, _check_no_grad, _check_softcap, _current_device, _dtype_code, _fits, _raw_stream)
+from .api import (_aux, _check, _check_input, _check_no_grad, _current_device, _dtype_code, _fits, _raw_stream, _usable_softcap)
 
 _CACHE_CODE = {torch.int8: 1, torch.float8_e4m3fn: 2}
 _BLOCK_TOKENS = (16, 32, 64, 128)
@@ -153,7 +153,7 @@ def flash_attn_cache_forward(Q, k_cache, v_cache, k_scales, v_scales, block_tabl
     lens = _aux(seq_lens, "seq_lens", torch.int32, (batch,), device)
     cu = _aux(cu_seqlens_q, "cu_seqlens_q", torch.int32, (batch + 1,), device)
     slopes = _aux(alibi_slopes, "alibi_slopes", torch.float32, (shape[1],), device) if alibi_slopes is not None else None
-    _check_softcap(softcap)
+    softcap = _usable_softcap(softcap)
     _check_no_grad(Q, alibi_slopes)
     most_q, most_kv = min(int(max_seqlen_q), 2 ** 31 - 1), min(int(max_seqlen_kv), 2 ** 31 - 1)  # (a C int would keep their low bits)
     sizes = (batch, most_q, most_kv, shape[0], cache[0], width, cache[2], shape[1], cache[1], shape[2])
