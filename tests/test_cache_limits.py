@@ -2,8 +2,10 @@
 import ctypes
 
 import pytest
+import torch
+from torch.autograd import forward_ad
 
-from tinyfa_b200 import _lib
+from tinyfa_b200 import _lib, api
 
 
 @pytest.fixture(scope="module")
@@ -22,3 +24,17 @@ def test_plan_lengths_that_overlap(p):
 
     for before, after in ((p + 3200, p + 3200), (p + 3200, p + 3212), (p + 3212, p + 3200)):
         assert call(before, after) == 3 and "overlap" in _lib.last_error()
+
+
+def test_gradients_of_either_mode():
+    x, y = torch.randn(3), torch.randn(3)
+    api._check_no_grad(x, None, y)
+    with pytest.raises(RuntimeError, match="forward only"):
+        api._check_no_grad(x, y.clone().requires_grad_())
+    with forward_ad.dual_level():
+        api._check_no_grad(x, y)
+        with pytest.raises(RuntimeError, match="forward only"):
+            api._check_no_grad(x, forward_ad.make_dual(y, x))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward only"):
+            api._check_no_grad(forward_ad.make_dual(x, y))
+    api._check_no_grad(x, y)

@@ -145,6 +145,19 @@ def test_rows_of_a_block_in_any_order(code, what):
         assert torch.equal(kc.view(torch.uint8), vc.view(torch.uint8)) and torch.equal(ks, vs)
 
 
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    cache = _cache("int8", [20], 1, 64, 16)
+    one, cu = torch.tensor([20], dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    Q, K = torch.randn(1, 2, 64, device="cuda").half(), torch.randn(1, 1, 64, device="cuda").half()
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward only"):
+            tfa.flash_attn_cache_forward(fwd.make_dual(Q, Q), *cache, one, cu, 1, 20)
+        with pytest.raises(RuntimeError, match="forward only"):
+            tfa.kv_cache_store(K, fwd.make_dual(K.clone(), K), *cache[:4], torch.tensor([3], device="cuda"))
+
+
 def test_maxima_that_a_c_int_does_not_hold(form):  # noqa: F811
     cache = _cache("int8", [300], 2, 64, 16, 14)
     one, cu = torch.tensor([300], dtype=torch.int32, device="cuda"), torch.tensor([0, 2], dtype=torch.int32, device="cuda")

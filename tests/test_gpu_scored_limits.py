@@ -94,3 +94,18 @@ def test_caps_below_and_above_what_fp32_holds(call):
     _compare(got, Q * 0, K, V, False, fp32_error=2.0 ** -19)
     got = tfa.flash_attn_scored_forward(Q, K, V, softcap=1e60)
     _compare(got, Q, K, V, False, fp32_error=2.0 ** -19)
+
+
+def test_tangents_are_refused():
+    """Forward-mode gradients are not dropped either."""
+    import torch.autograd.forward_ad as fwd
+
+    Q, K, V = _inputs("fp16", 1, 8, 8, 2, 1, 64, 8)
+    with fwd.dual_level():
+        dual = fwd.make_dual(Q, torch.ones_like(Q))
+        with pytest.raises(RuntimeError, match="forward only"):
+            tfa.flash_attn_scored_forward(dual, K, V)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward only"):
+            tfa.flash_attn_scored_forward(Q, K, fwd.make_dual(V, torch.ones_like(V)))
+        want = tfa.flash_attn_scored_forward(Q, K, V)
+        assert torch.equal(tfa.flash_attn_scored_forward(fwd.unpack_dual(dual).primal, K, V), want)

@@ -8,6 +8,7 @@ torch's current stream.  One addition: the call runs under a device guard for Q'
 reference launches on whichever device is current).
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -168,10 +169,13 @@ def flash_attn_varlen_forward(Q, K, V, cu_seqlens_q, cu_seqlens_kv, max_seqlen_q
 
 
 def _check_no_grad(*tensors):
-    """These operators have no backward pass: better an error than gradients that are silently missing."""
+    """These operators have no gradients, in either mode: better an error than gradients or tangents that are silently missing."""
     if torch.is_grad_enabled():
         for t in tensors:
             _check(not (t is not None and t.requires_grad), "forward only: call under torch.no_grad(), or on tensors that do not require gradients")
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # inside a dual level
+        for t in tensors:
+            _check(t is None or forward_ad.unpack_dual(t).tangent is None, "forward only: call on the primals of dual tensors")
 
 
 def _fits(x, dtype, shape, device):
