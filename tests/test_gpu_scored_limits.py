@@ -78,6 +78,24 @@ def test_largest_document_id_beside_padding(dtype, S, Hq, Hkv, D, fp32_tc, causa
     tfa.device_status()
 
 
+@pytest.mark.parametrize("q_start", [5000, 2 ** 24 + 3, 2 ** 30 + 1])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("cap", [0.0, 3.0])
+def test_distances_from_far_positions(call, q_start, causal, cap):
+    """All keys lie to the left of every row: |p - j| is (p - Skv + 1) + (Skv - 1 - j), and what all scores of a row share is nothing to its weights.
+    So the rows are those of position Skv - 1 with every key visible, in 64 bits too, and distances are as exact as there."""
+    dtype, Sq, Skv, Hq, Hkv, D = call
+    Q, K, V = _inputs(dtype, 2, Sq, Skv, Hq, Hkv, D, 4)
+    slopes = _slopes(Hq)
+    got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=causal, softcap=cap, alibi_slopes=slopes, q_start=q_start)
+    see = torch.ones(Sq, Skv, dtype=torch.bool, device="cuda")
+    distance = (Skv - 1 - torch.arange(Skv, device="cuda", dtype=torch.float64)).expand(Sq, Skv)
+    for b in range(2):
+        o, off, a = attend(Q[b].double(), K[b].double(), V[b].double(), see, cap, slopes, distance, 2.0 ** -19 if dtype == "fp32" else 8.6e-5)
+        check(got[b], o, off, a, U[Q.dtype], Skv * 2.0 ** -25 * V[b].abs().max().item() if dtype == "fp16" else 0.0)
+    tfa.device_status()
+
+
 def test_positions_that_a_c_int_does_not_hold():
     Q, K, V = _inputs("fp16", 1, 8, 20, 2, 1, 64, 5)
     f = tfa.flash_attn_scored_forward

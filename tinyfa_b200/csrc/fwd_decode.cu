@@ -446,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
       }
       if constexpr (kScore) {
         const int posA = p.qStart + qposA, posB = p.qStart + qposB;
+        const int fromA = score::bias_position(posA, p.seqLenKV), fromB = score::bias_position(posB, p.seqLenKV);
         int limA = keyEnd, limB = keyEnd;
         if (p.causal) {
           const int prefix = p.prefix != nullptr ? score::prefix_of(p, b, p.seqLenKV) : 0;
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
           for (int e = 0; e < 4; e++) {
             const int key = kb + n * 8 + 2 * tig + (e & 1);
             float x = sc[n][e];
-            if (p.slopes != nullptr) x = fmaf(e < 2 ? -slopeA : -slopeB, fabsf((float)((e < 2 ? posA : posB) - key)), x);
+            if (p.slopes != nullptr) x = fmaf(e < 2 ? -slopeA : -slopeB, fabsf((float)((e < 2 ? fromA : fromB) - key)), x);
             sc[n][e] = key < (e < 2 ? limA : limB) ? x : -INFINITY;
           }
         }

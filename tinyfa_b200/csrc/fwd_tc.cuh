@@ -692,7 +692,7 @@ struct ScoreRow {
   int last;        // last key that the causal mask (with the prefix) leaves to the row
   int seenByAll;   // ... to every row of the tile
   int seenByAllPos;  // position of the tile's first row
-  int pos;         // position of the row
+  int pos;         // position of the row, for the bias
   int docLo, docHi;  // keys of its document where they lie side by side; docLo below zero: by their ids
   int doc;         // its document; below zero: none
   float slope;     // log2(e) x slope of its head
@@ -725,6 +725,7 @@ struct ScoreRow {
         docHi = keys.y;
       }
     }
+    pos = score::bias_position(pos, w.skv);
     if constexpr ((kScore & kScoreBias) != 0) slope = qpos < w.sq ? p.slopes[head] * 1.44269504f : 0.f;
     if constexpr ((kScore & kScoreCap) != 0) {
       capArg = 2.f * p.scaleLog2 / p.cap;

@@ -89,6 +89,7 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
     if (!__any_sync(0xffffffffu, hidden)) return;
   }
   const int doc = docs ? f.docQ[row] : 0;
+  const int from = bias_position(pos, s.seqLenKV);
   const float scale = rsqrtf((float)D), slope = f.slopes != nullptr ? f.slopes[head] : 0.f;
 #pragma unroll 1
   for (int k0 = (end - 1) / 32 * 32; k0 >= 0; k0 -= 32) {
@@ -104,7 +105,7 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
       for (int d = 0; d < D / kPer; d++) x = dot16<T>(reinterpret_cast<const uint4*>(q)[d], k16[d], x);
       x *= scale;
       if (f.cap > 0.f) x = f.cap * tanhf(x / f.cap);
-      x = fmaf(-slope, fabsf((float)(pos - key)), x) * 1.44269504f;
+      x = fmaf(-slope, fabsf((float)(from - key)), x) * 1.44269504f;
     }
     float most = fmaxf(m, x);
 #pragma unroll
