@@ -127,3 +127,25 @@ def test_tangents_are_refused():
             tfa.flash_attn_scored_forward(Q, K, fwd.make_dual(V, torch.ones_like(V)))
         want = tfa.flash_attn_scored_forward(Q, K, V)
         assert torch.equal(tfa.flash_attn_scored_forward(fwd.unpack_dual(dual).primal, K, V), want)
+
+
+def test_rows_that_take_long_to_compute_again():
+    """A value that the mask hides from rows with very many keys: the other warps wait for as long as the rows take, which is more than a
+    wait without any progress may last."""
+    Sq, Skv, D = 40000, 6_000_000, 32
+    g = torch.Generator(device="cuda").manual_seed(9)
+    Q, K, V = (torch.randn(1, n, 1, D, device="cuda", generator=g).bfloat16() for n in (Sq, Skv, Skv))
+    V += 1
+    q_start = Skv - Sq
+    bad = q_start + 20 * 128 + 100  # hidden from the hundred rows before it in its block
+    V2 = V.clone()
+    V2[0, bad, 0, 5] = math.nan
+    got = tfa.flash_attn_scored_forward(Q, K, V2, is_causal=True, softcap=2.0, q_start=q_start)
+    tfa.device_status()
+    n = bad - q_start
+    assert torch.isfinite(got[:, :n]).all() and not torch.isfinite(got[:, n:, :, 5]).any()
+    for r in (0, n - 100, n - 50, n - 1):
+        i = q_start + r
+        see, dist = visible(1, i + 1, True, i)
+        o, off, a = attend(Q[0, r:r + 1].double(), K[0, :i + 1].double(), V[0, :i + 1].double(), see, 2.0, None, dist)
+        check(got[0, r:r + 1], o, off, a, U[torch.bfloat16])

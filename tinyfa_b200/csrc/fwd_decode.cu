@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
 #pragma unroll 1
       for (; spoilt != 0u; spoilt &= spoilt - 1) {
         const int r = __ffs(spoilt) - 1;
-        score::exact_row<Element<kBf16>, D>(p, qRow0 + r / p.group, hkv * p.group + r % p.group, p.O);
+        score::exact_row<Element<kBf16>, D, false>(p, qRow0 + r / p.group, hkv * p.group + r % p.group, p.O);
       }
     }
   };
@@ -632,7 +632,7 @@ combine_kernel(const float* partO, const float* partLse, void* O, long long rows
       if (threadIdx.x < 32) {
         bool bad = false;
         for (int i = threadIdx.x; i < kVec; i += 32) bad |= sBad[i];
-        if (__any_sync(0xffffffffu, bad)) score::exact_row<Element<kBf16>, D>(fields, row / headsQ, (int)(row % headsQ), O);
+        if (__any_sync(0xffffffffu, bad)) score::exact_row<Element<kBf16>, D, false>(fields, row / headsQ, (int)(row % headsQ), O);
       }
     }
     if (r + (int)gridDim.x < nRows) __syncthreads();  // sAcc is written again
@@ -688,7 +688,7 @@ combine_parts_kernel(const float* partO, const float* partLse, void* O, long lon
     if (kScore) bad = wsum > 0.f && wsum < INFINITY && !(fabsf(acc.x + acc.y + acc.z + acc.w) < INFINITY);
   }
   if constexpr (kScore) {
-    if (__syncthreads_or(bad)) score::exact_rows<Element<kBf16>, D>(fields, bad, row / headsQ, (int)(row % headsQ), O);
+    if (__syncthreads_or(bad)) score::exact_rows<Element<kBf16>, D, false>(fields, bad, row / headsQ, (int)(row % headsQ), O);
   }
 }
 

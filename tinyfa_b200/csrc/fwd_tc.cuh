@@ -33,6 +33,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <stddef.h>
+
 #include <type_traits>
 
 #include "cache_codes.cuh"
@@ -313,26 +315,36 @@ struct Ctl {
   int failed;
   WorkSlot work[2];
   int peerIdx[2];  // pair form, rank 1: work indices handed over by rank 0
+  int rowsAgain;   // scored calls: rows that were computed again
 };
+static_assert(sizeof(Ctl) <= 2048, "control block");
 
 struct WaitCtx {
   volatile int* failed;
   int* status;
   int epoch;
 };
+// ... where warps may have to compute rows again (score_row.cuh), for as long as those rows take: Ctl::rowsAgain changes with every one of them, and
+// a wait lasts while it does.
+struct WaitCtxRows : WaitCtx {};
+__device__ __forceinline__ int rows_again(const WaitCtx&) { return 0; }
+__device__ __forceinline__ int rows_again(const WaitCtxRows& c) { return c.failed[((int)offsetof(Ctl, rowsAgain) - (int)offsetof(Ctl, failed)) / (int)sizeof(int)]; }
 
 // Bounded wait: gives up after ~2 s, records (epoch << 8 | site) and lets the caller continue so that
 // every loop still terminates; later waits of the CTA return at once.
-__device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity, const WaitCtx& c, int site) {
+template <class Ctx>
+__device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity, const Ctx& c, int site) {
   if (ptx::mbar_try_wait(bar, parity)) return;
   uint32_t spins = 0;
   uint64_t t0 = 0;
+  int rows = 0;
   while (!ptx::mbar_try_wait(bar, parity)) {
     if ((++spins & 0x3FF) == 0) {
       if (*c.failed) return;
       const uint64_t now = ptx::global_timer_ns();
-      if (t0 == 0) {
+      if (t0 == 0 || rows_again(c) != rows) {
         t0 = now;
+        rows = rows_again(c);
       } else if (now - t0 > 2000000000ull) {
         *c.failed = 1;
         atomicExch(c.status, (c.epoch << 8) | site);
@@ -364,16 +376,19 @@ __device__ __forceinline__ void wait_bar_cluster(uint32_t bar, uint32_t parity, 
 
 // Same contract as wait_bar, polling with the non-blocking test_wait: lower wake-up latency, at the price of
 // issue slots - used only by the single-thread MMA issuers, whose reaction time is on the critical path.
-__device__ __forceinline__ void spin_bar(uint32_t bar, uint32_t parity, const WaitCtx& c, int site) {
+template <class Ctx>
+__device__ __forceinline__ void spin_bar(uint32_t bar, uint32_t parity, const Ctx& c, int site) {
   if (ptx::mbar_test_wait(bar, parity)) return;
   uint32_t spins = 0;
   uint64_t t0 = 0;
+  int rows = 0;
   while (!ptx::mbar_test_wait(bar, parity)) {
     if ((++spins & 0x3FFF) == 0) {
       if (*c.failed) return;
       const uint64_t now = ptx::global_timer_ns();
-      if (t0 == 0) {
+      if (t0 == 0 || rows_again(c) != rows) {
         t0 = now;
+        rows = rows_again(c);
       } else if (now - t0 > 2000000000ull) {
         *c.failed = 1;
         atomicExch(c.status, (c.epoch << 8) | site);
@@ -935,11 +950,11 @@ struct ScoreRow {
 
 // Rows of a tile that V has spoilt from a masked place.  Partial results: the kernel that joins them looks.
 template <bool kBf16, int kHD, class P, class W>
-__device__ __forceinline__ void exact_rows_of_tile(const P& p, const W& w, int t, bool bad, int qpos, int head) {
+__device__ __forceinline__ void exact_rows_of_tile(const P& p, const W& w, int t, bool bad, int qpos, int head, int* rowsAgain) {
   if constexpr (std::is_base_of<TcPartParams, P>::value) {
     if (!whole_tile(p, w, t)) return;
   }
-  score::exact_rows<typename std::conditional<kBf16, __nv_bfloat16, __half>::type, kHD>(p, bad, w.qRow0 + qpos, head, p.O);
+  score::exact_rows<typename std::conditional<kBf16, __nv_bfloat16, __half>::type, kHD>(p, bad, w.qRow0 + qpos, head, p.O, rowsAgain);
 }
 
 // ---- kModeCache
@@ -1019,6 +1034,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   constexpr int NT = C::kNT;
   // warp roles: softmax warps [0, 4 * NT'), epilogue warps, the two MMA-issuing warps, the loading warp
   constexpr bool kCache = (kMode == kModeCache);
+  constexpr bool kRowsAgain = (kScore != 0 && !kCache);
   static_assert(!kCache || (!kSolo && !kPair && kScore != 0), "cache form");
   constexpr int kSoftmaxWarps = (kSolo || (kCache && NT == 1)) ? 4 : 8;
   constexpr int kEpilogueEnd = kSolo ? 4 : 12;  // epilogue warps are [kSoftmaxWarps, kEpilogueEnd): none in the solo form
@@ -1101,6 +1117,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       for (int s = 0; s < 8; s++) ptx::mbar_init(ptx::smem_u32(&cctl->scaleFull[s]), kConvWarps);
     }
     ctl->failed = 0;
+    if constexpr (kRowsAgain) ctl->rowsAgain = 0;
     ptx::fence_barrier_init();
     ptx::fence_proxy_async_smem();
   }
@@ -1146,7 +1163,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     ptx::grid_wait_previous();
     ptx::grid_allow_next();
   }
-  const WaitCtx wc{&ctl->failed, p.status, p.epoch};
+  const typename std::conditional<kRowsAgain, WaitCtxRows, WaitCtx>::type wc{&ctl->failed, p.status, p.epoch};
 
   // Every consumer of work items (8 softmax warps, 4 epilogue warps, 2 MMA threads) reads item k from slot k & 1
   // and frees the slot; a negative index ends the loop.
@@ -1523,7 +1540,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             }
           }
         }
-        if constexpr (kScore != 0) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head);
+        if constexpr (kScore != 0) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head, &ctl->rowsAgain);
         items++;
         continue;
       }
@@ -1804,7 +1821,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             }
           }
         }
-        if constexpr (kScore != 0 && !kCache) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head);
+        if constexpr (kScore != 0 && !kCache) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head, &ctl->rowsAgain);
         items[t]++;
       }
     }

@@ -38,18 +38,19 @@ __device__ __forceinline__ float dot16(uint4 a, uint4 b, float x) {
   return x;
 }
 
+// kDocs: calls with documents come here too (they have neither few rows nor key ranges).
 // All lanes of a warp call it for the same row (batch entry x seqLenQ + query, head), of which some columns are not finite in memory; the others
 // stay as they are.  A lane scores every 32nd key and owns every 32nd column of O.  A value of V that the row does see stays what it is: nothing is
 // done where no hidden key near the row has such a value (only the causal mask: a tile reads no more than 255 keys past its rows'), and
 // keys are taken from the last to the first until none of the columns can become finite any more.  Capped causal prefill 2 x 4096, 32 heads of 128,
 // 0.4 ms: 1.9 with all of V NaN,
 // 3.0 with one value a head at key 2048.
-template <class T, int D>
+template <class T, int D, bool kDocs = true>
 __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, int head, void* O) {
   constexpr int kCols = D / 32, kPer = 16 / (int)sizeof(T);
   const int lane = threadIdx.x & 31;
   const ScoreSource& s = f.src;
-  const bool docs = f.docQ != nullptr;
+  const bool docs = kDocs && f.docQ != nullptr;
   if (!s.causal && !docs) return;  // nothing is hidden
   const int b = (int)(row / s.seqLenQ), pos = f.qStart + (int)(row - (long long)b * s.seqLenQ);
   const long long kvStride = (long long)s.headsKV * D;
@@ -89,10 +90,15 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
     if (!__any_sync(0xffffffffu, hidden)) return;
   }
   const int doc = docs ? f.docQ[row] : 0;
+  int low = 0;
+  if (docs && f.rowKeys[row].x >= 0) {  // documents in ascending order
+    low = f.rowKeys[row].x;
+    end = min(end, f.rowKeys[row].y);
+  }
   const int from = bias_position(pos, s.seqLenKV);
   const float scale = rsqrtf((float)D), slope = f.slopes != nullptr ? f.slopes[head] : 0.f;
 #pragma unroll 1
-  for (int k0 = (end - 1) / 32 * 32; k0 >= 0; k0 -= 32) {
+  for (int k0 = (end - 1) / 32 * 32; k0 >= low / 32 * 32; k0 -= 32) {
     const int key = k0 + lane;
     const bool see = key < end && (!docs || (doc >= 0 && f.docKV[(long long)b * s.seqLenKV + key] == doc));
     const unsigned seen = __ballot_sync(0xffffffffu, see);
@@ -144,9 +150,10 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
   }
 }
 
-// Rows of a warp's lanes, each bad or not: computes those that are.  Rows that several lanes name are computed once.
-template <class T, int D>
-__device__ __forceinline__ void exact_rows(const ScoreFields& f, bool bad, long long row, int head, void* O) {
+// Rows of a warp's lanes, each bad or not: computes those that are.  Rows that several lanes name are computed once.  count (or null), in shared
+// memory: goes up with every row, for those who wait meanwhile.
+template <class T, int D, bool kDocs = true>
+__device__ __forceinline__ void exact_rows(const ScoreFields& f, bool bad, long long row, int head, void* O, int* count = nullptr) {
   unsigned left = __ballot_sync(0xffffffffu, bad);
   if (left == 0u) return;
   __syncwarp();  // what the lanes have stored
@@ -155,7 +162,8 @@ __device__ __forceinline__ void exact_rows(const ScoreFields& f, bool bad, long 
     const int j = __ffs(left) - 1;
     const long long r = __shfl_sync(0xffffffffu, row, j);
     const int h = __shfl_sync(0xffffffffu, head, j);
-    exact_row<T, D>(f, r, h, O);
+    exact_row<T, D, kDocs>(f, r, h, O);
+    if (count != nullptr && (threadIdx.x & 31) == 0) atomicAdd(count, 1);
     left &= ~__ballot_sync(0xffffffffu, row == r && head == h);
   }
 }
