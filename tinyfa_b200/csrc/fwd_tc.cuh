@@ -33,8 +33,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <stddef.h>
-
 #include <type_traits>
 
 #include "cache_codes.cuh"
@@ -315,7 +313,6 @@ struct Ctl {
   int failed;
   WorkSlot work[2];
   int peerIdx[2];  // pair form, rank 1: work indices handed over by rank 0
-  int rowsAgain;   // scored calls: rows that were computed again
 };
 static_assert(sizeof(Ctl) <= 2048, "control block");
 
@@ -324,28 +321,28 @@ struct WaitCtx {
   int* status;
   int epoch;
 };
-// ... where warps may have to compute rows again (score_row.cuh), for as long as those rows take: Ctl::rowsAgain changes with every one of them, and
-// a wait lasts while it does.
-struct WaitCtxRows : WaitCtx {};
-__device__ __forceinline__ int rows_again(const WaitCtx&) { return 0; }
-__device__ __forceinline__ int rows_again(const WaitCtxRows& c) { return c.failed[((int)offsetof(Ctl, rowsAgain) - (int)offsetof(Ctl, failed)) / (int)sizeof(int)]; }
+// ... where warps may have to compute rows again (score_row.cuh) while the others wait: up to 64 rows one after the other for two tiles, 0.9 us for
+// every key where a CTA does so alone and 12 where all CTAs read K and V at once (head dim 256).
+struct WaitCtxRows : WaitCtx {
+  int keys;
+};
+__device__ __forceinline__ uint64_t wait_limit(const WaitCtx&) { return 2000000000ull; }
+__device__ __forceinline__ uint64_t wait_limit(const WaitCtxRows& c) { return 2000000000ull + ((uint64_t)(uint32_t)c.keys << 14); }
 
-// Bounded wait: gives up after ~2 s, records (epoch << 8 | site) and lets the caller continue so that
+// Bounded wait: gives up after wait_limit ns, records (epoch << 8 | site) and lets the caller continue so that
 // every loop still terminates; later waits of the CTA return at once.
 template <class Ctx>
 __device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity, const Ctx& c, int site) {
   if (ptx::mbar_try_wait(bar, parity)) return;
   uint32_t spins = 0;
   uint64_t t0 = 0;
-  int rows = 0;
   while (!ptx::mbar_try_wait(bar, parity)) {
     if ((++spins & 0x3FF) == 0) {
       if (*c.failed) return;
       const uint64_t now = ptx::global_timer_ns();
-      if (t0 == 0 || rows_again(c) != rows) {
+      if (t0 == 0) {
         t0 = now;
-        rows = rows_again(c);
-      } else if (now - t0 > 2000000000ull) {
+      } else if (now - t0 > wait_limit(c)) {
         *c.failed = 1;
         atomicExch(c.status, (c.epoch << 8) | site);
         return;
@@ -381,15 +378,13 @@ __device__ __forceinline__ void spin_bar(uint32_t bar, uint32_t parity, const Ct
   if (ptx::mbar_test_wait(bar, parity)) return;
   uint32_t spins = 0;
   uint64_t t0 = 0;
-  int rows = 0;
   while (!ptx::mbar_test_wait(bar, parity)) {
     if ((++spins & 0x3FFF) == 0) {
       if (*c.failed) return;
       const uint64_t now = ptx::global_timer_ns();
-      if (t0 == 0 || rows_again(c) != rows) {
+      if (t0 == 0) {
         t0 = now;
-        rows = rows_again(c);
-      } else if (now - t0 > 2000000000ull) {
+      } else if (now - t0 > wait_limit(c)) {
         *c.failed = 1;
         atomicExch(c.status, (c.epoch << 8) | site);
         return;
@@ -799,7 +794,7 @@ struct ScoreRow {
 
   // The bias; `scale`: what a score still has to be multiplied by (capped scores: nothing).  left: all keys that the row sees lie to its left,
   // where the bias is linear in the key - 2 packed operations on a pair of scores instead of 3 and two absolute values.
-  __device__ __forceinline__ void bias_scores(uint32_t (&v)[4][32], int kbase, float scale, bool left) const {
+  __device__ __forceinline__ void bias_scores(uint32_t (&v)[4][32], int kbase, float scale, bool left, int pos) const {
     if (__builtin_expect(left, 1)) {
       const float2 step = make_float2(2.f * slope, 2.f * slope);
 #pragma unroll
@@ -835,11 +830,11 @@ struct ScoreRow {
       }
     }
   }
-  // Scores of a key block -> capped and biased, times log2(e).
+  // Scores of a key block -> capped and biased, times log2(e).  pos: worked out anew for every block rather than kept in a register.
   template <class P>
-  __device__ __forceinline__ void transform(const P& p, uint32_t (&v)[4][32], int kbase) const {
+  __device__ __forceinline__ void transform(const P& p, uint32_t (&v)[4][32], int kbase, int pos) const {
     if constexpr ((kScore & kScoreCap) != 0) cap_scores(v, capArg);
-    if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, p.scaleLog2, (p.causal && p.prefix == nullptr) || kbase + kBlockN - 1 <= seenByAllPos);
+    if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, p.scaleLog2, (p.causal && p.prefix == nullptr) || kbase + kBlockN - 1 <= seenByAllPos, pos);
   }
 
   // The same for codes, whose scores are multiplied by kf (by groups of 16 keys: the scale of the keys x the row's factor) first.
@@ -899,7 +894,7 @@ struct ScoreRow {
           }
         }
       }
-      if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, 1.f, left);
+      if constexpr ((kScore & kScoreBias) != 0) bias_scores(v, kbase, 1.f, left, pos);
     }
   }
 
@@ -950,11 +945,11 @@ struct ScoreRow {
 
 // Rows of a tile that V has spoilt from a masked place.  Partial results: the kernel that joins them looks.
 template <bool kBf16, int kHD, class P, class W>
-__device__ __forceinline__ void exact_rows_of_tile(const P& p, const W& w, int t, bool bad, int qpos, int head, int* rowsAgain) {
+__device__ __forceinline__ void exact_rows_of_tile(const P& p, const W& w, int t, bool bad, int qpos, int head) {
   if constexpr (std::is_base_of<TcPartParams, P>::value) {
     if (!whole_tile(p, w, t)) return;
   }
-  score::exact_rows<typename std::conditional<kBf16, __nv_bfloat16, __half>::type, kHD>(p, bad, w.qRow0 + qpos, head, p.O, rowsAgain);
+  score::exact_rows<typename std::conditional<kBf16, __nv_bfloat16, __half>::type, kHD>(p, bad, w.qRow0 + qpos, head, p.O);
 }
 
 // ---- kModeCache
@@ -1034,7 +1029,6 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   constexpr int NT = C::kNT;
   // warp roles: softmax warps [0, 4 * NT'), epilogue warps, the two MMA-issuing warps, the loading warp
   constexpr bool kCache = (kMode == kModeCache);
-  constexpr bool kRowsAgain = (kScore != 0 && !kCache);
   static_assert(!kCache || (!kSolo && !kPair && kScore != 0), "cache form");
   constexpr int kSoftmaxWarps = (kSolo || (kCache && NT == 1)) ? 4 : 8;
   constexpr int kEpilogueEnd = kSolo ? 4 : 12;  // epilogue warps are [kSoftmaxWarps, kEpilogueEnd): none in the solo form
@@ -1117,7 +1111,6 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       for (int s = 0; s < 8; s++) ptx::mbar_init(ptx::smem_u32(&cctl->scaleFull[s]), kConvWarps);
     }
     ctl->failed = 0;
-    if constexpr (kRowsAgain) ctl->rowsAgain = 0;
     ptx::fence_barrier_init();
     ptx::fence_proxy_async_smem();
   }
@@ -1163,7 +1156,13 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     ptx::grid_wait_previous();
     ptx::grid_allow_next();
   }
-  const typename std::conditional<kRowsAgain, WaitCtxRows, WaitCtx>::type wc{&ctl->failed, p.status, p.epoch};
+  const auto wc = [&] {
+    if constexpr (kScore != 0 && !kCache) {
+      return WaitCtxRows{{&ctl->failed, p.status, p.epoch}, p.seqLenKV};
+    } else {
+      return WaitCtx{&ctl->failed, p.status, p.epoch};
+    }
+  }();
 
   // Every consumer of work items (8 softmax warps, 4 epilogue warps, 2 MMA threads) reads item k from slot k & 1
   // and frees the slot; a negative index ends the loop.
@@ -1282,7 +1281,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           row.cache_transform(v, kbase, keyFactors, p.causal || kbase + kBlockN - 1 <= row.seenByAll, gone);
           vGrow = vMax > vRef * kCacheSlack;
         } else if constexpr (kScore != 0) {
-          row.transform(p, v, kbase);
+          row.transform(p, v, kbase, score::bias_position(p.qStart + qpos, w.skv));
         }
         bool needMask = (kMode != kModeFixedNoMask) &&
                         ((kbase + kBlockN > w.skv) || (p.causal && (kbase + kBlockN - 1 > (kScore != 0 ? row.seenByAll : w.qlo[t]))));
@@ -1540,7 +1539,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             }
           }
         }
-        if constexpr (kScore != 0) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head, &ctl->rowsAgain);
+        if constexpr (kScore != 0) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head);
         items++;
         continue;
       }
@@ -1821,7 +1820,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             }
           }
         }
-        if constexpr (kScore != 0 && !kCache) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head, &ctl->rowsAgain);
+        if constexpr (kScore != 0 && !kCache) exact_rows_of_tile<kBf16, kHD>(p, w, t, valid && spoilt != 0.f && l > 0.f && l < INFINITY, qpos, head);
         items[t]++;
       }
     }

@@ -150,10 +150,9 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
   }
 }
 
-// Rows of a warp's lanes, each bad or not: computes those that are.  Rows that several lanes name are computed once.  count (or null), in shared
-// memory: goes up with every row, for those who wait meanwhile.
+// Rows of a warp's lanes, each bad or not: computes those that are.  Rows that several lanes name are computed once.
 template <class T, int D, bool kDocs = true>
-__device__ __forceinline__ void exact_rows(const ScoreFields& f, bool bad, long long row, int head, void* O, int* count = nullptr) {
+__device__ __forceinline__ void exact_rows(const ScoreFields& f, bool bad, long long row, int head, void* O) {
   unsigned left = __ballot_sync(0xffffffffu, bad);
   if (left == 0u) return;
   __syncwarp();  // what the lanes have stored
@@ -163,7 +162,6 @@ __device__ __forceinline__ void exact_rows(const ScoreFields& f, bool bad, long 
     const long long r = __shfl_sync(0xffffffffu, row, j);
     const int h = __shfl_sync(0xffffffffu, head, j);
     exact_row<T, D, kDocs>(f, r, h, O);
-    if (count != nullptr && (threadIdx.x & 31) == 0) atomicAdd(count, 1);
     left &= ~__ballot_sync(0xffffffffu, row == r && head == h);
   }
 }
