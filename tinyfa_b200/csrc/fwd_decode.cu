@@ -445,8 +445,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
         mma16816<kBf16>(sc[1], qf[ks], kf[2], kf[3]);
       }
       if constexpr (kScore) {
-        const int posA = p.qStart + qposA, posB = p.qStart + qposB;
-        const int fromA = score::bias_position(posA, p.seqLenKV), fromB = score::bias_position(posB, p.seqLenKV);
+        const int posA = score::bias_position(p.qStart + qposA, p.seqLenKV), posB = score::bias_position(p.qStart + qposB, p.seqLenKV);
         int limA = keyEnd, limB = keyEnd;
         if (p.causal) {
           const int prefix = p.prefix != nullptr ? score::prefix_of(p, b, p.seqLenKV) : 0;
@@ -462,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, (D == 32 && !kEven) ? 8 : 1) fwd_spl
           for (int e = 0; e < 4; e++) {
             const int key = kb + n * 8 + 2 * tig + (e & 1);
             float x = sc[n][e];
-            if (p.slopes != nullptr) x = fmaf(e < 2 ? -slopeA : -slopeB, fabsf((float)((e < 2 ? fromA : fromB) - key)), x);
+            if (p.slopes != nullptr) x = fmaf(e < 2 ? -slopeA : -slopeB, fabsf((float)((e < 2 ? posA : posB) - key)), x);
             sc[n][e] = key < (e < 2 ? limA : limB) ? x : -INFINITY;
           }
         }

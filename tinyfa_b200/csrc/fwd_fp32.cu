@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
       const float slope = p.slopes != nullptr ? p.slopes[h] : 0.f;
 #pragma unroll
       for (int r = 0; r < RPT; r++) {
-        const int row = q0 + ty * RPT + r, pos = p.qStart + row, from = score::bias_position(pos, p.seqLenKV);
+        const int row = q0 + ty * RPT + r, pos = score::bias_position(p.qStart + row, p.seqLenKV);
         const int lim = p.causal ? min(skv, max(pos + 1, prefix)) : skv;
         const int rowDoc = (p.docKV != nullptr && row < sq) ? p.docQ[qRow0 + row] : -1;  // (all keys by their ids: a few per thread)
 #pragma unroll
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(BR * 8 / kRowsPerThread) fwd_fp32_kernel(const
           const int key = kbase + tx + 8 * i;
           float x = s[r][i] * p.scale;
           if (p.cap > 0.f) x = p.cap * tanhf(x / p.cap);
-          if (p.slopes != nullptr) x = fmaf(-slope, fabsf((float)(from - key)), x);
+          if (p.slopes != nullptr) x = fmaf(-slope, fabsf((float)(pos - key)), x);
           const bool see = key < lim && (p.docKV == nullptr || (rowDoc >= 0 && doc[i] == rowDoc));
           s[r][i] = see ? x * 1.44269504f : -INFINITY;
         }

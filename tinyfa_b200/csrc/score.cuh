@@ -37,8 +37,9 @@ namespace score {
 // with it inside 32 bits.
 __device__ __forceinline__ int prefix_of(const ScoreFields& f, long long b, int seqLenKV) { return min(max(f.prefix[b], 0), seqLenKV); }
 
-// Position from which the bias of a row is measured.  Behind the last key all distances share pos - (seqLenKV - 1), which is nothing to a softmax
-// and, left in, would take the bits of the scores: at slope 1/2 and 2^24 keys past them they are rounded to whole numbers.
+// Position from which the bias of a row is measured (the masks are the same from there).  Behind the last key all distances share
+// pos - (seqLenKV - 1), which is nothing to a softmax and, left in, would take the bits of the scores: at slope 1/2 and 2^24 keys past them they are
+// rounded to whole numbers.
 __device__ __forceinline__ int bias_position(int pos, int seqLenKV) { return min(pos, seqLenKV - 1); }
 
 // tanh(t) / t = c0 + c1 t^2 + c2 t^4 + c3 t^6 for |t| <= 1/2, fitted to the smallest largest error of the tanh (1.3e-7)

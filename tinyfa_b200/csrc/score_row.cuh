@@ -52,7 +52,7 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
   const ScoreSource& s = f.src;
   const bool docs = kDocs && f.docQ != nullptr;
   if (!s.causal && !docs) return;  // nothing is hidden
-  const int b = (int)(row / s.seqLenQ), pos = f.qStart + (int)(row - (long long)b * s.seqLenQ);
+  const int b = (int)(row / s.seqLenQ), pos = bias_position(f.qStart + (int)(row - (long long)b * s.seqLenQ), s.seqLenKV);
   const long long kvStride = (long long)s.headsKV * D;
   const T* q = static_cast<const T*>(s.q) + (row * s.headsQ + head) * D;
   const long long kv0 = (long long)b * s.seqLenKV * kvStride + (long long)(head / (s.headsQ / s.headsKV)) * D;
@@ -95,7 +95,6 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
     low = f.rowKeys[row].x;
     end = min(end, f.rowKeys[row].y);
   }
-  const int from = bias_position(pos, s.seqLenKV);
   const float scale = rsqrtf((float)D), slope = f.slopes != nullptr ? f.slopes[head] : 0.f;
 #pragma unroll 1
   for (int k0 = (end - 1) / 32 * 32; k0 >= low / 32 * 32; k0 -= 32) {
@@ -111,7 +110,7 @@ __device__ __forceinline__ void exact_row(const ScoreFields& f, long long row, i
       for (int d = 0; d < D / kPer; d++) x = dot16<T>(reinterpret_cast<const uint4*>(q)[d], k16[d], x);
       x *= scale;
       if (f.cap > 0.f) x = f.cap * tanhf(x / f.cap);
-      x = fmaf(-slope, fabsf((float)(from - key)), x) * 1.44269504f;
+      x = fmaf(-slope, fabsf((float)(pos - key)), x) * 1.44269504f;
     }
     float most = fmaxf(m, x);
 #pragma unroll
