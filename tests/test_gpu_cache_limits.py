@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import tinyfa_b200 as tfa
-from test_gpu_cache import CODE, _cache, _expect, _store_by_hand, form  # noqa: F401
+from test_gpu_cache import CODE, DT, _cache, _expect, _store_by_hand, form  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -176,3 +176,15 @@ def test_caps_below_and_above_what_fp32_holds(form):  # noqa: F811
     _expect(got, Q * 0, cache, [300], [2])
     got = tfa.flash_attn_cache_forward(Q * 0.1, *cache, one, cu, 2, 300, softcap=1e60)
     _expect(got, Q * 0.1, cache, [300], [2])
+
+
+@pytest.mark.parametrize("dtype,code,D,block", [("fp16", "int8", 64, 16), ("bf16", "e4m3", 128, 64), ("fp16", "e4m3", 256, 32), ("bf16", "int8", 96, 128)])
+@pytest.mark.parametrize("factor", [4, 40])
+def test_scores_on_both_sides_of_half_a_cap(dtype, code, D, block, factor, form):  # noqa: F811
+    """Some below half the cap, where the tanh is a polynomial, some far above, in the same blocks."""
+    lens, new = [700, 90], [3, 70]
+    cache = _cache(code, lens, 2, D, block, 16, spread=0.3)
+    Q = (torch.randn(sum(new), 4, D, device="cuda") * factor).to(DT[dtype])
+    cu = torch.tensor([0, 3, 73], dtype=torch.int32, device="cuda")
+    got = tfa.flash_attn_cache_forward(Q, *cache, torch.tensor(lens, dtype=torch.int32, device="cuda"), cu, 70, 700, softcap=30.0)
+    _expect(got, Q, cache, lens, new, True, 30.0)

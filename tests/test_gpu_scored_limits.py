@@ -114,6 +114,22 @@ def test_caps_below_and_above_what_fp32_holds(call):
     _compare(got, Q, K, V, False, fp32_error=2.0 ** -19)
 
 
+@pytest.mark.parametrize("cap,factor", [(30.0, 3.0), (30.0, 12.0), (5.0, 2.0)])
+def test_scores_on_both_sides_of_half_a_cap(call, cap, factor):
+    """Scores of factor^2 standard normals: some below half the cap, where the tanh is a polynomial, some far above, in the same blocks."""
+    dtype, Sq, Skv, Hq, Hkv, D = call
+    Q, K, V = _inputs(dtype, 1, Sq, Skv, Hq, Hkv, D, 7)
+    Q, K = Q * factor, K * factor
+    for causal, q_start in ((False, 0), (True, Skv - Sq)):
+        got = tfa.flash_attn_scored_forward(Q, K, V, is_causal=causal, softcap=cap, q_start=q_start)
+        _compare(got, Q, K, V, causal, cap, q_start=q_start, fp32_error=2.0 ** -19)
+    # Q in a block of small scores only, and in one of large ones only
+    Q[:, : Sq // 2] /= 64
+    got = tfa.flash_attn_scored_forward(Q, K, V, softcap=cap, alibi_slopes=_slopes(Hq))
+    _compare(got, Q, K, V, False, cap, _slopes(Hq), fp32_error=2.0 ** -19)
+    tfa.device_status()
+
+
 def test_tangents_are_refused():
     """Forward-mode gradients are not dropped either."""
     import torch.autograd.forward_ad as fwd
