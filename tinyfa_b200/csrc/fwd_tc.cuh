@@ -1720,12 +1720,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           if (lane == 0) {
             if (!wasV && wasBlk > 0) ptx::mbar_arrive(ptx::smem_u32(&cctl->scaleFull[g]));  // the scales: before the scores can be there
             ptx::mbar_arrive(bar(kBarKvFull + s));
-            if (cw == 0) {  // the stage-free arrival of every tile that will not touch this block
-#pragma unroll
-              for (int t = 0; t < 2; t++) {
-                if (t >= NT || wasBlk >= w.nblk[t]) ptx::mbar_arrive(bar(kBarKvEmpty + s));
-              }
-            }
+            if (NT == 1 && cw == 0) ptx::mbar_arrive(bar(kBarKvEmpty + s));  // for the issuing thread that there is not
           }
           if (i == 0) {  // the row factors of both tiles belong to the first block
             if (NT == 2) fillQ(1);
@@ -1885,12 +1880,20 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       // One issuing thread per Q tile (warp 12: tile 0, warp kIssuerB: tile 1).  Every wait and commit costs the
       // issuing thread ~100 clocks during which it feeds nothing to the tensor pipe; with two issuers the other
       // tile's MMAs fill those gaps.  Both threads walk the same ring of K/V loads; a stage is free again after two
-      // arrivals: a tcgen05.commit from each tile that used the block, and for a tile that did not use it (causal:
-      // the last block belongs to tile 1 alone; one-tile head dims: tile 1 never) one from the loader when it issues
-      // the load.  A thread therefore never waits for a block it does not need, and the loader's arrival cannot be
-      // counted for the stage's previous use because the loader has waited for that phase before re-using the stage.
+      // arrivals: a tcgen05.commit from each tile that used the block, and a plain one from a tile that does not use it
+      // (causal: the last block belongs to tile 1 alone; an item may have no second tile), as soon as it sees the load.  So
+      // each thread sees every load once and the ring never gets ahead of it.  (Skipped loads would let the ring be two
+      // uses of a stage behind the next load that the thread needs - an item without a second tile whose loads are
+      // two rounds of the ring - and a parity wait for that load returns before it has landed; nor can they be looked at later,
+      // when the stage may have been loaded again.)  One-tile forms: the loader arrives for the thread that there is not.
       auto release = [&](int stage, bool used) {
         if (used) commit(bar(kBarKvEmpty + stage));
+      };
+      auto skip = [&](int stage, uint32_t parity) {  // a load that this tile does not use
+        if constexpr (NT == 2) {
+          wait_bar(bar(kBarKvFull + stage), parity, wc, 33);
+          ptx::mbar_arrive(bar(kBarKvEmpty + stage));
+        }
       };
       // The two issuers take strict turns (A: tile 0, B: tile 1, A, B, ...), which keeps the two tiles in
       // anti-phase: one tile's softmax runs while the other tile's MMAs run.  Without the turn token the two
@@ -1954,6 +1957,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           }
           passTurn();
           if constexpr (!kRingSig) release(s0, n > 0);
+          if (n == 0) skip(s0, ph0);
           ld++;
         }
         for (int j = 0; j < w.nmax; j++) {
@@ -1994,6 +1998,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                 commit(bar(kBarSFull + 2 * t + ((blk + 1) & 1)));
               }
               if (j + 2 == n) commit(bar(kBarQEmpty + 2 * t + (qc % C::kQBufs)));
+            } else if (hasNext) {
+              skip(sK, phK);
             }
             if (j < n) {
               wait_bar(bar(kBarKvFull + sV), phV, wc, 10);
@@ -2009,6 +2015,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
               } else {
                 commit(bar(kBarPvDone + 2 * t + (blk & 1)));
               }
+            } else {
+              skip(sV, phV);
             }
             if constexpr (!kRingSig) {
               if (hasNext) release(sK, j + 1 < n);
@@ -2050,8 +2058,10 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             passTurn();
           }
           release(sV, j < n);
+          if (j >= n) skip(sV, phV);
           if (hasNext) {
             release(sK, j + 1 < n);
+            if (j + 1 >= n) skip(sK, phK);
             ld++;
           }
         }
@@ -2306,11 +2316,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                                w.batchTma);
             }
           }
-          // the stage-free arrival of every tile that will not touch this block
-#pragma unroll
-          for (int t = 0; t < 2; t++) {
-            if (t >= NT || blkIdx >= w.nblk[t]) ptx::mbar_arrive(bar(kBarKvEmpty + s));
-          }
+          if constexpr (NT == 1) ptx::mbar_arrive(bar(kBarKvEmpty + s));  // for the issuing thread that there is not
         }
         if (!nextDone) more = publish(k + 1);
       }
