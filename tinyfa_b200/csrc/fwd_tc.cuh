@@ -1881,8 +1881,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       // issuing thread ~100 clocks during which it feeds nothing to the tensor pipe; with two issuers the other
       // tile's MMAs fill those gaps.  Both threads walk the same ring of K/V loads; a stage is free again after two
       // arrivals: a tcgen05.commit from each tile that used the block, and a plain one from a tile that does not use it
-      // (causal: the last block belongs to tile 1 alone; an item may have no second tile), as soon as it sees the load.  So
-      // each thread sees every load once and the ring never gets ahead of it.  (Skipped loads would let the ring be two
+      // (causal: the last block belongs to tile 1 alone; an item may have no second tile) that sees the load after its own
+      // work.  So each thread sees every load once and the ring never gets ahead of it.  (Skipped loads would let the ring be two
       // uses of a stage behind the next load that the thread needs - an item without a second tile whose loads are
       // two rounds of the ring - and a parity wait for that load returns before it has landed; nor can they be looked at later,
       // when the stage may have been loaded again.)  One-tile forms: the loader arrives for the thread that there is not.
@@ -1957,7 +1957,6 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           }
           passTurn();
           if constexpr (!kRingSig) release(s0, n > 0);
-          if (n == 0) skip(s0, ph0);
           ld++;
         }
         for (int j = 0; j < w.nmax; j++) {
@@ -1998,8 +1997,6 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                 commit(bar(kBarSFull + 2 * t + ((blk + 1) & 1)));
               }
               if (j + 2 == n) commit(bar(kBarQEmpty + 2 * t + (qc % C::kQBufs)));
-            } else if (hasNext) {
-              skip(sK, phK);
             }
             if (j < n) {
               wait_bar(bar(kBarKvFull + sV), phV, wc, 10);
@@ -2015,8 +2012,6 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
               } else {
                 commit(bar(kBarPvDone + 2 * t + (blk & 1)));
               }
-            } else {
-              skip(sV, phV);
             }
             if constexpr (!kRingSig) {
               if (hasNext) release(sK, j + 1 < n);
@@ -2058,11 +2053,20 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             passTurn();
           }
           release(sV, j < n);
-          if (j >= n) skip(sV, phV);
           if (hasNext) {
             release(sK, j + 1 < n);
-            if (j + 1 >= n) skip(sK, phK);
             ld++;
+          }
+        }
+        if constexpr (NT == 2) {
+          if (n < w.nmax) {
+            const int ld0 = ld - 2 * w.nmax;
+            int i = ld0 + 2 * n;
+            if (C::kTwoPos && n > 0) {  // K of block n comes ahead of V of block n - 1
+              skip((i - 1) % NS, ((i - 1) / NS) & 1);
+              i++;
+            }
+            for (; i < ld; i++) skip(i % NS, (i / NS) & 1);
           }
         }
         it += n;
