@@ -83,3 +83,32 @@ def test_packed(causal, D):
         see, _ = visible(lens[b], lens[b], causal)
         o, off, a = attend(Q[one].double(), K[one].double(), V[one].double(), see)
         check(got[one], o, off, a, U[torch.bfloat16])
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 96), ("bf16", 192), ("fp16", 256), ("bf16", 64)])
+@pytest.mark.parametrize("Skv", [100, 200, 300])
+def test_items_of_few_key_blocks_behind_a_slow_output(dtype, D, Skv):
+    """The warps that write a tile's output compute rows again, because a masked value is NaN; meanwhile the softmax of the next items, of one to
+    three key blocks each, is done."""
+    B, Sq = 700, 256
+    Q, K, V = _inputs(dtype, B, Sq, Skv, 2, 1, D)
+    V2 = V.clone()
+    V2[:, 50:, :, 5] = float("nan")
+    got = tfa.flash_attn_scored_forward(Q, K, V2, is_causal=True)
+    tfa.device_status()
+    see, _ = visible(50, Skv, True)
+    for b in range(0, B, 31):
+        o, off, a = attend(Q[b, :50].double(), K[b].double(), V[b].double(), see)
+        check(got[b, :50], o, off, a, U[Q.dtype], Skv * 2.0 ** -25 * V[b].abs().max().item() if Q.dtype == torch.float16 else 0.0)
+        assert not torch.isfinite(got[b, 50:, :, 5]).any() and torch.isfinite(got[b, 50:, :, 6:]).all()
+
+
+@pytest.mark.parametrize("D", [96, 128, 192, 256])
+@pytest.mark.parametrize("Skv", [1, 77, 128, 250])
+def test_items_of_one_and_two_key_blocks(D, Skv):
+    Q, K, V = _inputs("bf16", 300, 400, Skv, 4, 2, D)
+    got = _same(lambda: tfa.flash_attn_forward(Q, K, V), 60)
+    see, _ = visible(400, Skv, False)
+    for b in range(0, 300, 37):
+        o, off, a = attend(Q[b].double(), K[b].double(), V[b].double(), see)
+        check(got[b], o, off, a, U[torch.bfloat16])

@@ -279,6 +279,7 @@ enum Bar : int {
   kBarScaleFull = 20,  // [2]  softmax published the final row sums (once per tile and item)
   kBarTurn = 22,       // [2]  issue-turn token of the MMA thread of tile t
   kBarSFree = 24,      // [2]  softmax has read S into registers (rotating-S mode only)
+  kBarScaleRead = 24,  // [2]  epilogue has read the row sums (4 epilogue warps; forms without rotating S)
   kBarOFree = 26,      // [2]  epilogue has read O of the item into registers (4 epilogue warps)
   kBarWorkFull = 28,   // [2]  loader published the next work item in slot k & 1
   kBarWorkEmpty = 30,  // [2]  every consumer has read the slot
@@ -1066,6 +1067,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   Ctl* ctl = reinterpret_cast<Ctl*>(smem + NT * C::kQBufs * C::kTileBytes + NS * C::kStageBytes);
   const uint32_t barBase = ptx::smem_u32(&ctl->bars[0]);
   [[maybe_unused]] CacheCtl* cctl = reinterpret_cast<CacheCtl*>((reinterpret_cast<uintptr_t>(ctl + 1) + 15) & ~(uintptr_t)15);
+  constexpr bool kScaleRead = !kSolo && !kCache && !kPair && !C::kRot;  // kBarScaleRead is used
   constexpr int kConvWarps = kEpilogueEnd - kSoftmaxWarps;  // cache form: the warps that fill the tiles
   auto bar = [&](int slot) { return barBase + 8u * (uint32_t)slot; };
 
@@ -1756,6 +1758,10 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         pvTotal[t] += n;
         wait_bar(bar(kBarScaleFull + t), items[t] & 1, wc, 6);
         const float l = ctl->scale[t][r];
+        if constexpr (kScaleRead) {
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(kBarScaleRead + t));
+        }
         // Last P.V of the item.  Valid as a parity wait: the softmax published its row sums after storing the
         // last P, i.e. after all earlier P.V of the tile, and the next item's P.V waits for kBarOFree below.
         // (with two S positions P.V of block X-1 may still be running at this point: its barrier is the other one)
@@ -1943,6 +1949,14 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             wait_bar(bar(kBarKvFull + s0), ph0, wc, 8);
             wait_bar(bar(kBarQFull + 2 * t + (qc % C::kQBufs)), (qc / C::kQBufs) & 1, wc, 9);
             ptx::tc_fence_after();
+          }
+          // The softmax publishes an item's row sums in the place of the item's before, which the epilogue has to have read.  Scores that are
+          // issued behind the first P.V of the item come after that, since P.V waits for the epilogue; the last block's may be issued before it
+          // in items of one block (two S positions: of up to two), and wait here.
+          if constexpr (!kSolo && !kCache) {
+            if (n > 0 && n <= (C::kTwoPos ? 2 : 1) && qc > 0) {
+              wait_bar(bar(kScaleRead ? kBarScaleRead + t : kPair ? (int)kBarOFreePair : kBarOFree + t), (qc - 1) & 1, wc, 34);
+            }
           }
           takeTurn();
           if (n > 0) {
