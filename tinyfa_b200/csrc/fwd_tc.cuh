@@ -1722,7 +1722,12 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           if (lane == 0) {
             if (!wasV && wasBlk > 0) ptx::mbar_arrive(ptx::smem_u32(&cctl->scaleFull[g]));  // the scales: before the scores can be there
             ptx::mbar_arrive(bar(kBarKvFull + s));
-            if (NT == 1 && cw == 0) ptx::mbar_arrive(bar(kBarKvEmpty + s));  // for the issuing thread that there is not
+            if (cw == 0) {  // the stage-free arrival of every tile that will not touch this block
+#pragma unroll
+              for (int t = 0; t < 2; t++) {
+                if (t >= NT || wasBlk >= w.nblk[t]) ptx::mbar_arrive(bar(kBarKvEmpty + s));
+              }
+            }
           }
           if (i == 0) {  // the row factors of both tiles belong to the first block
             if (NT == 2) fillQ(1);
@@ -1892,6 +1897,9 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       // uses of a stage behind the next load that the thread needs - an item without a second tile whose loads are
       // two rounds of the ring - and a parity wait for that load returns before it has landed; nor can they be looked at later,
       // when the stage may have been loaded again.)  One-tile forms: the loader arrives for the thread that there is not.
+      // Cache form: the converter warps arrive for a tile that does not use a block.  They hand over tiles in order, Q of tile 1 behind the first K,
+      // so that what a thread waits for first in an item pins the ring, and tile 0 skips a block at most (the waits cost 15 % there, 238
+      // -> 274 us for 512 queries behind 8192 tokens without a bias).
       auto release = [&](int stage, bool used) {
         if (used) commit(bar(kBarKvEmpty + stage));
       };
@@ -2072,7 +2080,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             ld++;
           }
         }
-        if constexpr (NT == 2) {
+        if constexpr (NT == 2 && !kCache) {
           if (n < w.nmax) {
             const int ld0 = ld - 2 * w.nmax;
             int i = ld0 + 2 * n;
