@@ -160,11 +160,11 @@ int tfa_b200_fwd_decode_noalloc(const void* Q, const void* K, const void* V, voi
  * a chunk or a single token behind keys that are there already).
  *   s = q . k / sqrt(headDim);  softcap > 0: s <- softcap * tanh(s / softcap);  alibiSlopes [numHeadsQ]: s <- s - slope_h * |position - j|
  *   A row sees key j if (not isCausal, or j <= position, or j < prefixLens[b]) and (no documents, or docIdsQ[b][i] == docIdsKV[b][j] >= 0).
- * prefixLens int32 [batchSize] (with isCausal only); docIdsQ int32 [batchSize, seqLenQ], docIdsKV int32 [batchSize, seqLenKV]: both or
- * neither; negative ids belong to no document (padding): such a key is seen by no row and such a row sees no key.  Ids may come in any
- * order; keys outside the range of blocks that a 128-row tile of queries can see are not read, so runs of equal ids in ascending order
- * are fast.  A row that sees no key is zero.  What a row does not see has no effect on it, NaN and infinities included.  softcap 0 and
- * null pointers switch a part off.
+ * prefixLens int32 [batchSize] (with isCausal only; below zero: none, past the keys: all of them); docIdsQ int32 [batchSize, seqLenQ],
+ * docIdsKV int32 [batchSize, seqLenKV]: both or neither; negative ids belong to no document (padding): such a key is seen by no row and such
+ * a row sees no key.  Ids may come in any order; keys outside the range of blocks that a 128-row tile of queries can see are not read, so runs
+ * of equal ids in ascending order are fast.  A row that sees no key is zero.  What a row does not see has no effect on it, NaN and infinities
+ * included.  softcap 0 and null pointers switch a part off.
  */
 int tfa_b200_fwd_scored(const void* Q, const void* K, const void* V, void* O, int dtype, int batchSize, int seqLenQ, int seqLenKV,
                         int numHeadsQ, int numHeadsKV, int headDim, int isCausal, int qStart, float softcap, const float* alibiSlopes,

@@ -1,8 +1,8 @@
 // Codes of the 8-bit cache -> fp16, exactly: int8 and e4m3 both fit its 11 bits.
 //
 // e4m3 is converted.  Widening it with shifts and masks instead (sign, exponent and mantissa moved to where fp16 has them are the code times
-// 2^-8) was slower in both attention kernels, which are bound by issue slots there: decode of 64 requests of 4000 tokens 103 -> 119 us, chunks of
-// queries 350 -> 366.
+// 2^-8) was slower in both attention kernels, where it lengthens the chain of the warps that convert: decode of 64 requests of 4000 tokens
+// 103 -> 119 us, chunks of queries 350 -> 366.
 #pragma once
 
 #include <cuda_fp16.h>
